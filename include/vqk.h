@@ -385,6 +385,105 @@ int vqk_linear_apply(const vqk_weights *w, const void *x, int32_t x_type, int64_
 int vqk_skipzero_row_table_host(const uint8_t *rowmask, int64_t E,
                                 int64_t OUT, int32_t *table, int64_t *n_live);
 
+/* ---- MXFP4: microscaled 4-bit weights ---------------------------------------
+ * No counterpart in the reference (its formats are vector-quantised): the
+ * OCP microscaling format with 4-bit elements, which the matrix cores of
+ * gfx950 take as operands, for checkpoints that hold it beside VQ modules.
+ * A row of C values is NB = ceil(C / 32) blocks of 32; block b is 16 bytes of
+ * codes (element 2i in the low half of byte i; zeros past C) and a scale byte
+ * s: value = e2m1(code) * 2^(s - 127), with e2m1 in {0, .5, 1, 1.5, 2, 3, 4, 6}
+ * and the sign in a code's top bit. s = 255: the whole block is NaN.
+ *
+ *   codes   uint8 [E, OUT, NB * 16], 16-byte aligned
+ *   scales  uint8 [E, OUT, NB]
+ * A dense linear is E = 1. */
+typedef struct vqk_mx_weights {
+    const uint8_t *codes;
+    const uint8_t *scales;
+    int64_t        E;
+    int64_t        OUT;
+    int64_t        IN;
+} vqk_mx_weights;
+
+/* x [rows, cols] (rows ldx elements apart) -> codes [rows, NB * 16] (4-byte
+ * aligned) and scales [rows, NB]: s - 127 = floor(log2(largest magnitude)) - 2,
+ * at least -127; elements rounded to nearest, ties to the even code, past 6 to
+ * 6. A block that holds an infinity or NaN becomes s = 255, codes 0. x: fp16,
+ * bf16 or fp32. vqk_mx_dequantize is the way back, into out [rows, cols]. */
+int vqk_mx_quantize(const void *x, int32_t x_type, int64_t rows, int64_t cols, int64_t ldx,
+                    uint8_t *codes, uint8_t *scales, void *stream);
+int vqk_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols,
+                      void *out, int32_t out_type, void *stream);
+
+/* y [N, OUT] = x [N, IN] . W^T, fp32 accumulation, one rounding into y_type
+ * (VQK_VIA_F16 as elsewhere). act: VQK_MX_ACT_NONE takes x as it is (every
+ * weight and every x enters the matrix cores exactly); VQK_MX_ACT_MXFP4
+ * quantises x's rows as vqk_mx_quantize does and multiplies 4-bit operands.
+ * The workspace is 256-byte aligned. */
+#define VQK_MX_ACT_NONE  0
+#define VQK_MX_ACT_MXFP4 1
+int vqk_mx_linear_workspace(const vqk_mx_weights *w, int32_t x_type, int64_t N, int32_t act,
+                            size_t *bytes);
+int vqk_mx_linear(const vqk_mx_weights *w, const void *x, int32_t x_type, int64_t N, int32_t act,
+                  void *y, int32_t y_type, void *workspace, size_t ws_bytes, void *stream);
+/* The gradient of x of that product (act NONE): dx [N, IN] = dy [N, OUT] . W. */
+int vqk_mx_linear_dx_workspace(const vqk_mx_weights *w, int32_t dy_type, int64_t N, size_t *bytes);
+int vqk_mx_linear_dx(const vqk_mx_weights *w, const void *dy, int32_t dy_type, int64_t N, void *dx,
+                     int32_t dx_type, void *workspace, size_t ws_bytes, void *stream);
+
+/* Routed experts, the contract of vqk_moe_expert_gemv: pair n multiplies row
+ * n / xkrep of x [T, IN] with expert eidx[n], y [N, OUT], N = T * xkrep; a pair
+ * whose id is outside [0, E) gives a row of zeros. E at most 4096. */
+int vqk_mx_switch_workspace(const vqk_mx_weights *w, int32_t x_type, int64_t T, int64_t N,
+                            size_t *bytes);
+int vqk_mx_switch(const vqk_mx_weights *w, const void *x, int32_t x_type, int64_t T,
+                  const int32_t *eidx, int64_t N, int64_t xkrep, void *y, int32_t y_type,
+                  void *workspace, size_t ws_bytes, void *stream);
+
+/* The block of experts: y_t = sum_j wts[t, j] down_e(silu(gate_e x_t) * (up_e x_t)),
+ * e = ids[t, j]; gate, up [E, I, H], down [E, H, I]. Pairs whose id is outside
+ * [0, E) add nothing, whatever their weight. The SwiGLU rows are rounded to
+ * x's type. ids, wts: [T, top_k], as vqk_route leaves them. */
+int vqk_mx_experts_workspace(const vqk_mx_weights *gate, const vqk_mx_weights *up,
+                             const vqk_mx_weights *down, int32_t x_type, int64_t T, int32_t top_k,
+                             size_t *bytes);
+int vqk_mx_experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, const vqk_mx_weights *down,
+                   const void *x, int32_t x_type, int64_t T, const int32_t *ids, const float *wts,
+                   int32_t top_k, void *y, int32_t y_type, void *workspace, size_t ws_bytes,
+                   void *stream);
+
+/* ---- router -------------------------------------------------------------------
+ * The layer calls' routing (softmax, top_k, renormalised when norm_topk != 0)
+ * as a call of its own, with what training it needs. logits [T, E] rows ld
+ * elements apart, fp16, bf16 or fp32; E at most 2048, top_k at most 64.
+ *   mask    [T] bytes or NULL: 0 marks a padding token. It, and a token whose
+ *           logits are all -inf, gets ids -1 and weights 0 and counts nowhere
+ *   ids     int32 [T, top_k], largest logit first, ties to the lower id; -1
+ *           (weight 0) where no expert above -inf is left
+ *   wts     fp32 [T, top_k]
+ *   counts  int32 [E]: tokens that chose each expert
+ *   stats   fp32 [3]: balance = E sum_e counts_e / (n top_k) * mean_t p_te,
+ *           z = mean_t logsumexp(l_t)^2, and n, the tokens both means run over
+ *           (n = 0: both 0)
+ *   saved   fp32 [T, 2], for vqk_route_backward; may be NULL
+ * counts and stats are both given or both NULL; without them no workspace is
+ * needed. A NaN logit is never chosen and makes its token's weights NaN, and
+ * with them the losses. Results are the same from call to call.
+ *
+ * vqk_route_backward: the gradient of the logits [T, E] (contiguous, in their
+ * type) from those of the weights [T, top_k], balance and z (fp32 in device
+ * memory, each may be NULL). counts, as a number of choices, has none. */
+int vqk_route_workspace(int64_t T, int64_t E, size_t *bytes);
+int vqk_route(const void *logits, int32_t l_type, int64_t T, int64_t E, int64_t ld,
+              const uint8_t *mask, int32_t top_k, int32_t norm_topk, int32_t *ids, float *wts,
+              int32_t *counts, float *stats, float *saved, void *workspace, size_t ws_bytes,
+              void *stream);
+int vqk_route_backward(const void *logits, int32_t l_type, int64_t T, int64_t E, int64_t ld,
+                       int32_t top_k, int32_t norm_topk, const int32_t *ids, const float *wts,
+                       const int32_t *counts, const float *stats, const float *saved,
+                       const float *dw, const float *dbalance, const float *dz, void *dlogits,
+                       void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,7 @@ VQK_NOALLOC_SCRATCH_BYTES = 32 << 20     # include/vqk.h
 VQK_MOE_HEADER_BYTES = 49152             # include/vqk.h: zero before a layer workspace's first call
 VQK_VIA_F16 = 0x100                      # output type flag: round through fp16 first
 VQK_X_KEEP = 0x200                       # x type flag (d=8 GEMV): x enters the products unrounded
+VQK_MX_ACT_NONE, VQK_MX_ACT_MXFP4 = range(2)   # include/vqk.h: x of an MXFP4 linear as it is / in 4 bits
 
 c_i32, c_i64, c_p, c_sz = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t
 
@@ -44,6 +45,12 @@ class VQKOptions(ctypes.Structure):
                 ("decode_bf16io", c_i32), ("prefill_bf16io", c_i32),
                 ("crowded_grouped", c_i32)]
 
+
+class VQKMXWeights(ctypes.Structure):
+    _fields_ = [("codes", c_p), ("scales", c_p), ("E", c_i64), ("OUT", c_i64), ("IN", c_i64)]
+
+
+_MXW = ctypes.POINTER(VQKMXWeights)
 
 # name -> (restype, argtypes), one entry per function of include/vqk.h
 SIGNATURES = {
@@ -96,6 +103,24 @@ SIGNATURES = {
                                          ctypes.POINTER(VQKOptions), ctypes.POINTER(c_sz)]),
     "vqk_linear_apply": (c_i32, [ctypes.POINTER(VQKWeights), c_p, c_i32, c_i64, c_p, c_i32, c_p,
                                  c_sz, ctypes.POINTER(VQKOptions), c_p]),
+    "vqk_mx_quantize": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, c_p, c_p, c_p]),
+    "vqk_mx_dequantize": (c_i32, [c_p, c_p, c_i64, c_i64, c_p, c_i32, c_p]),
+    "vqk_mx_linear_workspace": (c_i32, [_MXW, c_i32, c_i64, c_i32, ctypes.POINTER(c_sz)]),
+    "vqk_mx_linear": (c_i32, [_MXW, c_p, c_i32, c_i64, c_i32, c_p, c_i32, c_p, c_sz, c_p]),
+    "vqk_mx_linear_dx_workspace": (c_i32, [_MXW, c_i32, c_i64, ctypes.POINTER(c_sz)]),
+    "vqk_mx_linear_dx": (c_i32, [_MXW, c_p, c_i32, c_i64, c_p, c_i32, c_p, c_sz, c_p]),
+    "vqk_mx_switch_workspace": (c_i32, [_MXW, c_i32, c_i64, c_i64, ctypes.POINTER(c_sz)]),
+    "vqk_mx_switch": (c_i32, [_MXW, c_p, c_i32, c_i64, c_p, c_i64, c_i64, c_p, c_i32, c_p, c_sz,
+                              c_p]),
+    "vqk_mx_experts_workspace": (c_i32, [_MXW, _MXW, _MXW, c_i32, c_i64, c_i32,
+                                         ctypes.POINTER(c_sz)]),
+    "vqk_mx_experts": (c_i32, [_MXW, _MXW, _MXW, c_p, c_i32, c_i64, c_p, c_p, c_i32, c_p, c_i32,
+                               c_p, c_sz, c_p]),
+    "vqk_route_workspace": (c_i32, [c_i64, c_i64, ctypes.POINTER(c_sz)]),
+    "vqk_route": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, c_p, c_i32, c_i32, c_p, c_p, c_p, c_p,
+                          c_p, c_p, c_sz, c_p]),
+    "vqk_route_backward": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, c_i32, c_i32, c_p, c_p, c_p,
+                                   c_p, c_p, c_p, c_p, c_p, c_p, c_p]),
 }
 
 _LIB = None

@@ -3,6 +3,7 @@ the current HIP stream. torch provides device memory and streams only; the
 arithmetic runs in libvqk."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -31,6 +32,16 @@ def code_type(t: torch.Tensor) -> int:
 
 def stream(device=None) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(t: torch.Tensor):
+    """Context with t's device current: kernels launch on the current device."""
+    if t.device.index is None or t.device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(t.device)
 
 
 def ptr(t) -> ctypes.c_void_p:

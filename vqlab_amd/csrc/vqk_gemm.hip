@@ -583,6 +583,13 @@ int seg_sort(const uint32_t *eidx, int64_t N, int64_t E, int tok, void *ws, hipS
     return launch_with_lds<k_group_sort>(dim3(1), dim3(kSortThreads), sort_lds, st, a);
 }
 
+SegTiles seg_tiles(const void *ws, int64_t N, int64_t E) {
+    const uint8_t *b = static_cast<const uint8_t *>(ws);
+    const size_t meta = sort_order_bytes(N), count = meta + sort_meta_bytes(N, E);
+    return SegTiles{reinterpret_cast<const int32_t *>(b), reinterpret_cast<const int32_t *>(b + meta),
+                    reinterpret_cast<const int32_t *>(b + count)};
+}
+
 int seg_run(const vqk_weights *w, const SegCall &c, const void *sort_ws, hipStream_t st) {
     Geom g;
     int rc = make_geom(w, &g);

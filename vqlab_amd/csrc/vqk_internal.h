@@ -76,6 +76,10 @@ bool seg_ok(const vqk_weights *w, int64_t N);
 // or 4) and the tile count.
 int seg_sort(const uint32_t *eidx, int64_t N, int64_t E, int tok, void *ws, hipStream_t st);
 
+// Where seg_sort leaves its results in `ws`.
+struct SegTiles { const int32_t *order, *meta, *ntiles; };
+SegTiles seg_tiles(const void *ws, int64_t N, int64_t E);
+
 // One projection over a routing sorted into `sort_ws` (or over N dense rows
 // of expert 0 when sort_ws is NULL).
 int seg_run(const vqk_weights *w, const SegCall &c, const void *sort_ws, hipStream_t st);

@@ -1,0 +1,147 @@
+// MXFP4 (microscaled 4-bit) weights: shared declarations of the vqk_mx*
+// sources. A row of C values is NB = ceil(C / 32) blocks; block b holds 32
+// codes of 4 bits in 16 bytes (the earlier element in the low half of a byte,
+// codes past C zero) and one scale byte s: element = e2m1(code) * 2^(s - 127),
+// s = 255 a block of NaN.
+//
+// Two facts carry every kernel here:
+//   * e2m1 * 2^(s - 127) has at most two significant bits and an exponent
+//     inside bf16's, so a bf16 weight is the exact weight
+//     (v_cvt_scalef32_pk_bf16_fp4 makes two of them, scale included);
+//   * the sum over k may be taken in any order, so a lane of a 16x16x32 MFMA
+//     owns one whole block (16 bytes, one scale): lane group g = lane / 16
+//     holds block 4c + g of the 128-wide chunk c, and step s of four
+//     multiplies elements 8s..8s+7 of each group's block. Weights then go
+//     from global memory to registers with one 16-byte load, no LDS, and the
+//     x operand is the matching 16-byte piece of its row.
+#pragma once
+
+#include "vqk_gemv.h"
+#include "vqk_internal.h"
+
+namespace vqk {
+
+typedef __bf16 mx_b2 __attribute__((ext_vector_type(2)));
+typedef __bf16 mx_b8 __attribute__((ext_vector_type(8)));
+
+constexpr int kMxBlock = 32;
+constexpr int kMxChunk = 128;                 // k of one weight load: 4 lane groups x 32
+
+struct MxGeom { int64_t E, OUT, IN, NB; };
+// Validates `w` and fills `g`; returns a VQK_* status and sets the message.
+int make_mx_geom(const vqk_mx_weights *w, MxGeom *g, const char *what);
+
+// 2^(s - 127) as fp32 (s = 0 is the subnormal 2^-127; s = 255 NaN).
+__device__ __forceinline__ float mx_scale(uint32_t s) {
+    return __uint_as_float(s == 0u ? 0x00400000u : (s == 255u ? 0x7fc00000u : s << 23));
+}
+
+// Eight codes (one word) as bf16 weights, scale included.
+__device__ __forceinline__ u32x4 mx_decode8(uint32_t w, float sc) {
+    u32x4 r;
+    r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0));
+    r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1));
+    r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2));
+    r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3));
+    return r;
+}
+
+// Activations enter the matrix cores as bf16 planes whose sum is exact: one
+// for bf16, two for fp16 (11 significant bits = 8 + 3), three for fp32 (24).
+constexpr int mx_planes(int32_t type) { return type == VQK_BF16 ? 1 : (type == VQK_F16 ? 2 : 3); }
+
+// Plane pl of v: bf16 of what the planes before it leave. A value that is not
+// finite stands in plane 0 alone.
+__device__ __forceinline__ uint16_t mx_plane_next(float &rest) {
+    const uint16_t h = f32_to_bf16(rest);
+    const float f = bf16_to_f32(h);
+    const bool fin = (__float_as_uint(f) & 0x7f800000u) != 0x7f800000u;
+    rest = fin ? rest - f : 0.f;
+    return h;
+}
+
+// Largest magnitude bits of a block -> its scale byte: floor(log2) - 2 in the
+// biased exponents, at least 0 (2^-127); 255 where a value is not finite.
+__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax_bits) {
+    const int e = int(amax_bits >> 23);
+    return e == 255 ? 255u : uint32_t(max(e - 2, 0));
+}
+
+// Eight values as codes under the scale byte s (255: zeros).
+__device__ __forceinline__ uint32_t mx_encode8(const float (&v)[8], uint32_t s) {
+    if (s == 255u) return 0u;
+    const float sc = mx_scale(s);
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], sc, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], sc, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], sc, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], sc, 3);
+    return w;
+}
+
+// Eight activations k0..k0+7 of a row (vec: 16-byte aligned and whole), zero
+// at and past `cols`.
+__device__ __forceinline__ void mx_load8(const void *x, int32_t type, int64_t base, int64_t k0,
+                                         int64_t cols, bool vec, float (&v)[8]) {
+    if (vec && k0 + 8 <= cols) {
+        if (type == VQK_F32) {
+            const u32x4 a = *reinterpret_cast<const u32x4 *>(static_cast<const float *>(x) + base + k0);
+            const u32x4 b = *reinterpret_cast<const u32x4 *>(static_cast<const float *>(x) + base + k0 + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = __uint_as_float(a[i]);
+                v[4 + i] = __uint_as_float(b[i]);
+            }
+        } else {
+            const u32x4 a = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(x) + base + k0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint16_t lo = uint16_t(a[i] & 0xffffu), hi = uint16_t(a[i] >> 16);
+                v[2 * i] = type == VQK_BF16 ? bf16_to_f32(lo) : h_to_f32(lo);
+                v[2 * i + 1] = type == VQK_BF16 ? bf16_to_f32(hi) : h_to_f32(hi);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k0 + i < cols ? load_act(x, type, base + k0 + i) : 0.f;
+}
+
+// Largest value over each aligned group of four lanes, in every lane of it.
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+    v = max(v, dpp_u<kDppQuadXor1>(v));
+    return max(v, dpp_u<kDppQuadXor2>(v));
+}
+
+// x [N, IN] (rows ldx apart) -> bf16 planes [P][N][NB * 32], zero past IN; or
+// (quant) the values of its MXFP4 form, one plane.
+int launch_mx_planes(const void *x, int32_t type, int64_t N, int64_t IN, int64_t ldx, bool quant,
+                     uint16_t *out, hipStream_t st);
+// The quantiser without argument checks.
+int launch_mx_quant(const void *x, int32_t type, int64_t rows, int64_t cols, int64_t ldx,
+                    uint8_t *codes, uint8_t *scales, hipStream_t st);
+
+// Rows of x as the product kernels read them: bf16 planes of rows ld apart.
+struct MxX {
+    const uint16_t *x;
+    int64_t ld, plane;                        // elements between rows / planes
+    int P;
+};
+
+// One product, over dense rows, single pairs, or tiles of a sorted routing.
+struct MxCall {
+    const uint8_t *codes[2], *scales[2];      // [1]: the second projection of a SwiGLU pair
+    int64_t E, OUT, IN, NB;
+    MxX x;
+    int64_t N;                                // rows or pairs
+    // routing: none (dense) | ids (tile = pair) | order, meta, ntiles (sorted tiles)
+    const int32_t *ids, *order, *meta, *ntiles;
+    int64_t xkrep;                            // x row = pair / xkrep; 0: x rows are sorted positions (or pairs)
+    void *y;                                  // [row][OUT] in y_type; a SwiGLU pair: bf16 planes
+    int32_t y_type;
+    int64_t ldy, yplane;                      // elements between rows / planes of y
+    int yp;                                   // planes of a SwiGLU pair's output
+    bool ysorted;                             // y rows by sorted position
+};
+
+}  // namespace vqk

@@ -1,0 +1,237 @@
+// Routed experts with MXFP4 weights: one projection for (token, expert) pairs,
+// and the whole block of experts,
+//     y_t = sum_j w_tj * down_e( silu(gate_e x_t) * (up_e x_t) ),  e = ids_tj.
+//
+// Few pairs run pair by pair; more are sorted by expert on the device, so that
+// an expert's weights are read once for a tile of its rows. Gate and up are one
+// launch whose epilogue leaves silu(g) * u as the bf16 planes that down reads
+// (in x's precision: one plane for bf16, two for fp16, three for fp32); down
+// leaves fp32 rows by pair, and the last kernel adds them in order of j.
+#include "vqk_mxs.h"
+
+namespace vqk {
+
+static size_t al256(size_t v) { return (v + 255) & ~size_t(255); }
+
+// Pairs up to which the products run pair by pair.
+constexpr int64_t kMxPairsUnsorted = 64;
+constexpr int64_t kMxMaxExperts = 4096;
+
+// Row tiles of 16 for a routing of N pairs over E experts.
+static int mx_row_tiles(int64_t N, int64_t E) {
+    const int64_t avg = N / E;
+    return avg <= 12 ? 1 : (avg <= 40 ? 2 : 4);
+}
+
+struct CombineArgs {
+    const float *part;
+    const int32_t *ids;
+    const float *wts;
+    int64_t T, H, E;
+    int32_t k;
+    void *y;
+    int32_t y_type;
+};
+
+// y_t = sum_j w_tj part[t k + j]; pairs without an expert are not read.
+__global__ void __launch_bounds__(256) k_mx_combine(const CombineArgs p) {
+    const int64_t t = blockIdx.y;
+    const int64_t h = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4;
+    if (h >= p.H) return;
+    float v[4] = {};
+    const bool vec = p.H % 4 == 0;
+    for (int j = 0; j < p.k; ++j) {
+        const int64_t pair = t * p.k + j;
+        const int64_t e = p.ids[pair];
+        if (e < 0 || e >= p.E) continue;
+        const float w = p.wts[pair];
+        const float *src = p.part + pair * p.H + h;
+        if (vec) {
+            const float4 q = *reinterpret_cast<const float4 *>(src);
+            v[0] += w * q.x; v[1] += w * q.y; v[2] += w * q.z; v[3] += w * q.w;
+        } else {
+            for (int u = 0; u < 4 && h + u < p.H; ++u) v[u] += w * src[u];
+        }
+    }
+    for (int u = 0; u < 4 && h + u < p.H; ++u) store_act(p.y, p.y_type, t * p.H + h + u, v[u]);
+}
+
+static int check_pairs(int64_t T, int64_t N, int64_t E, const char *what) {
+    if (T < 0 || N < 0 || N > INT32_MAX / 4) return set_error(VQK_EINVAL, "%s: T=%lld N=%lld", what, (long long)T, (long long)N);
+    if (E > kMxMaxExperts) return set_error(VQK_ENOTIMPL, "%s: E=%lld > %lld", what, (long long)E, (long long)kMxMaxExperts);
+    return VQK_OK;
+}
+
+// x rows as planes: in place, or laid out at `ws` (bytes: plane_bytes).
+static bool x_in_place(const void *x, int32_t type, int64_t IN) {
+    return type == VQK_BF16 && IN % kMxBlock == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+}
+static size_t plane_bytes(int64_t rows, int64_t NB, int P) { return al256(size_t(rows) * NB * kMxBlock * 2 * P); }
+static int make_x(const void *x, int32_t type, int64_t rows, int64_t IN, int64_t NB, uint16_t *ws, MxX *out,
+                  hipStream_t st) {
+    if (x_in_place(x, type, IN)) {
+        *out = MxX{static_cast<const uint16_t *>(x), IN, 0, 1};
+        return VQK_OK;
+    }
+    *out = MxX{ws, NB * kMxBlock, rows * NB * kMxBlock, mx_planes(type)};
+    return launch_mx_planes(x, type, rows, IN, IN, false, ws, st);
+}
+
+static size_t sort_bytes(int64_t N, int64_t E) {
+    return N <= kMxPairsUnsorted ? 0 : al256(seg_sort_bytes(N, E));
+}
+// Sets a call's routing from the ids: unsorted pairs, or sorted into `ws`.
+static int set_routing(MxCall *c, const int32_t *ids, int64_t N, int64_t E, int nt, void *ws, hipStream_t st) {
+    if (N <= kMxPairsUnsorted) {
+        c->ids = ids;
+        return VQK_OK;
+    }
+    const int rc = seg_sort(reinterpret_cast<const uint32_t *>(ids), N, E, 16 * nt, ws, st);
+    const SegTiles t = seg_tiles(ws, N, E);
+    c->order = t.order;
+    c->meta = t.meta;
+    c->ntiles = t.ntiles;
+    return rc;
+}
+
+struct ExpertsPlan {
+    int64_t N, IP;
+    int P;
+    size_t x, h, part, sort, total;
+};
+static int plan_experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, const vqk_mx_weights *down,
+                        int32_t x_type, int64_t T, int32_t top_k, MxGeom *g1, MxGeom *g2, ExpertsPlan *p) {
+    MxGeom gu;
+    int rc;
+    if ((rc = make_mx_geom(gate, g1, "mx experts: gate")) || (rc = make_mx_geom(up, &gu, "mx experts: up")) ||
+        (rc = make_mx_geom(down, g2, "mx experts: down")))
+        return rc;
+    if (gu.E != g1->E || gu.OUT != g1->OUT || gu.IN != g1->IN || g2->E != g1->E || g2->IN != g1->OUT ||
+        g2->OUT != g1->IN)
+        return set_error(VQK_EINVAL, "mx experts: gate, up [E, I, H] and down [E, H, I] do not fit together");
+    if (!act_size(x_type)) return set_error(VQK_EINVAL, "mx experts: x type %d", x_type);
+    if (top_k < 1 || top_k > g1->E)
+        return set_error(VQK_EINVAL, "mx experts: top_k=%d of %lld experts", top_k, (long long)g1->E);
+    if (T < 0 || T > INT32_MAX / 4 / top_k) return set_error(VQK_EINVAL, "mx experts: T=%lld", (long long)T);
+    p->N = T * top_k;
+    if ((rc = check_pairs(T, p->N, g1->E, "mx experts"))) return rc;
+    p->IP = g2->NB * kMxBlock;
+    p->P = mx_planes(x_type);
+    p->x = 0;
+    p->h = plane_bytes(T, g1->NB, p->P);
+    p->part = p->h + plane_bytes(p->N, g2->NB, p->P);
+    p->sort = p->part + al256(size_t(p->N) * g2->OUT * 4);
+    p->total = p->sort + sort_bytes(p->N, g1->E);
+    return VQK_OK;
+}
+
+}  // namespace vqk
+
+using namespace vqk;
+
+extern "C" int vqk_mx_switch_workspace(const vqk_mx_weights *w, int32_t x_type, int64_t T, int64_t N,
+                                       size_t *bytes) {
+    MxGeom g;
+    int rc = make_mx_geom(w, &g, "mx switch");
+    if (rc || (rc = check_pairs(T, N, g.E, "mx switch"))) return rc;
+    if (!act_size(x_type)) return set_error(VQK_EINVAL, "mx switch: x type %d", x_type);
+    if (!bytes) return set_error(VQK_EINVAL, "mx switch: NULL bytes");
+    *bytes = plane_bytes(T, g.NB, mx_planes(x_type)) + sort_bytes(N, g.E);
+    return VQK_OK;
+}
+
+extern "C" int vqk_mx_switch(const vqk_mx_weights *w, const void *x, int32_t x_type, int64_t T,
+                             const int32_t *eidx, int64_t N, int64_t xkrep, void *y, int32_t y_type,
+                             void *workspace, size_t ws_bytes, void *stream) {
+    MxGeom g;
+    int rc = make_mx_geom(w, &g, "mx switch");
+    if (rc || (rc = check_pairs(T, N, g.E, "mx switch"))) return rc;
+    if (!act_size(x_type)) return set_error(VQK_EINVAL, "mx switch: x type %d", x_type);
+    if (!out_size(y_type)) return set_error(VQK_EINVAL, "mx switch: y type %d", y_type);
+    if (xkrep < 1 || T > INT64_MAX / xkrep || N != T * xkrep)
+        return set_error(VQK_EINVAL, "mx switch: N=%lld pairs for T=%lld rows x %lld", (long long)N,
+                         (long long)T, (long long)xkrep);
+    if (N == 0) return VQK_OK;
+    if (!x || !eidx || !y) return set_error(VQK_EINVAL, "mx switch: NULL pointer");
+    const size_t sort_at = plane_bytes(T, g.NB, mx_planes(x_type));
+    const size_t need = sort_at + sort_bytes(N, g.E);
+    if (!workspace || ws_bytes < need)
+        return set_error(VQK_ENOSPACE, "mx switch: workspace %zu < %zu", ws_bytes, need);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255)
+        return set_error(VQK_EINVAL, "mx switch: workspace must be 256-byte aligned");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    MxCall c{};
+    c.codes[0] = w->codes; c.scales[0] = w->scales;
+    c.E = g.E; c.OUT = g.OUT; c.IN = g.IN; c.NB = g.NB;
+    c.N = N; c.xkrep = xkrep;
+    c.y = y; c.y_type = y_type; c.ldy = g.OUT;
+    if ((rc = make_x(x, x_type, T, g.IN, g.NB, reinterpret_cast<uint16_t *>(ws), &c.x, st))) return rc;
+    const int nt = N <= kMxPairsUnsorted ? 1 : mx_row_tiles(N, g.E);
+    if ((rc = set_routing(&c, eidx, N, g.E, nt, ws + sort_at, st))) return rc;
+    return mx_stream(c, nt, st);
+}
+
+extern "C" int vqk_mx_experts_workspace(const vqk_mx_weights *gate, const vqk_mx_weights *up,
+                                        const vqk_mx_weights *down, int32_t x_type, int64_t T,
+                                        int32_t top_k, size_t *bytes) {
+    MxGeom g1, g2;
+    ExpertsPlan p;
+    const int rc = plan_experts(gate, up, down, x_type, T, top_k, &g1, &g2, &p);
+    if (rc) return rc;
+    if (!bytes) return set_error(VQK_EINVAL, "mx experts: NULL bytes");
+    *bytes = p.total;
+    return VQK_OK;
+}
+
+extern "C" int vqk_mx_experts(const vqk_mx_weights *gate, const vqk_mx_weights *up,
+                              const vqk_mx_weights *down, const void *x, int32_t x_type, int64_t T,
+                              const int32_t *ids, const float *wts, int32_t top_k, void *y, int32_t y_type,
+                              void *workspace, size_t ws_bytes, void *stream) {
+    MxGeom g1, g2;
+    ExpertsPlan p;
+    int rc = plan_experts(gate, up, down, x_type, T, top_k, &g1, &g2, &p);
+    if (rc) return rc;
+    if (!out_size(y_type)) return set_error(VQK_EINVAL, "mx experts: y type %d", y_type);
+    if (T == 0) return VQK_OK;
+    if (!x || !ids || !wts || !y) return set_error(VQK_EINVAL, "mx experts: NULL pointer");
+    if (!workspace || ws_bytes < p.total)
+        return set_error(VQK_ENOSPACE, "mx experts: workspace %zu < %zu", ws_bytes, p.total);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255)
+        return set_error(VQK_EINVAL, "mx experts: workspace must be 256-byte aligned");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    const bool sorted = p.N > kMxPairsUnsorted;
+    const int nt = sorted ? mx_row_tiles(p.N, g1.E) : 1;
+    MxCall c{};
+    c.codes[0] = gate->codes; c.scales[0] = gate->scales;
+    c.codes[1] = up->codes; c.scales[1] = up->scales;
+    c.E = g1.E; c.OUT = g1.OUT; c.IN = g1.IN; c.NB = g1.NB;
+    c.N = p.N; c.xkrep = top_k;
+    uint16_t *h = reinterpret_cast<uint16_t *>(ws + p.h);
+    c.y = h; c.ldy = p.IP; c.yplane = p.N * p.IP; c.yp = p.P; c.ysorted = true;
+    if ((rc = make_x(x, x_type, T, g1.IN, g1.NB, reinterpret_cast<uint16_t *>(ws), &c.x, st))) return rc;
+    if ((rc = set_routing(&c, ids, p.N, g1.E, nt, ws + p.sort, st))) return rc;
+    if ((rc = mx_stream(c, nt, st))) return rc;
+    MxCall d = c;                              // the same routing, over the SwiGLU rows
+    d.codes[0] = down->codes; d.scales[0] = down->scales;
+    d.codes[1] = nullptr; d.scales[1] = nullptr;
+    d.OUT = g2.OUT; d.IN = g2.IN; d.NB = g2.NB;
+    d.x = MxX{h, p.IP, p.N * p.IP, p.P};
+    d.xkrep = 0;
+    float *part = reinterpret_cast<float *>(ws + p.part);
+    d.y = part; d.y_type = VQK_F32; d.ldy = g2.OUT; d.ysorted = false;
+    if ((rc = mx_stream(d, nt, st))) return rc;
+    const CombineArgs a{part, ids, wts, T, g2.OUT, g1.E, top_k, y, y_type};
+    for (int64_t t0 = 0; t0 < T; t0 += 65535) {          // grid.y holds 65535 tokens
+        CombineArgs b = a;
+        b.part += t0 * top_k * g2.OUT;
+        b.ids += t0 * top_k;
+        b.wts += t0 * top_k;
+        b.y = static_cast<uint8_t *>(y) + t0 * g2.OUT * out_size(y_type);
+        const int64_t n = T - t0 < 65535 ? T - t0 : 65535;
+        hipLaunchKernelGGL(k_mx_combine, dim3(unsigned((g2.OUT + 1023) / 1024), unsigned(n)), dim3(256), 0, st, b);
+        if ((rc = hip_status(hipGetLastError(), "combine launch"))) return rc;
+    }
+    return VQK_OK;
+}

@@ -1,0 +1,288 @@
+"""MXFP4 (microscaled 4-bit) weights for PyTorch-ROCm, beside the VQ modules. No counterpart in
+the reference, whose formats are vector-quantised: this is the OCP microscaling format that
+gfx950's matrix cores multiply directly.
+
+A row of C values is ceil(C / 32) blocks of 32: 16 bytes of 4-bit codes each (element 2i in the
+low half of byte i) and one scale byte s, value = e2m1(code) * 2^(s - 127); s = 255 is a block of
+NaN (include/vqk.h).
+
+  mx_quantize(x) -> codes, scales         mx_dequantize(codes, scales, cols, dtype)
+  MXLinear(codes, scales, in_features)    bias-free linear, like VQLinear
+  MXSwitchLinear, MXSwitchGLU             routed experts, like VQSwitchLinear / VQSwitchGLU
+  MXSparseMoeBlock                        routing + experts, like VQSparseMoeBlock
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib as L
+from . import _torch as T
+from . import router
+
+BLOCK = 32
+
+
+def _blocks(cols):
+    return -(-int(cols) // BLOCK)
+
+
+def mx_quantize(x):
+    """x [..., C] (fp16, bf16, fp32) -> codes uint8 [..., 16 B], scales uint8 [..., B],
+    B = ceil(C / 32). Each block's scale is 2^(floor(log2(max |x|)) - 2), at least 2^-127; elements
+    are rounded to nearest (ties to even), past 6 to 6. A block with an infinity or NaN becomes NaN.
+    Not differentiable."""
+    T.require_cuda(x)
+    xt = T.act_type(x)
+    if x.ndim == 0:
+        raise ValueError("mx_quantize takes rows, got a scalar")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError("mx_quantize has no gradient: detach x, or call it under no_grad")
+    C, B = x.shape[-1], _blocks(x.shape[-1])
+    with T.on_device(x):
+        if x.ndim == 2 and x.stride(1) == 1 and x.stride(0) >= C:
+            rows, ld = x, x.stride(0)                  # rows apart: read where they are
+        else:
+            rows, ld = x.contiguous(), C
+        n = x.numel() // C if C else 0
+        codes = torch.empty((*x.shape[:-1], 16 * B), dtype=torch.uint8, device=x.device)
+        scales = torch.empty((*x.shape[:-1], B), dtype=torch.uint8, device=x.device)
+        L.check(L.lib().vqk_mx_quantize(rows.data_ptr(), xt, n, C, ld, codes.data_ptr(),
+                                        scales.data_ptr(), T.stream(x.device)), "mx_quantize")
+    return codes, scales
+
+
+def _check_mx(codes, scales, cols, what):
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise ValueError(f"{what}: codes and scales must be uint8, got {codes.dtype}, {scales.dtype}")
+    B = _blocks(cols)
+    if codes.shape[:-1] != scales.shape[:-1] or codes.shape[-1] != 16 * B or scales.shape[-1] != B:
+        raise ValueError(f"{what}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not "
+                         f"hold rows of {cols} values ({16 * B} and {B} bytes)")
+
+
+def mx_dequantize(codes, scales, cols, dtype=torch.bfloat16):
+    """The values [..., cols] that codes and scales stand for, in dtype (exact in bf16 and fp32)."""
+    T.require_cuda(codes, scales)
+    _check_mx(codes, scales, cols, "mx_dequantize")
+    if dtype not in T.ACT_TYPES:
+        raise ValueError(f"dtype must be float16, bfloat16 or float32, got {dtype}")
+    with T.on_device(codes):
+        codes, scales = _aligned(codes, 4), scales.contiguous()
+        out = torch.empty((*scales.shape[:-1], int(cols)), dtype=dtype, device=codes.device)
+        n = out.numel() // int(cols) if cols else 0
+        L.check(L.lib().vqk_mx_dequantize(codes.data_ptr(), scales.data_ptr(), n, int(cols),
+                                          out.data_ptr(), T.ACT_TYPES[dtype],
+                                          T.stream(codes.device)), "mx_dequantize")
+    return out
+
+
+def _aligned(t, n):
+    """t contiguous, its first byte at a multiple of n."""
+    t = t.contiguous()
+    return t if t.data_ptr() % n == 0 else t.clone()
+
+
+def _ids32(ids, E):
+    """ids as int32; a wider id keeps being outside [0, E) when it is."""
+    return (ids if ids.dtype == torch.int32 else ids.clamp(-1, E).to(torch.int32)).contiguous()
+
+
+def _desc(codes, scales, E, OUT, IN):
+    return L.VQKMXWeights(codes.data_ptr(), scales.data_ptr(), E, OUT, IN)
+
+
+def _work(query, dev, *args):
+    ws = ctypes.c_size_t()
+    L.check(query(*args, ctypes.byref(ws)), "workspace")
+    return (torch.empty(ws.value, dtype=torch.uint8, device=dev) if ws.value else None), ws.value
+
+
+class _LinearFn(torch.autograd.Function):
+    """y = x . W^T with a frozen W; the gradient reaches x."""
+
+    @staticmethod
+    def forward(ctx, x, mod):
+        ctx.mod = mod
+        return mod._product(x)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return ctx.mod._dx(dy), None
+
+
+class MXLinear(torch.nn.Module):
+    """Bias-free linear whose weight is MXFP4: codes uint8 [OUT, 16 B], scales uint8 [OUT, B].
+    in_features may be any width of the last block (default: all 32 of it). act: None multiplies x
+    as it is (bf16, fp16 and fp32 enter exactly, fp32 sums); "mxfp4" quantises x's rows as
+    mx_quantize does. Differentiable in x with act None; the weight is frozen."""
+
+    def __init__(self, codes, scales, in_features=None, act=None):
+        super().__init__()
+        if act not in (None, "mxfp4"):
+            raise ValueError(f"act must be None or 'mxfp4', got {act!r}")
+        if codes.ndim != 2:
+            raise ValueError(f"codes must be [OUT, bytes], got {tuple(codes.shape)}")
+        IN = int(scales.shape[-1]) * BLOCK if in_features is None else int(in_features)
+        _check_mx(codes, scales, IN, "MXLinear")
+        self.codes, self.scales = _aligned(codes, 16), scales.contiguous()
+        self.in_features, self.out_features, self.act = IN, int(codes.shape[0]), act
+
+    @classmethod
+    def from_weight(cls, weight, act=None):
+        """The linear of a weight [OUT, IN], quantised here."""
+        return cls(*mx_quantize(weight.detach()), weight.shape[1], act)
+
+    input_dims = property(lambda self: self.in_features)
+    output_dims = property(lambda self: self.out_features)
+
+    def _product(self, x):
+        IN, OUT = self.in_features, self.out_features
+        act = L.VQK_MX_ACT_NONE if self.act is None else L.VQK_MX_ACT_MXFP4
+        xt, lib = T.act_type(x), L.lib()
+        with T.on_device(x):
+            xf = x.reshape(-1, IN).contiguous()
+            N = xf.shape[0]
+            w = _desc(self.codes, self.scales, 1, OUT, IN)
+            y = torch.empty((*x.shape[:-1], OUT), dtype=x.dtype, device=x.device)
+            work, size = _work(lib.vqk_mx_linear_workspace, x.device, ctypes.byref(w), xt, N, act)
+            L.check(lib.vqk_mx_linear(ctypes.byref(w), xf.data_ptr(), xt, N, act, y.data_ptr(), xt,
+                                      work.data_ptr() if size else None, size, T.stream(x.device)),
+                    "MXLinear")
+        return y
+
+    def _dx(self, dy):
+        IN, OUT = self.in_features, self.out_features
+        dt, lib = T.act_type(dy), L.lib()
+        with T.on_device(dy):
+            d = dy.reshape(-1, OUT).contiguous()
+            N = d.shape[0]
+            w = _desc(self.codes, self.scales, 1, OUT, IN)
+            dx = torch.empty((*dy.shape[:-1], IN), dtype=dy.dtype, device=dy.device)
+            work, size = _work(lib.vqk_mx_linear_dx_workspace, dy.device, ctypes.byref(w), dt, N)
+            L.check(lib.vqk_mx_linear_dx(ctypes.byref(w), d.data_ptr(), dt, N, dx.data_ptr(), dt,
+                                         work.data_ptr() if size else None, size,
+                                         T.stream(dy.device)), "MXLinear gradient")
+        return dx
+
+    def forward(self, x):
+        T.require_cuda(x, self.codes, self.scales)
+        if x.ndim == 0 or x.shape[-1] != self.in_features:
+            raise ValueError(f"MXLinear: x {tuple(x.shape)} for in_features {self.in_features}")
+        if torch.is_grad_enabled() and x.requires_grad:
+            if self.act is not None:
+                raise RuntimeError("MXLinear(act='mxfp4') has no gradient: the rounding of x has none")
+            return _LinearFn.apply(x, self)
+        return self._product(x)
+
+
+def _no_grad(what, *ts):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise RuntimeError(f"{what} has no gradient: run it under no_grad, or detach its inputs")
+
+
+class MXSwitchLinear(torch.nn.Module):
+    """E bias-free linears in MXFP4, one picked by each index: codes uint8 [E, OUT, 16 B], scales
+    uint8 [E, OUT, B]. forward(x [..., 1, 1, IN] or [..., k, 1, IN], indices [..., k]) ->
+    [..., k, 1, OUT], as VQSwitchLinear; an index outside [0, E) gives zeros. Serving only: no
+    gradient."""
+
+    def __init__(self, codes, scales, in_features=None):
+        super().__init__()
+        if codes.ndim != 3:
+            raise ValueError(f"codes must be [E, OUT, bytes], got {tuple(codes.shape)}")
+        IN = int(scales.shape[-1]) * BLOCK if in_features is None else int(in_features)
+        _check_mx(codes, scales, IN, "MXSwitchLinear")
+        self.codes, self.scales = _aligned(codes, 16), scales.contiguous()
+        self.num_experts, self.output_dims, self.input_dims = int(codes.shape[0]), int(codes.shape[1]), IN
+
+    @classmethod
+    def from_weight(cls, weight):
+        """The experts of a weight [E, OUT, IN], quantised here."""
+        return cls(*mx_quantize(weight.detach()), weight.shape[2])
+
+    def _weights(self):
+        return _desc(self.codes, self.scales, self.num_experts, self.output_dims, self.input_dims)
+
+    def forward(self, x, indices):
+        T.require_cuda(x, indices, self.codes, self.scales)
+        _no_grad("MXSwitchLinear", x)
+        IN, OUT, k = self.input_dims, self.output_dims, int(indices.shape[-1])
+        lead = tuple(indices.shape[:-1])
+        if x.shape[-1] != IN or tuple(x.shape[:-3]) != lead or x.shape[-2] != 1 or x.shape[-3] not in (1, k):
+            raise ValueError(f"MXSwitchLinear: x {tuple(x.shape)} for indices {tuple(indices.shape)}, "
+                             f"in_features {IN}")
+        xt, lib = T.act_type(x), L.lib()
+        with T.on_device(x):
+            xf = x.reshape(-1, IN).contiguous()
+            eidx = _ids32(indices.reshape(-1), self.num_experts)
+            rows, N = xf.shape[0], eidx.numel()
+            w = self._weights()
+            y = torch.empty((*lead, k, 1, OUT), dtype=x.dtype, device=x.device)
+            work, size = _work(lib.vqk_mx_switch_workspace, x.device, ctypes.byref(w), xt, rows, N)
+            L.check(lib.vqk_mx_switch(ctypes.byref(w), xf.data_ptr(), xt, rows, eidx.data_ptr(), N,
+                                      N // rows if rows else 1, y.data_ptr(), xt,
+                                      work.data_ptr() if size else None, size, T.stream(x.device)),
+                    "MXSwitchLinear")
+        return y
+
+
+class MXSwitchGLU(torch.nn.Module):
+    """SwitchGLU with MXFP4 projections: forward(x [T, H], ids [T, k], weights [T, k]) ->
+    sum_j weights_j * down_j(silu(gate_j(x)) * up_j(x)), [T, H]. Ids outside [0, E) add nothing.
+    The SwiGLU rows are rounded to x's type. Serving only: no gradient."""
+
+    def __init__(self, gate_proj: MXSwitchLinear, up_proj: MXSwitchLinear, down_proj: MXSwitchLinear):
+        super().__init__()
+        g, u, d = gate_proj, up_proj, down_proj
+        if (g.num_experts, g.output_dims, g.input_dims) != (u.num_experts, u.output_dims, u.input_dims) or \
+                (d.num_experts, d.output_dims, d.input_dims) != (g.num_experts, g.input_dims, g.output_dims):
+            raise ValueError("MXSwitchGLU: gate, up [E, I, H] and down [E, H, I] do not fit together")
+        self.gate_proj, self.up_proj, self.down_proj = g, u, d
+
+    def forward(self, x, ids, weights):
+        T.require_cuda(x, ids, weights, self.gate_proj.codes)
+        _no_grad("MXSwitchGLU", x, weights)
+        H = self.gate_proj.input_dims
+        if x.ndim != 2 or x.shape[1] != H or ids.ndim != 2 or ids.shape[0] != x.shape[0] or \
+                ids.shape != weights.shape:
+            raise ValueError(f"MXSwitchGLU: x {tuple(x.shape)}, ids {tuple(ids.shape)}, weights "
+                             f"{tuple(weights.shape)} for hidden size {H}")
+        xt, lib = T.act_type(x), L.lib()
+        n, k = ids.shape
+        with T.on_device(x):
+            x = x.contiguous()
+            ids = _ids32(ids, self.gate_proj.num_experts)
+            wts = weights.to(torch.float32).contiguous()
+            ws = [m._weights() for m in (self.gate_proj, self.up_proj, self.down_proj)]
+            refs = [ctypes.byref(w) for w in ws]
+            y = torch.empty_like(x)
+            work, size = _work(lib.vqk_mx_experts_workspace, x.device, *refs, xt, n, k)
+            L.check(lib.vqk_mx_experts(*refs, x.data_ptr(), xt, n, ids.data_ptr(), wts.data_ptr(), k,
+                                       y.data_ptr(), xt, work.data_ptr() if size else None, size,
+                                       T.stream(x.device)), "MXSwitchGLU")
+        return y
+
+
+class MXSparseMoeBlock(torch.nn.Module):
+    """Softmax top-k routing and MXFP4 experts: forward(x [T, H], logits [T, E], mask [T]) ->
+    [T, H]; without logits they are x . router_weight^T. mask: 0 marks padding, whose rows are
+    zero and take no expert's time."""
+
+    def __init__(self, switch_mlp: MXSwitchGLU, top_k: int, norm_topk_prob: bool = True,
+                 router_weight=None):
+        super().__init__()
+        self.switch_mlp, self.top_k = switch_mlp, int(top_k)
+        self.norm_topk_prob, self.router_weight = bool(norm_topk_prob), router_weight
+
+    def forward(self, x, logits=None, mask=None):
+        if logits is None:
+            logits = x.float() @ self.router_weight.float().T
+        _no_grad("MXSparseMoeBlock", x, logits)
+        if logits.ndim != 2 or logits.shape != (x.shape[0], self.switch_mlp.gate_proj.num_experts):
+            raise ValueError(f"MXSparseMoeBlock: logits {tuple(logits.shape)} for x {tuple(x.shape)} and "
+                             f"{self.switch_mlp.gate_proj.num_experts} experts")
+        ids, w = router.top_k(logits, self.top_k, self.norm_topk_prob, mask)
+        return self.switch_mlp(x, ids, w)

@@ -1,0 +1,125 @@
+"""Router of a mixture of experts: softmax top-k routing with the counts and losses that training
+it needs. No counterpart in the reference, whose routers are trained elsewhere; the routing itself
+is the one of its MoE block (see vqlab_amd.moe).
+
+    p = softmax(logits); ids = top_k(p); weights = p[ids] (renormalised)
+    over the n live tokens:  counts_e = tokens that chose expert e
+    balance = E * sum_e counts_e / (n k) * mean_t p_te      (1 where the load is even)
+    z       = mean_t logsumexp(logits_t)^2
+
+Gradients reach the logits from weights, balance and z.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import torch
+
+from . import _lib as L
+from . import _torch as T
+
+
+class Route(NamedTuple):
+    """ids int32 [T, k] (-1: none), weights fp32 [T, k], counts int32 [E], balance and z fp32
+    scalars, tokens fp32 scalar (the live tokens n)."""
+    ids: torch.Tensor
+    weights: torch.Tensor
+    counts: torch.Tensor
+    balance: torch.Tensor
+    z: torch.Tensor
+    tokens: torch.Tensor
+
+
+def _mask_ptr(mask, logits):
+    if mask is None:
+        return None, None
+    if mask.dtype not in (torch.bool, torch.uint8):
+        raise ValueError(f"mask must be bool or uint8, got {mask.dtype}")
+    if mask.shape != logits.shape[:1]:
+        raise ValueError(f"mask {tuple(mask.shape)} for logits {tuple(logits.shape)}")
+    mask = mask.contiguous()
+    return mask, mask.data_ptr()
+
+
+def _check(logits, mask):
+    if logits.ndim != 2:
+        raise ValueError(f"logits must be [T, E], got {tuple(logits.shape)}")
+    T.act_type(logits)
+    T.require_cuda(logits, mask)
+
+
+def _rows(logits):
+    """logits with contiguous rows, and the elements between them."""
+    E = logits.shape[1]
+    if logits.stride(1) != 1 or logits.stride(0) < E:
+        logits = logits.contiguous()
+    return logits, max(logits.stride(0), E)
+
+
+def top_k(logits, k, norm_topk_prob=True, mask=None):
+    """ids int32 [T, k] and weights fp32 [T, k] of logits [T, E], one launch and no gradient: the
+    routing of a serving step. mask [T] (bool / uint8): 0 marks padding, whose ids are -1."""
+    _check(logits, mask)
+    with T.on_device(logits):
+        lg, ld = _rows(logits)
+        m, mp = _mask_ptr(mask, lg)
+        n, E = lg.shape
+        ids = torch.empty((n, k), dtype=torch.int32, device=lg.device)
+        w = torch.empty((n, k), dtype=torch.float32, device=lg.device)
+        L.check(L.lib().vqk_route(lg.data_ptr(), T.act_type(lg), n, E, ld, mp, k,
+                                  int(norm_topk_prob), ids.data_ptr(), w.data_ptr(), None, None,
+                                  None, None, 0, T.stream(lg.device)), "route")
+    return ids, w
+
+
+class _RouteFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, norm, mask):
+        with T.on_device(logits):
+            lg, ld = _rows(logits)
+            m, mp = _mask_ptr(mask, lg)
+            n, E = lg.shape
+            dev = lg.device
+            ids = torch.empty((n, k), dtype=torch.int32, device=dev)
+            w = torch.empty((n, k), dtype=torch.float32, device=dev)
+            counts = torch.empty(E, dtype=torch.int32, device=dev)
+            stats = torch.empty(3, dtype=torch.float32, device=dev)
+            saved = torch.empty((n, 2), dtype=torch.float32, device=dev)
+            lib = L.lib()
+            ws = ctypes.c_size_t()
+            L.check(lib.vqk_route_workspace(n, E, ctypes.byref(ws)), "route")
+            work = torch.empty(ws.value, dtype=torch.uint8, device=dev)
+            L.check(lib.vqk_route(lg.data_ptr(), T.act_type(lg), n, E, ld, mp, k, norm,
+                                  ids.data_ptr(), w.data_ptr(), counts.data_ptr(),
+                                  stats.data_ptr(), saved.data_ptr(), work.data_ptr(), ws.value,
+                                  T.stream(dev)), "route")
+        balance, z, tokens = stats.unbind()
+        ctx.save_for_backward(lg, ids, w, counts, stats, saved)
+        ctx.k, ctx.norm, ctx.ld = k, norm, ld
+        ctx.mark_non_differentiable(ids, counts, tokens)
+        ctx.set_materialize_grads(False)
+        return ids, w, counts, balance, z, tokens
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, _ids, dw, _counts, db, dz, _tokens):
+        lg, ids, w, counts, stats, saved = ctx.saved_tensors
+        n, E = lg.shape
+        with T.on_device(lg):
+            d = torch.empty((n, E), dtype=lg.dtype, device=lg.device)
+            grads = [None if g is None else g.to(torch.float32).contiguous() for g in (dw, db, dz)]
+            L.check(L.lib().vqk_route_backward(
+                lg.data_ptr(), T.act_type(lg), n, E, ctx.ld, ctx.k, ctx.norm, ids.data_ptr(),
+                w.data_ptr(), counts.data_ptr(), stats.data_ptr(), saved.data_ptr(),
+                *(None if g is None else g.data_ptr() for g in grads), d.data_ptr(),
+                T.stream(lg.device)), "route backward")
+        return d, None, None, None
+
+
+def route(logits, k, norm_topk_prob=True, mask=None):
+    """Route of logits [T, E] (fp16, bf16 or fp32), differentiable in the logits. mask [T] (bool /
+    uint8): 0 marks padding, which gets ids -1, weights 0 and a zero gradient and enters neither
+    counts nor losses; so does a token whose logits are all -inf."""
+    _check(logits, mask)
+    return Route(*_RouteFn.apply(logits, int(k), int(norm_topk_prob), mask))
