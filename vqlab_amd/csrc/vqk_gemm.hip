@@ -570,8 +570,8 @@ int seg_tile_rows(const vqk_weights *w, int64_t N, int64_t E) {
 
 int seg_sort(const uint32_t *eidx, int64_t N, int64_t E, int tok, void *ws, hipStream_t st) {
     if (N == 0) return VQK_OK;
-    if (tok != kSegTok && tok != kSegTokNarrow && tok != kHalfTile && tok != 64 && tok != 96)
-        return set_error(VQK_EINVAL, "sort tiles of %d rows (16, %d, 32, 64 or 96)", tok, kSegTokNarrow);
+    if (tok != kSegTok && tok != kSegTokNarrow && tok != kHalfTile && tok != 64 && tok != 96 && tok != 128)
+        return set_error(VQK_EINVAL, "sort tiles of %d rows (16, %d, 32, 64, 96 or 128)", tok, kSegTokNarrow);
     uint8_t *b = static_cast<uint8_t *>(ws);
     const int64_t mt = group_max_tiles(N, E, tok);
     int32_t *order = reinterpret_cast<int32_t *>(b);

@@ -113,6 +113,31 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
     return max(v, dpp_u<kDppQuadXor2>(v));
 }
 
+// n (up to 4) neighbouring outputs at element i; al: whole fours are aligned
+// wherever i is a multiple of 4.
+__device__ __forceinline__ void mx_store4(void *y, int32_t type, int64_t i, const float (&v)[4], int n,
+                                          bool al) {
+    if (al && n == 4 && (i & 3) == 0) {
+        if (type == VQK_F32) {
+            *reinterpret_cast<float4 *>(static_cast<float *>(y) + i) = float4{v[0], v[1], v[2], v[3]};
+            return;
+        }
+        if (type == VQK_BF16 || type == VQK_F16) {
+            uint32_t q[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) q[u] = type == VQK_BF16 ? f32_to_bf16(v[u]) : f32_to_h(v[u]);
+            u32x2 o;
+            o.x = q[0] | (q[1] << 16);
+            o.y = q[2] | (q[3] << 16);
+            *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(y) + i) = o;
+            return;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        if (u < n) store_act(y, type, i + u, v[u]);
+}
+
 // x [N, IN] (rows ldx apart) -> bf16 planes [P][N][NB * 32], zero past IN; or
 // (quant) the values of its MXFP4 form, one plane.
 int launch_mx_planes(const void *x, int32_t type, int64_t N, int64_t IN, int64_t ldx, bool quant,
@@ -143,5 +168,11 @@ struct MxCall {
     int yp;                                   // planes of a SwiGLU pair's output
     bool ysorted;                             // y rows by sorted position
 };
+
+// The many-row products (vqk_mxg.h): x tiles of tile_rows (32, 64, 128); part:
+// room for fp32 K slices of a dense product, or NULL.
+int mx_gemm(const MxCall &c, int tile_rows, float *part, size_t part_bytes, hipStream_t st);
+// Bytes of the K slices that a dense product of N rows makes use of.
+size_t mxg_part_bytes(int64_t N, int64_t OUT, int64_t NB);
 
 }  // namespace vqk

@@ -116,9 +116,16 @@ static int check_lin(const vqk_mx_weights *w, int32_t x_type, int64_t N, MxGeom 
     return VQK_OK;
 }
 
-static size_t lin_bytes(const MxGeom &g, int32_t x_type, int64_t N, int32_t act) {
+// Rows up to which the weights are streamed past all rows (vqk_mxs.h).
+constexpr int64_t kMxStreamRows = 64;
+
+// Workspace: x's planes, then the K slices of the many-row product.
+static size_t lin_x_bytes(const MxGeom &g, int32_t x_type, int64_t N, int32_t act) {
     const int P = act == VQK_MX_ACT_MXFP4 ? 1 : mx_planes(x_type);
     return al256(size_t(N) * g.NB * kMxBlock * 2 * P);
+}
+static size_t lin_bytes(const MxGeom &g, int32_t x_type, int64_t N, int32_t act) {
+    return lin_x_bytes(g, x_type, N, act) + (N > kMxStreamRows ? mxg_part_bytes(N, g.OUT, g.NB) : 0);
 }
 
 }  // namespace vqk
@@ -154,20 +161,24 @@ extern "C" int vqk_mx_linear(const vqk_mx_weights *w, const void *x, int32_t x_t
     c.E = 1; c.OUT = g.OUT; c.IN = g.IN; c.NB = g.NB;
     c.N = N; c.xkrep = 1;
     c.y = y; c.y_type = y_type; c.ldy = g.OUT;
-    if (act == VQK_MX_ACT_NONE && x_in_place(x, x_type, g.IN, g.IN)) {
+    const bool place = act == VQK_MX_ACT_NONE && x_in_place(x, x_type, g.IN, g.IN);
+    const size_t need = lin_bytes(g, x_type, N, act);
+    if ((!place || N > kMxStreamRows) && need && (!workspace || ws_bytes < need))
+        return set_error(VQK_ENOSPACE, "mx linear: workspace %zu < %zu", ws_bytes, need);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255)
+        return set_error(VQK_EINVAL, "mx linear: workspace must be 256-byte aligned");
+    if (place) {
         c.x = MxX{static_cast<const uint16_t *>(x), g.IN, 0, 1};
     } else {
-        if (!workspace || ws_bytes < lin_bytes(g, x_type, N, act))
-            return set_error(VQK_ENOSPACE, "mx linear: workspace %zu < %zu", ws_bytes,
-                             lin_bytes(g, x_type, N, act));
-        if (reinterpret_cast<uintptr_t>(workspace) & 15)
-            return set_error(VQK_EINVAL, "mx linear: workspace must be 16-byte aligned");
         uint16_t *xs = static_cast<uint16_t *>(workspace);
         if ((rc = launch_mx_planes(x, x_type, N, g.IN, g.IN, act == VQK_MX_ACT_MXFP4, xs, st))) return rc;
         c.x = MxX{xs, g.NB * kMxBlock, N * g.NB * kMxBlock,
                   act == VQK_MX_ACT_MXFP4 ? 1 : mx_planes(x_type)};
     }
-    return mx_stream(c, N <= 16 ? 1 : (N <= 32 ? 2 : 4), st);
+    if (N <= kMxStreamRows) return mx_stream(c, N <= 16 ? 1 : (N <= 32 ? 2 : 4), st);
+    const size_t xb = lin_x_bytes(g, x_type, N, act);
+    return mx_gemm(c, 128, need > xb ? reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + xb) : nullptr,
+                   need - xb, st);
 }
 
 extern "C" int vqk_mx_linear_dx_workspace(const vqk_mx_weights *w, int32_t type, int64_t N, size_t *bytes) {

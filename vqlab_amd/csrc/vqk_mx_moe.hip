@@ -17,10 +17,14 @@ static size_t al256(size_t v) { return (v + 255) & ~size_t(255); }
 constexpr int64_t kMxPairsUnsorted = 64;
 constexpr int64_t kMxMaxExperts = 4096;
 
-// Row tiles of 16 for a routing of N pairs over E experts.
-static int mx_row_tiles(int64_t N, int64_t E) {
+// Rows per tile of a routing of N pairs over E experts: 16 (the streaming kernel) while
+// experts have a few pairs each, then 32, 64 or 128 (the many-row kernel).
+static int mx_tile_rows(int64_t N, int64_t E) {
     const int64_t avg = N / E;
-    return avg <= 12 ? 1 : (avg <= 40 ? 2 : 4);
+    return avg <= 12 ? 16 : (avg <= 24 ? 32 : (avg <= 80 ? 64 : 128));
+}
+static int run(const MxCall &c, int rows, hipStream_t st) {
+    return rows == 16 ? mx_stream(c, 1, st) : mx_gemm(c, rows, nullptr, 0, st);
 }
 
 struct CombineArgs {
@@ -81,12 +85,12 @@ static size_t sort_bytes(int64_t N, int64_t E) {
     return N <= kMxPairsUnsorted ? 0 : al256(seg_sort_bytes(N, E));
 }
 // Sets a call's routing from the ids: unsorted pairs, or sorted into `ws`.
-static int set_routing(MxCall *c, const int32_t *ids, int64_t N, int64_t E, int nt, void *ws, hipStream_t st) {
+static int set_routing(MxCall *c, const int32_t *ids, int64_t N, int64_t E, int rows, void *ws, hipStream_t st) {
     if (N <= kMxPairsUnsorted) {
         c->ids = ids;
         return VQK_OK;
     }
-    const int rc = seg_sort(reinterpret_cast<const uint32_t *>(ids), N, E, 16 * nt, ws, st);
+    const int rc = seg_sort(reinterpret_cast<const uint32_t *>(ids), N, E, rows, ws, st);
     const SegTiles t = seg_tiles(ws, N, E);
     c->order = t.order;
     c->meta = t.meta;
@@ -167,9 +171,9 @@ extern "C" int vqk_mx_switch(const vqk_mx_weights *w, const void *x, int32_t x_t
     c.N = N; c.xkrep = xkrep;
     c.y = y; c.y_type = y_type; c.ldy = g.OUT;
     if ((rc = make_x(x, x_type, T, g.IN, g.NB, reinterpret_cast<uint16_t *>(ws), &c.x, st))) return rc;
-    const int nt = N <= kMxPairsUnsorted ? 1 : mx_row_tiles(N, g.E);
-    if ((rc = set_routing(&c, eidx, N, g.E, nt, ws + sort_at, st))) return rc;
-    return mx_stream(c, nt, st);
+    const int rows = N <= kMxPairsUnsorted ? 16 : mx_tile_rows(N, g.E);
+    if ((rc = set_routing(&c, eidx, N, g.E, rows, ws + sort_at, st))) return rc;
+    return run(c, rows, st);
 }
 
 extern "C" int vqk_mx_experts_workspace(const vqk_mx_weights *gate, const vqk_mx_weights *up,
@@ -202,7 +206,7 @@ extern "C" int vqk_mx_experts(const vqk_mx_weights *gate, const vqk_mx_weights *
     hipStream_t st = static_cast<hipStream_t>(stream);
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     const bool sorted = p.N > kMxPairsUnsorted;
-    const int nt = sorted ? mx_row_tiles(p.N, g1.E) : 1;
+    const int rows = sorted ? mx_tile_rows(p.N, g1.E) : 16;
     MxCall c{};
     c.codes[0] = gate->codes; c.scales[0] = gate->scales;
     c.codes[1] = up->codes; c.scales[1] = up->scales;
@@ -211,8 +215,8 @@ extern "C" int vqk_mx_experts(const vqk_mx_weights *gate, const vqk_mx_weights *
     uint16_t *h = reinterpret_cast<uint16_t *>(ws + p.h);
     c.y = h; c.ldy = p.IP; c.yplane = p.N * p.IP; c.yp = p.P; c.ysorted = true;
     if ((rc = make_x(x, x_type, T, g1.IN, g1.NB, reinterpret_cast<uint16_t *>(ws), &c.x, st))) return rc;
-    if ((rc = set_routing(&c, ids, p.N, g1.E, nt, ws + p.sort, st))) return rc;
-    if ((rc = mx_stream(c, nt, st))) return rc;
+    if ((rc = set_routing(&c, ids, p.N, g1.E, rows, ws + p.sort, st))) return rc;
+    if ((rc = run(c, rows, st))) return rc;
     MxCall d = c;                              // the same routing, over the SwiGLU rows
     d.codes[0] = down->codes; d.scales[0] = down->scales;
     d.codes[1] = nullptr; d.scales[1] = nullptr;
@@ -221,7 +225,7 @@ extern "C" int vqk_mx_experts(const vqk_mx_weights *gate, const vqk_mx_weights *
     d.xkrep = 0;
     float *part = reinterpret_cast<float *>(ws + p.part);
     d.y = part; d.y_type = VQK_F32; d.ldy = g2.OUT; d.ysorted = false;
-    if ((rc = mx_stream(d, nt, st))) return rc;
+    if ((rc = run(d, rows, st))) return rc;
     const CombineArgs a{part, ids, wts, T, g2.OUT, g1.E, top_k, y, y_type};
     for (int64_t t0 = 0; t0 < T; t0 += 65535) {          // grid.y holds 65535 tokens
         CombineArgs b = a;

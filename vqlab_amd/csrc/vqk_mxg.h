@@ -1,0 +1,231 @@
+// Products of MXFP4 weights with many rows: decoded in registers, multiplied
+// on 32x32x16 bf16 matrix instructions.
+//
+// A workgroup of four waves takes 256 weight rows (128 of each projection of a
+// SwiGLU pair) and a tile of 32 * BT x rows; a wave owns 64 weight rows and all
+// of the tile's x rows, so every weight is decoded by one wave only. Per chunk
+// of 128 k:
+//   * weights: 32 bytes per lane and 32-row tile straight from global memory.
+//     The sum over k has no order of its own, so lane group g = lane / 32 holds
+//     blocks 2g and 2g + 1 of the chunk and step (q, h) multiplies elements
+//     8h..8h+7 of block 2g + q: a lane decodes with one scale per block.
+//   * x: the tile's 256-byte row pieces, copied global -> LDS without registers
+//     (16 bytes a lane); piece p of row n is stored at p ^ (n & 15), so the 16
+//     rows of a read phase fall on 16 different bank groups.
+// The loads of the next chunk are in flight while one multiplies; two
+// workgroups share a CU and fill each other's waits. The four conversions of a
+// fragment (v_cvt_scalef32_pk_bf16_fp4) issue in the shadow of the matrix
+// instructions: one conversion for each of them at BT = 4.
+// x in planes (fp16, fp32): the chunk's planes one after the other, weights
+// loaded once.
+#pragma once
+
+#include "vqk_mxs.h"
+
+namespace vqk {
+
+typedef float f32x16v __attribute__((ext_vector_type(16)));
+
+constexpr int kMxgWaves = 4;
+constexpr int kMxgRows = 256;                 // weight rows per workgroup
+
+struct MxgArgs {
+    MxsArgs a;
+    int32_t ntiles_host;                      // x tiles when they are not counted on the device
+    int32_t splits, per;                      // K slices and chunks in each (splits = 1: none)
+    float *part;                              // [splits][N][OUT] when splits > 1
+};
+
+template <int BT, bool GLU, int P>
+__global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga) {
+    const MxsArgs &p = ga.a;
+    constexpr int ROWS = 32 * BT;
+    constexpr int STAGE = ROWS * 256;         // bytes of x per chunk
+    constexpr int CPW = STAGE / 1024 / kMxgWaves;
+    static_assert(CPW * kMxgWaves * 1024 == STAGE, "whole copies per wave");
+    extern __shared__ __align__(16) uint8_t xs[];       // [2][STAGE]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r = lane & 31, g = lane >> 5;
+
+    // tiles in contiguous bands per XCD (workgroup b runs on XCD b % 8)
+    const int nt = p.meta ? p.ntiles[0] : ga.ntiles_host;
+    const int total = nt * p.nob * ga.splits;
+    int t = int(blockIdx.x);
+    if (t >= total) return;
+    {
+        const int x = t % 8, q = total / 8, rest = total % 8;
+        t = x * q + min(x, rest) + t / 8;
+    }
+    const int slice = t % ga.splits;
+    t /= ga.splits;
+    const int tt = p.meta ? t / p.nob : t % nt, ob = p.meta ? t % p.nob : t / nt;
+    MxTile tile;
+    if (!mx_tile<ROWS>(p, tt, &tile)) return;
+    const int o0 = ob * (GLU ? kMxgRows / 2 : kMxgRows);
+    const int ow = o0 + wave * (GLU ? 32 : 64);         // this wave's first output
+    const int c_lo = slice * ga.per, c_hi = min(p.NC, c_lo + ga.per);
+
+    f32x16v acc[2][BT];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < BT; ++b) acc[a][b] = f32x16v{};
+    bool nan[2] = {};
+
+    if (tile.expert >= 0) {
+        const uint8_t *wp[2], *sp[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            const int64_t row = tile.expert * p.OUT + min(int64_t(ow + (GLU ? 0 : 32 * a) + r), p.OUT - 1);
+            wp[a] = (GLU && a ? p.codes1 : p.codes0) + row * p.NB * 16;
+            sp[a] = (GLU && a ? p.scales1 : p.scales0) + row * p.NB;
+        }
+        // the x copies of this lane: 16 bytes of one row each
+        const uint16_t *src[CPW];
+        int piece[CPW];
+#pragma unroll
+        for (int j = 0; j < CPW; ++j) {
+            const int n = (wave * CPW + j) * 4 + (lane >> 4);
+            piece[j] = (lane & 15) ^ (n & 15);
+            src[j] = p.x + mx_x_row(p, tile.row0 + min(n, tile.nrows - 1)) * p.xld + piece[j] * 8;
+        }
+        auto issue = [&](int c, int pl, int buf) {
+#pragma unroll
+            for (int j = 0; j < CPW; ++j) {
+                // past the row's last block: the row's start again (multiplied by no weight, masked below)
+                const bool in = 4 * int64_t(c) + piece[j] / 4 < p.NB;
+                const uint16_t *s = src[j] + pl * p.xplane + (in ? int64_t(c) * kMxChunk : -int64_t(piece[j] * 8));
+                __builtin_amdgcn_global_load_lds((global_void *)s,
+                                                 (lds_void *)(xs + buf * STAGE + (wave * CPW + j) * 1024), 16, 0, 0);
+            }
+        };
+        u32x4 w[2][2], wn[2][2];
+        uint32_t s[2][2], sn[2][2];
+        auto load_w = [&](int c, u32x4 (&ww)[2][2], uint32_t (&ss)[2][2]) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const int64_t blk = 4 * int64_t(c) + 2 * g + q;
+                    const bool in = blk < p.NB;
+                    ww[a][q] = in ? *reinterpret_cast<const u32x4 *>(wp[a] + blk * 16) : u32x4{};
+                    ss[a][q] = in ? sp[a][blk] : 127u;
+                }
+        };
+        auto mul = [&](int c, int buf) {
+            const bool tail = 4 * int64_t(c) + 4 > p.NB;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                float sc[2];
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    nan[a] = nan[a] || s[a][q] == 255u;
+                    sc[a] = mx_scale(s[a][q] == 255u ? 127u : s[a][q]);
+                }
+                const bool in = !tail || 4 * int64_t(c) + 2 * g + q < p.NB;
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    mx_b8 wf[2];
+#pragma unroll
+                    for (int a = 0; a < 2; ++a) wf[a] = __builtin_bit_cast(mx_b8, mx_decode8(w[a][q][h], sc[a]));
+                    const int at = ((8 * g + 4 * q + h) ^ (lane & 15)) * 16 + r * 256;
+#pragma unroll
+                    for (int b = 0; b < BT; ++b) {
+                        u32x4 xv = *reinterpret_cast<const u32x4 *>(xs + buf * STAGE + b * 8192 + at);
+                        if (tail && !in) xv = u32x4{};
+                        const mx_b8 xf = __builtin_bit_cast(mx_b8, xv);
+#pragma unroll
+                        for (int a = 0; a < 2; ++a)
+                            acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[a], xf, acc[a][b], 0, 0, 0);
+                    }
+                }
+            }
+        };
+        int buf = 0;
+        if (c_lo < c_hi) {
+            issue(c_lo, 0, 0);
+            load_w(c_lo, wn, sn);
+        }
+        for (int c = c_lo; c < c_hi; ++c) {
+#pragma unroll
+            for (int pl = 0; pl < P; ++pl) {
+                wait_vmem();                  // this wave's copies of the step, and its weights
+                __syncthreads();              // every wave's copies; every wave is done with the other buffer
+                if (pl == 0) {
+#pragma unroll
+                    for (int a = 0; a < 2; ++a)
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            w[a][q] = wn[a][q];
+                            s[a][q] = sn[a][q];
+                        }
+                }
+                if (pl + 1 < P) issue(c, pl + 1, buf ^ 1);
+                else if (c + 1 < c_hi) {
+                    issue(c + 1, 0, buf ^ 1);
+                    load_w(c + 1, wn, sn);
+                }
+                mul(c, buf);
+                buf ^= 1;
+            }
+        }
+    }
+
+    // register i of lane l: weight row 8 * (i / 4) + 4 * (l / 32) + i % 4, x row l % 32. A NaN block
+    // makes its output NaN: the flag of weight row r is in lanes r and r + 32
+    uint64_t nm[2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+        const uint64_t m = __ballot(nan[a]);
+        nm[a] = (m | (m >> 32)) & 0xffffffffu;
+    }
+    auto value = [&](int a, int b, int i) {
+        const int o = 8 * (i / 4) + 4 * g + i % 4;
+        return (nm[a] >> o) & 1 ? __uint_as_float(0x7fc00000u) : acc[a][b][i];
+    };
+#pragma unroll
+    for (int b = 0; b < BT; ++b) {
+        const int n = 32 * b + r;
+        if (n >= tile.nrows) continue;
+        const int64_t yr = mx_y_row(p, tile.row0 + n);
+        if constexpr (GLU) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int o = ow + 8 * j + 4 * g;
+                if (o >= p.ocover) continue;  // ocover is whole blocks of 32
+                float h[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float v = value(0, b, 4 * j + i), u = value(1, b, 4 * j + i);
+                    h[i] = o + i < p.OUT ? v / (1.f + __expf(-v)) * u : 0.f;
+                }
+                for (int pl = 0; pl < p.yp; ++pl) {
+                    uint16_t q[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) q[i] = mx_plane_next(h[i]);
+                    u32x2 v2;
+                    v2.x = q[0] | (uint32_t(q[1]) << 16);
+                    v2.y = q[2] | (uint32_t(q[3]) << 16);
+                    *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(p.y) + pl * p.yplane + yr * p.ldy + o) = v2;
+                }
+            }
+        } else {
+            void *y = ga.splits > 1 ? static_cast<void *>(ga.part + int64_t(slice) * p.N * p.OUT) : p.y;
+            const int32_t yt = ga.splits > 1 ? VQK_F32 : p.y_type;
+            const bool al = (p.ldy & 3) == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int o = ow + 32 * a + 8 * j + 4 * g;
+                    if (o >= p.OUT) continue;
+                    float v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = value(a, b, 4 * j + i);
+                    mx_store4(y, yt, yr * p.ldy + o, v, int(min(int64_t(4), p.OUT - o)), al);
+                }
+        }
+    }
+}
+
+}  // namespace vqk

@@ -1,0 +1,107 @@
+// Launch of the many-row MXFP4 products (kernel in vqk_mxg.h).
+#include "vqk_mxg.h"
+
+namespace vqk {
+
+struct MxRedArgs {
+    const float *part;
+    int64_t n, plane;                         // outputs; floats between slices
+    int32_t splits, y_type;
+    void *y;
+};
+
+// Sum of the K slices in slice order, four outputs a thread.
+__global__ void __launch_bounds__(256) k_mx_reduce(const MxRedArgs p) {
+    const int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4;
+    if (i >= p.n) return;
+    float v[4] = {};
+    const int n = int(min(int64_t(4), p.n - i));
+    const bool al = (p.plane & 3) == 0;
+    for (int s = 0; s < p.splits; ++s) {
+        const float *src = p.part + s * p.plane + i;
+        if (al && n == 4) {
+            const float4 q = *reinterpret_cast<const float4 *>(src);
+            v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+        } else {
+            for (int u = 0; u < n; ++u) v[u] += src[u];
+        }
+    }
+    mx_store4(p.y, p.y_type, i, v, n, (reinterpret_cast<uintptr_t>(p.y) & 15) == 0);
+}
+
+// K slices for T tiles of NC chunks: enough workgroups for two on every CU, at
+// least 8 chunks each.
+int mxg_splits(int64_t T, int64_t NC) {
+    const int64_t want = 512;
+    int64_t s = T > 0 ? want / T : 1;
+    s = s > NC / 8 ? NC / 8 : s;
+    return int(s < 1 ? 1 : (s > 16 ? 16 : s));
+}
+
+static int mxg_bt(int64_t rows) { return rows <= 32 ? 1 : (rows <= 64 ? 2 : 4); }
+
+size_t mxg_part_bytes(int64_t N, int64_t OUT, int64_t NB) {
+    const int64_t T = ((N + 127) / 128) * ((OUT + kMxgRows - 1) / kMxgRows);
+    const int s = mxg_splits(T, (NB + 3) / 4);
+    return s > 1 ? size_t(s) * N * OUT * 4 : 0;
+}
+
+template <int BT, bool GLU, int P>
+static int go(MxgArgs ga, int64_t tiles, hipStream_t st) {
+    MxsArgs &a = ga.a;
+    a.nob = int32_t((a.ocover + (GLU ? kMxgRows / 2 : kMxgRows) - 1) / (GLU ? kMxgRows / 2 : kMxgRows));
+    const int64_t grid = int64_t(a.nob) * tiles * ga.splits;
+    if (grid > INT32_MAX) return set_error(VQK_ENOTIMPL, "MXFP4 product: grid too large");
+    ga.ntiles_host = int32_t(tiles);
+    int rc = launch_with_lds<k_mx_gemm<BT, GLU, P>>(dim3(unsigned(grid)), dim3(64 * kMxgWaves),
+                                                    size_t(2) * 32 * BT * 256, st, ga);
+    if (rc || ga.splits == 1) return rc;
+    const MxRedArgs r{ga.part, a.N * a.OUT, a.N * a.OUT, ga.splits, a.y_type, a.y};
+    const int64_t wgs = (r.n + 1023) / 1024;
+    if (wgs > INT32_MAX) return set_error(VQK_ENOTIMPL, "MXFP4 product: too many outputs");
+    hipLaunchKernelGGL(k_mx_reduce, dim3(unsigned(wgs)), dim3(256), 0, st, r);
+    return hip_status(hipGetLastError(), "slice sum launch");
+}
+
+template <int BT, bool GLU>
+static int go_p(const MxgArgs &a, int P, int64_t tiles, hipStream_t st) {
+    switch (P) {
+        case 1: return go<BT, GLU, 1>(a, tiles, st);
+        case 2: return go<BT, GLU, 2>(a, tiles, st);
+        default: return go<BT, GLU, 3>(a, tiles, st);
+    }
+}
+
+// tile_rows: x rows per tile (32, 64 or 128; the sort's for a sorted routing).
+int mx_gemm(const MxCall &c, int tile_rows, float *part, size_t part_bytes, hipStream_t st) {
+    const bool glu = c.codes[1] != nullptr;
+    MxgArgs ga{};
+    mx_args(c, &ga.a);
+    const int64_t tiles = mx_tiles(c, tile_rows);
+    if (tiles == 0) return VQK_OK;
+    ga.splits = 1;
+    ga.per = ga.a.NC;
+    if (part && !c.meta && !glu) {
+        const int64_t T = tiles * ((c.OUT + kMxgRows - 1) / kMxgRows);
+        const int s = mxg_splits(T, ga.a.NC);
+        if (s > 1 && size_t(s) * c.N * c.OUT * 4 <= part_bytes) {
+            ga.per = int32_t((ga.a.NC + s - 1) / s);
+            ga.splits = int32_t((ga.a.NC + ga.per - 1) / ga.per);
+            ga.part = part;
+        }
+    }
+    if (glu) {
+        switch (mxg_bt(tile_rows)) {
+            case 1: return go_p<1, true>(ga, c.x.P, tiles, st);
+            case 2: return go_p<2, true>(ga, c.x.P, tiles, st);
+            default: return go_p<4, true>(ga, c.x.P, tiles, st);
+        }
+    }
+    switch (mxg_bt(tile_rows)) {
+        case 1: return go_p<1, false>(ga, c.x.P, tiles, st);
+        case 2: return go_p<2, false>(ga, c.x.P, tiles, st);
+        default: return go_p<4, false>(ga, c.x.P, tiles, st);
+    }
+}
+
+}  // namespace vqk

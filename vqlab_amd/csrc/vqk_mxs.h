@@ -165,6 +165,9 @@ __global__ void __launch_bounds__(64 * kMxsMaxWaves) k_mx_stream(const MxsArgs p
     }
 }
 
+// Kernel arguments of a call, and the tiles of `rows` x rows that it makes.
+void mx_args(const MxCall &c, MxsArgs *a);
+int64_t mx_tiles(const MxCall &c, int rows);
 // Launches k_mx_stream for a call; NT row tiles of 16.
 int mx_stream(const MxCall &c, int NT, hipStream_t st);
 

@@ -24,22 +24,31 @@ static int go_p(const MxsArgs &a, int P, int64_t tiles, hipStream_t st) {
     }
 }
 
+void mx_args(const MxCall &c, MxsArgs *a) {
+    *a = MxsArgs{};
+    a->codes0 = c.codes[0]; a->scales0 = c.scales[0];
+    a->codes1 = c.codes[1]; a->scales1 = c.scales[1];
+    a->NB = c.NB; a->OUT = c.OUT; a->E = c.E;
+    a->NC = int32_t((c.NB + 3) / 4);
+    a->x = c.x.x; a->xld = c.x.ld; a->xplane = c.x.plane;
+    a->N = c.N; a->xkrep = c.xkrep;
+    a->ids = c.ids; a->order = c.order; a->meta = c.meta; a->ntiles = c.ntiles;
+    a->y = c.y; a->y_type = c.y_type; a->yp = c.yp; a->ysorted = c.ysorted;
+    a->ldy = c.ldy; a->yplane = c.yplane;
+    a->ocover = c.codes[1] ? c.ldy : c.OUT;
+}
+
+int64_t mx_tiles(const MxCall &c, int rows) {
+    if (c.ids) return c.N;
+    const int64_t full = (c.N + rows - 1) / rows;
+    return c.meta ? full + (c.N < c.E + 1 ? c.N : c.E + 1) : full;
+}
+
 int mx_stream(const MxCall &c, int NT, hipStream_t st) {
     const bool glu = c.codes[1] != nullptr;
-    MxsArgs a{};
-    a.codes0 = c.codes[0]; a.scales0 = c.scales[0];
-    a.codes1 = c.codes[1]; a.scales1 = c.scales[1];
-    a.NB = c.NB; a.OUT = c.OUT; a.E = c.E;
-    a.NC = int32_t((c.NB + 3) / 4);
-    a.x = c.x.x; a.xld = c.x.ld; a.xplane = c.x.plane;
-    a.N = c.N; a.xkrep = c.xkrep;
-    a.ids = c.ids; a.order = c.order; a.meta = c.meta; a.ntiles = c.ntiles;
-    a.y = c.y; a.y_type = c.y_type; a.yp = c.yp; a.ysorted = c.ysorted;
-    a.ldy = c.ldy; a.yplane = c.yplane;
-    a.ocover = glu ? c.ldy : c.OUT;
-    const int rows = 16 * NT;
-    const int64_t tiles = c.meta ? (c.N + rows - 1) / rows + (c.N < c.E + 1 ? c.N : c.E + 1)
-                                 : (c.ids ? c.N : (c.N + rows - 1) / rows);
+    MxsArgs a;
+    mx_args(c, &a);
+    const int64_t tiles = mx_tiles(c, 16 * NT);
     if (tiles == 0) return VQK_OK;
     if (glu) {
         switch (NT) {
