@@ -124,7 +124,8 @@ def test_linear(dtype, N, OUT, IN):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("N,OUT,IN", [(1, 64, 512), (5, 33, 96), (16, 40, 70), (70, 64, 256), (130, 272, 640),
-                                      (257, 130, 1000), (300, 520, 1152)])
+                                      (257, 130, 1000), (300, 520, 1152), (65, 33, 128), (129, 257, 384),
+                                      (200, 16, 4096)])
 def test_linear_4_bit_activations(dtype, N, OUT, IN):
     rng = np.random.default_rng(N * 11 + OUT + IN)
     lin, w = _linear(rng, OUT, IN, act="mxfp4")
@@ -136,31 +137,33 @@ def test_linear_4_bit_activations(dtype, N, OUT, IN):
 
 @pytest.mark.parametrize("act", [None, "mxfp4"])
 @pytest.mark.parametrize("N", [1, 20, 70, 200])
-def test_linear_scales_far_apart(N, act):
+@pytest.mark.parametrize("IN", [320, 384])
+def test_linear_scales_far_apart(N, act, IN):
     """Scales over 200 powers of two, 0 (a subnormal 2^-127) among them: every weight is exact."""
     rng = np.random.default_rng(N)
     from vqlab_amd import mx
-    codes, _ = mc.weight(rng, 48, 320)
-    scales = rng.integers(0, 200, (48, 10)).astype(np.uint8)
-    lin, w = mx.MXLinear(*_dev(codes, scales), 320, act), mc.values(codes, scales, 320)
-    x, xv = mc.acts(rng, "fp32", N, 320)
+    codes, _ = mc.weight(rng, 48, IN)
+    scales = rng.integers(0, 200, (48, IN // 32)).astype(np.uint8)
+    lin, w = mx.MXLinear(*_dev(codes, scales), IN, act), mc.values(codes, scales, IN)
+    x, xv = mc.acts(rng, "fp32", N, IN)
     if act:
-        xv = mc.values(*mc.quantize(xv), 320)
+        xv = mc.values(*mc.quantize(xv), IN)
     y, bar = mc.product_bar(xv, w, "fp32")
-    # sums of values below fp32's normal range may be flushed: 320 terms of up to 2^-126 each
-    mc.assert_within(lin(x), y, bar + 320 * 2.0 ** -126, "far scales")
+    # sums of values below fp32's normal range may be flushed: IN terms of up to 2^-126 each
+    mc.assert_within(lin(x), y, bar + IN * 2.0 ** -126, "far scales")
 
 
 @pytest.mark.parametrize("act", [None, "mxfp4"])
 @pytest.mark.parametrize("N", [1, 20, 70, 200])
-def test_linear_nan_blocks_stay_in_their_column(N, act):
+@pytest.mark.parametrize("IN", [384, 416])
+def test_linear_nan_blocks_stay_in_their_column(N, act, IN):
     from vqlab_amd import mx
     rng = np.random.default_rng(N + 50)
-    codes, scales = mc.weight(rng, 70, 416)
+    codes, scales = mc.weight(rng, 70, IN)
     scales[5, 3] = 255
-    scales[33, 0] = scales[69, 12] = 255
-    lin = mx.MXLinear(*_dev(codes, scales), 416, act)
-    x, _ = mc.acts(rng, "bf16", N, 416)
+    scales[33, 0] = scales[69, 11] = 255
+    lin = mx.MXLinear(*_dev(codes, scales), IN, act)
+    x, _ = mc.acts(rng, "bf16", N, IN)
     x[0] = 0
     y = lin(x).float().cpu().numpy()
     assert np.isnan(y[:, [5, 33, 69]]).all()
@@ -170,12 +173,13 @@ def test_linear_nan_blocks_stay_in_their_column(N, act):
 @pytest.mark.parametrize("act", [None, "mxfp4"])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("N", [1, 20, 70, 200])
-def test_linear_not_finite_x_stays_in_its_row(dtype, N, act):
+@pytest.mark.parametrize("IN", [200, 256])
+def test_linear_not_finite_x_stays_in_its_row(dtype, N, act, IN):
     rng = np.random.default_rng(N)
-    lin, _ = _linear(rng, 40, 200, act)
-    x, _ = mc.acts(rng, dtype, N, 200)
+    lin, _ = _linear(rng, 40, IN, act)
+    x, _ = mc.acts(rng, dtype, N, IN)
     x[N // 2, 7] = float("nan")
-    x[N - 1, 199] = float("inf")
+    x[N - 1, IN - 1] = float("inf")
     bad = {N // 2, N - 1}
     y = lin(x).float().cpu().numpy()
     for r in range(N):

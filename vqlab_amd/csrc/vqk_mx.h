@@ -142,8 +142,9 @@ __device__ __forceinline__ void mx_store4(void *y, int32_t type, int64_t i, cons
 // (quant) the values of its MXFP4 form, one plane.
 int launch_mx_planes(const void *x, int32_t type, int64_t N, int64_t IN, int64_t ldx, bool quant,
                      uint16_t *out, hipStream_t st);
-// The quantiser without argument checks.
-int launch_mx_quant(const void *x, int32_t type, int64_t rows, int64_t cols, int64_t ldx,
+// The quantiser without argument checks, into rows of NB >= ceil(cols / 32)
+// blocks (those past the row: zeros).
+int launch_mx_quant(const void *x, int32_t type, int64_t rows, int64_t cols, int64_t ldx, int64_t NB,
                     uint8_t *codes, uint8_t *scales, hipStream_t st);
 
 // Rows of x as the product kernels read them: bf16 planes of rows ld apart.
@@ -174,5 +175,22 @@ struct MxCall {
 int mx_gemm(const MxCall &c, int tile_rows, float *part, size_t part_bytes, hipStream_t st);
 // Bytes of the K slices that a dense product of N rows makes use of.
 size_t mxg_part_bytes(int64_t N, int64_t OUT, int64_t NB);
+
+// K slices of a dense product, four outputs a thread, and how many pay.
+int mxg_splits(int64_t T, int64_t NC);
+int launch_mx_reduce(const float *part, int splits, int64_t n, void *y, int32_t y_type, hipStream_t st);
+
+// Products of 4-bit rows with 4-bit weights (vqk_mxf.h): x as codes and scales
+// in rows of xNB blocks, a multiple of 8.
+struct MxfCall {
+    const uint8_t *codes, *scales;            // weights [OUT, NB], NB % 4 == 0
+    int64_t OUT, NB, N, xNB;
+    const uint8_t *xcodes, *xscales;
+    void *y;
+    int32_t y_type;
+};
+bool mxf_ok(const uint8_t *scales, int64_t IN, int64_t N);
+int mxf_gemm(const MxfCall &c, float *part, size_t part_bytes, hipStream_t st);
+size_t mxf_part_bytes(int64_t N, int64_t OUT, int64_t NB);
 
 }  // namespace vqk

@@ -58,7 +58,7 @@ static int go_quant(const QuantArgs &a, hipStream_t st) {
     const int esz = XT == VQK_F32 ? 4 : 2;
     const bool al = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
     const bool vec = al && (a.ldx * esz) % 16 == 0;
-    const bool flat = vec && a.ldx == a.cols && a.cols % kMxBlock == 0;
+    const bool flat = vec && a.ldx == a.cols && a.cols == a.NB * kMxBlock;
     const int64_t wgs = (a.pieces + 255) / 256;
     const dim3 grid(unsigned(wgs < 16384 ? wgs : 16384));
     if (flat) hipLaunchKernelGGL((k_mx_quant<XT, true, true>), grid, dim3(256), 0, st, a);
@@ -67,9 +67,8 @@ static int go_quant(const QuantArgs &a, hipStream_t st) {
     return hip_status(hipGetLastError(), "MXFP4 quantiser launch");
 }
 
-int launch_mx_quant(const void *x, int32_t type, int64_t rows, int64_t cols, int64_t ldx,
+int launch_mx_quant(const void *x, int32_t type, int64_t rows, int64_t cols, int64_t ldx, int64_t NB,
                     uint8_t *codes, uint8_t *scales, hipStream_t st) {
-    const int64_t NB = (cols + kMxBlock - 1) / kMxBlock;
     const QuantArgs a{x, cols, ldx, NB, rows * NB * 4, codes, scales};
     switch (type) {
         case VQK_F16: return go_quant<VQK_F16>(a, st);
@@ -211,7 +210,8 @@ extern "C" int vqk_mx_quantize(const void *x, int32_t x_type, int64_t rows, int6
     if (!x || !codes || !scales) return set_error(VQK_EINVAL, "mx quantize: NULL pointer");
     if (reinterpret_cast<uintptr_t>(codes) & 3)
         return set_error(VQK_EINVAL, "mx quantize: codes must be 4-byte aligned");
-    return launch_mx_quant(x, x_type, rows, cols, ldx, codes, scales, static_cast<hipStream_t>(stream));
+    return launch_mx_quant(x, x_type, rows, cols, ldx, (cols + kMxBlock - 1) / kMxBlock, codes, scales,
+                           static_cast<hipStream_t>(stream));
 }
 
 extern "C" int vqk_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols,

@@ -124,7 +124,14 @@ static size_t lin_x_bytes(const MxGeom &g, int32_t x_type, int64_t N, int32_t ac
     const int P = act == VQK_MX_ACT_MXFP4 ? 1 : mx_planes(x_type);
     return al256(size_t(N) * g.NB * kMxBlock * 2 * P);
 }
-static size_t lin_bytes(const MxGeom &g, int32_t x_type, int64_t N, int32_t act) {
+// 4-bit x for the 4-bit matrix instructions: rows of whole 256-wide chunks.
+static int64_t mxf_blocks(const MxGeom &g) { return (g.NB + 7) / 8 * 8; }
+static size_t mxf_x_bytes(const MxGeom &g, int64_t N) { return al256(size_t(N) * mxf_blocks(g) * 17); }
+static bool lin_4bit(const vqk_mx_weights *w, const MxGeom &g, int64_t N, int32_t act) {
+    return act == VQK_MX_ACT_MXFP4 && N > kMxStreamRows && mxf_ok(w->scales, g.IN, N);
+}
+static size_t lin_bytes(const vqk_mx_weights *w, const MxGeom &g, int32_t x_type, int64_t N, int32_t act) {
+    if (lin_4bit(w, g, N, act)) return mxf_x_bytes(g, N) + mxf_part_bytes(N, g.OUT, g.NB);
     return lin_x_bytes(g, x_type, N, act) + (N > kMxStreamRows ? mxg_part_bytes(N, g.OUT, g.NB) : 0);
 }
 
@@ -143,7 +150,7 @@ extern "C" int vqk_mx_linear_workspace(const vqk_mx_weights *w, int32_t x_type, 
     int rc = check_lin(w, x_type, N, &g, "mx linear");
     if (rc || (rc = check_act(act))) return rc;
     if (!bytes) return set_error(VQK_EINVAL, "mx linear: NULL bytes");
-    *bytes = lin_bytes(g, x_type, N, act);
+    *bytes = lin_bytes(w, g, x_type, N, act);
     return VQK_OK;
 }
 
@@ -162,11 +169,19 @@ extern "C" int vqk_mx_linear(const vqk_mx_weights *w, const void *x, int32_t x_t
     c.N = N; c.xkrep = 1;
     c.y = y; c.y_type = y_type; c.ldy = g.OUT;
     const bool place = act == VQK_MX_ACT_NONE && x_in_place(x, x_type, g.IN, g.IN);
-    const size_t need = lin_bytes(g, x_type, N, act);
+    const size_t need = lin_bytes(w, g, x_type, N, act);
     if ((!place || N > kMxStreamRows) && need && (!workspace || ws_bytes < need))
         return set_error(VQK_ENOSPACE, "mx linear: workspace %zu < %zu", ws_bytes, need);
     if (reinterpret_cast<uintptr_t>(workspace) & 255)
         return set_error(VQK_EINVAL, "mx linear: workspace must be 256-byte aligned");
+    if (lin_4bit(w, g, N, act)) {
+        const int64_t xNB = mxf_blocks(g);
+        uint8_t *xc = static_cast<uint8_t *>(workspace), *xsc = xc + size_t(N) * xNB * 16;
+        if ((rc = launch_mx_quant(x, x_type, N, g.IN, g.IN, xNB, xc, xsc, st))) return rc;
+        const size_t xb = mxf_x_bytes(g, N);
+        const MxfCall f{w->codes, w->scales, g.OUT, g.NB, N, xNB, xc, xsc, y, y_type};
+        return mxf_gemm(f, need > xb ? reinterpret_cast<float *>(xc + xb) : nullptr, need - xb, st);
+    }
     if (place) {
         c.x = MxX{static_cast<const uint16_t *>(x), g.IN, 0, 1};
     } else {

@@ -32,11 +32,13 @@ constexpr int kMxgRows = 256;                 // weight rows per workgroup
 struct MxgArgs {
     MxsArgs a;
     int32_t ntiles_host;                      // x tiles when they are not counted on the device
+    int32_t planes;                           // bf16 planes of x
     int32_t splits, per;                      // K slices and chunks in each (splits = 1: none)
     float *part;                              // [splits][N][OUT] when splits > 1
 };
 
-template <int BT, bool GLU, int P>
+// PL: x in more planes than one.
+template <int BT, bool GLU, bool PL>
 __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga) {
     const MxsArgs &p = ga.a;
     constexpr int ROWS = 32 * BT;
@@ -141,33 +143,36 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
                 }
             }
         };
-        int buf = 0;
-        if (c_lo < c_hi) {
+        // steps: chunk c_lo + step / P, plane step % P
+        const int P = PL ? ga.planes : 1, steps = (c_hi - c_lo) * P;
+        if (steps > 0) {
             issue(c_lo, 0, 0);
             load_w(c_lo, wn, sn);
         }
-        for (int c = c_lo; c < c_hi; ++c) {
+        int c = c_lo, pl = 0;
+#pragma unroll 1
+        for (int step = 0; step < steps; ++step) {
+            wait_vmem();                      // this wave's copies of the step, and its weights
+            __syncthreads();                  // every wave's copies; every wave is done with the other buffer
+            if (!PL || pl == 0) {
 #pragma unroll
-            for (int pl = 0; pl < P; ++pl) {
-                wait_vmem();                  // this wave's copies of the step, and its weights
-                __syncthreads();              // every wave's copies; every wave is done with the other buffer
-                if (pl == 0) {
+                for (int a = 0; a < 2; ++a)
 #pragma unroll
-                    for (int a = 0; a < 2; ++a)
-#pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            w[a][q] = wn[a][q];
-                            s[a][q] = sn[a][q];
-                        }
-                }
-                if (pl + 1 < P) issue(c, pl + 1, buf ^ 1);
-                else if (c + 1 < c_hi) {
-                    issue(c + 1, 0, buf ^ 1);
-                    load_w(c + 1, wn, sn);
-                }
-                mul(c, buf);
-                buf ^= 1;
+                    for (int q = 0; q < 2; ++q) {
+                        w[a][q] = wn[a][q];
+                        s[a][q] = sn[a][q];
+                    }
             }
+            const int cc = c;
+            if (!PL || ++pl == P) {
+                pl = 0;
+                ++c;
+            }
+            if (step + 1 < steps) {
+                issue(c, pl, (step + 1) & 1);
+                if (!PL || pl == 0) load_w(c, wn, sn);
+            }
+            mul(cc, step & 1);
         }
     }
 

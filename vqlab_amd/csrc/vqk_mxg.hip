@@ -29,6 +29,14 @@ __global__ void __launch_bounds__(256) k_mx_reduce(const MxRedArgs p) {
     mx_store4(p.y, p.y_type, i, v, n, (reinterpret_cast<uintptr_t>(p.y) & 15) == 0);
 }
 
+int launch_mx_reduce(const float *part, int splits, int64_t n, void *y, int32_t y_type, hipStream_t st) {
+    const MxRedArgs r{part, n, n, splits, y_type, y};
+    const int64_t wgs = (n + 1023) / 1024;
+    if (wgs > INT32_MAX) return set_error(VQK_ENOTIMPL, "MXFP4 product: too many outputs");
+    hipLaunchKernelGGL(k_mx_reduce, dim3(unsigned(wgs)), dim3(256), 0, st, r);
+    return hip_status(hipGetLastError(), "slice sum launch");
+}
+
 // K slices for T tiles of NC chunks: enough workgroups for two on every CU, at
 // least 8 chunks each.
 int mxg_splits(int64_t T, int64_t NC) {
@@ -46,30 +54,22 @@ size_t mxg_part_bytes(int64_t N, int64_t OUT, int64_t NB) {
     return s > 1 ? size_t(s) * N * OUT * 4 : 0;
 }
 
-template <int BT, bool GLU, int P>
+template <int BT, bool GLU, bool PL>
 static int go(MxgArgs ga, int64_t tiles, hipStream_t st) {
     MxsArgs &a = ga.a;
     a.nob = int32_t((a.ocover + (GLU ? kMxgRows / 2 : kMxgRows) - 1) / (GLU ? kMxgRows / 2 : kMxgRows));
     const int64_t grid = int64_t(a.nob) * tiles * ga.splits;
     if (grid > INT32_MAX) return set_error(VQK_ENOTIMPL, "MXFP4 product: grid too large");
     ga.ntiles_host = int32_t(tiles);
-    int rc = launch_with_lds<k_mx_gemm<BT, GLU, P>>(dim3(unsigned(grid)), dim3(64 * kMxgWaves),
+    int rc = launch_with_lds<k_mx_gemm<BT, GLU, PL>>(dim3(unsigned(grid)), dim3(64 * kMxgWaves),
                                                     size_t(2) * 32 * BT * 256, st, ga);
     if (rc || ga.splits == 1) return rc;
-    const MxRedArgs r{ga.part, a.N * a.OUT, a.N * a.OUT, ga.splits, a.y_type, a.y};
-    const int64_t wgs = (r.n + 1023) / 1024;
-    if (wgs > INT32_MAX) return set_error(VQK_ENOTIMPL, "MXFP4 product: too many outputs");
-    hipLaunchKernelGGL(k_mx_reduce, dim3(unsigned(wgs)), dim3(256), 0, st, r);
-    return hip_status(hipGetLastError(), "slice sum launch");
+    return launch_mx_reduce(ga.part, ga.splits, a.N * a.OUT, a.y, a.y_type, st);
 }
 
 template <int BT, bool GLU>
-static int go_p(const MxgArgs &a, int P, int64_t tiles, hipStream_t st) {
-    switch (P) {
-        case 1: return go<BT, GLU, 1>(a, tiles, st);
-        case 2: return go<BT, GLU, 2>(a, tiles, st);
-        default: return go<BT, GLU, 3>(a, tiles, st);
-    }
+static int go_p(const MxgArgs &a, int64_t tiles, hipStream_t st) {
+    return a.planes == 1 ? go<BT, GLU, false>(a, tiles, st) : go<BT, GLU, true>(a, tiles, st);
 }
 
 // tile_rows: x rows per tile (32, 64 or 128; the sort's for a sorted routing).
@@ -77,6 +77,7 @@ int mx_gemm(const MxCall &c, int tile_rows, float *part, size_t part_bytes, hipS
     const bool glu = c.codes[1] != nullptr;
     MxgArgs ga{};
     mx_args(c, &ga.a);
+    ga.planes = c.x.P;
     const int64_t tiles = mx_tiles(c, tile_rows);
     if (tiles == 0) return VQK_OK;
     ga.splits = 1;
@@ -92,15 +93,15 @@ int mx_gemm(const MxCall &c, int tile_rows, float *part, size_t part_bytes, hipS
     }
     if (glu) {
         switch (mxg_bt(tile_rows)) {
-            case 1: return go_p<1, true>(ga, c.x.P, tiles, st);
-            case 2: return go_p<2, true>(ga, c.x.P, tiles, st);
-            default: return go_p<4, true>(ga, c.x.P, tiles, st);
+            case 1: return go_p<1, true>(ga, tiles, st);
+            case 2: return go_p<2, true>(ga, tiles, st);
+            default: return go_p<4, true>(ga, tiles, st);
         }
     }
     switch (mxg_bt(tile_rows)) {
-        case 1: return go_p<1, false>(ga, c.x.P, tiles, st);
-        case 2: return go_p<2, false>(ga, c.x.P, tiles, st);
-        default: return go_p<4, false>(ga, c.x.P, tiles, st);
+        case 1: return go_p<1, false>(ga, tiles, st);
+        case 2: return go_p<2, false>(ga, tiles, st);
+        default: return go_p<4, false>(ga, tiles, st);
     }
 }
 
