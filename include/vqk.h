@@ -394,9 +394,17 @@ int vqk_skipzero_row_table_host(const uint8_t *rowmask, int64_t E,
  * s: value = e2m1(code) * 2^(s - 127), with e2m1 in {0, .5, 1, 1.5, 2, 3, 4, 6}
  * and the sign in a code's top bit. s = 255: the whole block is NaN.
  *
- *   codes   uint8 [E, OUT, NB * 16], 16-byte aligned
- *   scales  uint8 [E, OUT, NB]
- * A dense linear is E = 1. */
+ *
+ * Weights are kept in operand order, as vqk_mx_pack lays them out once from rows
+ * of codes [E, OUT, NB * 16] and scales [E, OUT, NB] (both as vqk_mx_quantize
+ * leaves them; codes 16-byte aligned): with RT = ceil(OUT / 16) and
+ * NC = ceil(IN / 128),
+ *   codes   uint8 [E, RT, NC, 64, 16], 16-byte aligned: unit i of a tile is block
+ *           4 c + i / 16 of weight row 16 rt + i % 16
+ *   scales  uint8 [E, RT, ceil(NC / 4), 64, 4], 4-byte aligned: byte j of unit i
+ *           belongs to its block in chunk 4 group + j
+ * with codes 0 and scales 127 past the rows' ends. vqk_mx_pack_bytes gives both
+ * sizes. A dense linear is E = 1; one expert holds less than 4 GB. */
 typedef struct vqk_mx_weights {
     const uint8_t *codes;
     const uint8_t *scales;
@@ -404,6 +412,9 @@ typedef struct vqk_mx_weights {
     int64_t        OUT;
     int64_t        IN;
 } vqk_mx_weights;
+int vqk_mx_pack_bytes(int64_t E, int64_t OUT, int64_t IN, size_t *codes, size_t *scales);
+int vqk_mx_pack(const uint8_t *codes, const uint8_t *scales, int64_t E, int64_t OUT, int64_t IN,
+                uint8_t *packed_codes, uint8_t *packed_scales, void *stream);
 
 /* x [rows, cols] (rows ldx elements apart) -> codes [rows, NB * 16] (4-byte
  * aligned) and scales [rows, NB]: s - 127 = floor(log2(largest magnitude)) - 2,

@@ -105,6 +105,8 @@ SIGNATURES = {
                                  c_sz, ctypes.POINTER(VQKOptions), c_p]),
     "vqk_mx_quantize": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, c_p, c_p, c_p]),
     "vqk_mx_dequantize": (c_i32, [c_p, c_p, c_i64, c_i64, c_p, c_i32, c_p]),
+    "vqk_mx_pack_bytes": (c_i32, [c_i64, c_i64, c_i64, ctypes.POINTER(c_sz), ctypes.POINTER(c_sz)]),
+    "vqk_mx_pack": (c_i32, [c_p, c_p, c_i64, c_i64, c_i64, c_p, c_p, c_p]),
     "vqk_mx_linear_workspace": (c_i32, [_MXW, c_i32, c_i64, c_i32, ctypes.POINTER(c_sz)]),
     "vqk_mx_linear": (c_i32, [_MXW, c_p, c_i32, c_i64, c_i32, c_p, c_i32, c_p, c_sz, c_p]),
     "vqk_mx_linear_dx_workspace": (c_i32, [_MXW, c_i32, c_i64, ctypes.POINTER(c_sz)]),

@@ -4,16 +4,25 @@
 // codes past C zero) and one scale byte s: element = e2m1(code) * 2^(s - 127),
 // s = 255 a block of NaN.
 //
-// Two facts carry every kernel here:
+// Three facts carry every kernel here:
 //   * e2m1 * 2^(s - 127) has at most two significant bits and an exponent
 //     inside bf16's, so a bf16 weight is the exact weight
 //     (v_cvt_scalef32_pk_bf16_fp4 makes two of them, scale included);
-//   * the sum over k may be taken in any order, so a lane of a 16x16x32 MFMA
-//     owns one whole block (16 bytes, one scale): lane group g = lane / 16
-//     holds block 4c + g of the 128-wide chunk c, and step s of four
-//     multiplies elements 8s..8s+7 of each group's block. Weights then go
-//     from global memory to registers with one 16-byte load, no LDS, and the
-//     x operand is the matching 16-byte piece of its row.
+//   * the sum over k may be taken in any order, so a lane of a matrix
+//     instruction can own whole blocks (16 bytes, one scale): in a chunk of 128 k
+//     the lane groups take the chunk's four blocks, and step h multiplies
+//     elements 8h..8h+7 of each group's block. Weights then go from global
+//     memory to registers, no LDS, and the x operand is a 16-byte piece of a row;
+//   * the L1 serves one 128-byte line per cycle, and 16 lanes a cycle. Read
+//     row by row, a lane's 16 bytes lie in a line of their own: 64 cycles for the
+//     1 KB of a wave's load instead of 16 (47 MB of weights at 4.1 TB/s instead of 5.5,
+//     and the many-row kernels bound by it). So weights are laid out once in
+//     operand order:
+//       codes  [E][RT][NC][64][16]   RT = ceil(OUT / 16) row tiles, NC = ceil(IN / 128)
+//              unit (lane) i of a tile: row i % 16, block 4 chunk + i / 16
+//       scales [E][RT][ceil(NC / 4)][64][4]   byte j of unit i: the scale of its block in
+//              chunk 4 group + j (the block-scaled matrix instruction picks a byte itself)
+//     with codes 0 and scales 127 past the row's and the weight's end.
 #pragma once
 
 #include "vqk_gemv.h"
@@ -27,7 +36,9 @@ typedef __bf16 mx_b8 __attribute__((ext_vector_type(8)));
 constexpr int kMxBlock = 32;
 constexpr int kMxChunk = 128;                 // k of one weight load: 4 lane groups x 32
 
-struct MxGeom { int64_t E, OUT, IN, NB; };
+struct MxGeom { int64_t E, OUT, IN, NB, RT, NC; };
+__host__ __device__ constexpr int64_t mx_expert_codes(int64_t RT, int64_t NC) { return RT * NC * 1024; }
+__host__ __device__ constexpr int64_t mx_expert_scales(int64_t RT, int64_t NC) { return RT * ((NC + 3) / 4) * 256; }
 // Validates `w` and fills `g`; returns a VQK_* status and sets the message.
 int make_mx_geom(const vqk_mx_weights *w, MxGeom *g, const char *what);
 
@@ -143,9 +154,9 @@ __device__ __forceinline__ void mx_store4(void *y, int32_t type, int64_t i, cons
 int launch_mx_planes(const void *x, int32_t type, int64_t N, int64_t IN, int64_t ldx, bool quant,
                      uint16_t *out, hipStream_t st);
 // The quantiser without argument checks, into rows of NB >= ceil(cols / 32)
-// blocks (those past the row: zeros).
+// blocks (those past the row: zeros); permute: scales placed by mxf_scale_at.
 int launch_mx_quant(const void *x, int32_t type, int64_t rows, int64_t cols, int64_t ldx, int64_t NB,
-                    uint8_t *codes, uint8_t *scales, hipStream_t st);
+                    bool permute, uint8_t *codes, uint8_t *scales, hipStream_t st);
 
 // Rows of x as the product kernels read them: bf16 planes of rows ld apart.
 struct MxX {
@@ -157,7 +168,7 @@ struct MxX {
 // One product, over dense rows, single pairs, or tiles of a sorted routing.
 struct MxCall {
     const uint8_t *codes[2], *scales[2];      // [1]: the second projection of a SwiGLU pair
-    int64_t E, OUT, IN, NB;
+    MxGeom g;
     MxX x;
     int64_t N;                                // rows or pairs
     // routing: none (dense) | ids (tile = pair) | order, meta, ntiles (sorted tiles)
@@ -173,24 +184,31 @@ struct MxCall {
 // The many-row products (vqk_mxg.h): x tiles of tile_rows (32, 64, 128); part:
 // room for fp32 K slices of a dense product, or NULL.
 int mx_gemm(const MxCall &c, int tile_rows, float *part, size_t part_bytes, hipStream_t st);
+// x rows per tile of a dense product of N rows.
+int mxg_dense_rows(int64_t N);
 // Bytes of the K slices that a dense product of N rows makes use of.
-size_t mxg_part_bytes(int64_t N, int64_t OUT, int64_t NB);
+size_t mxg_part_bytes(int64_t N, const MxGeom &g);
 
 // K slices of a dense product, four outputs a thread, and how many pay.
 int mxg_splits(int64_t T, int64_t NC);
 int launch_mx_reduce(const float *part, int splits, int64_t n, void *y, int32_t y_type, hipStream_t st);
 
-// Products of 4-bit rows with 4-bit weights (vqk_mxf.h): x as codes and scales
-// in rows of xNB blocks, a multiple of 8.
+// Products of 4-bit rows with 4-bit weights (vqk_mxf.h): x as codes in rows of
+// xNB blocks, a multiple of 16, and scales in the order of mxf_scale_at.
 struct MxfCall {
-    const uint8_t *codes, *scales;            // weights [OUT, NB], NB % 4 == 0
-    int64_t OUT, NB, N, xNB;
+    const uint8_t *codes, *scales;
+    MxGeom g;
+    int64_t N, xNB;
     const uint8_t *xcodes, *xscales;
     void *y;
     int32_t y_type;
 };
-bool mxf_ok(const uint8_t *scales, int64_t IN, int64_t N);
+// Place of block b's scale in a row of x scales: the four chunks' bytes of a
+// block position side by side, as in the weights' scales.
+__host__ __device__ constexpr int64_t mxf_scale_at(int64_t b) {
+    return b / 16 * 16 + b % 4 * 4 + b / 4 % 4;
+}
 int mxf_gemm(const MxfCall &c, float *part, size_t part_bytes, hipStream_t st);
-size_t mxf_part_bytes(int64_t N, int64_t OUT, int64_t NB);
+size_t mxf_part_bytes(int64_t N, const MxGeom &g);
 
 }  // namespace vqk

@@ -21,13 +21,20 @@ int make_mx_geom(const vqk_mx_weights *w, MxGeom *g, const char *what) {
     if (!w->codes || !w->scales) return set_error(VQK_EINVAL, "%s: codes and scales are required", what);
     if (reinterpret_cast<uintptr_t>(w->codes) & 15)
         return set_error(VQK_EINVAL, "%s: codes must be 16-byte aligned", what);
-    *g = MxGeom{w->E, w->OUT, w->IN, (w->IN + kMxBlock - 1) / kMxBlock};
+    if (reinterpret_cast<uintptr_t>(w->scales) & 3)
+        return set_error(VQK_EINVAL, "%s: scales must be 4-byte aligned", what);
+    *g = MxGeom{w->E, w->OUT, w->IN, (w->IN + kMxBlock - 1) / kMxBlock, (w->OUT + 15) / 16,
+                (w->IN + kMxChunk - 1) / kMxChunk};
+    // kernels reach an expert's weights by 32-bit offsets
+    if (mx_expert_codes(g->RT, g->NC) > INT64_C(0xffffffff))
+        return set_error(VQK_ENOTIMPL, "%s: an expert of 4 GB or more", what);
     return VQK_OK;
 }
 
 struct QuantArgs {
     const void *x;
     int64_t cols, ldx, NB, pieces;            // pieces of 8 values: rows * NB * 4
+    int32_t permute;
     uint8_t *codes, *scales;
 };
 
@@ -49,7 +56,7 @@ __global__ void __launch_bounds__(256) k_mx_quant(const QuantArgs p) {
         // pieces come in whole quads (pieces % 4 == 0 and 256 % 4 == 0): all four lanes are here
         const uint32_t s = mx_scale_byte(quad_max(m));
         reinterpret_cast<uint32_t *>(p.codes)[i] = mx_encode8(v, s);
-        if ((i & 3) == 0) p.scales[i >> 2] = uint8_t(s);
+        if ((i & 3) == 0) p.scales[p.permute ? mxf_scale_at(i >> 2) : i >> 2] = uint8_t(s);   // NB % 16 == 0 then
     }
 }
 
@@ -68,8 +75,8 @@ static int go_quant(const QuantArgs &a, hipStream_t st) {
 }
 
 int launch_mx_quant(const void *x, int32_t type, int64_t rows, int64_t cols, int64_t ldx, int64_t NB,
-                    uint8_t *codes, uint8_t *scales, hipStream_t st) {
-    const QuantArgs a{x, cols, ldx, NB, rows * NB * 4, codes, scales};
+                    bool permute, uint8_t *codes, uint8_t *scales, hipStream_t st) {
+    const QuantArgs a{x, cols, ldx, NB, rows * NB * 4, permute, codes, scales};
     switch (type) {
         case VQK_F16: return go_quant<VQK_F16>(a, st);
         case VQK_BF16: return go_quant<VQK_BF16>(a, st);
@@ -196,9 +203,64 @@ int launch_mx_planes(const void *x, int32_t type, int64_t N, int64_t IN, int64_t
     return hip_status(hipGetLastError(), "activation plane launch");
 }
 
+// ------------------------------------------------------- operand order
+struct PackArgs {
+    const uint8_t *codes, *scales;
+    int64_t E, OUT, NB, RT, NC, units;        // units of 16 bytes: E * RT * NC * 64
+    uint8_t *pcodes, *pscales;
+};
+
+// One unit a thread: 16 bytes of codes from their row to their place.
+__global__ void __launch_bounds__(256) k_mx_pack(const PackArgs p) {
+    const int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (u >= p.units) return;
+    const int i = int(u & 63);
+    const int64_t tile = u >> 6, c = tile % p.NC, et = tile / p.NC, rt = et % p.RT, e = et / p.RT;
+    const int64_t row = rt * 16 + (i & 15), blk = 4 * c + (i >> 4);
+    const bool in = row < p.OUT && blk < p.NB;
+    const int64_t at = (e * p.OUT + row) * p.NB + blk;
+    reinterpret_cast<u32x4 *>(p.pcodes)[u] = in ? reinterpret_cast<const u32x4 *>(p.codes)[at] : u32x4{};
+    uint8_t *sc = p.pscales + ((et * ((p.NC + 3) / 4) + c / 4) * 64 + i) * 4;
+    sc[c & 3] = in ? p.scales[at] : uint8_t(127);
+    if (c == p.NC - 1)                        // the bytes of chunks past the end
+        for (int j = int(c & 3) + 1; j < 4; ++j) sc[j] = 127;
+}
+
 }  // namespace vqk
 
 using namespace vqk;
+
+static int check_pack(int64_t E, int64_t OUT, int64_t IN) {
+    if (E < 1 || OUT < 1 || IN < 1 || E > INT32_MAX || OUT > INT32_MAX / 2 || IN > INT32_MAX / 2)
+        return set_error(VQK_EINVAL, "mx pack: bad shape E=%lld OUT=%lld IN=%lld", (long long)E, (long long)OUT,
+                         (long long)IN);
+    return VQK_OK;
+}
+
+extern "C" int vqk_mx_pack_bytes(int64_t E, int64_t OUT, int64_t IN, size_t *codes, size_t *scales) {
+    const int rc = check_pack(E, OUT, IN);
+    if (rc) return rc;
+    if (!codes || !scales) return set_error(VQK_EINVAL, "mx pack: NULL sizes");
+    const int64_t RT = (OUT + 15) / 16, NC = (IN + kMxChunk - 1) / kMxChunk;
+    *codes = size_t(E) * mx_expert_codes(RT, NC);
+    *scales = size_t(E) * mx_expert_scales(RT, NC);
+    return VQK_OK;
+}
+
+extern "C" int vqk_mx_pack(const uint8_t *codes, const uint8_t *scales, int64_t E, int64_t OUT, int64_t IN,
+                           uint8_t *pcodes, uint8_t *pscales, void *stream) {
+    const int rc = check_pack(E, OUT, IN);
+    if (rc) return rc;
+    if (!codes || !scales || !pcodes || !pscales) return set_error(VQK_EINVAL, "mx pack: NULL pointer");
+    if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(pcodes)) & 15)
+        return set_error(VQK_EINVAL, "mx pack: codes must be 16-byte aligned");
+    const int64_t RT = (OUT + 15) / 16, NC = (IN + kMxChunk - 1) / kMxChunk, units = E * RT * NC * 64;
+    if ((units + 255) / 256 > INT32_MAX) return set_error(VQK_ENOTIMPL, "mx pack: weight too large");
+    const PackArgs a{codes, scales, E, OUT, (IN + kMxBlock - 1) / kMxBlock, RT, NC, units, pcodes, pscales};
+    hipLaunchKernelGGL(k_mx_pack, dim3(unsigned((units + 255) / 256)), dim3(256), 0,
+                       static_cast<hipStream_t>(stream), a);
+    return hip_status(hipGetLastError(), "MXFP4 pack launch");
+}
 
 extern "C" int vqk_mx_quantize(const void *x, int32_t x_type, int64_t rows, int64_t cols, int64_t ldx,
                                uint8_t *codes, uint8_t *scales, void *stream) {
@@ -210,7 +272,7 @@ extern "C" int vqk_mx_quantize(const void *x, int32_t x_type, int64_t rows, int6
     if (!x || !codes || !scales) return set_error(VQK_EINVAL, "mx quantize: NULL pointer");
     if (reinterpret_cast<uintptr_t>(codes) & 3)
         return set_error(VQK_EINVAL, "mx quantize: codes must be 4-byte aligned");
-    return launch_mx_quant(x, x_type, rows, cols, ldx, (cols + kMxBlock - 1) / kMxBlock, codes, scales,
+    return launch_mx_quant(x, x_type, rows, cols, ldx, (cols + kMxBlock - 1) / kMxBlock, false, codes, scales,
                            static_cast<hipStream_t>(stream));
 }
 

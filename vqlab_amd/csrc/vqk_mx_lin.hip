@@ -1,9 +1,10 @@
 // Dense linears with MXFP4 weights: y = x . W^T and the gradient of x,
 // dx = dy . W.
 //
-// The forward product runs on the kernels of vqk_mxs.h. x that is bf16, 16-byte
-// aligned and whole blocks wide is read in place; other x is laid out once in
-// the workspace as exact bf16 planes (vqk_mx.h). The gradient sums over the
+// The forward product streams the weights past few rows (vqk_mxs.h) or
+// multiplies tiles of many (vqk_mxg.h; 4-bit x: vqk_mxf.h). x that is bf16,
+// 16-byte aligned and whole blocks wide is read in place; other x is laid out
+// once in the workspace as exact bf16 planes (vqk_mx.h). The gradient sums over the
 // weight's rows, along which its codes do not lie: the weight is decoded,
 // transposed, into the workspace as bf16 (exact) and multiplied by the
 // matrix-core GEMM of the dense prefill path.
@@ -21,23 +22,22 @@ static bool x_in_place(const void *x, int32_t type, int64_t IN, int64_t ld) {
 // ------------------------------------------------------- transposed decode
 struct DecTArgs {
     const uint8_t *codes, *scales;
-    int64_t OUT, IN, NB, KO;                  // KO: columns of one copy of the transposed weight
+    int64_t IN, RT, NC, KO;                   // KO: columns of one copy of the transposed weight
     int32_t P;
     uint16_t *out;                            // [IN][P * KO], zero past OUT
 };
 
-// 64 weight rows x 128 columns through LDS: 16 bytes of codes in per thread,
+// 64 weight rows x one chunk through LDS: 16 bytes of codes in per thread,
 // 16-byte pieces of a transposed row out.
 __global__ void __launch_bounds__(256) k_mx_dec_t(const DecTArgs p) {
     __shared__ uint16_t tile[128][72];
-    const int64_t o0 = int64_t(blockIdx.x) * 64, k0 = int64_t(blockIdx.y) * 128;
+    const int64_t o0 = int64_t(blockIdx.x) * 64, c = blockIdx.y, k0 = c * kMxChunk;
     {
-        const int o = threadIdx.x >> 2, g = threadIdx.x & 3;
-        const int64_t blk = k0 / kMxBlock + g;
-        const bool ok = o0 + o < p.OUT && blk < p.NB;
-        const int64_t at = (o0 + o) * p.NB + blk;
-        const u32x4 w = ok ? *reinterpret_cast<const u32x4 *>(p.codes + at * 16) : u32x4{};
-        const uint32_t s = ok ? p.scales[at] : 127u;
+        const int unit = threadIdx.x & 63, o = (threadIdx.x >> 6) * 16 + (unit & 15), g = unit >> 4;
+        const int64_t rt = o0 / 16 + (threadIdx.x >> 6);
+        const bool ok = rt < p.RT;
+        const u32x4 w = ok ? *reinterpret_cast<const u32x4 *>(p.codes + ((rt * p.NC + c) * 64 + unit) * 16) : u32x4{};
+        const uint32_t s = ok ? p.scales[((rt * ((p.NC + 3) / 4) + c / 4) * 64 + unit) * 4 + c % 4] : 127u;
         const float sc = mx_scale(s == 255u ? 127u : s);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -116,23 +116,25 @@ static int check_lin(const vqk_mx_weights *w, int32_t x_type, int64_t N, MxGeom 
     return VQK_OK;
 }
 
-// Rows up to which the weights are streamed past all rows (vqk_mxs.h).
-constexpr int64_t kMxStreamRows = 64;
+// Rows up to which the weights are streamed past all rows (vqk_mxs.h), where x
+// fits its registers; more run as tiles.
+constexpr int64_t kMxStreamRows = 32;
+// Rows from which x that is quantised runs on the 4-bit matrix instructions;
+// fewer enter as the values they are rounded to.
+constexpr int64_t kMxfMinRows = 65;
 
 // Workspace: x's planes, then the K slices of the many-row product.
 static size_t lin_x_bytes(const MxGeom &g, int32_t x_type, int64_t N, int32_t act) {
     const int P = act == VQK_MX_ACT_MXFP4 ? 1 : mx_planes(x_type);
     return al256(size_t(N) * g.NB * kMxBlock * 2 * P);
 }
-// 4-bit x for the 4-bit matrix instructions: rows of whole 256-wide chunks.
-static int64_t mxf_blocks(const MxGeom &g) { return (g.NB + 7) / 8 * 8; }
+// 4-bit x: rows of whole groups of four chunks.
+static int64_t mxf_blocks(const MxGeom &g) { return (g.NB + 15) / 16 * 16; }
 static size_t mxf_x_bytes(const MxGeom &g, int64_t N) { return al256(size_t(N) * mxf_blocks(g) * 17); }
-static bool lin_4bit(const vqk_mx_weights *w, const MxGeom &g, int64_t N, int32_t act) {
-    return act == VQK_MX_ACT_MXFP4 && N > kMxStreamRows && mxf_ok(w->scales, g.IN, N);
-}
-static size_t lin_bytes(const vqk_mx_weights *w, const MxGeom &g, int32_t x_type, int64_t N, int32_t act) {
-    if (lin_4bit(w, g, N, act)) return mxf_x_bytes(g, N) + mxf_part_bytes(N, g.OUT, g.NB);
-    return lin_x_bytes(g, x_type, N, act) + (N > kMxStreamRows ? mxg_part_bytes(N, g.OUT, g.NB) : 0);
+static bool lin_4bit(int64_t N, int32_t act) { return act == VQK_MX_ACT_MXFP4 && N >= kMxfMinRows; }
+static size_t lin_bytes(const MxGeom &g, int32_t x_type, int64_t N, int32_t act) {
+    if (lin_4bit(N, act)) return mxf_x_bytes(g, N) + mxf_part_bytes(N, g);
+    return lin_x_bytes(g, x_type, N, act) + mxg_part_bytes(N, g);
 }
 
 }  // namespace vqk
@@ -150,7 +152,7 @@ extern "C" int vqk_mx_linear_workspace(const vqk_mx_weights *w, int32_t x_type, 
     int rc = check_lin(w, x_type, N, &g, "mx linear");
     if (rc || (rc = check_act(act))) return rc;
     if (!bytes) return set_error(VQK_EINVAL, "mx linear: NULL bytes");
-    *bytes = lin_bytes(w, g, x_type, N, act);
+    *bytes = lin_bytes(g, x_type, N, act);
     return VQK_OK;
 }
 
@@ -165,35 +167,37 @@ extern "C" int vqk_mx_linear(const vqk_mx_weights *w, const void *x, int32_t x_t
     hipStream_t st = static_cast<hipStream_t>(stream);
     MxCall c{};
     c.codes[0] = w->codes; c.scales[0] = w->scales;
-    c.E = 1; c.OUT = g.OUT; c.IN = g.IN; c.NB = g.NB;
+    c.g = g;
     c.N = N; c.xkrep = 1;
     c.y = y; c.y_type = y_type; c.ldy = g.OUT;
     const bool place = act == VQK_MX_ACT_NONE && x_in_place(x, x_type, g.IN, g.IN);
-    const size_t need = lin_bytes(w, g, x_type, N, act);
-    if ((!place || N > kMxStreamRows) && need && (!workspace || ws_bytes < need))
+    c.x.P = act == VQK_MX_ACT_MXFP4 ? 1 : mx_planes(x_type);
+    const int nt = N <= 16 ? 1 : 2;
+    const bool stream_w = N <= kMxStreamRows && mx_rows_ok(c, nt);
+    const size_t need = lin_bytes(g, x_type, N, act);
+    if (!(place && stream_w) && need && (!workspace || ws_bytes < need))
         return set_error(VQK_ENOSPACE, "mx linear: workspace %zu < %zu", ws_bytes, need);
     if (reinterpret_cast<uintptr_t>(workspace) & 255)
         return set_error(VQK_EINVAL, "mx linear: workspace must be 256-byte aligned");
-    if (lin_4bit(w, g, N, act)) {
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    if (lin_4bit(N, act)) {
         const int64_t xNB = mxf_blocks(g);
-        uint8_t *xc = static_cast<uint8_t *>(workspace), *xsc = xc + size_t(N) * xNB * 16;
-        if ((rc = launch_mx_quant(x, x_type, N, g.IN, g.IN, xNB, xc, xsc, st))) return rc;
+        uint8_t *xsc = ws + size_t(N) * xNB * 16;
+        if ((rc = launch_mx_quant(x, x_type, N, g.IN, g.IN, xNB, true, ws, xsc, st))) return rc;
         const size_t xb = mxf_x_bytes(g, N);
-        const MxfCall f{w->codes, w->scales, g.OUT, g.NB, N, xNB, xc, xsc, y, y_type};
-        return mxf_gemm(f, need > xb ? reinterpret_cast<float *>(xc + xb) : nullptr, need - xb, st);
+        const MxfCall f{w->codes, w->scales, g, N, xNB, ws, xsc, y, y_type};
+        return mxf_gemm(f, need > xb ? reinterpret_cast<float *>(ws + xb) : nullptr, need - xb, st);
     }
     if (place) {
         c.x = MxX{static_cast<const uint16_t *>(x), g.IN, 0, 1};
     } else {
-        uint16_t *xs = static_cast<uint16_t *>(workspace);
+        uint16_t *xs = reinterpret_cast<uint16_t *>(ws);
         if ((rc = launch_mx_planes(x, x_type, N, g.IN, g.IN, act == VQK_MX_ACT_MXFP4, xs, st))) return rc;
-        c.x = MxX{xs, g.NB * kMxBlock, N * g.NB * kMxBlock,
-                  act == VQK_MX_ACT_MXFP4 ? 1 : mx_planes(x_type)};
+        c.x = MxX{xs, g.NB * kMxBlock, N * g.NB * kMxBlock, c.x.P};
     }
-    if (N <= kMxStreamRows) return mx_stream(c, N <= 16 ? 1 : (N <= 32 ? 2 : 4), st);
+    if (stream_w) return mx_rows(c, nt, st);
     const size_t xb = lin_x_bytes(g, x_type, N, act);
-    return mx_gemm(c, 128, need > xb ? reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + xb) : nullptr,
-                   need - xb, st);
+    return mx_gemm(c, mxg_dense_rows(N), need > xb ? reinterpret_cast<float *>(ws + xb) : nullptr, need - xb, st);
 }
 
 extern "C" int vqk_mx_linear_dx_workspace(const vqk_mx_weights *w, int32_t type, int64_t N, size_t *bytes) {
@@ -237,8 +241,8 @@ extern "C" int vqk_mx_linear_dx(const vqk_mx_weights *w, const void *dy, int32_t
         A = out;
     }
     uint16_t *wt = reinterpret_cast<uint16_t *>(ws + d.wt);
-    const DecTArgs t{w->codes, w->scales, g.OUT, g.IN, g.NB, d.KO, int32_t(d.P), wt};
-    const int64_t gy = (g.IN + 127) / 128;
+    const DecTArgs t{w->codes, w->scales, g.IN, g.RT, g.NC, d.KO, int32_t(d.P), wt};
+    const int64_t gy = g.NC;
     if (gy > 65535) return set_error(VQK_ENOTIMPL, "mx linear dx: IN=%lld", (long long)g.IN);
     hipLaunchKernelGGL(k_mx_dec_t, dim3(unsigned(d.KO / 64), unsigned(gy)), dim3(256), 0, st, t);
     if ((rc = hip_status(hipGetLastError(), "transposed decode launch"))) return rc;

@@ -24,7 +24,7 @@ static int mx_tile_rows(int64_t N, int64_t E) {
     return avg <= 12 ? 16 : (avg <= 24 ? 32 : (avg <= 80 ? 64 : 128));
 }
 static int run(const MxCall &c, int rows, hipStream_t st) {
-    return rows == 16 ? mx_stream(c, 1, st) : mx_gemm(c, rows, nullptr, 0, st);
+    return rows == 16 && mx_rows_ok(c, 1) ? mx_rows(c, 1, st) : mx_gemm(c, rows, nullptr, 0, st);
 }
 
 struct CombineArgs {
@@ -167,7 +167,7 @@ extern "C" int vqk_mx_switch(const vqk_mx_weights *w, const void *x, int32_t x_t
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     MxCall c{};
     c.codes[0] = w->codes; c.scales[0] = w->scales;
-    c.E = g.E; c.OUT = g.OUT; c.IN = g.IN; c.NB = g.NB;
+    c.g = g;
     c.N = N; c.xkrep = xkrep;
     c.y = y; c.y_type = y_type; c.ldy = g.OUT;
     if ((rc = make_x(x, x_type, T, g.IN, g.NB, reinterpret_cast<uint16_t *>(ws), &c.x, st))) return rc;
@@ -210,7 +210,7 @@ extern "C" int vqk_mx_experts(const vqk_mx_weights *gate, const vqk_mx_weights *
     MxCall c{};
     c.codes[0] = gate->codes; c.scales[0] = gate->scales;
     c.codes[1] = up->codes; c.scales[1] = up->scales;
-    c.E = g1.E; c.OUT = g1.OUT; c.IN = g1.IN; c.NB = g1.NB;
+    c.g = g1;
     c.N = p.N; c.xkrep = top_k;
     uint16_t *h = reinterpret_cast<uint16_t *>(ws + p.h);
     c.y = h; c.ldy = p.IP; c.yplane = p.N * p.IP; c.yp = p.P; c.ysorted = true;
@@ -220,7 +220,7 @@ extern "C" int vqk_mx_experts(const vqk_mx_weights *gate, const vqk_mx_weights *
     MxCall d = c;                              // the same routing, over the SwiGLU rows
     d.codes[0] = down->codes; d.scales[0] = down->scales;
     d.codes[1] = nullptr; d.scales[1] = nullptr;
-    d.OUT = g2.OUT; d.IN = g2.IN; d.NB = g2.NB;
+    d.g = g2;
     d.x = MxX{h, p.IP, p.N * p.IP, p.P};
     d.xkrep = 0;
     float *part = reinterpret_cast<float *>(ws + p.part);

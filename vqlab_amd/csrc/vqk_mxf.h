@@ -3,15 +3,14 @@
 // 32 x 32 outputs in the time that bf16 takes for 16.
 //
 // A workgroup of four waves takes 256 weight rows and 32 * BT x rows, a wave 64
-// weight rows and all of the x rows. k runs in chunks of 256 = 8 blocks; lane
-// group g = lane / 32 holds blocks 4g .. 4g+3 of its row, so that a step
-// multiplies one whole block per lane (16 bytes), the chunk's four scales are
-// one 32-bit load and the instruction picks the step's byte itself. Weights go
-// straight to registers; x pieces go global -> LDS without registers, piece p of
-// row n at p ^ (n / 2 % 8): the 16 rows of a read phase, two to 256 bytes, then
-// fall on 16 different bank groups.
-// Bound by the traffic from L2: a chunk of 256 x 32 BT outputs reads
-// 32 KB + 4 KB * BT for 256 * BT clocks of matrix work per SIMD.
+// weight rows and all of the x rows. k runs in groups of four chunks of 128; lane
+// group g = lane / 32 holds blocks 2g and 2g + 1 of each chunk, and a step
+// multiplies one block per lane (16 bytes). The four chunks' scales of a block
+// position are one 32-bit load, and the instruction picks the chunk's byte itself.
+// Weights go straight to registers in operand order; x pieces go global -> LDS
+// without registers, two chunks (128 bytes of a row) a stage, piece p of row n at
+// p ^ (n / 2 % 8): the 16 rows of a read phase, two to 256 bytes, then fall on 16
+// different bank groups.
 #pragma once
 
 #include <type_traits>
@@ -25,10 +24,10 @@ typedef int mxf_i8 __attribute__((ext_vector_type(8)));
 
 struct MxfArgs {
     const uint8_t *codes, *scales, *xcodes, *xscales;
-    int64_t OUT, NB, N, xNB;
+    int64_t OUT, N, xNB;
     void *y;
     int32_t y_type;
-    int32_t nob, nt, NC, splits, per;
+    int32_t RT, NC, nob, nt, splits, per;     // per: groups of four chunks in a K slice
     float *part;
 };
 
@@ -58,7 +57,8 @@ __global__ void __launch_bounds__(256, WPE) k_mxf_gemm(const MxfArgs p) {
     const int64_t row0 = int64_t(t % p.nt) * ROWS;
     const int nrows = int(min(int64_t(ROWS), p.N - row0));
     const int ow = t / p.nt * 256 + wave * 64;
-    const int c_lo = slice * p.per, c_hi = min(p.NC, c_lo + p.per);
+    const int NC4 = (p.NC + 3) / 4;
+    const int h_lo = 2 * slice * p.per, h_hi = min((p.NC + 1) / 2, h_lo + 2 * p.per);   // halves of a group
 
     f32x16f acc[2][BT];
 #pragma unroll
@@ -66,73 +66,106 @@ __global__ void __launch_bounds__(256, WPE) k_mxf_gemm(const MxfArgs p) {
 #pragma unroll
         for (int b = 0; b < BT; ++b) acc[a][b] = f32x16f{};
 
-    const uint8_t *wp[2], *sp[2];
+    uint32_t wo[2], so[2];                    // block 2g of this lane's row tile
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
-        const int64_t row = min(int64_t(ow + 32 * a + r), p.OUT - 1);
-        wp[a] = p.codes + row * p.NB * 16;
-        sp[a] = p.scales + row * p.NB;
+        const uint32_t rt = uint32_t(min((ow + 32 * a) / 16 + (r >> 4), p.RT - 1));
+        const uint32_t unit = uint32_t(2 * g * 16 + (r & 15));
+        wo[a] = (rt * uint32_t(p.NC) * 64 + unit) * 16;
+        so[a] = (rt * uint32_t(NC4) * 64 + unit) * 4;
     }
-    const uint8_t *src[CPW], *xsp[BT];
+    // x by 32-bit offsets from the tile's first row
+    const uint8_t *xc0 = p.xcodes + row0 * p.xNB * 16, *xs0 = p.xscales + row0 * p.xNB;
+    uint32_t src[CPW], xso[BT];
 #pragma unroll
     for (int j = 0; j < CPW; ++j) {
         const int n = (wave * CPW + j) * 8 + (lane >> 3);
-        src[j] = p.xcodes + (row0 + min(n, nrows - 1)) * p.xNB * 16 + ((lane & 7) ^ ((n >> 1) & 7)) * 16;
+        src[j] = uint32_t(min(n, nrows - 1)) * uint32_t(p.xNB) * 16 + ((lane & 7) ^ ((n >> 1) & 7)) * 16;
     }
 #pragma unroll
-    for (int b = 0; b < BT; ++b) xsp[b] = p.xscales + (row0 + min(32 * b + r, nrows - 1)) * p.xNB + 4 * g;
+    for (int b = 0; b < BT; ++b) xso[b] = uint32_t(min(32 * b + r, nrows - 1)) * uint32_t(p.xNB) + 8 * g;
 
-    u32x4 w[2][4], wn[2][4];
-    int ws[2], wsn[2], xsc[BT], xscn[BT];
-    auto issue = [&](int c, int buf) {
+    u32x4 w[2][4], wn[2][4];                  // [tile][2 * chunk of the half + block]
+    int ws[2][2], wsn[2][2], xsc[BT][2], xscn[BT][2];   // [..][block]: a group's scales
+    // half h: chunks 2h and 2h + 1. x is padded to whole groups; a weight chunk past the end is none
+    auto issue = [&](int h, int buf) {
 #pragma unroll
         for (int j = 0; j < CPW; ++j)
-            __builtin_amdgcn_global_load_lds((global_void *)(src[j] + int64_t(c) * 128),
+            __builtin_amdgcn_global_load_lds((global_void *)(xc0 + (src[j] + uint32_t(h) * 128u)),
                                              (lds_void *)(xs + buf * STAGE + (wave * CPW + j) * 1024), 16, 0, 0);
-        const int64_t blk = 8 * int64_t(c) + 4 * g;       // NB % 4 == 0: a lane's four blocks are in or out together
-        const bool in = blk < p.NB;
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-                wn[a][s] = in ? *reinterpret_cast<const u32x4 *>(wp[a] + (blk + s) * 16) : u32x4{};
-            wsn[a] = in ? *reinterpret_cast<const int *>(sp[a] + blk) : 0;
-        }
-#pragma unroll
-        for (int b = 0; b < BT; ++b) xscn[b] = *reinterpret_cast<const int *>(xsp[b] + 8 * int64_t(c));
-    };
-    const int at0 = r * 128, sw = (r >> 1) & 7;
-    auto step = [&](int buf, auto s_c) {
-        constexpr int S = decltype(s_c)::value;
-        const int at = at0 + ((4 * g + S) ^ sw) * 16;
-#pragma unroll
-        for (int b = 0; b < BT; ++b) {
-            const mxf_i8 xf = mxf_operand(*reinterpret_cast<const u32x4 *>(xs + buf * STAGE + b * 4096 + at));
+        for (int c = 0; c < 2; ++c) {
+            const uint32_t ch = uint32_t(min(2 * h + c, p.NC - 1));
 #pragma unroll
             for (int a = 0; a < 2; ++a)
-                acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mxf_operand(w[a][S]), xf, acc[a][b], 4, 4,
-                                                                            S, ws[a], S, xsc[b]);
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    wn[a][2 * c + q] = *reinterpret_cast<const u32x4 *>(p.codes + (wo[a] + ch * 1024u + q * 256u));
         }
     };
-    if (c_lo < c_hi) issue(c_lo, 0);
-#pragma unroll 1
-    for (int c = c_lo; c < c_hi; ++c) {
-        const int buf = (c - c_lo) & 1;
-        wait_vmem();
-        __syncthreads();                      // copies of chunk c are in; the other buffer is free
+    auto scales = [&](int grp) {
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+                wsn[a][q] = *reinterpret_cast<const int *>(p.scales + (so[a] + uint32_t(grp) * 256u + q * 64u));
+#pragma unroll
+            for (int b = 0; b < BT; ++b)
+                xscn[b][q] = *reinterpret_cast<const int *>(xs0 + (xso[b] + uint32_t(grp) * 16u + q * 4u));
+        }
+    };
+    const int at0 = r * 128, sw = (r >> 1) & 7;
+    auto half = [&](int h, auto odd) {
+        constexpr int ODD = decltype(odd)::value;
+        const int buf = h & 1;
+        wait_vmem();
+        __syncthreads();                      // copies of the half are in; the other buffer is free
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
 #pragma unroll
             for (int s = 0; s < 4; ++s) w[a][s] = wn[a][s];
-            ws[a] = wsn[a];
-        }
+        if (!ODD) {
 #pragma unroll
-        for (int b = 0; b < BT; ++b) xsc[b] = xscn[b];
-        if (c + 1 < c_hi) issue(c + 1, buf ^ 1);
-        step(buf, std::integral_constant<int, 0>{});
-        step(buf, std::integral_constant<int, 1>{});
-        step(buf, std::integral_constant<int, 2>{});
-        step(buf, std::integral_constant<int, 3>{});
+            for (int q = 0; q < 2; ++q) {
+#pragma unroll
+                for (int a = 0; a < 2; ++a) ws[a][q] = wsn[a][q];
+#pragma unroll
+                for (int b = 0; b < BT; ++b) xsc[b][q] = xscn[b][q];
+            }
+        }
+        if (h + 1 < h_hi) {
+            issue(h + 1, buf ^ 1);
+            if (ODD) scales(h / 2 + 1);
+        }
+        auto step = [&](auto c_c, auto q_c) {
+            constexpr int C = decltype(c_c)::value, Q = decltype(q_c)::value;
+            const int at = at0 + ((4 * C + 2 * g + Q) ^ sw) * 16;
+#pragma unroll
+            for (int b = 0; b < BT; ++b) {
+                const mxf_i8 xf = mxf_operand(*reinterpret_cast<const u32x4 *>(xs + buf * STAGE + b * 4096 + at));
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+                    acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                        mxf_operand(w[a][2 * C + Q]), xf, acc[a][b], 4, 4, 2 * ODD + C, ws[a][Q], 2 * ODD + C, xsc[b][Q]);
+            }
+        };
+        using c0 = std::integral_constant<int, 0>;
+        using c1 = std::integral_constant<int, 1>;
+        step(c0{}, c0{});
+        step(c0{}, c1{});
+        if (2 * h + 1 < p.NC) {
+            step(c1{}, c0{});
+            step(c1{}, c1{});
+        }
+    };
+    if (h_lo < h_hi) {                        // h_lo is even
+        issue(h_lo, 0);
+        scales(h_lo / 2);
+    }
+#pragma unroll 1
+    for (int h = h_lo; h < h_hi; h += 2) {
+        half(h, std::integral_constant<int, 0>{});
+        if (h + 1 < h_hi) half(h + 1, std::integral_constant<int, 1>{});
     }
 
     void *y = p.splits > 1 ? static_cast<void *>(p.part + int64_t(slice) * p.N * p.OUT) : p.y;

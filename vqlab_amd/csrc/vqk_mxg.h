@@ -5,10 +5,10 @@
 // SwiGLU pair) and a tile of 32 * BT x rows; a wave owns 64 weight rows and all
 // of the tile's x rows, so every weight is decoded by one wave only. Per chunk
 // of 128 k:
-//   * weights: 32 bytes per lane and 32-row tile straight from global memory.
-//     The sum over k has no order of its own, so lane group g = lane / 32 holds
-//     blocks 2g and 2g + 1 of the chunk and step (q, h) multiplies elements
-//     8h..8h+7 of block 2g + q: a lane decodes with one scale per block.
+//   * weights: 32 bytes per lane and 32-row tile straight from global memory,
+//     in operand order. Lane group g = lane / 32 holds blocks 2g and 2g + 1 of
+//     the chunk and step (q, h) multiplies elements 8h..8h+7 of block 2g + q: a
+//     lane decodes with one scale per block.
 //   * x: the tile's 256-byte row pieces, copied global -> LDS without registers
 //     (16 bytes a lane); piece p of row n is stored at p ^ (n & 15), so the 16
 //     rows of a read phase fall on 16 different bank groups.
@@ -75,12 +75,19 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
     bool nan[2] = {};
 
     if (tile.expert >= 0) {
-        const uint8_t *wp[2], *sp[2];
+        // unit of block 2g in this lane's row tile; the second block's is 16 further
+        const uint32_t NC = uint32_t(p.NC), NC4 = (NC + 3) / 4;
+        const uint8_t *cb[2], *sb[2];
+        uint32_t wo[2], so[2];
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
-            const int64_t row = tile.expert * p.OUT + min(int64_t(ow + (GLU ? 0 : 32 * a) + r), p.OUT - 1);
-            wp[a] = (GLU && a ? p.codes1 : p.codes0) + row * p.NB * 16;
-            sp[a] = (GLU && a ? p.scales1 : p.scales0) + row * p.NB;
+            const int m = GLU ? a : 0;
+            cb[a] = p.codes[m] + int64_t(tile.expert) * mx_expert_codes(p.RT, p.NC);
+            sb[a] = p.scales[m] + int64_t(tile.expert) * mx_expert_scales(p.RT, p.NC);
+            const uint32_t rt = uint32_t(min((ow + (GLU ? 0 : 32 * a)) / 16 + (r >> 4), p.RT - 1));
+            const uint32_t unit = uint32_t(2 * g * 16 + (r & 15));
+            wo[a] = (rt * NC * 64 + unit) * 16;
+            so[a] = (rt * NC4 * 64 + unit) * 4;
         }
         // the x copies of this lane: 16 bytes of one row each
         const uint16_t *src[CPW];
@@ -89,13 +96,13 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
         for (int j = 0; j < CPW; ++j) {
             const int n = (wave * CPW + j) * 4 + (lane >> 4);
             piece[j] = (lane & 15) ^ (n & 15);
-            src[j] = p.x + mx_x_row(p, tile.row0 + min(n, tile.nrows - 1)) * p.xld + piece[j] * 8;
+            src[j] = p.x + int64_t(mx_x_row(p, tile.row0 + min(n, tile.nrows - 1))) * p.xld + piece[j] * 8;
         }
         auto issue = [&](int c, int pl, int buf) {
 #pragma unroll
             for (int j = 0; j < CPW; ++j) {
                 // past the row's last block: the row's start again (multiplied by no weight, masked below)
-                const bool in = 4 * int64_t(c) + piece[j] / 4 < p.NB;
+                const bool in = 4 * c + piece[j] / 4 < p.NB;
                 const uint16_t *s = src[j] + pl * p.xplane + (in ? int64_t(c) * kMxChunk : -int64_t(piece[j] * 8));
                 __builtin_amdgcn_global_load_lds((global_void *)s,
                                                  (lds_void *)(xs + buf * STAGE + (wave * CPW + j) * 1024), 16, 0, 0);
@@ -108,14 +115,12 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
             for (int a = 0; a < 2; ++a)
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    const int64_t blk = 4 * int64_t(c) + 2 * g + q;
-                    const bool in = blk < p.NB;
-                    ww[a][q] = in ? *reinterpret_cast<const u32x4 *>(wp[a] + blk * 16) : u32x4{};
-                    ss[a][q] = in ? sp[a][blk] : 127u;
+                    ww[a][q] = *reinterpret_cast<const u32x4 *>(cb[a] + (wo[a] + uint32_t(c) * 1024u + q * 256u));
+                    ss[a][q] = sb[a][so[a] + uint32_t(c / 4) * 256u + q * 64u + uint32_t(c % 4)];
                 }
         };
         auto mul = [&](int c, int buf) {
-            const bool tail = 4 * int64_t(c) + 4 > p.NB;
+            const bool tail = 4 * c + 4 > p.NB;
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 float sc[2];
@@ -124,7 +129,7 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
                     nan[a] = nan[a] || s[a][q] == 255u;
                     sc[a] = mx_scale(s[a][q] == 255u ? 127u : s[a][q]);
                 }
-                const bool in = !tail || 4 * int64_t(c) + 2 * g + q < p.NB;
+                const bool in = !tail || 4 * c + 2 * g + q < p.NB;
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
                     mx_b8 wf[2];

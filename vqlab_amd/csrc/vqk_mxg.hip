@@ -48,10 +48,16 @@ int mxg_splits(int64_t T, int64_t NC) {
 
 static int mxg_bt(int64_t rows) { return rows <= 32 ? 1 : (rows <= 64 ? 2 : 4); }
 
-size_t mxg_part_bytes(int64_t N, int64_t OUT, int64_t NB) {
-    const int64_t T = ((N + 127) / 128) * ((OUT + kMxgRows - 1) / kMxgRows);
-    const int s = mxg_splits(T, (NB + 3) / 4);
-    return s > 1 ? size_t(s) * N * OUT * 4 : 0;
+static int dense_splits(int64_t N, const MxGeom &g) {
+    const int rows = mxg_dense_rows(N);
+    return mxg_splits(((N + rows - 1) / rows) * ((g.OUT + kMxgRows - 1) / kMxgRows), g.NC);
+}
+
+int mxg_dense_rows(int64_t N) { return N <= 32 ? 32 : (N <= 64 ? 64 : 128); }
+
+size_t mxg_part_bytes(int64_t N, const MxGeom &g) {
+    const int s = dense_splits(N, g);
+    return s > 1 ? size_t(s) * N * g.OUT * 4 : 0;
 }
 
 template <int BT, bool GLU, bool PL>
@@ -82,10 +88,9 @@ int mx_gemm(const MxCall &c, int tile_rows, float *part, size_t part_bytes, hipS
     if (tiles == 0) return VQK_OK;
     ga.splits = 1;
     ga.per = ga.a.NC;
-    if (part && !c.meta && !glu) {
-        const int64_t T = tiles * ((c.OUT + kMxgRows - 1) / kMxgRows);
-        const int s = mxg_splits(T, ga.a.NC);
-        if (s > 1 && size_t(s) * c.N * c.OUT * 4 <= part_bytes) {
+    if (part && !c.meta && !c.ids && !glu) {
+        const int s = dense_splits(c.N, c.g);
+        if (s > 1 && size_t(s) * c.N * c.g.OUT * 4 <= part_bytes) {
             ga.per = int32_t((ga.a.NC + s - 1) / s);
             ga.splits = int32_t((ga.a.NC + ga.per - 1) / ga.per);
             ga.part = part;

@@ -1,42 +1,49 @@
-// Products of MXFP4 weights with a few rows at a time: each weight is read
-// once for up to 16 * NT rows.
+// Products of MXFP4 weights with few rows of x: the weights are streamed once
+// past up to 16 * NT rows.
 //
 //     y[n, o] = sum_k x[n, k] * W[o, k]
 //
-// A workgroup takes 16 * MT weight rows (of each projection of a SwiGLU pair)
-// and a tile of x rows; its waves split k by chunks of 128 (wave w takes
-// chunks w, w + NW, ...: side by side they read whole lines of a row) and
-// their fp32 sums meet in LDS, added in wave order. Weights go from global
-// memory to matrix-core operands in registers (vqk_mx.h); x pieces come from
-// L2 in the same order, so nothing is staged. Bound by the weight stream: a
-// wave decodes and multiplies a 16 x 128 piece (1088 bytes) in ~100 cycles,
-// several times the rate at which HBM delivers them.
+// A workgroup keeps its tile of x in registers and walks over weight rows, so
+// its loop is the weight stream and little else. Eight waves: KW along k, NCW
+// chunks of 128 each (x takes 16 * NCW * NT * P registers), and 8 / KW along the
+// weight rows, 16 a step. The next step's weights (16 bytes a lane and chunk, a
+// contiguous KB a wave) load while the last ones are decoded and multiplied. The
+// fp32 sums of KW > 1 waves meet in LDS in wave order, two buffers in turn, one
+// barrier a step.
+// x comes straight from its rows where a tile has at most two, and otherwise
+// through LDS, copied in whole lines and read in operand order (16 rows read
+// directly cost 64 L1 cycles a load: 8 us of a 20-row product).
+// Bound by HBM: a wave decodes and multiplies a 16 x 128 piece (1088 bytes) in
+// ~100 cycles, several times the rate at which it can arrive.
 #pragma once
 
 #include "vqk_mx.h"
 
 namespace vqk {
 
-constexpr int kMxsMaxWaves = 8;
+constexpr int kMxsWaves = 8;
 
 struct MxsArgs {
-    const uint8_t *codes0, *scales0, *codes1, *scales1;
-    int64_t NB, OUT, E;
-    int32_t NC, nob;                          // chunks of k; output blocks of 16 * MT rows
+    const uint8_t *codes[2], *scales[2];
+    int64_t OUT, E;
+    int32_t RT, NC, NB;
     const uint16_t *x;
     int64_t xld, xplane;
-    int64_t N, xkrep;
+    int64_t N;
+    int32_t xkrep;
     const int32_t *ids, *order, *meta, *ntiles;
     void *y;
     int32_t y_type, yp, ysorted;
     int64_t ldy, yplane, ocover;              // columns of y to write (OUT, or its padding to whole blocks)
+    int32_t nob;                              // workgroups per tile
+    // k_mx_rows: waves along k, row steps per workgroup and in all, x through LDS
+    int32_t kw, steps, total_steps, stage;
 };
 
 // Rows of x that a tile multiplies, and where they lie.
 struct MxTile {
-    int64_t expert;                           // < 0: no expert (rows of zeros)
-    int64_t row0;
-    int nrows;
+    int expert;                               // < 0: none (rows of zeros)
+    int row0, nrows;
 };
 template <int ROWS>
 __device__ __forceinline__ bool mx_tile(const MxsArgs &p, int t, MxTile *out) {
@@ -45,122 +52,199 @@ __device__ __forceinline__ bool mx_tile(const MxsArgs &p, int t, MxTile *out) {
         *out = MxTile{p.meta[3 * t], p.meta[3 * t + 1], p.meta[3 * t + 2]};
         if (out->nrows < 1) return false;
     } else if (p.ids) {
-        const int64_t e = p.ids[t];
+        const int e = p.ids[t];
         *out = MxTile{e >= 0 && e < p.E ? e : -1, t, 1};
     } else {
-        const int64_t r = int64_t(t) * ROWS;
+        const int r = t * ROWS;
         *out = MxTile{0, r, int(min(int64_t(ROWS), p.N - r))};
     }
+    out->expert = __builtin_amdgcn_readfirstlane(out->expert);
+    out->row0 = __builtin_amdgcn_readfirstlane(out->row0);
+    out->nrows = __builtin_amdgcn_readfirstlane(out->nrows);
     return true;
 }
-__device__ __forceinline__ int64_t mx_x_row(const MxsArgs &p, int64_t pos) {
+__device__ __forceinline__ int mx_x_row(const MxsArgs &p, int pos) {
     if (p.xkrep == 0) return pos;
-    const int64_t pair = p.meta ? p.order[pos] : pos;
-    return p.xkrep == 1 ? pair : pair / p.xkrep;
+    const int pair = p.meta ? p.order[pos] : pos;
+    return p.xkrep == 1 ? pair : int(uint32_t(pair) / uint32_t(p.xkrep));
 }
-__device__ __forceinline__ int64_t mx_y_row(const MxsArgs &p, int64_t pos) {
+__device__ __forceinline__ int mx_y_row(const MxsArgs &p, int pos) {
     return p.meta && !p.ysorted ? p.order[pos] : pos;
 }
 
-template <int NT, int MT, bool GLU, int P>
-__global__ void __launch_bounds__(64 * kMxsMaxWaves) k_mx_stream(const MxsArgs p) {
-    constexpr int TT = GLU ? 2 * MT : MT;
-    extern __shared__ __align__(16) float red[];      // [waves][TT * NT][256]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, NW = blockDim.x >> 6;
+template <int NT, int P, int NCW, bool GLU>
+__global__ void __launch_bounds__(64 * kMxsWaves, 2) k_mx_rows(const MxsArgs p) {
+    constexpr int TT = GLU ? 2 : 1;
+    // sums [2][8 waves][TT * NT][256] floats (KW > 1); before them x, [8 waves][16 rows][NCW * 256 bytes]
+    extern __shared__ __align__(16) uint8_t smem[];
+    float *red = reinterpret_cast<float *>(smem);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 15, g = lane >> 4;
-    const int ob = int(blockIdx.x % unsigned(p.nob)), t = int(blockIdx.x / unsigned(p.nob));
+    const int KW = p.kw, RW = kMxsWaves / KW;
+    const int kw = wave % KW, rw = wave / KW;
+    const int t = int(blockIdx.x / unsigned(p.nob)), part = int(blockIdx.x % unsigned(p.nob));
     MxTile tile;
     if (!mx_tile<16 * NT>(p, t, &tile)) return;
-    const int o0 = ob * 16 * MT;
+    const int s_lo = part * p.steps, s_hi = min(p.total_steps, s_lo + p.steps);
+    if (s_lo >= s_hi) return;
 
-    f32x4 acc[TT][NT];
+    const bool live = tile.expert >= 0;
+    const int64_t ex = live ? tile.expert : 0;
+    const uint8_t *cb[2], *sb[2];
 #pragma unroll
-    for (int a = 0; a < TT; ++a)
+    for (int a = 0; a < 2; ++a) {
+        cb[a] = p.codes[a] + ex * mx_expert_codes(p.RT, p.NC);
+        sb[a] = p.scales[a] + ex * mx_expert_scales(p.RT, p.NC);
+    }
+    // this wave's chunks: kw * NCW ..; past the last one the last stands in, against x of zero
+    const uint32_t NC = uint32_t(p.NC), NC4 = (NC + 3) / 4;
+    u32x4 w[TT][NCW], wn[TT][NCW];
+    uint32_t sc[TT][NCW], scn[TT][NCW];
+    auto load_w = [&](int step) {
+        const uint32_t rt = uint32_t(min(step * RW + rw, p.RT - 1));
 #pragma unroll
-        for (int b = 0; b < NT; ++b) acc[a][b] = f32x4{};
-    bool nan[TT] = {};
-    if (tile.expert >= 0) {
-        const uint8_t *wp[TT], *sp[TT];
+        for (int a = 0; a < TT; ++a)
 #pragma unroll
-        for (int a = 0; a < TT; ++a) {
-            const int64_t row = tile.expert * p.OUT + min(int64_t(o0 + (a % MT) * 16 + r), p.OUT - 1);
-            wp[a] = (a < MT ? p.codes0 : p.codes1) + row * p.NB * 16;
-            sp[a] = (a < MT ? p.scales0 : p.scales1) + row * p.NB;
-        }
-        const uint16_t *xp[NT];
-#pragma unroll
-        for (int b = 0; b < NT; ++b)
-            xp[b] = p.x + mx_x_row(p, tile.row0 + min(b * 16 + r, tile.nrows - 1)) * p.xld;
-        for (int c = wave; c < p.NC; c += NW) {
-            const int64_t blk = 4 * c + g;
-            const bool ok = blk < p.NB;
-            u32x4 w[TT];
-            uint32_t s[TT];
-#pragma unroll
-            for (int a = 0; a < TT; ++a) {
-                w[a] = ok ? *reinterpret_cast<const u32x4 *>(wp[a] + blk * 16) : u32x4{};
-                s[a] = ok ? sp[a][blk] : 127u;
+            for (int c = 0; c < NCW; ++c) {
+                const uint32_t ch = min(uint32_t(kw * NCW + c), NC - 1);
+                wn[a][c] = *reinterpret_cast<const u32x4 *>(cb[a] + ((rt * NC + ch) * 64 + lane) * 16u);
+                scn[a][c] = sb[a][((rt * NC4 + ch / 4) * 64 + lane) * 4 + ch % 4];
             }
-            u32x4 xf[P][NT][4];
+    };
+    load_w(s_lo);
+
+    u32x4 xf[P][NT][NCW][4];
+    auto x_in = [&](int c) { return 4 * (kw * NCW + c) + g < p.NB; };   // this lane's block of x exists
+    if (p.stage) {
+        uint8_t *xl = smem + wave * (NCW * 4096);
+#pragma unroll
+        for (int pl = 0; pl < P; ++pl)
+#pragma unroll
+            for (int b = 0; b < NT; ++b) {
+#pragma unroll
+                for (int i = 0; i < 4 * NCW; ++i) {
+                    // LDS unit i * 64 + lane: row / 16-byte slot; the slot holds piece slot ^ row of the
+                    // wave's part of that row (past the row's end its start: zeroed below)
+                    const int u = i * 64 + lane, row = u / (16 * NCW), piece = (u % (16 * NCW)) ^ row;
+                    const int64_t k = int64_t(kw) * NCW * kMxChunk + piece * 8;
+                    const int pos = tile.row0 + min(b * 16 + row, tile.nrows - 1);
+                    const uint16_t *src = p.x + pl * p.xplane + int64_t(mx_x_row(p, pos)) * p.xld +
+                                          (k < int64_t(p.NB) * kMxBlock ? k : 0);
+                    __builtin_amdgcn_global_load_lds((global_void *)src, (lds_void *)(xl + i * 1024), 16, 0, 0);
+                }
+                wait_vmem();
+#pragma unroll
+                for (int c = 0; c < NCW; ++c)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const u32x4 v = *reinterpret_cast<const u32x4 *>(
+                            xl + r * (NCW * 256) + (((c * 16 + g * 4 + k) ^ r) << 4));
+                        xf[pl][b][c][k] = live && x_in(c) && b * 16 + r < tile.nrows ? v : u32x4{};
+                    }
+                __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): read before the next rows land
+            }
+        __syncthreads();                      // the sums use the same LDS
+    } else {
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
+            const bool row_in = live && b * 16 + r < tile.nrows;
+            const uint16_t *xp = p.x + (row_in ? int64_t(mx_x_row(p, tile.row0 + b * 16 + r)) : 0) * p.xld;
 #pragma unroll
             for (int pl = 0; pl < P; ++pl)
 #pragma unroll
-                for (int b = 0; b < NT; ++b)
+                for (int c = 0; c < NCW; ++c)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        xf[pl][b][k] = ok ? *reinterpret_cast<const u32x4 *>(xp[b] + pl * p.xplane +
-                                                                             blk * kMxBlock + 8 * k)
-                                          : u32x4{};
+                        xf[pl][b][c][k] = row_in && x_in(c)
+                            ? *reinterpret_cast<const u32x4 *>(xp + pl * p.xplane +
+                                                               (4 * (kw * NCW + c) + g) * kMxBlock + 8 * k)
+                            : u32x4{};
+        }
+    }
+
+    for (int step = s_lo; step < s_hi; ++step) {
 #pragma unroll
-            for (int a = 0; a < TT; ++a) {
-                nan[a] = nan[a] || s[a] == 255u;
-                const float sc = mx_scale(s[a] == 255u ? 127u : s[a]);
+        for (int a = 0; a < TT; ++a)
+#pragma unroll
+            for (int c = 0; c < NCW; ++c) {
+                w[a][c] = wn[a][c];
+                sc[a][c] = scn[a][c];
+            }
+        if (step + 1 < s_hi) load_w(step + 1);
+        f32x4 acc[TT][NT];
+#pragma unroll
+        for (int a = 0; a < TT; ++a) {
+            bool nan = false;
+#pragma unroll
+            for (int b = 0; b < NT; ++b) acc[a][b] = f32x4{};
+#pragma unroll
+            for (int c = 0; c < NCW; ++c) {
+                const bool bad = sc[a][c] == 255u;
+                nan = nan || bad;             // a chunk that stands in is of the same row
+                const float s = mx_scale(bad ? 127u : sc[a][c]);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const mx_b8 wf = __builtin_bit_cast(mx_b8, mx_decode8(w[a][k], sc));
+                    const mx_b8 wf = __builtin_bit_cast(mx_b8, mx_decode8(w[a][c][k], s));
 #pragma unroll
                     for (int pl = 0; pl < P; ++pl)
 #pragma unroll
                         for (int b = 0; b < NT; ++b)
                             acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                __builtin_bit_cast(mx_b8, xf[pl][b][k]), wf, acc[a][b], 0, 0, 0);
+                                __builtin_bit_cast(mx_b8, xf[pl][b][c][k]), wf, acc[a][b], 0, 0, 0);
                 }
             }
-        }
-    }
-    // a NaN block makes its whole output column NaN: any of the column's four lane groups may hold it
+            // a NaN block makes its whole output column NaN, whichever of its lane groups holds it
+            if (__ballot(nan && live)) {
+                int f = nan && live;
+                f |= __shfl_xor(f, 16);
+                f |= __shfl_xor(f, 32);
 #pragma unroll
-    for (int a = 0; a < TT; ++a) {
-        int f = nan[a];
-        f |= __shfl_xor(f, 16);
-        f |= __shfl_xor(f, 32);
-        if (f) {
+                for (int b = 0; b < NT; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[a][b][i] = f ? __uint_as_float(0x7fc00000u) : acc[a][b][i];
+            }
+        }
+        auto put = [&](int row, int o, float v, float u) {
+            const int64_t yr = mx_y_row(p, tile.row0 + row);
+            if constexpr (GLU) {
+                float h = o < p.OUT ? v / (1.f + __expf(-v)) * u : 0.f;
+                for (int pl = 0; pl < p.yp; ++pl)
+                    static_cast<uint16_t *>(p.y)[pl * p.yplane + yr * p.ldy + o] = mx_plane_next(h);
+            } else {
+                store_act(p.y, p.y_type, yr * p.ldy + o, v);
+            }
+        };
+        if (KW == 1) {
+            // register i of lane l: x row 4 * (l / 16) + i, weight row l % 16
+            const int o = (step * RW + rw) * 16 + r;
 #pragma unroll
             for (int b = 0; b < NT; ++b)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[a][b][i] = __uint_as_float(0x7fc00000u);
+                for (int i = 0; i < 4; ++i)
+                    if (b * 16 + 4 * g + i < tile.nrows && o < p.ocover)
+                        put(b * 16 + 4 * g + i, o, acc[0][b][i], acc[TT - 1][b][i]);
+            continue;
         }
+        float *buf = red + (step & 1) * kMxsWaves * TT * NT * 256;
 #pragma unroll
-        for (int b = 0; b < NT; ++b)
-            *reinterpret_cast<f32x4 *>(red + ((wave * TT + a) * NT + b) * 256 + lane * 4) = acc[a][b];
-    }
-    __syncthreads();
-    // element (m, n) of a tile: lane (m / 4) * 16 + n, register m % 4
-    for (int e = threadIdx.x; e < MT * NT * 256; e += blockDim.x) {
-        const int n = e & 15, a = (e >> 4) % MT, m = (e >> 4) / MT % 16, b = (e >> 8) / MT;
-        const int row = b * 16 + m, o = o0 + a * 16 + n;
-        if (row >= tile.nrows || o >= p.ocover) continue;
-        const int off = ((m >> 2) * 16 + n) * 4 + (m & 3);
-        float v = 0.f, u = 0.f;
-        for (int w = 0; w < NW; ++w) v += red[((w * TT + a) * NT + b) * 256 + off];
-        const int64_t yr = mx_y_row(p, tile.row0 + row);
-        if constexpr (GLU) {
-            for (int w = 0; w < NW; ++w) u += red[((w * TT + MT + a) * NT + b) * 256 + off];
-            float h = o < p.OUT ? v / (1.f + __expf(-v)) * u : 0.f;
-            for (int pl = 0; pl < p.yp; ++pl)
-                static_cast<uint16_t *>(p.y)[pl * p.yplane + yr * p.ldy + o] = mx_plane_next(h);
-        } else {
-            store_act(p.y, p.y_type, yr * p.ldy + o, v);
+        for (int a = 0; a < TT; ++a)
+#pragma unroll
+            for (int b = 0; b < NT; ++b)
+                *reinterpret_cast<f32x4 *>(buf + ((wave * TT + a) * NT + b) * 256 + lane * 4) = acc[a][b];
+        __syncthreads();
+        // outputs (x row, weight row) of the step, weight rows fastest
+        const int n_out = 16 * RW;
+        for (int e = threadIdx.x; e < n_out * min(tile.nrows, 16 * NT); e += 64 * kMxsWaves) {
+            const int row = e / n_out, c = e - row * n_out, n = c & 15, m = row & 15, b = row >> 4;
+            const int o = step * n_out + c;
+            if (o >= p.ocover) continue;
+            const float *src = buf + ((c >> 4) * KW * TT * NT + b) * 256 + ((m >> 2) * 16 + n) * 4 + (m & 3);
+            float v = 0.f, u = 0.f;
+            for (int k = 0; k < KW; ++k) {
+                v += src[k * TT * NT * 256];
+                if constexpr (GLU) u += src[(k * TT + 1) * NT * 256];
+            }
+            put(row, o, v, u);
         }
     }
 }
@@ -168,7 +252,8 @@ __global__ void __launch_bounds__(64 * kMxsMaxWaves) k_mx_stream(const MxsArgs p
 // Kernel arguments of a call, and the tiles of `rows` x rows that it makes.
 void mx_args(const MxCall &c, MxsArgs *a);
 int64_t mx_tiles(const MxCall &c, int rows);
-// Launches k_mx_stream for a call; NT row tiles of 16.
-int mx_stream(const MxCall &c, int NT, hipStream_t st);
+// Whether k_mx_rows takes a call in tiles of 16 * NT rows; its launch.
+bool mx_rows_ok(const MxCall &c, int NT);
+int mx_rows(const MxCall &c, int NT, hipStream_t st);
 
 }  // namespace vqk

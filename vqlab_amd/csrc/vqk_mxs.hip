@@ -3,64 +3,91 @@
 
 namespace vqk {
 
-template <int NT, int MT, bool GLU, int P>
-static int go(MxsArgs a, int64_t tiles, hipStream_t st) {
-    const int64_t cover = a.ocover;
-    a.nob = int32_t((cover + 16 * MT - 1) / (16 * MT));
-    const int64_t grid = int64_t(a.nob) * tiles;
-    if (grid > INT32_MAX) return set_error(VQK_ENOTIMPL, "MXFP4 product: grid too large");
-    int nw = 1;                               // no wave without a chunk of k
-    while (nw < kMxsMaxWaves && nw < a.NC) nw *= 2;
-    const size_t lds = size_t(nw) * (GLU ? 2 : 1) * MT * NT * 1024;
-    return launch_with_lds<k_mx_stream<NT, MT, GLU, P>>(dim3(unsigned(grid)), dim3(64 * nw), lds, st, a);
-}
-
-template <int NT, int MT, bool GLU>
-static int go_p(const MxsArgs &a, int P, int64_t tiles, hipStream_t st) {
-    switch (P) {
-        case 1: return go<NT, MT, GLU, 1>(a, tiles, st);
-        case 2: return go<NT, MT, GLU, 2>(a, tiles, st);
-        default: return go<NT, MT, GLU, 3>(a, tiles, st);
-    }
-}
-
 void mx_args(const MxCall &c, MxsArgs *a) {
     *a = MxsArgs{};
-    a->codes0 = c.codes[0]; a->scales0 = c.scales[0];
-    a->codes1 = c.codes[1]; a->scales1 = c.scales[1];
-    a->NB = c.NB; a->OUT = c.OUT; a->E = c.E;
-    a->NC = int32_t((c.NB + 3) / 4);
+    for (int i = 0; i < 2; ++i) {
+        a->codes[i] = c.codes[i];
+        a->scales[i] = c.scales[i];
+    }
+    a->OUT = c.g.OUT; a->E = c.g.E;
+    a->RT = int32_t(c.g.RT); a->NC = int32_t(c.g.NC); a->NB = int32_t(c.g.NB);
     a->x = c.x.x; a->xld = c.x.ld; a->xplane = c.x.plane;
-    a->N = c.N; a->xkrep = c.xkrep;
+    a->N = c.N; a->xkrep = int32_t(c.xkrep);
     a->ids = c.ids; a->order = c.order; a->meta = c.meta; a->ntiles = c.ntiles;
     a->y = c.y; a->y_type = c.y_type; a->yp = c.yp; a->ysorted = c.ysorted;
     a->ldy = c.ldy; a->yplane = c.yplane;
-    a->ocover = c.codes[1] ? c.ldy : c.OUT;
+    a->ocover = c.codes[1] ? c.ldy : c.g.OUT;
 }
 
 int64_t mx_tiles(const MxCall &c, int rows) {
     if (c.ids) return c.N;
     const int64_t full = (c.N + rows - 1) / rows;
-    return c.meta ? full + (c.N < c.E + 1 ? c.N : c.E + 1) : full;
+    return c.meta ? full + (c.N < c.g.E + 1 ? c.N : c.g.E + 1) : full;
 }
 
-int mx_stream(const MxCall &c, int NT, hipStream_t st) {
+// Chunks per wave that the registers hold: 16 per chunk and x operand, 9 for two
+// buffers of weights, 210 in all.
+constexpr int rows_cap(int xn, bool glu) { return 210 / (16 * xn + (glu ? 18 : 9)); }
+
+// Waves along k and chunks per wave, or kw = 0 where x does not fit.
+struct RowsPlan { int kw, ncw; };
+static RowsPlan rows_plan(int64_t NC, int xn, bool glu) {
+    const int cap = rows_cap(xn, glu);
+    // about four chunks a wave keep enough weights in flight; fewer waves along k save the sums
+    int kw = 1;
+    while (kw < kMxsWaves && (NC + kw - 1) / kw > (cap < 4 ? cap : 4)) kw *= 2;
+    const int64_t ncw = (NC + kw - 1) / kw;
+    return ncw <= cap ? RowsPlan{kw, int(ncw)} : RowsPlan{0, 0};
+}
+
+bool mx_rows_ok(const MxCall &c, int NT) {
+    return (NT == 1 || (NT == 2 && c.x.P == 1)) && rows_plan(c.g.NC, NT * c.x.P, c.codes[1] != nullptr).kw > 0;
+}
+
+template <int NT, int P, int NCW, bool GLU>
+static int go(MxsArgs a, int64_t tiles, int kw, hipStream_t st) {
+    const int RW = kMxsWaves / kw;
+    a.kw = kw;
+    a.total_steps = int32_t((a.ocover + 16 * RW - 1) / (16 * RW));
+    // row steps per workgroup: long walks, while every CU gets two workgroups
+    const int64_t want = tiles > 0 ? (512 + tiles - 1) / tiles : 1;
+    int64_t steps = a.total_steps / (want < 1 ? 1 : want);
+    steps = steps < 1 ? 1 : (steps > 8 ? 8 : steps);
+    a.steps = int32_t(steps);
+    a.nob = int32_t((a.total_steps + steps - 1) / steps);
+    const int64_t grid = int64_t(a.nob) * tiles;
+    if (grid > INT32_MAX) return set_error(VQK_ENOTIMPL, "MXFP4 product: grid too large");
+    // dense tiles of more than two rows; sorted ones hold few as long as this kernel takes them
+    a.stage = !a.ids && !a.meta && a.N > 2;
+    const size_t sums = kw > 1 ? size_t(2) * kMxsWaves * (GLU ? 2 : 1) * NT * 1024 : 0;
+    const size_t xl = a.stage ? size_t(kMxsWaves) * NCW * 4096 : 0;
+    return launch_with_lds<k_mx_rows<NT, P, NCW, GLU>>(dim3(unsigned(grid)), dim3(64 * kMxsWaves),
+                                                       sums > xl ? sums : xl, st, a);
+}
+
+template <int NT, int P, bool GLU, int NCW = 1>
+static int go_ncw(const MxsArgs &a, int64_t tiles, RowsPlan pl, hipStream_t st) {
+    if (pl.ncw == NCW) return go<NT, P, NCW, GLU>(a, tiles, pl.kw, st);
+    if constexpr (NCW < rows_cap(NT * P, GLU)) return go_ncw<NT, P, GLU, NCW + 1>(a, tiles, pl, st);
+    return set_error(VQK_EINVAL, "MXFP4 product: no instance of %d chunks", pl.ncw);
+}
+template <int NT, int P>
+static int go_glu(const MxsArgs &a, bool glu, int64_t tiles, RowsPlan pl, hipStream_t st) {
+    return glu ? go_ncw<NT, P, true>(a, tiles, pl, st) : go_ncw<NT, P, false>(a, tiles, pl, st);
+}
+
+int mx_rows(const MxCall &c, int NT, hipStream_t st) {
     const bool glu = c.codes[1] != nullptr;
     MxsArgs a;
     mx_args(c, &a);
     const int64_t tiles = mx_tiles(c, 16 * NT);
     if (tiles == 0) return VQK_OK;
-    if (glu) {
-        switch (NT) {
-            case 1: return go_p<1, 1, true>(a, c.x.P, tiles, st);
-            case 2: return go_p<2, 1, true>(a, c.x.P, tiles, st);
-            default: return go_p<4, 1, true>(a, c.x.P, tiles, st);
-        }
-    }
-    switch (NT) {
-        case 1: return go_p<1, 1, false>(a, c.x.P, tiles, st);
-        case 2: return go_p<2, 2, false>(a, c.x.P, tiles, st);
-        default: return go_p<4, 2, false>(a, c.x.P, tiles, st);
+    const RowsPlan pl = rows_plan(c.g.NC, NT * c.x.P, glu);
+    if (NT == 2) return go_glu<2, 1>(a, glu, tiles, pl, st);
+    switch (c.x.P) {
+        case 1: return go_glu<1, 1>(a, glu, tiles, pl, st);
+        case 2: return go_glu<1, 2>(a, glu, tiles, pl, st);
+        default: return go_glu<1, 3>(a, glu, tiles, pl, st);
     }
 }
 

@@ -93,6 +93,20 @@ def _desc(codes, scales, E, OUT, IN):
     return L.VQKMXWeights(codes.data_ptr(), scales.data_ptr(), E, OUT, IN)
 
 
+def _pack(codes, scales, E, OUT, IN):
+    """Codes and scales of E weights in the kernels' operand order (laid out once)."""
+    T.require_cuda(codes, scales)
+    nc, ns = ctypes.c_size_t(), ctypes.c_size_t()
+    L.check(L.lib().vqk_mx_pack_bytes(E, OUT, IN, ctypes.byref(nc), ctypes.byref(ns)), "MXFP4 weight")
+    with T.on_device(codes):
+        codes, scales = _aligned(codes, 16), scales.contiguous()
+        pc = torch.empty(nc.value, dtype=torch.uint8, device=codes.device)
+        ps = torch.empty(ns.value, dtype=torch.uint8, device=codes.device)
+        L.check(L.lib().vqk_mx_pack(codes.data_ptr(), scales.data_ptr(), E, OUT, IN, pc.data_ptr(),
+                                    ps.data_ptr(), T.stream(codes.device)), "MXFP4 weight")
+    return pc, ps
+
+
 def _work(query, dev, *args):
     ws = ctypes.c_size_t()
     L.check(query(*args, ctypes.byref(ws)), "workspace")
@@ -115,7 +129,8 @@ class _LinearFn(torch.autograd.Function):
 
 class MXLinear(torch.nn.Module):
     """Bias-free linear whose weight is MXFP4: codes uint8 [OUT, 16 B], scales uint8 [OUT, B].
-    in_features may be any width of the last block (default: all 32 of it). act: None multiplies x
+    (the module keeps its own copy, in the kernels' operand order). in_features may be any width of
+    the last block (default: all 32 of it). act: None multiplies x
     as it is (bf16, fp16 and fp32 enter exactly, fp32 sums); "mxfp4" quantises x's rows as
     mx_quantize does. Differentiable in x with act None; the weight is frozen."""
 
@@ -127,8 +142,8 @@ class MXLinear(torch.nn.Module):
             raise ValueError(f"codes must be [OUT, bytes], got {tuple(codes.shape)}")
         IN = int(scales.shape[-1]) * BLOCK if in_features is None else int(in_features)
         _check_mx(codes, scales, IN, "MXLinear")
-        self.codes, self.scales = _aligned(codes, 16), scales.contiguous()
         self.in_features, self.out_features, self.act = IN, int(codes.shape[0]), act
+        self.packed, self.packed_scales = _pack(codes, scales, 1, self.out_features, IN)
 
     @classmethod
     def from_weight(cls, weight, act=None):
@@ -145,7 +160,7 @@ class MXLinear(torch.nn.Module):
         with T.on_device(x):
             xf = x.reshape(-1, IN).contiguous()
             N = xf.shape[0]
-            w = _desc(self.codes, self.scales, 1, OUT, IN)
+            w = _desc(self.packed, self.packed_scales, 1, OUT, IN)
             y = torch.empty((*x.shape[:-1], OUT), dtype=x.dtype, device=x.device)
             work, size = _work(lib.vqk_mx_linear_workspace, x.device, ctypes.byref(w), xt, N, act)
             L.check(lib.vqk_mx_linear(ctypes.byref(w), xf.data_ptr(), xt, N, act, y.data_ptr(), xt,
@@ -159,7 +174,7 @@ class MXLinear(torch.nn.Module):
         with T.on_device(dy):
             d = dy.reshape(-1, OUT).contiguous()
             N = d.shape[0]
-            w = _desc(self.codes, self.scales, 1, OUT, IN)
+            w = _desc(self.packed, self.packed_scales, 1, OUT, IN)
             dx = torch.empty((*dy.shape[:-1], IN), dtype=dy.dtype, device=dy.device)
             work, size = _work(lib.vqk_mx_linear_dx_workspace, dy.device, ctypes.byref(w), dt, N)
             L.check(lib.vqk_mx_linear_dx(ctypes.byref(w), d.data_ptr(), dt, N, dx.data_ptr(), dt,
@@ -168,7 +183,7 @@ class MXLinear(torch.nn.Module):
         return dx
 
     def forward(self, x):
-        T.require_cuda(x, self.codes, self.scales)
+        T.require_cuda(x, self.packed, self.packed_scales)
         if x.ndim == 0 or x.shape[-1] != self.in_features:
             raise ValueError(f"MXLinear: x {tuple(x.shape)} for in_features {self.in_features}")
         if torch.is_grad_enabled() and x.requires_grad:
@@ -195,8 +210,8 @@ class MXSwitchLinear(torch.nn.Module):
             raise ValueError(f"codes must be [E, OUT, bytes], got {tuple(codes.shape)}")
         IN = int(scales.shape[-1]) * BLOCK if in_features is None else int(in_features)
         _check_mx(codes, scales, IN, "MXSwitchLinear")
-        self.codes, self.scales = _aligned(codes, 16), scales.contiguous()
         self.num_experts, self.output_dims, self.input_dims = int(codes.shape[0]), int(codes.shape[1]), IN
+        self.packed, self.packed_scales = _pack(codes, scales, *codes.shape[:2], IN)
 
     @classmethod
     def from_weight(cls, weight):
@@ -204,10 +219,10 @@ class MXSwitchLinear(torch.nn.Module):
         return cls(*mx_quantize(weight.detach()), weight.shape[2])
 
     def _weights(self):
-        return _desc(self.codes, self.scales, self.num_experts, self.output_dims, self.input_dims)
+        return _desc(self.packed, self.packed_scales, self.num_experts, self.output_dims, self.input_dims)
 
     def forward(self, x, indices):
-        T.require_cuda(x, indices, self.codes, self.scales)
+        T.require_cuda(x, indices, self.packed, self.packed_scales)
         _no_grad("MXSwitchLinear", x)
         IN, OUT, k = self.input_dims, self.output_dims, int(indices.shape[-1])
         lead = tuple(indices.shape[:-1])
@@ -243,7 +258,7 @@ class MXSwitchGLU(torch.nn.Module):
         self.gate_proj, self.up_proj, self.down_proj = g, u, d
 
     def forward(self, x, ids, weights):
-        T.require_cuda(x, ids, weights, self.gate_proj.codes)
+        T.require_cuda(x, ids, weights, self.gate_proj.packed)
         _no_grad("MXSwitchGLU", x, weights)
         H = self.gate_proj.input_dims
         if x.ndim != 2 or x.shape[1] != H or ids.ndim != 2 or ids.shape[0] != x.shape[0] or \
