@@ -56,7 +56,8 @@ def _check(lg, k, norm, mask, r, grads=None):
 
 
 CASES = [(1, 1, 1), (1, 8, 2), (5, 8, 8), (33, 60, 6), (64, 64, 4), (100, 65, 10), (257, 256, 8), (40, 300, 10),
-         (130, 512, 10), (19, 1000, 3), (9, 2048, 64)]
+         (130, 512, 10), (19, 1000, 3), (9, 2048, 64),
+         (2048, 8, 2), (2049, 60, 6), (3001, 96, 10), (2500, 130, 7), (2100, 256, 8), (2222, 300, 10), (2050, 512, 16)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -77,47 +78,64 @@ def test_route(dtype, norm, T, E, k):
     assert torch.equal(ids, r.ids) and torch.equal(w, r.weights)
 
 
-def test_ties_go_to_the_lower_id():
+@pytest.mark.parametrize("T", [3, 3000])
+def test_ties_go_to_the_lower_id(T):
     from vqlab_amd import router
-    lg = torch.zeros(3, 200, device="cuda")
+    lg = torch.zeros(T, 200, device="cuda")
     lg[1, 70:] = 1.0
     lg[2, ::2] = -0.0
     ids, w = router.top_k(lg, 5)
-    assert ids.tolist() == [[0, 1, 2, 3, 4], [70, 71, 72, 73, 74], [0, 1, 2, 3, 4]]
+    assert ids[:3].tolist() == [[0, 1, 2, 3, 4], [70, 71, 72, 73, 74], [0, 1, 2, 3, 4]]
+    assert (ids[3:] == torch.arange(5, device="cuda")).all()
     assert torch.allclose(w, torch.full_like(w, 0.2))
 
 
-@pytest.mark.parametrize("E,k", [(8, 4), (96, 6), (512, 10)])
-def test_rows_with_few_or_no_experts_left(E, k):
+@pytest.mark.parametrize("E,k", [(64, 6), (256, 8), (500, 16)])
+def test_many_tokens_with_few_distinct_logits(E, k):
+    """Coarse logits: rows with more equal candidates than the ranking holds, beside ordinary ones."""
     from vqlab_amd import router
     rng = np.random.default_rng(E)
-    lg = _logits(rng, "fp32", 12, E)
+    lg = torch.from_numpy(np.round(rng.standard_normal((2400, E)) * 2).astype(np.float32) / 2)
+    lg[::3] = torch.from_numpy(rng.standard_normal((800, E)).astype(np.float32))
+    lg = lg.cuda()
+    r = router.route(lg, k)
+    _check(lg, k, True, None, r)
+
+
+@pytest.mark.parametrize("E,k", [(8, 4), (96, 6), (512, 10)])
+@pytest.mark.parametrize("more", [0, 2100])
+def test_rows_with_few_or_no_experts_left(E, k, more):
+    from vqlab_amd import router
+    rng = np.random.default_rng(E)
+    T = 12 + more
+    lg = _logits(rng, "fp32", T, E)
     lg[3] = float("-inf")
     lg[5, 2:] = float("-inf")                              # two experts for k places
     lg[7, 1:] = float("-inf")
     lg[8] = torch.finfo(torch.float32).min                 # the type's lowest value is a number
     lg[9] = 1e30
-    mask = torch.ones(12, dtype=torch.bool, device="cuda")
+    mask = torch.ones(T, dtype=torch.bool, device="cuda")
     mask[10] = False
     lg[10] = float("nan")
     lg.requires_grad_(True)
     r = router.route(lg, k, True, mask)
-    dw = torch.randn(12, k, device="cuda")
+    dw = torch.randn(T, k, device="cuda")
     zero = torch.tensor(0.0, device="cuda")
     gb = torch.tensor(1.0, device="cuda")
     d = torch.autograd.grad((r.weights, r.balance, r.z), lg, (dw, gb, zero))[0]
     assert (r.ids[3] == -1).all() and (r.weights[3] == 0).all() and (d[3] == 0).all()
     assert (r.ids[10] == -1).all() and (r.weights[10] == 0).all() and (d[10] == 0).all()
     assert r.ids[5].tolist()[2:] == [-1] * (k - 2) and abs(float(r.weights[5].sum().detach()) - 1) < 1e-6
-    assert r.ids[7].tolist() == [0] + [-1] * (k - 1) and float(r.weights[7, 0]) == 1.0
+    assert r.ids[7].tolist() == [0] + [-1] * (k - 1) and float(r.weights[7, 0].detach()) == 1.0
     assert r.ids[8].tolist() == list(range(k)) and torch.isfinite(r.weights).all()
-    assert float(r.tokens) == 10 and int(r.counts.sum()) == 10 * k - (k - 2) - (k - 1)
+    assert float(r.tokens) == T - 2 and int(r.counts.sum()) == (T - 2) * k - (k - 2) - (k - 1)
     assert torch.isfinite(d).all()
 
 
-def test_nan_logits_are_loud():
+@pytest.mark.parametrize("T", [4, 2400])
+def test_nan_logits_are_loud(T):
     from vqlab_amd import router
-    lg = torch.randn(4, 40, device="cuda")
+    lg = torch.randn(T, 40, device="cuda")
     lg[1, 7] = float("nan")
     lg[2, 3] = float("inf")
     r = router.route(lg, 3)

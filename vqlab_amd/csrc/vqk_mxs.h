@@ -127,10 +127,12 @@ __global__ void __launch_bounds__(64 * kMxsWaves, 2) k_mx_rows(const MxsArgs p) 
                     // wave's part of that row (past the row's end its start: zeroed below)
                     const int u = i * 64 + lane, row = u / (16 * NCW), piece = (u % (16 * NCW)) ^ row;
                     const int64_t k = int64_t(kw) * NCW * kMxChunk + piece * 8;
-                    const int pos = tile.row0 + min(b * 16 + row, tile.nrows - 1);
-                    const uint16_t *src = p.x + pl * p.xplane + int64_t(mx_x_row(p, pos)) * p.xld +
-                                          (k < int64_t(p.NB) * kMxBlock ? k : 0);
-                    __builtin_amdgcn_global_load_lds((global_void *)src, (lds_void *)(xl + i * 1024), 16, 0, 0);
+                    if (b * 16 + row < tile.nrows) {          // else the unit stays as it is: zeroed below
+                        const uint16_t *src = p.x + pl * p.xplane +
+                                              int64_t(mx_x_row(p, tile.row0 + b * 16 + row)) * p.xld +
+                                              (k < int64_t(p.NB) * kMxBlock ? k : 0);
+                        __builtin_amdgcn_global_load_lds((global_void *)src, (lds_void *)(xl + i * 1024), 16, 0, 0);
+                    }
                 }
                 wait_vmem();
 #pragma unroll

@@ -49,10 +49,12 @@ static int go(MxsArgs a, int64_t tiles, int kw, hipStream_t st) {
     const int RW = kMxsWaves / kw;
     a.kw = kw;
     a.total_steps = int32_t((a.ocover + 16 * RW - 1) / (16 * RW));
-    // row steps per workgroup: long walks, while every CU gets two workgroups
-    const int64_t want = tiles > 0 ? (512 + tiles - 1) / tiles : 1;
-    int64_t steps = a.total_steps / (want < 1 ? 1 : want);
-    steps = steps < 1 ? 1 : (steps > 8 ? 8 : steps);
+    // row steps per workgroup: one round of workgroups, two to a CU where the registers let them;
+    // tiles of a routing are an upper bound, so walks stay short enough to balance
+    const int64_t room = 45 + NCW * (16 * NT * P + (GLU ? 18 : 9)) <= 128 ? 512 : 256;
+    const int64_t want = tiles > 0 ? (room + tiles - 1) / tiles : 1;
+    int64_t steps = (a.total_steps + want - 1) / want;
+    if (a.meta || a.ids) steps = steps > 8 ? 8 : steps;
     a.steps = int32_t(steps);
     a.nob = int32_t((a.total_steps + steps - 1) / steps);
     const int64_t grid = int64_t(a.nob) * tiles;
