@@ -404,17 +404,22 @@ int vqk_skipzero_row_table_host(const uint8_t *rowmask, int64_t E,
  *   scales  uint8 [E, RT, ceil(NC / 4), 64, 4], 4-byte aligned: byte j of unit i
  *           belongs to its block in chunk 4 group + j
  * with codes 0 and scales 127 past the rows' ends. vqk_mx_pack_bytes gives both
- * sizes. A dense linear is E = 1; one expert holds less than 4 GB. */
+ * sizes. A dense linear is E = 1; one expert holds less than 4 GB.
+ * vqk_mx_pack sets *not_f16 (device memory, zeroed by the caller; may be NULL) to 1
+ * where some weight is no fp16 number (a scale outside 2^-23 .. 2^13). f16_exact:
+ * nonzero when the caller knows that it stayed 0; fp16 x then enters the matrix
+ * cores as it is, otherwise as two bf16 parts (the same products at half the rate). */
 typedef struct vqk_mx_weights {
     const uint8_t *codes;
     const uint8_t *scales;
     int64_t        E;
     int64_t        OUT;
     int64_t        IN;
+    int32_t        f16_exact;
 } vqk_mx_weights;
 int vqk_mx_pack_bytes(int64_t E, int64_t OUT, int64_t IN, size_t *codes, size_t *scales);
 int vqk_mx_pack(const uint8_t *codes, const uint8_t *scales, int64_t E, int64_t OUT, int64_t IN,
-                uint8_t *packed_codes, uint8_t *packed_scales, void *stream);
+                uint8_t *packed_codes, uint8_t *packed_scales, int32_t *not_f16, void *stream);
 
 /* x [rows, cols] (rows ldx elements apart) -> codes [rows, NB * 16] (4-byte
  * aligned) and scales [rows, NB]: s - 127 = floor(log2(largest magnitude)) - 2,

@@ -153,6 +153,24 @@ def test_linear_scales_far_apart(N, act, IN):
     mc.assert_within(lin(x), y, bar + IN * 2.0 ** -126, "far scales")
 
 
+@pytest.mark.parametrize("N", [1, 20, 70, 200])
+@pytest.mark.parametrize("lo,hi", [(104, 120), (80, 120)])
+def test_linear_fp16_x_and_weights_beyond_fp16(N, lo, hi):
+    """Weights that are fp16 numbers down to the last subnormal, and weights that are not, among
+    blocks of zeros under the smallest scale: exact either way."""
+    from vqlab_amd import mx
+    rng = np.random.default_rng(N + lo)
+    codes, _ = mc.weight(rng, 48, 320)
+    scales = rng.integers(lo, hi + 1, (48, 10)).astype(np.uint8)
+    scales[0] = lo
+    codes[3, :16], scales[3, 0] = 0, 0
+    lin, w = mx.MXLinear(*_dev(codes, scales), 320), mc.values(codes, scales, 320)
+    assert bool(lin._w.f16_exact) == (lo >= 104)
+    x, xv = mc.acts(rng, "fp16", N, 320)
+    y, bar = mc.product_bar(xv, w, "fp16")
+    mc.assert_within(lin(x), y, bar + 2.0 ** -25, "fp16")     # half a step of fp16's subnormals
+
+
 @pytest.mark.parametrize("act", [None, "mxfp4"])
 @pytest.mark.parametrize("N", [1, 20, 70, 200])
 @pytest.mark.parametrize("IN", [384, 416])

@@ -47,7 +47,8 @@ class VQKOptions(ctypes.Structure):
 
 
 class VQKMXWeights(ctypes.Structure):
-    _fields_ = [("codes", c_p), ("scales", c_p), ("E", c_i64), ("OUT", c_i64), ("IN", c_i64)]
+    _fields_ = [("codes", c_p), ("scales", c_p), ("E", c_i64), ("OUT", c_i64), ("IN", c_i64),
+                ("f16_exact", c_i32)]
 
 
 _MXW = ctypes.POINTER(VQKMXWeights)
@@ -106,7 +107,7 @@ SIGNATURES = {
     "vqk_mx_quantize": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, c_p, c_p, c_p]),
     "vqk_mx_dequantize": (c_i32, [c_p, c_p, c_i64, c_i64, c_p, c_i32, c_p]),
     "vqk_mx_pack_bytes": (c_i32, [c_i64, c_i64, c_i64, ctypes.POINTER(c_sz), ctypes.POINTER(c_sz)]),
-    "vqk_mx_pack": (c_i32, [c_p, c_p, c_i64, c_i64, c_i64, c_p, c_p, c_p]),
+    "vqk_mx_pack": (c_i32, [c_p, c_p, c_i64, c_i64, c_i64, c_p, c_p, c_p, c_p]),
     "vqk_mx_linear_workspace": (c_i32, [_MXW, c_i32, c_i64, c_i32, ctypes.POINTER(c_sz)]),
     "vqk_mx_linear": (c_i32, [_MXW, c_p, c_i32, c_i64, c_i32, c_p, c_i32, c_p, c_sz, c_p]),
     "vqk_mx_linear_dx_workspace": (c_i32, [_MXW, c_i32, c_i64, ctypes.POINTER(c_sz)]),

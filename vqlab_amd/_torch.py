@@ -34,14 +34,33 @@ def stream(device=None) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+# The current stream of a device index as a plain handle: an eighth of the time that building a
+# Stream object takes, which is half of a small call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def raw_stream(t: torch.Tensor) -> int:
+    """Handle of the current stream on t's device."""
+    if _raw_stream is None:
+        return torch.cuda.current_stream(t.device).cuda_stream
+    return _raw_stream(t.device.index)
+
+
 _HERE = contextlib.nullcontext()
 
 
 def on_device(t: torch.Tensor):
     """Context with t's device current: kernels launch on the current device."""
-    if t.device.index is None or t.device.index == torch.cuda.current_device():
+    if t.device.index == torch.cuda.current_device():
         return _HERE
     return torch.cuda.device(t.device)
+
+
+def rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """t [..., cols] as contiguous rows [n, cols]."""
+    if t.dim() == 2 and t.is_contiguous():
+        return t
+    return t.reshape(-1, cols).contiguous()
 
 
 def ptr(t) -> ctypes.c_void_p:

@@ -42,6 +42,12 @@ __host__ __device__ constexpr int64_t mx_expert_scales(int64_t RT, int64_t NC) {
 // Validates `w` and fills `g`; returns a VQK_* status and sets the message.
 int make_mx_geom(const vqk_mx_weights *w, MxGeom *g, const char *what);
 
+// Whether rows of x [., IN] enter as they lie.
+inline bool mx_x_in_place(const vqk_mx_weights *w, const void *x, int32_t type) {
+    return (type == VQK_BF16 || (type == VQK_F16 && w->f16_exact)) && w->IN % kMxBlock == 0 &&
+           (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+}
+
 // 2^(s - 127) as fp32 (s = 0 is the subnormal 2^-127; s = 255 NaN).
 __device__ __forceinline__ float mx_scale(uint32_t s) {
     return __uint_as_float(s == 0u ? 0x00400000u : (s == 255u ? 0x7fc00000u : s << 23));
@@ -57,7 +63,24 @@ __device__ __forceinline__ u32x4 mx_decode8(uint32_t w, float sc) {
     return r;
 }
 
-// Activations enter the matrix cores as bf16 planes whose sum is exact: one
+// The same for fp16 operands, exact for weights that are fp16 numbers (f16_exact).
+template <int OP>
+__device__ __forceinline__ u32x4 mx_decode8_op(uint32_t w, float sc) {
+    if constexpr (OP == kOpBF16) return mx_decode8(w, sc);
+    u32x4 r;
+    r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 0));
+    r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 1));
+    r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 2));
+    r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 3));
+    return r;
+}
+
+// Scale bytes under which every code but 0 is an fp16 number: 0.5 * 2^-23 is the
+// smallest subnormal, 6 * 2^13 below the largest number.
+constexpr uint32_t kMxF16ScaleMin = 104, kMxF16ScaleMax = 140;
+
+// fp16 x enters as it is where the weights are fp16 numbers. Otherwise
+// activations enter the matrix cores as bf16 planes whose sum is exact: one
 // for bf16, two for fp16 (11 significant bits = 8 + 3), three for fp32 (24).
 constexpr int mx_planes(int32_t type) { return type == VQK_BF16 ? 1 : (type == VQK_F16 ? 2 : 3); }
 
@@ -158,11 +181,12 @@ int launch_mx_planes(const void *x, int32_t type, int64_t N, int64_t IN, int64_t
 int launch_mx_quant(const void *x, int32_t type, int64_t rows, int64_t cols, int64_t ldx, int64_t NB,
                     bool permute, uint8_t *codes, uint8_t *scales, hipStream_t st);
 
-// Rows of x as the product kernels read them: bf16 planes of rows ld apart.
+// Rows of x as the product kernels read them: bf16 planes (or fp16 rows) ld apart.
 struct MxX {
     const uint16_t *x;
     int64_t ld, plane;                        // elements between rows / planes
     int P;
+    int op;                                   // kOpBF16, or kOpF16 (P = 1): fp16 rows
 };
 
 // One product, over dense rows, single pairs, or tiles of a sorted routing.
@@ -174,7 +198,7 @@ struct MxCall {
     // routing: none (dense) | ids (tile = pair) | order, meta, ntiles (sorted tiles)
     const int32_t *ids, *order, *meta, *ntiles;
     int64_t xkrep;                            // x row = pair / xkrep; 0: x rows are sorted positions (or pairs)
-    void *y;                                  // [row][OUT] in y_type; a SwiGLU pair: bf16 planes
+    void *y;                                  // [row][OUT] in y_type; a SwiGLU pair: rows like x's
     int32_t y_type;
     int64_t ldy, yplane;                      // elements between rows / planes of y
     int yp;                                   // planes of a SwiGLU pair's output
@@ -190,7 +214,7 @@ int mxg_dense_rows(int64_t N);
 size_t mxg_part_bytes(int64_t N, const MxGeom &g);
 
 // K slices of a dense product, four outputs a thread, and how many pay.
-int mxg_splits(int64_t T, int64_t NC);
+int mx_splits(int64_t T, int64_t NC, int64_t n, float t1, float t2);
 int launch_mx_reduce(const float *part, int splits, int64_t n, void *y, int32_t y_type, hipStream_t st);
 
 // Products of 4-bit rows with 4-bit weights (vqk_mxf.h): x as codes in rows of

@@ -208,6 +208,7 @@ struct PackArgs {
     const uint8_t *codes, *scales;
     int64_t E, OUT, NB, RT, NC, units;        // units of 16 bytes: E * RT * NC * 64
     uint8_t *pcodes, *pscales;
+    int32_t *not_f16;
 };
 
 // One unit a thread: 16 bytes of codes from their row to their place.
@@ -219,9 +220,14 @@ __global__ void __launch_bounds__(256) k_mx_pack(const PackArgs p) {
     const int64_t row = rt * 16 + (i & 15), blk = 4 * c + (i >> 4);
     const bool in = row < p.OUT && blk < p.NB;
     const int64_t at = (e * p.OUT + row) * p.NB + blk;
-    reinterpret_cast<u32x4 *>(p.pcodes)[u] = in ? reinterpret_cast<const u32x4 *>(p.codes)[at] : u32x4{};
+    const u32x4 w = in ? reinterpret_cast<const u32x4 *>(p.codes)[at] : u32x4{};
+    reinterpret_cast<u32x4 *>(p.pcodes)[u] = w;
     uint8_t *sc = p.pscales + ((et * ((p.NC + 3) / 4) + c / 4) * 64 + i) * 4;
-    sc[c & 3] = in ? p.scales[at] : uint8_t(127);
+    const uint32_t s = in ? p.scales[at] : 127u;
+    sc[c & 3] = uint8_t(s);
+    if (p.not_f16 && ((w.x | w.y | w.z | w.w) & 0x77777777u) != 0 && s != 255u &&
+        (s < kMxF16ScaleMin || s > kMxF16ScaleMax))
+        *p.not_f16 = 1;                       // every thread that writes it writes the same
     if (c == p.NC - 1)                        // the bytes of chunks past the end
         for (int j = int(c & 3) + 1; j < 4; ++j) sc[j] = 127;
 }
@@ -248,7 +254,7 @@ extern "C" int vqk_mx_pack_bytes(int64_t E, int64_t OUT, int64_t IN, size_t *cod
 }
 
 extern "C" int vqk_mx_pack(const uint8_t *codes, const uint8_t *scales, int64_t E, int64_t OUT, int64_t IN,
-                           uint8_t *pcodes, uint8_t *pscales, void *stream) {
+                           uint8_t *pcodes, uint8_t *pscales, int32_t *not_f16, void *stream) {
     const int rc = check_pack(E, OUT, IN);
     if (rc) return rc;
     if (!codes || !scales || !pcodes || !pscales) return set_error(VQK_EINVAL, "mx pack: NULL pointer");
@@ -256,7 +262,7 @@ extern "C" int vqk_mx_pack(const uint8_t *codes, const uint8_t *scales, int64_t 
         return set_error(VQK_EINVAL, "mx pack: codes must be 16-byte aligned");
     const int64_t RT = (OUT + 15) / 16, NC = (IN + kMxChunk - 1) / kMxChunk, units = E * RT * NC * 64;
     if ((units + 255) / 256 > INT32_MAX) return set_error(VQK_ENOTIMPL, "mx pack: weight too large");
-    const PackArgs a{codes, scales, E, OUT, (IN + kMxBlock - 1) / kMxBlock, RT, NC, units, pcodes, pscales};
+    const PackArgs a{codes, scales, E, OUT, (IN + kMxBlock - 1) / kMxBlock, RT, NC, units, pcodes, pscales, not_f16};
     hipLaunchKernelGGL(k_mx_pack, dim3(unsigned((units + 255) / 256)), dim3(256), 0,
                        static_cast<hipStream_t>(stream), a);
     return hip_status(hipGetLastError(), "MXFP4 pack launch");

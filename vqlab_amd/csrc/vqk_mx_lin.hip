@@ -2,8 +2,9 @@
 // dx = dy . W.
 //
 // The forward product streams the weights past few rows (vqk_mxs.h) or
-// multiplies tiles of many (vqk_mxg.h; 4-bit x: vqk_mxf.h). x that is bf16,
-// 16-byte aligned and whole blocks wide is read in place; other x is laid out
+// multiplies tiles of many (vqk_mxg.h; 4-bit x: vqk_mxf.h). x that is bf16 (or
+// fp16, for weights that are fp16 numbers), 16-byte aligned and whole blocks wide
+// is read in place; other x is laid out
 // once in the workspace as exact bf16 planes (vqk_mx.h). The gradient sums over the
 // weight's rows, along which its codes do not lie: the weight is decoded,
 // transposed, into the workspace as bf16 (exact) and multiplied by the
@@ -14,10 +15,6 @@ namespace vqk {
 
 static size_t al256(size_t v) { return (v + 255) & ~size_t(255); }
 
-static bool x_in_place(const void *x, int32_t type, int64_t IN, int64_t ld) {
-    return type == VQK_BF16 && IN % kMxBlock == 0 && ld % 8 == 0 &&
-           (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-}
 
 // ------------------------------------------------------- transposed decode
 struct DecTArgs {
@@ -170,8 +167,9 @@ extern "C" int vqk_mx_linear(const vqk_mx_weights *w, const void *x, int32_t x_t
     c.g = g;
     c.N = N; c.xkrep = 1;
     c.y = y; c.y_type = y_type; c.ldy = g.OUT;
-    const bool place = act == VQK_MX_ACT_NONE && x_in_place(x, x_type, g.IN, g.IN);
-    c.x.P = act == VQK_MX_ACT_MXFP4 ? 1 : mx_planes(x_type);
+    const bool place = act == VQK_MX_ACT_NONE && mx_x_in_place(w, x, x_type);
+    c.x.P = place || act == VQK_MX_ACT_MXFP4 ? 1 : mx_planes(x_type);
+    c.x.op = place && x_type == VQK_F16 ? kOpF16 : kOpBF16;
     const int nt = N <= 16 ? 1 : 2;
     const bool stream_w = N <= kMxStreamRows && mx_rows_ok(c, nt);
     const size_t need = lin_bytes(g, x_type, N, act);
@@ -189,11 +187,11 @@ extern "C" int vqk_mx_linear(const vqk_mx_weights *w, const void *x, int32_t x_t
         return mxf_gemm(f, need > xb ? reinterpret_cast<float *>(ws + xb) : nullptr, need - xb, st);
     }
     if (place) {
-        c.x = MxX{static_cast<const uint16_t *>(x), g.IN, 0, 1};
+        c.x = MxX{static_cast<const uint16_t *>(x), g.IN, 0, 1, c.x.op};
     } else {
         uint16_t *xs = reinterpret_cast<uint16_t *>(ws);
         if ((rc = launch_mx_planes(x, x_type, N, g.IN, g.IN, act == VQK_MX_ACT_MXFP4, xs, st))) return rc;
-        c.x = MxX{xs, g.NB * kMxBlock, N * g.NB * kMxBlock, c.x.P};
+        c.x = MxX{xs, g.NB * kMxBlock, N * g.NB * kMxBlock, c.x.P, kOpBF16};
     }
     if (stream_w) return mx_rows(c, nt, st);
     const size_t xb = lin_x_bytes(g, x_type, N, act);

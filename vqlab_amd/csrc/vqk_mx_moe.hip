@@ -21,7 +21,7 @@ constexpr int64_t kMxMaxExperts = 4096;
 // experts have a few pairs each, then 32, 64 or 128 (the many-row kernel).
 static int mx_tile_rows(int64_t N, int64_t E) {
     const int64_t avg = N / E;
-    return avg <= 12 ? 16 : (avg <= 24 ? 32 : (avg <= 80 ? 64 : 128));
+    return avg <= 12 ? 16 : (avg <= 20 ? 32 : (avg <= 40 ? 64 : 128));
 }
 static int run(const MxCall &c, int rows, hipStream_t st) {
     return rows == 16 && mx_rows_ok(c, 1) ? mx_rows(c, 1, st) : mx_gemm(c, rows, nullptr, 0, st);
@@ -66,19 +66,16 @@ static int check_pairs(int64_t T, int64_t N, int64_t E, const char *what) {
     return VQK_OK;
 }
 
-// x rows as planes: in place, or laid out at `ws` (bytes: plane_bytes).
-static bool x_in_place(const void *x, int32_t type, int64_t IN) {
-    return type == VQK_BF16 && IN % kMxBlock == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-}
+// x rows in place, or laid out as planes at `ws` (bytes: plane_bytes).
 static size_t plane_bytes(int64_t rows, int64_t NB, int P) { return al256(size_t(rows) * NB * kMxBlock * 2 * P); }
-static int make_x(const void *x, int32_t type, int64_t rows, int64_t IN, int64_t NB, uint16_t *ws, MxX *out,
-                  hipStream_t st) {
-    if (x_in_place(x, type, IN)) {
-        *out = MxX{static_cast<const uint16_t *>(x), IN, 0, 1};
+static int make_x(const vqk_mx_weights *w, bool place, const void *x, int32_t type, int64_t rows, int64_t NB,
+                  uint16_t *ws, MxX *out, hipStream_t st) {
+    if (place) {
+        *out = MxX{static_cast<const uint16_t *>(x), w->IN, 0, 1, type == VQK_F16 ? kOpF16 : kOpBF16};
         return VQK_OK;
     }
-    *out = MxX{ws, NB * kMxBlock, rows * NB * kMxBlock, mx_planes(type)};
-    return launch_mx_planes(x, type, rows, IN, IN, false, ws, st);
+    *out = MxX{ws, NB * kMxBlock, rows * NB * kMxBlock, mx_planes(type), kOpBF16};
+    return launch_mx_planes(x, type, rows, w->IN, w->IN, false, ws, st);
 }
 
 static size_t sort_bytes(int64_t N, int64_t E) {
@@ -170,7 +167,8 @@ extern "C" int vqk_mx_switch(const vqk_mx_weights *w, const void *x, int32_t x_t
     c.g = g;
     c.N = N; c.xkrep = xkrep;
     c.y = y; c.y_type = y_type; c.ldy = g.OUT;
-    if ((rc = make_x(x, x_type, T, g.IN, g.NB, reinterpret_cast<uint16_t *>(ws), &c.x, st))) return rc;
+    if ((rc = make_x(w, mx_x_in_place(w, x, x_type), x, x_type, T, g.NB, reinterpret_cast<uint16_t *>(ws),
+                     &c.x, st))) return rc;
     const int rows = N <= kMxPairsUnsorted ? 16 : mx_tile_rows(N, g.E);
     if ((rc = set_routing(&c, eidx, N, g.E, rows, ws + sort_at, st))) return rc;
     return run(c, rows, st);
@@ -213,15 +211,18 @@ extern "C" int vqk_mx_experts(const vqk_mx_weights *gate, const vqk_mx_weights *
     c.g = g1;
     c.N = p.N; c.xkrep = top_k;
     uint16_t *h = reinterpret_cast<uint16_t *>(ws + p.h);
-    c.y = h; c.ldy = p.IP; c.yplane = p.N * p.IP; c.yp = p.P; c.ysorted = true;
-    if ((rc = make_x(x, x_type, T, g1.IN, g1.NB, reinterpret_cast<uint16_t *>(ws), &c.x, st))) return rc;
+    // fp16 x and SwiGLU rows, or bf16 planes of both
+    const bool place = mx_x_in_place(gate, x, x_type) && (x_type != VQK_F16 || (up->f16_exact && down->f16_exact));
+    if ((rc = make_x(gate, place, x, x_type, T, g1.NB, reinterpret_cast<uint16_t *>(ws), &c.x, st))) return rc;
+    const int hp = c.x.op == kOpF16 ? 1 : p.P;
+    c.y = h; c.ldy = p.IP; c.yplane = p.N * p.IP; c.yp = hp; c.ysorted = true;
     if ((rc = set_routing(&c, ids, p.N, g1.E, rows, ws + p.sort, st))) return rc;
     if ((rc = run(c, rows, st))) return rc;
     MxCall d = c;                              // the same routing, over the SwiGLU rows
     d.codes[0] = down->codes; d.scales[0] = down->scales;
     d.codes[1] = nullptr; d.scales[1] = nullptr;
     d.g = g2;
-    d.x = MxX{h, p.IP, p.N * p.IP, p.P};
+    d.x = MxX{h, p.IP, p.N * p.IP, hp, c.x.op};
     d.xkrep = 0;
     float *part = reinterpret_cast<float *>(ws + p.part);
     d.y = part; d.y_type = VQK_F32; d.ldy = g2.OUT; d.ysorted = false;

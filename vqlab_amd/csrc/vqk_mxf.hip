@@ -9,8 +9,13 @@ static int64_t mxf_tiles(int64_t N, int64_t OUT) {
     return ((N + kMxfRows - 1) / kMxfRows) * ((OUT + 255) / 256);
 }
 
+// In groups of four chunks: 3.6 us with one workgroup on a CU, 6.1 with two.
+static int splits_of(int64_t N, const MxGeom &g) {
+    return mx_splits(mxf_tiles(N, g.OUT), (g.NC + 3) / 4, N * g.OUT, 3.6f, 6.1f);
+}
+
 size_t mxf_part_bytes(int64_t N, const MxGeom &g) {
-    const int s = mxg_splits(mxf_tiles(N, g.OUT), (g.NC + 1) / 2);
+    const int s = splits_of(N, g);
     return s > 1 ? size_t(s) * N * g.OUT * 4 : 0;
 }
 
@@ -25,7 +30,7 @@ int mxf_gemm(const MxfCall &c, float *part, size_t part_bytes, hipStream_t st) {
     const int groups = (a.NC + 3) / 4;
     a.splits = 1;
     a.per = groups;
-    const int s = mxg_splits(mxf_tiles(c.N, c.g.OUT), (c.g.NC + 1) / 2);
+    const int s = splits_of(c.N, c.g);
     if (s > 1 && part && size_t(s) * c.N * c.g.OUT * 4 <= part_bytes) {
         a.per = (groups + s - 1) / s;
         a.splits = (groups + a.per - 1) / a.per;

@@ -16,9 +16,12 @@
 // workgroups share a CU and fill each other's waits. The four conversions of a
 // fragment (v_cvt_scalef32_pk_bf16_fp4) issue in the shadow of the matrix
 // instructions: one conversion for each of them at BT = 4.
-// x in planes (fp16, fp32): the chunk's planes one after the other, weights
-// loaded once.
+// The loop exists for every number of 32-row groups that a tile may hold: a
+// routed expert's last rows cost what they are. x in planes (fp16 beyond exact
+// weights, fp32): the chunk's planes one after the other, weights loaded once.
 #pragma once
+
+#include <type_traits>
 
 #include "vqk_mxs.h"
 
@@ -37,8 +40,17 @@ struct MxgArgs {
     float *part;                              // [splits][N][OUT] when splits > 1
 };
 
+template <int OP>
+__device__ __forceinline__ f32x16v mx_mma32(u32x4 w, u32x4 x, f32x16v c) {
+    if constexpr (OP == kOpBF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(mx_b8, w), __builtin_bit_cast(mx_b8, x), c,
+                                                       0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, w), __builtin_bit_cast(h8, x), c, 0, 0, 0);
+}
+
 // PL: x in more planes than one.
-template <int BT, bool GLU, bool PL>
+template <int OP, int BT, bool GLU, bool PL>
 __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga) {
     const MxsArgs &p = ga.a;
     constexpr int ROWS = 32 * BT;
@@ -94,18 +106,19 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
         int piece[CPW];
 #pragma unroll
         for (int j = 0; j < CPW; ++j) {
-            const int n = (wave * CPW + j) * 4 + (lane >> 4);
+            const int n = (j * kMxgWaves + wave) * 4 + (lane >> 4);
             piece[j] = (lane & 15) ^ (n & 15);
             src[j] = p.x + int64_t(mx_x_row(p, tile.row0 + min(n, tile.nrows - 1))) * p.xld + piece[j] * 8;
         }
-        auto issue = [&](int c, int pl, int buf) {
+        // NA: groups of 32 rows that the tile holds
+        auto issue = [&](int c, int pl, int buf, auto na) {
 #pragma unroll
-            for (int j = 0; j < CPW; ++j) {
+            for (int j = 0; j < 2 * decltype(na)::value; ++j) {
                 // past the row's last block: the row's start again (multiplied by no weight, masked below)
                 const bool in = 4 * c + piece[j] / 4 < p.NB;
                 const uint16_t *s = src[j] + pl * p.xplane + (in ? int64_t(c) * kMxChunk : -int64_t(piece[j] * 8));
                 __builtin_amdgcn_global_load_lds((global_void *)s,
-                                                 (lds_void *)(xs + buf * STAGE + (wave * CPW + j) * 1024), 16, 0, 0);
+                                                 (lds_void *)(xs + buf * STAGE + (j * kMxgWaves + wave) * 1024), 16, 0, 0);
             }
         };
         u32x4 w[2][2], wn[2][2];
@@ -119,7 +132,7 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
                     ss[a][q] = sb[a][so[a] + uint32_t(c / 4) * 256u + q * 64u + uint32_t(c % 4)];
                 }
         };
-        auto mul = [&](int c, int buf) {
+        auto mul = [&](int c, int buf, auto na) {
             const bool tail = 4 * c + 4 > p.NB;
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
@@ -132,53 +145,58 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
                 const bool in = !tail || 4 * c + 2 * g + q < p.NB;
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
-                    mx_b8 wf[2];
+                    u32x4 wf[2];
 #pragma unroll
-                    for (int a = 0; a < 2; ++a) wf[a] = __builtin_bit_cast(mx_b8, mx_decode8(w[a][q][h], sc[a]));
+                    for (int a = 0; a < 2; ++a) wf[a] = mx_decode8_op<OP>(w[a][q][h], sc[a]);
                     const int at = ((8 * g + 4 * q + h) ^ (lane & 15)) * 16 + r * 256;
 #pragma unroll
-                    for (int b = 0; b < BT; ++b) {
+                    for (int b = 0; b < decltype(na)::value; ++b) {
                         u32x4 xv = *reinterpret_cast<const u32x4 *>(xs + buf * STAGE + b * 8192 + at);
                         if (tail && !in) xv = u32x4{};
-                        const mx_b8 xf = __builtin_bit_cast(mx_b8, xv);
 #pragma unroll
-                        for (int a = 0; a < 2; ++a)
-                            acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[a], xf, acc[a][b], 0, 0, 0);
+                        for (int a = 0; a < 2; ++a) acc[a][b] = mx_mma32<OP>(wf[a], xv, acc[a][b]);
                     }
                 }
             }
         };
         // steps: chunk c_lo + step / P, plane step % P
-        const int P = PL ? ga.planes : 1, steps = (c_hi - c_lo) * P;
-        if (steps > 0) {
-            issue(c_lo, 0, 0);
-            load_w(c_lo, wn, sn);
-        }
-        int c = c_lo, pl = 0;
+        auto walk = [&](auto na) {
+            const int P = PL ? ga.planes : 1, steps = (c_hi - c_lo) * P;
+            if (steps > 0) {
+                issue(c_lo, 0, 0, na);
+                load_w(c_lo, wn, sn);
+            }
+            int c = c_lo, pl = 0;
 #pragma unroll 1
-        for (int step = 0; step < steps; ++step) {
-            wait_vmem();                      // this wave's copies of the step, and its weights
-            __syncthreads();                  // every wave's copies; every wave is done with the other buffer
-            if (!PL || pl == 0) {
+            for (int step = 0; step < steps; ++step) {
+                wait_vmem();                  // this wave's copies of the step, and its weights
+                __syncthreads();              // every wave's copies; every wave is done with the other buffer
+                if (!PL || pl == 0) {
 #pragma unroll
-                for (int a = 0; a < 2; ++a)
+                    for (int a = 0; a < 2; ++a)
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        w[a][q] = wn[a][q];
-                        s[a][q] = sn[a][q];
-                    }
+                        for (int q = 0; q < 2; ++q) {
+                            w[a][q] = wn[a][q];
+                            s[a][q] = sn[a][q];
+                        }
+                }
+                const int cc = c;
+                if (!PL || ++pl == P) {
+                    pl = 0;
+                    ++c;
+                }
+                if (step + 1 < steps) {
+                    issue(c, pl, (step + 1) & 1, na);
+                    if (!PL || pl == 0) load_w(c, wn, sn);
+                }
+                mul(cc, step & 1, na);
             }
-            const int cc = c;
-            if (!PL || ++pl == P) {
-                pl = 0;
-                ++c;
-            }
-            if (step + 1 < steps) {
-                issue(c, pl, (step + 1) & 1);
-                if (!PL || pl == 0) load_w(c, wn, sn);
-            }
-            mul(cc, step & 1);
-        }
+        };
+        const int groups = (tile.nrows + 31) / 32;
+        if (BT > 1 && groups <= 1) walk(std::integral_constant<int, 1>{});
+        else if (BT > 2 && groups == 2) walk(std::integral_constant<int, (BT > 2 ? 2 : BT)>{});
+        else if (BT > 3 && groups == 3) walk(std::integral_constant<int, (BT > 3 ? 3 : BT)>{});
+        else walk(std::integral_constant<int, BT>{});
     }
 
     // register i of lane l: weight row 8 * (i / 4) + 4 * (l / 32) + i % 4, x row l % 32. A NaN block
@@ -207,12 +225,12 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float v = value(0, b, 4 * j + i), u = value(1, b, 4 * j + i);
-                    h[i] = o + i < p.OUT ? v / (1.f + __expf(-v)) * u : 0.f;
+                    h[i] = o + i < p.OUT ? mx_swiglu(v, u) : 0.f;
                 }
-                for (int pl = 0; pl < p.yp; ++pl) {
+                for (int pl = 0; pl < (OP == kOpF16 ? 1 : p.yp); ++pl) {
                     uint16_t q[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) q[i] = mx_plane_next(h[i]);
+                    for (int i = 0; i < 4; ++i) q[i] = OP == kOpF16 ? f32_to_h(h[i]) : mx_plane_next(h[i]);
                     u32x2 v2;
                     v2.x = q[0] | (uint32_t(q[1]) << 16);
                     v2.y = q[2] | (uint32_t(q[3]) << 16);

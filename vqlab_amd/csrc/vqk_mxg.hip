@@ -37,20 +37,33 @@ int launch_mx_reduce(const float *part, int splits, int64_t n, void *y, int32_t 
     return hip_status(hipGetLastError(), "slice sum launch");
 }
 
-// K slices for T tiles of NC chunks: enough workgroups for two on every CU, at
-// least 8 chunks each.
-int mxg_splits(int64_t T, int64_t NC) {
-    const int64_t want = 512;
-    int64_t s = T > 0 ? want / T : 1;
-    s = s > NC / 8 ? NC / 8 : s;
-    return int(s < 1 ? 1 : (s > 16 ? 16 : s));
+// K slices of a dense product of T tiles over NC chunks with n outputs, by an
+// estimate of its time in us. One workgroup on a CU takes a chunk in t1, two
+// together in t2 (128-row tiles: 2.2 and 3.6); slices are written and read as
+// fp32 at ~4.5 TB/s and cost one more launch.
+int mx_splits(int64_t T, int64_t NC, int64_t n, float t1, float t2) {
+    int best = 1;
+    float cost = -1.f;
+    for (int s = 1; s <= 16 && (s == 1 || NC / s >= 4); ++s) {
+        const int64_t wgs = T * s, per = (NC + s - 1) / s;
+        const int64_t rounds = wgs / 512, rest = wgs % 512;
+        float c = float(per) * (float(rounds) * t2 + (rest == 0 ? 0.f : (rest <= 256 ? t1 : t2)));
+        if (s > 1) c += 3.f + float(s) * float(n) * 8.f / 4.5e6f;
+        if (cost < 0.f || c < cost * 0.97f) {
+            best = s;
+            cost = c;
+        }
+    }
+    return best;
 }
 
 static int mxg_bt(int64_t rows) { return rows <= 32 ? 1 : (rows <= 64 ? 2 : 4); }
 
 static int dense_splits(int64_t N, const MxGeom &g) {
     const int rows = mxg_dense_rows(N);
-    return mxg_splits(((N + rows - 1) / rows) * ((g.OUT + kMxgRows - 1) / kMxgRows), g.NC);
+    const float f = rows == 128 ? 1.f : (rows == 64 ? 0.7f : 0.55f);
+    return mx_splits(((N + rows - 1) / rows) * ((g.OUT + kMxgRows - 1) / kMxgRows), g.NC, N * g.OUT, 2.2f * f,
+                     3.6f * f);
 }
 
 int mxg_dense_rows(int64_t N) { return N <= 32 ? 32 : (N <= 64 ? 64 : 128); }
@@ -60,22 +73,31 @@ size_t mxg_part_bytes(int64_t N, const MxGeom &g) {
     return s > 1 ? size_t(s) * N * g.OUT * 4 : 0;
 }
 
-template <int BT, bool GLU, bool PL>
+template <int OP, int BT, bool GLU, bool PL>
 static int go(MxgArgs ga, int64_t tiles, hipStream_t st) {
     MxsArgs &a = ga.a;
     a.nob = int32_t((a.ocover + (GLU ? kMxgRows / 2 : kMxgRows) - 1) / (GLU ? kMxgRows / 2 : kMxgRows));
     const int64_t grid = int64_t(a.nob) * tiles * ga.splits;
     if (grid > INT32_MAX) return set_error(VQK_ENOTIMPL, "MXFP4 product: grid too large");
     ga.ntiles_host = int32_t(tiles);
-    int rc = launch_with_lds<k_mx_gemm<BT, GLU, PL>>(dim3(unsigned(grid)), dim3(64 * kMxgWaves),
-                                                    size_t(2) * 32 * BT * 256, st, ga);
+    int rc = launch_with_lds<k_mx_gemm<OP, BT, GLU, PL>>(dim3(unsigned(grid)), dim3(64 * kMxgWaves),
+                                                        size_t(2) * 32 * BT * 256, st, ga);
     if (rc || ga.splits == 1) return rc;
     return launch_mx_reduce(ga.part, ga.splits, a.N * a.OUT, a.y, a.y_type, st);
 }
 
 template <int BT, bool GLU>
-static int go_p(const MxgArgs &a, int64_t tiles, hipStream_t st) {
-    return a.planes == 1 ? go<BT, GLU, false>(a, tiles, st) : go<BT, GLU, true>(a, tiles, st);
+static int go_op(const MxgArgs &a, int op, int64_t tiles, hipStream_t st) {
+    if (op == kOpF16) return go<kOpF16, BT, GLU, false>(a, tiles, st);
+    return a.planes == 1 ? go<kOpBF16, BT, GLU, false>(a, tiles, st) : go<kOpBF16, BT, GLU, true>(a, tiles, st);
+}
+template <bool GLU>
+static int go_bt(const MxgArgs &a, int op, int tile_rows, int64_t tiles, hipStream_t st) {
+    switch (mxg_bt(tile_rows)) {
+        case 1: return go_op<1, GLU>(a, op, tiles, st);
+        case 2: return go_op<2, GLU>(a, op, tiles, st);
+        default: return go_op<4, GLU>(a, op, tiles, st);
+    }
 }
 
 // tile_rows: x rows per tile (32, 64 or 128; the sort's for a sorted routing).
@@ -96,18 +118,7 @@ int mx_gemm(const MxCall &c, int tile_rows, float *part, size_t part_bytes, hipS
             ga.part = part;
         }
     }
-    if (glu) {
-        switch (mxg_bt(tile_rows)) {
-            case 1: return go_p<1, true>(ga, tiles, st);
-            case 2: return go_p<2, true>(ga, tiles, st);
-            default: return go_p<4, true>(ga, tiles, st);
-        }
-    }
-    switch (mxg_bt(tile_rows)) {
-        case 1: return go_p<1, false>(ga, tiles, st);
-        case 2: return go_p<2, false>(ga, tiles, st);
-        default: return go_p<4, false>(ga, tiles, st);
-    }
+    return glu ? go_bt<true>(ga, c.x.op, tile_rows, tiles, st) : go_bt<false>(ga, c.x.op, tile_rows, tiles, st);
 }
 
 }  // namespace vqk

@@ -72,7 +72,17 @@ __device__ __forceinline__ int mx_y_row(const MxsArgs &p, int pos) {
     return p.meta && !p.ysorted ? p.order[pos] : pos;
 }
 
-template <int NT, int P, int NCW, bool GLU>
+template <int OP>
+__device__ __forceinline__ f32x4 mx_mma16(u32x4 x, u32x4 w, f32x4 c) {
+    if constexpr (OP == kOpBF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mx_b8, x), __builtin_bit_cast(mx_b8, w), c,
+                                                       0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, w), c, 0, 0, 0);
+}
+__device__ __forceinline__ float mx_swiglu(float g, float u) { return g / (1.f + __expf(-g)) * u; }
+
+template <int OP, int NT, int P, int NCW, bool GLU>
 __global__ void __launch_bounds__(64 * kMxsWaves, 2) k_mx_rows(const MxsArgs p) {
     constexpr int TT = GLU ? 2 : 1;
     // sums [2][8 waves][TT * NT][256] floats (KW > 1); before them x, [8 waves][16 rows][NCW * 256 bytes]
@@ -186,13 +196,12 @@ __global__ void __launch_bounds__(64 * kMxsWaves, 2) k_mx_rows(const MxsArgs p) 
                 const float s = mx_scale(bad ? 127u : sc[a][c]);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const mx_b8 wf = __builtin_bit_cast(mx_b8, mx_decode8(w[a][c][k], s));
+                    const u32x4 wf = mx_decode8_op<OP>(w[a][c][k], s);
 #pragma unroll
                     for (int pl = 0; pl < P; ++pl)
 #pragma unroll
                         for (int b = 0; b < NT; ++b)
-                            acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                __builtin_bit_cast(mx_b8, xf[pl][b][c][k]), wf, acc[a][b], 0, 0, 0);
+                            acc[a][b] = mx_mma16<OP>(xf[pl][b][c][k], wf, acc[a][b]);
                 }
             }
             // a NaN block makes its whole output column NaN, whichever of its lane groups holds it
@@ -209,9 +218,11 @@ __global__ void __launch_bounds__(64 * kMxsWaves, 2) k_mx_rows(const MxsArgs p) 
         auto put = [&](int row, int o, float v, float u) {
             const int64_t yr = mx_y_row(p, tile.row0 + row);
             if constexpr (GLU) {
-                float h = o < p.OUT ? v / (1.f + __expf(-v)) * u : 0.f;
-                for (int pl = 0; pl < p.yp; ++pl)
-                    static_cast<uint16_t *>(p.y)[pl * p.yplane + yr * p.ldy + o] = mx_plane_next(h);
+                float h = o < p.OUT ? mx_swiglu(v, u) : 0.f;
+                uint16_t *y = static_cast<uint16_t *>(p.y) + yr * p.ldy + o;
+                if constexpr (OP == kOpF16) *y = f32_to_h(h);
+                else
+                    for (int pl = 0; pl < p.yp; ++pl) y[pl * p.yplane] = mx_plane_next(h);
             } else {
                 store_act(p.y, p.y_type, yr * p.ldy + o, v);
             }

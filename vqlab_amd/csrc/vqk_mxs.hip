@@ -26,25 +26,28 @@ int64_t mx_tiles(const MxCall &c, int rows) {
 }
 
 // Chunks per wave that the registers hold: 16 per chunk and x operand, 9 for two
-// buffers of weights, 210 in all.
-constexpr int rows_cap(int xn, bool glu) { return 210 / (16 * xn + (glu ? 18 : 9)); }
+// buffers of weights, 200 in all. (20 rows of 5120 -> 17408, five chunks a wave at
+// 210: 25.6 us, the tiles of vqk_mxg.h 20.4; four chunks, 4096 -> 4096: 8.5 and 14.7.)
+constexpr int rows_cap(int xn, bool glu) { return 200 / (16 * xn + (glu ? 18 : 9)); }
 
 // Waves along k and chunks per wave, or kw = 0 where x does not fit.
 struct RowsPlan { int kw, ncw; };
-static RowsPlan rows_plan(int64_t NC, int xn, bool glu) {
+static RowsPlan rows_plan(int64_t NC, int xn, bool glu, int64_t row_tiles) {
     const int cap = rows_cap(xn, glu);
-    // about four chunks a wave keep enough weights in flight; fewer waves along k save the sums
+    // about four chunks a wave keep enough weights in flight, and fewer waves along k save the sums;
+    // a small product takes more of them, until each CU has a workgroup
     int kw = 1;
-    while (kw < kMxsWaves && (NC + kw - 1) / kw > (cap < 4 ? cap : 4)) kw *= 2;
+    while (kw < kMxsWaves && ((NC + kw - 1) / kw > (cap < 4 ? cap : 4) ||
+                              (NC > kw && row_tiles * kw < 256 * kMxsWaves))) kw *= 2;
     const int64_t ncw = (NC + kw - 1) / kw;
     return ncw <= cap ? RowsPlan{kw, int(ncw)} : RowsPlan{0, 0};
 }
 
 bool mx_rows_ok(const MxCall &c, int NT) {
-    return (NT == 1 || (NT == 2 && c.x.P == 1)) && rows_plan(c.g.NC, NT * c.x.P, c.codes[1] != nullptr).kw > 0;
+    return (NT == 1 || (NT == 2 && c.x.P == 1)) && rows_plan(c.g.NC, NT * c.x.P, c.codes[1] != nullptr, mx_tiles(c, 16 * NT) * c.g.RT).kw > 0;
 }
 
-template <int NT, int P, int NCW, bool GLU>
+template <int OP, int NT, int P, int NCW, bool GLU>
 static int go(MxsArgs a, int64_t tiles, int kw, hipStream_t st) {
     const int RW = kMxsWaves / kw;
     a.kw = kw;
@@ -63,19 +66,19 @@ static int go(MxsArgs a, int64_t tiles, int kw, hipStream_t st) {
     a.stage = !a.ids && !a.meta && a.N > 2;
     const size_t sums = kw > 1 ? size_t(2) * kMxsWaves * (GLU ? 2 : 1) * NT * 1024 : 0;
     const size_t xl = a.stage ? size_t(kMxsWaves) * NCW * 4096 : 0;
-    return launch_with_lds<k_mx_rows<NT, P, NCW, GLU>>(dim3(unsigned(grid)), dim3(64 * kMxsWaves),
+    return launch_with_lds<k_mx_rows<OP, NT, P, NCW, GLU>>(dim3(unsigned(grid)), dim3(64 * kMxsWaves),
                                                        sums > xl ? sums : xl, st, a);
 }
 
-template <int NT, int P, bool GLU, int NCW = 1>
+template <int OP, int NT, int P, bool GLU, int NCW = 1>
 static int go_ncw(const MxsArgs &a, int64_t tiles, RowsPlan pl, hipStream_t st) {
-    if (pl.ncw == NCW) return go<NT, P, NCW, GLU>(a, tiles, pl.kw, st);
-    if constexpr (NCW < rows_cap(NT * P, GLU)) return go_ncw<NT, P, GLU, NCW + 1>(a, tiles, pl, st);
+    if (pl.ncw == NCW) return go<OP, NT, P, NCW, GLU>(a, tiles, pl.kw, st);
+    if constexpr (NCW < rows_cap(NT * P, GLU)) return go_ncw<OP, NT, P, GLU, NCW + 1>(a, tiles, pl, st);
     return set_error(VQK_EINVAL, "MXFP4 product: no instance of %d chunks", pl.ncw);
 }
-template <int NT, int P>
+template <int OP, int NT, int P>
 static int go_glu(const MxsArgs &a, bool glu, int64_t tiles, RowsPlan pl, hipStream_t st) {
-    return glu ? go_ncw<NT, P, true>(a, tiles, pl, st) : go_ncw<NT, P, false>(a, tiles, pl, st);
+    return glu ? go_ncw<OP, NT, P, true>(a, tiles, pl, st) : go_ncw<OP, NT, P, false>(a, tiles, pl, st);
 }
 
 int mx_rows(const MxCall &c, int NT, hipStream_t st) {
@@ -84,12 +87,14 @@ int mx_rows(const MxCall &c, int NT, hipStream_t st) {
     mx_args(c, &a);
     const int64_t tiles = mx_tiles(c, 16 * NT);
     if (tiles == 0) return VQK_OK;
-    const RowsPlan pl = rows_plan(c.g.NC, NT * c.x.P, glu);
-    if (NT == 2) return go_glu<2, 1>(a, glu, tiles, pl, st);
+    const RowsPlan pl = rows_plan(c.g.NC, NT * c.x.P, glu, tiles * c.g.RT);
+    if (c.x.op == kOpF16)
+        return NT == 2 ? go_glu<kOpF16, 2, 1>(a, glu, tiles, pl, st) : go_glu<kOpF16, 1, 1>(a, glu, tiles, pl, st);
+    if (NT == 2) return go_glu<kOpBF16, 2, 1>(a, glu, tiles, pl, st);
     switch (c.x.P) {
-        case 1: return go_glu<1, 1>(a, glu, tiles, pl, st);
-        case 2: return go_glu<1, 2>(a, glu, tiles, pl, st);
-        default: return go_glu<1, 3>(a, glu, tiles, pl, st);
+        case 1: return go_glu<kOpBF16, 1, 1>(a, glu, tiles, pl, st);
+        case 2: return go_glu<kOpBF16, 1, 2>(a, glu, tiles, pl, st);
+        default: return go_glu<kOpBF16, 1, 3>(a, glu, tiles, pl, st);
     }
 }
 

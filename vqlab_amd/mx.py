@@ -37,7 +37,7 @@ def mx_quantize(x):
     xt = T.act_type(x)
     if x.ndim == 0:
         raise ValueError("mx_quantize takes rows, got a scalar")
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("mx_quantize has no gradient: detach x, or call it under no_grad")
     C, B = x.shape[-1], _blocks(x.shape[-1])
     with T.on_device(x):
@@ -46,10 +46,11 @@ def mx_quantize(x):
         else:
             rows, ld = x.contiguous(), C
         n = x.numel() // C if C else 0
-        codes = torch.empty((*x.shape[:-1], 16 * B), dtype=torch.uint8, device=x.device)
-        scales = torch.empty((*x.shape[:-1], B), dtype=torch.uint8, device=x.device)
+        lead = x.shape[:-1]
+        codes = torch.empty((*lead, 16 * B), dtype=torch.uint8, device=x.device)
+        scales = torch.empty((*lead, B), dtype=torch.uint8, device=x.device)
         L.check(L.lib().vqk_mx_quantize(rows.data_ptr(), xt, n, C, ld, codes.data_ptr(),
-                                        scales.data_ptr(), T.stream(x.device)), "mx_quantize")
+                                        scales.data_ptr(), T.raw_stream(x)), "mx_quantize")
     return codes, scales
 
 
@@ -74,7 +75,7 @@ def mx_dequantize(codes, scales, cols, dtype=torch.bfloat16):
         n = out.numel() // int(cols) if cols else 0
         L.check(L.lib().vqk_mx_dequantize(codes.data_ptr(), scales.data_ptr(), n, int(cols),
                                           out.data_ptr(), T.ACT_TYPES[dtype],
-                                          T.stream(codes.device)), "mx_dequantize")
+                                          T.raw_stream(codes)), "mx_dequantize")
     return out
 
 
@@ -89,12 +90,14 @@ def _ids32(ids, E):
     return (ids if ids.dtype == torch.int32 else ids.clamp(-1, E).to(torch.int32)).contiguous()
 
 
-def _desc(codes, scales, E, OUT, IN):
-    return L.VQKMXWeights(codes.data_ptr(), scales.data_ptr(), E, OUT, IN)
+def _desc(packed, E, OUT, IN):
+    codes, scales, f16_exact = packed
+    return L.VQKMXWeights(codes.data_ptr(), scales.data_ptr(), E, OUT, IN, f16_exact)
 
 
 def _pack(codes, scales, E, OUT, IN):
-    """Codes and scales of E weights in the kernels' operand order (laid out once)."""
+    """Codes and scales of E weights in the kernels' operand order (laid out once), and whether
+    every weight is an fp16 number (looked up once: the one wait for the GPU here)."""
     T.require_cuda(codes, scales)
     nc, ns = ctypes.c_size_t(), ctypes.c_size_t()
     L.check(L.lib().vqk_mx_pack_bytes(E, OUT, IN, ctypes.byref(nc), ctypes.byref(ns)), "MXFP4 weight")
@@ -102,15 +105,31 @@ def _pack(codes, scales, E, OUT, IN):
         codes, scales = _aligned(codes, 16), scales.contiguous()
         pc = torch.empty(nc.value, dtype=torch.uint8, device=codes.device)
         ps = torch.empty(ns.value, dtype=torch.uint8, device=codes.device)
+        inexact = torch.zeros(1, dtype=torch.int32, device=codes.device)
         L.check(L.lib().vqk_mx_pack(codes.data_ptr(), scales.data_ptr(), E, OUT, IN, pc.data_ptr(),
-                                    ps.data_ptr(), T.stream(codes.device)), "MXFP4 weight")
-    return pc, ps
+                                    ps.data_ptr(), inexact.data_ptr(), T.raw_stream(codes)),
+                "MXFP4 weight")
+        return pc, ps, int(inexact.item() == 0)
 
 
-def _work(query, dev, *args):
-    ws = ctypes.c_size_t()
-    L.check(query(*args, ctypes.byref(ws)), "workspace")
-    return (torch.empty(ws.value, dtype=torch.uint8, device=dev) if ws.value else None), ws.value
+def _ws_bytes(sizes, key, query, *args):
+    """Workspace bytes of a call, asked of the library once for each (shape, type)."""
+    n = sizes.get(key)
+    if n is None:
+        ws = ctypes.c_size_t()
+        L.check(query(*args, ctypes.byref(ws)), "workspace")
+        if len(sizes) > 4096:
+            sizes.clear()
+        n = sizes[key] = ws.value
+    return n
+
+
+def _work(like, n):
+    """A workspace of n bytes beside `like`, and its address (None, None: none needed)."""
+    if not n:
+        return None, None
+    t = torch.empty(n, dtype=torch.uint8, device=like.device)
+    return t, t.data_ptr()
 
 
 class _LinearFn(torch.autograd.Function):
@@ -128,11 +147,11 @@ class _LinearFn(torch.autograd.Function):
 
 
 class MXLinear(torch.nn.Module):
-    """Bias-free linear whose weight is MXFP4: codes uint8 [OUT, 16 B], scales uint8 [OUT, B].
+    """Bias-free linear whose weight is MXFP4: codes uint8 [OUT, 16 B], scales uint8 [OUT, B]
     (the module keeps its own copy, in the kernels' operand order). in_features may be any width of
-    the last block (default: all 32 of it). act: None multiplies x
-    as it is (bf16, fp16 and fp32 enter exactly, fp32 sums); "mxfp4" quantises x's rows as
-    mx_quantize does. Differentiable in x with act None; the weight is frozen."""
+    the last block (default: all 32 of it). act: None multiplies x as it is (bf16, fp16 and fp32
+    enter exactly, fp32 sums); "mxfp4" quantises x's rows as mx_quantize does. Differentiable in x
+    with act None; the weight is frozen."""
 
     def __init__(self, codes, scales, in_features=None, act=None):
         super().__init__()
@@ -143,7 +162,9 @@ class MXLinear(torch.nn.Module):
         IN = int(scales.shape[-1]) * BLOCK if in_features is None else int(in_features)
         _check_mx(codes, scales, IN, "MXLinear")
         self.in_features, self.out_features, self.act = IN, int(codes.shape[0]), act
-        self.packed, self.packed_scales = _pack(codes, scales, 1, self.out_features, IN)
+        self._packed = _pack(codes, scales, 1, self.out_features, IN)
+        self._w = _desc(self._packed, 1, self.out_features, IN)
+        self._sizes = {}
 
     @classmethod
     def from_weight(cls, weight, act=None):
@@ -156,37 +177,38 @@ class MXLinear(torch.nn.Module):
     def _product(self, x):
         IN, OUT = self.in_features, self.out_features
         act = L.VQK_MX_ACT_NONE if self.act is None else L.VQK_MX_ACT_MXFP4
-        xt, lib = T.act_type(x), L.lib()
+        xt, lib, w = T.act_type(x), L.lib(), ctypes.byref(self._w)
         with T.on_device(x):
-            xf = x.reshape(-1, IN).contiguous()
+            xf = T.rows_of(x, IN)
             N = xf.shape[0]
-            w = _desc(self.packed, self.packed_scales, 1, OUT, IN)
-            y = torch.empty((*x.shape[:-1], OUT), dtype=x.dtype, device=x.device)
-            work, size = _work(lib.vqk_mx_linear_workspace, x.device, ctypes.byref(w), xt, N, act)
-            L.check(lib.vqk_mx_linear(ctypes.byref(w), xf.data_ptr(), xt, N, act, y.data_ptr(), xt,
-                                      work.data_ptr() if size else None, size, T.stream(x.device)),
-                    "MXLinear")
+            y = x.new_empty((*x.shape[:-1], OUT))
+            size = _ws_bytes(self._sizes, (N, xt), lib.vqk_mx_linear_workspace, w, xt, N, act)
+            work, wp = _work(x, size)
+            rc = lib.vqk_mx_linear(w, xf.data_ptr(), xt, N, act, y.data_ptr(), xt, wp, size,
+                                   T.raw_stream(x))
+            if rc:
+                L.check(rc, "MXLinear")
         return y
 
     def _dx(self, dy):
         IN, OUT = self.in_features, self.out_features
-        dt, lib = T.act_type(dy), L.lib()
+        dt, lib, w = T.act_type(dy), L.lib(), ctypes.byref(self._w)
         with T.on_device(dy):
-            d = dy.reshape(-1, OUT).contiguous()
+            d = T.rows_of(dy, OUT)
             N = d.shape[0]
-            w = _desc(self.packed, self.packed_scales, 1, OUT, IN)
-            dx = torch.empty((*dy.shape[:-1], IN), dtype=dy.dtype, device=dy.device)
-            work, size = _work(lib.vqk_mx_linear_dx_workspace, dy.device, ctypes.byref(w), dt, N)
-            L.check(lib.vqk_mx_linear_dx(ctypes.byref(w), d.data_ptr(), dt, N, dx.data_ptr(), dt,
-                                         work.data_ptr() if size else None, size,
-                                         T.stream(dy.device)), "MXLinear gradient")
+            dx = dy.new_empty((*dy.shape[:-1], IN))
+            size = _ws_bytes(self._sizes, (N, dt, "dx"), lib.vqk_mx_linear_dx_workspace, w, dt, N)
+            work, wp = _work(dy, size)
+            L.check(lib.vqk_mx_linear_dx(w, d.data_ptr(), dt, N, dx.data_ptr(), dt, wp, size,
+                                         T.raw_stream(dy)), "MXLinear gradient")
         return dx
 
     def forward(self, x):
-        T.require_cuda(x, self.packed, self.packed_scales)
+        if x.device != self._packed[0].device:
+            raise ValueError(f"MXLinear on {self._packed[0].device}, x on {x.device}")
         if x.ndim == 0 or x.shape[-1] != self.in_features:
             raise ValueError(f"MXLinear: x {tuple(x.shape)} for in_features {self.in_features}")
-        if torch.is_grad_enabled() and x.requires_grad:
+        if x.requires_grad and torch.is_grad_enabled():
             if self.act is not None:
                 raise RuntimeError("MXLinear(act='mxfp4') has no gradient: the rounding of x has none")
             return _LinearFn.apply(x, self)
@@ -194,7 +216,7 @@ class MXLinear(torch.nn.Module):
 
 
 def _no_grad(what, *ts):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+    if any(t.requires_grad for t in ts) and torch.is_grad_enabled():
         raise RuntimeError(f"{what} has no gradient: run it under no_grad, or detach its inputs")
 
 
@@ -211,36 +233,35 @@ class MXSwitchLinear(torch.nn.Module):
         IN = int(scales.shape[-1]) * BLOCK if in_features is None else int(in_features)
         _check_mx(codes, scales, IN, "MXSwitchLinear")
         self.num_experts, self.output_dims, self.input_dims = int(codes.shape[0]), int(codes.shape[1]), IN
-        self.packed, self.packed_scales = _pack(codes, scales, *codes.shape[:2], IN)
+        self._packed = _pack(codes, scales, self.num_experts, self.output_dims, IN)
+        self._w = _desc(self._packed, self.num_experts, self.output_dims, IN)
+        self._sizes = {}
 
     @classmethod
     def from_weight(cls, weight):
         """The experts of a weight [E, OUT, IN], quantised here."""
         return cls(*mx_quantize(weight.detach()), weight.shape[2])
 
-    def _weights(self):
-        return _desc(self.packed, self.packed_scales, self.num_experts, self.output_dims, self.input_dims)
-
     def forward(self, x, indices):
-        T.require_cuda(x, indices, self.packed, self.packed_scales)
+        T.require_cuda(x, indices, self._packed[0])
         _no_grad("MXSwitchLinear", x)
         IN, OUT, k = self.input_dims, self.output_dims, int(indices.shape[-1])
         lead = tuple(indices.shape[:-1])
-        if x.shape[-1] != IN or tuple(x.shape[:-3]) != lead or x.shape[-2] != 1 or x.shape[-3] not in (1, k):
+        if x.ndim < 3 or x.shape[-1] != IN or tuple(x.shape[:-3]) != lead or x.shape[-2] != 1 or \
+                x.shape[-3] not in (1, k):
             raise ValueError(f"MXSwitchLinear: x {tuple(x.shape)} for indices {tuple(indices.shape)}, "
                              f"in_features {IN}")
-        xt, lib = T.act_type(x), L.lib()
+        xt, lib, w = T.act_type(x), L.lib(), ctypes.byref(self._w)
         with T.on_device(x):
-            xf = x.reshape(-1, IN).contiguous()
+            xf = T.rows_of(x, IN)
             eidx = _ids32(indices.reshape(-1), self.num_experts)
             rows, N = xf.shape[0], eidx.numel()
-            w = self._weights()
-            y = torch.empty((*lead, k, 1, OUT), dtype=x.dtype, device=x.device)
-            work, size = _work(lib.vqk_mx_switch_workspace, x.device, ctypes.byref(w), xt, rows, N)
-            L.check(lib.vqk_mx_switch(ctypes.byref(w), xf.data_ptr(), xt, rows, eidx.data_ptr(), N,
-                                      N // rows if rows else 1, y.data_ptr(), xt,
-                                      work.data_ptr() if size else None, size, T.stream(x.device)),
-                    "MXSwitchLinear")
+            y = x.new_empty((*lead, k, 1, OUT))
+            size = _ws_bytes(self._sizes, (rows, N, xt), lib.vqk_mx_switch_workspace, w, xt, rows, N)
+            work, wp = _work(x, size)
+            L.check(lib.vqk_mx_switch(w, xf.data_ptr(), xt, rows, eidx.data_ptr(), N,
+                                      N // rows if rows else 1, y.data_ptr(), xt, wp, size,
+                                      T.raw_stream(x)), "MXSwitchLinear")
         return y
 
 
@@ -256,28 +277,32 @@ class MXSwitchGLU(torch.nn.Module):
                 (d.num_experts, d.output_dims, d.input_dims) != (g.num_experts, g.input_dims, g.output_dims):
             raise ValueError("MXSwitchGLU: gate, up [E, I, H] and down [E, H, I] do not fit together")
         self.gate_proj, self.up_proj, self.down_proj = g, u, d
+        self._sizes = {}
 
     def forward(self, x, ids, weights):
-        T.require_cuda(x, ids, weights, self.gate_proj.packed)
+        T.require_cuda(x, ids, weights, self.gate_proj._packed[0])
         _no_grad("MXSwitchGLU", x, weights)
         H = self.gate_proj.input_dims
         if x.ndim != 2 or x.shape[1] != H or ids.ndim != 2 or ids.shape[0] != x.shape[0] or \
                 ids.shape != weights.shape:
             raise ValueError(f"MXSwitchGLU: x {tuple(x.shape)}, ids {tuple(ids.shape)}, weights "
                              f"{tuple(weights.shape)} for hidden size {H}")
+        return self._run(x, _ids32(ids, self.gate_proj.num_experts),
+                         weights.to(torch.float32).contiguous())
+
+    def _run(self, x, ids, wts):
         xt, lib = T.act_type(x), L.lib()
         n, k = ids.shape
+        ws = [ctypes.byref(m._w) for m in (self.gate_proj, self.up_proj, self.down_proj)]
         with T.on_device(x):
             x = x.contiguous()
-            ids = _ids32(ids, self.gate_proj.num_experts)
-            wts = weights.to(torch.float32).contiguous()
-            ws = [m._weights() for m in (self.gate_proj, self.up_proj, self.down_proj)]
-            refs = [ctypes.byref(w) for w in ws]
-            y = torch.empty_like(x)
-            work, size = _work(lib.vqk_mx_experts_workspace, x.device, *refs, xt, n, k)
-            L.check(lib.vqk_mx_experts(*refs, x.data_ptr(), xt, n, ids.data_ptr(), wts.data_ptr(), k,
-                                       y.data_ptr(), xt, work.data_ptr() if size else None, size,
-                                       T.stream(x.device)), "MXSwitchGLU")
+            y = x.new_empty(x.shape)
+            size = _ws_bytes(self._sizes, (n, k, xt), lib.vqk_mx_experts_workspace, *ws, xt, n, k)
+            work, wp = _work(x, size)
+            rc = lib.vqk_mx_experts(*ws, x.data_ptr(), xt, n, ids.data_ptr(), wts.data_ptr(), k,
+                                    y.data_ptr(), xt, wp, size, T.raw_stream(x))
+            if rc:
+                L.check(rc, "MXSwitchGLU")
         return y
 
 
@@ -296,8 +321,10 @@ class MXSparseMoeBlock(torch.nn.Module):
         if logits is None:
             logits = x.float() @ self.router_weight.float().T
         _no_grad("MXSparseMoeBlock", x, logits)
-        if logits.ndim != 2 or logits.shape != (x.shape[0], self.switch_mlp.gate_proj.num_experts):
-            raise ValueError(f"MXSparseMoeBlock: logits {tuple(logits.shape)} for x {tuple(x.shape)} and "
-                             f"{self.switch_mlp.gate_proj.num_experts} experts")
+        g = self.switch_mlp.gate_proj
+        T.require_cuda(x, logits, g._packed[0])
+        if x.ndim != 2 or x.shape[1] != g.input_dims or logits.shape != (x.shape[0], g.num_experts):
+            raise ValueError(f"MXSparseMoeBlock: x {tuple(x.shape)}, logits {tuple(logits.shape)} for "
+                             f"{g.num_experts} experts of width {g.input_dims}")
         ids, w = router.top_k(logits, self.top_k, self.norm_topk_prob, mask)
-        return self.switch_mlp(x, ids, w)
+        return self.switch_mlp._run(x, ids, w)

@@ -49,6 +49,10 @@ def _check(logits, mask):
     T.require_cuda(logits, mask)
 
 
+def _f32(g):
+    return g if g.dtype == torch.float32 and g.is_contiguous() else g.float().contiguous()
+
+
 def _rows(logits):
     """logits with contiguous rows, and the elements between them."""
     E = logits.shape[1]
@@ -69,8 +73,11 @@ def top_k(logits, k, norm_topk_prob=True, mask=None):
         w = torch.empty((n, k), dtype=torch.float32, device=lg.device)
         L.check(L.lib().vqk_route(lg.data_ptr(), T.act_type(lg), n, E, ld, mp, k,
                                   int(norm_topk_prob), ids.data_ptr(), w.data_ptr(), None, None,
-                                  None, None, 0, T.stream(lg.device)), "route")
+                                  None, None, 0, T.raw_stream(lg)), "route")
     return ids, w
+
+
+_sizes = {}                                     # (tokens, experts) -> workspace bytes
 
 
 class _RouteFn(torch.autograd.Function):
@@ -87,13 +94,18 @@ class _RouteFn(torch.autograd.Function):
             stats = torch.empty(3, dtype=torch.float32, device=dev)
             saved = torch.empty((n, 2), dtype=torch.float32, device=dev)
             lib = L.lib()
-            ws = ctypes.c_size_t()
-            L.check(lib.vqk_route_workspace(n, E, ctypes.byref(ws)), "route")
-            work = torch.empty(ws.value, dtype=torch.uint8, device=dev)
+            size = _sizes.get((n, E))
+            if size is None:
+                ws = ctypes.c_size_t()
+                L.check(lib.vqk_route_workspace(n, E, ctypes.byref(ws)), "route")
+                if len(_sizes) > 4096:
+                    _sizes.clear()
+                size = _sizes[(n, E)] = ws.value
+            work = torch.empty(size, dtype=torch.uint8, device=dev)
             L.check(lib.vqk_route(lg.data_ptr(), T.act_type(lg), n, E, ld, mp, k, norm,
                                   ids.data_ptr(), w.data_ptr(), counts.data_ptr(),
-                                  stats.data_ptr(), saved.data_ptr(), work.data_ptr(), ws.value,
-                                  T.stream(dev)), "route")
+                                  stats.data_ptr(), saved.data_ptr(), work.data_ptr(), size,
+                                  T.raw_stream(lg)), "route")
         balance, z, tokens = stats.unbind()
         ctx.save_for_backward(lg, ids, w, counts, stats, saved)
         ctx.k, ctx.norm, ctx.ld = k, norm, ld
@@ -108,12 +120,12 @@ class _RouteFn(torch.autograd.Function):
         n, E = lg.shape
         with T.on_device(lg):
             d = torch.empty((n, E), dtype=lg.dtype, device=lg.device)
-            grads = [None if g is None else g.to(torch.float32).contiguous() for g in (dw, db, dz)]
+            grads = [None if g is None else _f32(g) for g in (dw, db, dz)]
             L.check(L.lib().vqk_route_backward(
                 lg.data_ptr(), T.act_type(lg), n, E, ctx.ld, ctx.k, ctx.norm, ids.data_ptr(),
                 w.data_ptr(), counts.data_ptr(), stats.data_ptr(), saved.data_ptr(),
                 *(None if g is None else g.data_ptr() for g in grads), d.data_ptr(),
-                T.stream(lg.device)), "route backward")
+                T.raw_stream(lg)), "route backward")
         return d, None, None, None
 
 
