@@ -21,7 +21,7 @@ constexpr int64_t kMxMaxExperts = 4096;
 // experts have a few pairs each, then 32, 64 or 128 (the many-row kernel).
 static int mx_tile_rows(int64_t N, int64_t E) {
     const int64_t avg = N / E;
-    return avg <= 12 ? 16 : (avg <= 20 ? 32 : (avg <= 40 ? 64 : 128));
+    return avg <= 12 ? 16 : (avg <= 20 ? 32 : (avg <= 40 ? 64 : (avg <= 80 ? 96 : 128)));
 }
 static int run(const MxCall &c, int rows, hipStream_t st) {
     return rows == 16 && mx_rows_ok(c, 1) ? mx_rows(c, 1, st) : mx_gemm(c, rows, nullptr, 0, st);

@@ -12,7 +12,7 @@
 //   * x: the tile's 256-byte row pieces, copied global -> LDS without registers
 //     (16 bytes a lane); piece p of row n is stored at p ^ (n & 15), so the 16
 //     rows of a read phase fall on 16 different bank groups.
-// The loads of the next chunk are in flight while one multiplies; two
+// The loads of the next chunk (or two) are in flight while one multiplies; two
 // workgroups share a CU and fill each other's waits. The four conversions of a
 // fragment (v_cvt_scalef32_pk_bf16_fp4) issue in the shadow of the matrix
 // instructions: one conversion for each of them at BT = 4.
@@ -49,15 +49,26 @@ __device__ __forceinline__ f32x16v mx_mma32(u32x4 w, u32x4 x, f32x16v c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, w), __builtin_bit_cast(h8, x), c, 0, 0, 0);
 }
 
+// What x is past its rows' ends.
+static __device__ __align__(16) uint8_t mxg_zeros[16];
+
+// The counted waits need the loads of a stage where the source has them: none may
+// move across this.
+__device__ __forceinline__ void mxg_keep_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// ST: stages of x in LDS and of weights in registers (ST - 1 chunks in flight).
 // PL: x in more planes than one.
-template <int OP, int BT, bool GLU, bool PL>
+template <int OP, int BT, int ST, bool GLU, bool PL>
 __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga) {
     const MxsArgs &p = ga.a;
     constexpr int ROWS = 32 * BT;
     constexpr int STAGE = ROWS * 256;         // bytes of x per chunk
     constexpr int CPW = STAGE / 1024 / kMxgWaves;
     static_assert(CPW * kMxgWaves * 1024 == STAGE, "whole copies per wave");
-    extern __shared__ __align__(16) uint8_t xs[];       // [2][STAGE]
+    extern __shared__ __align__(16) uint8_t xs[];       // [ST][STAGE]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 31, g = lane >> 5;
 
@@ -103,56 +114,66 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
         }
         // the x copies of this lane: 16 bytes of one row each
         const uint16_t *src[CPW];
-        int piece[CPW];
+        int piece[CPW], xrow[CPW];
+#pragma unroll
+        for (int j = 0; j < CPW; ++j)
+            xrow[j] = tile.row0 + min((j * kMxgWaves + wave) * 4 + (lane >> 4), tile.nrows - 1);
+        mx_x_rows(p, xrow);
 #pragma unroll
         for (int j = 0; j < CPW; ++j) {
             const int n = (j * kMxgWaves + wave) * 4 + (lane >> 4);
             piece[j] = (lane & 15) ^ (n & 15);
-            src[j] = p.x + int64_t(mx_x_row(p, tile.row0 + min(n, tile.nrows - 1))) * p.xld + piece[j] * 8;
+            src[j] = p.x + int64_t(xrow[j]) * p.xld + piece[j] * 8;
         }
-        // NA: groups of 32 rows that the tile holds
-        auto issue = [&](int c, int pl, int buf, auto na) {
+        struct Weights {
+            u32x4 w[2][2];
+            uint32_t s[2][2];
+        };
+        Weights wb[ST];
+        // steps: chunk c_lo + step / P, plane step % P (the weights again for each plane). NA: groups of
+        // 32 rows that the tile holds
+        const int P = PL ? ga.planes : 1, steps = (c_hi - c_lo) * P;
+        auto issue = [&](int step, auto slot, auto na) {
+            const int c = c_lo + (PL ? step / P : step), pl = PL ? step % P : 0;
+            constexpr int S = decltype(slot)::value;
 #pragma unroll
             for (int j = 0; j < 2 * decltype(na)::value; ++j) {
-                // past the row's last block: the row's start again (multiplied by no weight, masked below)
-                const bool in = 4 * c + piece[j] / 4 < p.NB;
-                const uint16_t *s = src[j] + pl * p.xplane + (in ? int64_t(c) * kMxChunk : -int64_t(piece[j] * 8));
-                __builtin_amdgcn_global_load_lds((global_void *)s,
-                                                 (lds_void *)(xs + buf * STAGE + (j * kMxgWaves + wave) * 1024), 16, 0, 0);
+                // past the row's last block: zeros
+                const uint16_t *from = src[j] + pl * p.xplane + int64_t(c) * kMxChunk;
+                from = 4 * c + piece[j] / 4 < p.NB ? from : reinterpret_cast<const uint16_t *>(mxg_zeros);
+                __builtin_amdgcn_global_load_lds((global_void *)from,
+                                                 (lds_void *)(xs + S * STAGE + (j * kMxgWaves + wave) * 1024), 16, 0, 0);
             }
-        };
-        u32x4 w[2][2], wn[2][2];
-        uint32_t s[2][2], sn[2][2];
-        auto load_w = [&](int c, u32x4 (&ww)[2][2], uint32_t (&ss)[2][2]) {
 #pragma unroll
             for (int a = 0; a < 2; ++a)
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    ww[a][q] = *reinterpret_cast<const u32x4 *>(cb[a] + (wo[a] + uint32_t(c) * 1024u + q * 256u));
-                    ss[a][q] = sb[a][so[a] + uint32_t(c / 4) * 256u + q * 64u + uint32_t(c % 4)];
+                    wb[S].w[a][q] = *reinterpret_cast<const u32x4 *>(cb[a] + (wo[a] + uint32_t(c) * 1024u + q * 256u));
+                    wb[S].s[a][q] = *reinterpret_cast<const uint32_t *>(sb[a] + (so[a] + uint32_t(c / 4) * 256u + q * 64u));
                 }
         };
-        auto mul = [&](int c, int buf, auto na) {
-            const bool tail = 4 * c + 4 > p.NB;
+        auto mul = [&](int step, auto slot, auto na) {
+            constexpr int S = decltype(slot)::value;
+            const Weights &d = wb[S];
+            const int c = c_lo + (PL ? step / P : step);
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 float sc[2];
 #pragma unroll
                 for (int a = 0; a < 2; ++a) {
-                    nan[a] = nan[a] || s[a][q] == 255u;
-                    sc[a] = mx_scale(s[a][q] == 255u ? 127u : s[a][q]);
+                    const uint32_t b = (d.s[a][q] >> (8 * (c & 3))) & 255u;
+                    nan[a] = nan[a] || b == 255u;
+                    sc[a] = mx_scale(b == 255u ? 127u : b);
                 }
-                const bool in = !tail || 4 * c + 2 * g + q < p.NB;
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
                     u32x4 wf[2];
 #pragma unroll
-                    for (int a = 0; a < 2; ++a) wf[a] = mx_decode8_op<OP>(w[a][q][h], sc[a]);
+                    for (int a = 0; a < 2; ++a) wf[a] = mx_decode8_op<OP>(d.w[a][q][h], sc[a]);
                     const int at = ((8 * g + 4 * q + h) ^ (lane & 15)) * 16 + r * 256;
 #pragma unroll
                     for (int b = 0; b < decltype(na)::value; ++b) {
-                        u32x4 xv = *reinterpret_cast<const u32x4 *>(xs + buf * STAGE + b * 8192 + at);
-                        if (tail && !in) xv = u32x4{};
+                        const u32x4 xv = *reinterpret_cast<const u32x4 *>(xs + S * STAGE + b * 8192 + at);
 #pragma unroll
                         for (int a = 0; a < 2; ++a) acc[a][b] = mx_mma32<OP>(wf[a], xv, acc[a][b]);
                     }
@@ -161,36 +182,40 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
         };
         // steps: chunk c_lo + step / P, plane step % P
         auto walk = [&](auto na) {
-            const int P = PL ? ga.planes : 1, steps = (c_hi - c_lo) * P;
-            if (steps > 0) {
-                issue(c_lo, 0, 0, na);
-                load_w(c_lo, wn, sn);
+            constexpr int OPS = 2 * decltype(na)::value + 8;      // loads of a stage
+            using s0 = std::integral_constant<int, 0>;
+            using s1 = std::integral_constant<int, 1>;
+            using s2 = std::integral_constant<int, ST - 1>;
+            // past the last step it is loaded again, into a slot that no step reads, and the steps run in
+            // whole rounds of the slots: on every path a step issues the same loads, so that the counted
+            // wait stands for the compiler as well (it adds none of its own)
+            auto one = [&](int step, auto slot) {
+                // this wave's loads of the step (those of the next may be on their way), then every
+                // wave's; every wave is done with the slot that is filled next
+                mxg_keep_order();
+                wait_vmcnt<(ST - 2) * OPS>();
+                __builtin_amdgcn_s_waitcnt(0xC07F);       // lgkmcnt(0): this wave's reads of that slot
+                __builtin_amdgcn_s_barrier();             // (a __syncthreads would wait for every load)
+                mxg_keep_order();
+                issue(min(step + ST - 1, steps - 1),
+                      std::integral_constant<int, (decltype(slot)::value + ST - 1) % ST>{}, na);
+                mxg_keep_order();
+                if (step < steps) mul(step, slot, na);
+            };
+            if (steps <= 0) return;
+            issue(0, s0{}, na);
+            mxg_keep_order();
+            if constexpr (ST == 3) {
+                issue(min(1, steps - 1), s1{}, na);
+                mxg_keep_order();
             }
-            int c = c_lo, pl = 0;
 #pragma unroll 1
-            for (int step = 0; step < steps; ++step) {
-                wait_vmem();                  // this wave's copies of the step, and its weights
-                __syncthreads();              // every wave's copies; every wave is done with the other buffer
-                if (!PL || pl == 0) {
-#pragma unroll
-                    for (int a = 0; a < 2; ++a)
-#pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            w[a][q] = wn[a][q];
-                            s[a][q] = sn[a][q];
-                        }
-                }
-                const int cc = c;
-                if (!PL || ++pl == P) {
-                    pl = 0;
-                    ++c;
-                }
-                if (step + 1 < steps) {
-                    issue(c, pl, (step + 1) & 1, na);
-                    if (!PL || pl == 0) load_w(c, wn, sn);
-                }
-                mul(cc, step & 1, na);
+            for (int step = 0; step < steps; step += ST) {
+                one(step, s0{});
+                one(step + 1, s1{});
+                if constexpr (ST == 3) one(step + 2, s2{});
             }
+            wait_vmem();
         };
         const int groups = (tile.nrows + 31) / 32;
         if (BT > 1 && groups <= 1) walk(std::integral_constant<int, 1>{});
@@ -211,11 +236,15 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
         const int o = 8 * (i / 4) + 4 * g + i % 4;
         return (nm[a] >> o) & 1 ? __uint_as_float(0x7fc00000u) : acc[a][b][i];
     };
+    int yrow[BT];
+#pragma unroll
+    for (int b = 0; b < BT; ++b) yrow[b] = tile.row0 + min(32 * b + r, tile.nrows - 1);
+    mx_y_rows(p, yrow);
 #pragma unroll
     for (int b = 0; b < BT; ++b) {
         const int n = 32 * b + r;
         if (n >= tile.nrows) continue;
-        const int64_t yr = mx_y_row(p, tile.row0 + n);
+        const int64_t yr = yrow[b];
         if constexpr (GLU) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {

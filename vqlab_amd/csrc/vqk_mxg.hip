@@ -1,6 +1,11 @@
 // Launch of the many-row MXFP4 products (kernel in vqk_mxg.h).
 #include "vqk_mxg.h"
 
+#ifndef VQ_ST1
+#define VQ_ST1 3
+#define VQ_ST2 3
+#define VQ_ST3 3
+#endif
 namespace vqk {
 
 struct MxRedArgs {
@@ -57,8 +62,6 @@ int mx_splits(int64_t T, int64_t NC, int64_t n, float t1, float t2) {
     return best;
 }
 
-static int mxg_bt(int64_t rows) { return rows <= 32 ? 1 : (rows <= 64 ? 2 : 4); }
-
 static int dense_splits(int64_t N, const MxGeom &g) {
     const int rows = mxg_dense_rows(N);
     const float f = rows == 128 ? 1.f : (rows == 64 ? 0.7f : 0.55f);
@@ -73,34 +76,34 @@ size_t mxg_part_bytes(int64_t N, const MxGeom &g) {
     return s > 1 ? size_t(s) * N * g.OUT * 4 : 0;
 }
 
-template <int OP, int BT, bool GLU, bool PL>
+template <int OP, int BT, int ST, bool GLU, bool PL>
 static int go(MxgArgs ga, int64_t tiles, hipStream_t st) {
     MxsArgs &a = ga.a;
     a.nob = int32_t((a.ocover + (GLU ? kMxgRows / 2 : kMxgRows) - 1) / (GLU ? kMxgRows / 2 : kMxgRows));
     const int64_t grid = int64_t(a.nob) * tiles * ga.splits;
     if (grid > INT32_MAX) return set_error(VQK_ENOTIMPL, "MXFP4 product: grid too large");
     ga.ntiles_host = int32_t(tiles);
-    int rc = launch_with_lds<k_mx_gemm<OP, BT, GLU, PL>>(dim3(unsigned(grid)), dim3(64 * kMxgWaves),
-                                                        size_t(2) * 32 * BT * 256, st, ga);
+    int rc = launch_with_lds<k_mx_gemm<OP, BT, ST, GLU, PL>>(dim3(unsigned(grid)), dim3(64 * kMxgWaves),
+                                                        size_t(ST) * 32 * BT * 256, st, ga);
     if (rc || ga.splits == 1) return rc;
     return launch_mx_reduce(ga.part, ga.splits, a.N * a.OUT, a.y, a.y_type, st);
 }
 
-template <int BT, bool GLU>
+template <int BT, int ST, bool GLU>
 static int go_op(const MxgArgs &a, int op, int64_t tiles, hipStream_t st) {
-    if (op == kOpF16) return go<kOpF16, BT, GLU, false>(a, tiles, st);
-    return a.planes == 1 ? go<kOpBF16, BT, GLU, false>(a, tiles, st) : go<kOpBF16, BT, GLU, true>(a, tiles, st);
+    if (op == kOpF16) return go<kOpF16, BT, ST, GLU, false>(a, tiles, st);
+    return a.planes == 1 ? go<kOpBF16, BT, ST, GLU, false>(a, tiles, st)
+                         : go<kOpBF16, BT, ST, GLU, true>(a, tiles, st);
 }
 template <bool GLU>
 static int go_bt(const MxgArgs &a, int op, int tile_rows, int64_t tiles, hipStream_t st) {
-    switch (mxg_bt(tile_rows)) {
-        case 1: return go_op<1, GLU>(a, op, tiles, st);
-        case 2: return go_op<2, GLU>(a, op, tiles, st);
-        default: return go_op<4, GLU>(a, op, tiles, st);
-    }
+    if (tile_rows <= 32) return go_op<1, VQ_ST1, GLU>(a, op, tiles, st);
+    if (tile_rows <= 64) return go_op<2, VQ_ST2, GLU>(a, op, tiles, st);
+    if (tile_rows <= 96) return go_op<3, VQ_ST3, GLU>(a, op, tiles, st);
+    return go_op<4, 2, GLU>(a, op, tiles, st);
 }
 
-// tile_rows: x rows per tile (32, 64 or 128; the sort's for a sorted routing).
+// tile_rows: x rows per tile (32, 64, 96 or 128; the sort's for a sorted routing).
 int mx_gemm(const MxCall &c, int tile_rows, float *part, size_t part_bytes, hipStream_t st) {
     const bool glu = c.codes[1] != nullptr;
     MxgArgs ga{};

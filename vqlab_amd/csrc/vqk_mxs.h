@@ -63,13 +63,24 @@ __device__ __forceinline__ bool mx_tile(const MxsArgs &p, int t, MxTile *out) {
     out->nrows = __builtin_amdgcn_readfirstlane(out->nrows);
     return true;
 }
-__device__ __forceinline__ int mx_x_row(const MxsArgs &p, int pos) {
-    if (p.xkrep == 0) return pos;
-    const int pair = p.meta ? p.order[pos] : pos;
-    return p.xkrep == 1 ? pair : int(uint32_t(pair) / uint32_t(p.xkrep));
+// Tile positions -> rows of x / of y, in place; the loads of one call run together.
+template <int N>
+__device__ __forceinline__ void mx_x_rows(const MxsArgs &p, int (&pos)[N]) {
+    if (p.xkrep == 0) return;
+    if (p.meta) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) pos[i] = load_global(p.order, pos[i]);
+    }
+    if (p.xkrep != 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) pos[i] = int(uint32_t(pos[i]) / uint32_t(p.xkrep));
+    }
 }
-__device__ __forceinline__ int mx_y_row(const MxsArgs &p, int pos) {
-    return p.meta && !p.ysorted ? p.order[pos] : pos;
+template <int N>
+__device__ __forceinline__ void mx_y_rows(const MxsArgs &p, int (&pos)[N]) {
+    if (!p.meta || p.ysorted) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) pos[i] = load_global(p.order, pos[i]);
 }
 
 template <int OP>
@@ -125,7 +136,7 @@ __global__ void __launch_bounds__(64 * kMxsWaves, 2) k_mx_rows(const MxsArgs p) 
 
     u32x4 xf[P][NT][NCW][4];
     auto x_in = [&](int c) { return 4 * (kw * NCW + c) + g < p.NB; };   // this lane's block of x exists
-    if (p.stage) {
+    if (p.stage) {                            // dense rows only: a tile's rows lie one after the other
         uint8_t *xl = smem + wave * (NCW * 4096);
 #pragma unroll
         for (int pl = 0; pl < P; ++pl)
@@ -138,8 +149,7 @@ __global__ void __launch_bounds__(64 * kMxsWaves, 2) k_mx_rows(const MxsArgs p) 
                     const int u = i * 64 + lane, row = u / (16 * NCW), piece = (u % (16 * NCW)) ^ row;
                     const int64_t k = int64_t(kw) * NCW * kMxChunk + piece * 8;
                     if (b * 16 + row < tile.nrows) {          // else the unit stays as it is: zeroed below
-                        const uint16_t *src = p.x + pl * p.xplane +
-                                              int64_t(mx_x_row(p, tile.row0 + b * 16 + row)) * p.xld +
+                        const uint16_t *src = p.x + pl * p.xplane + int64_t(tile.row0 + b * 16 + row) * p.xld +
                                               (k < int64_t(p.NB) * kMxBlock ? k : 0);
                         __builtin_amdgcn_global_load_lds((global_void *)src, (lds_void *)(xl + i * 1024), 16, 0, 0);
                     }
@@ -157,10 +167,14 @@ __global__ void __launch_bounds__(64 * kMxsWaves, 2) k_mx_rows(const MxsArgs p) 
             }
         __syncthreads();                      // the sums use the same LDS
     } else {
+        int xrow[NT];
+#pragma unroll
+        for (int b = 0; b < NT; ++b) xrow[b] = tile.row0 + min(b * 16 + r, tile.nrows - 1);
+        mx_x_rows(p, xrow);
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
             const bool row_in = live && b * 16 + r < tile.nrows;
-            const uint16_t *xp = p.x + (row_in ? int64_t(mx_x_row(p, tile.row0 + b * 16 + r)) : 0) * p.xld;
+            const uint16_t *xp = p.x + int64_t(xrow[b]) * p.xld;
 #pragma unroll
             for (int pl = 0; pl < P; ++pl)
 #pragma unroll
@@ -216,7 +230,9 @@ __global__ void __launch_bounds__(64 * kMxsWaves, 2) k_mx_rows(const MxsArgs p) 
             }
         }
         auto put = [&](int row, int o, float v, float u) {
-            const int64_t yr = mx_y_row(p, tile.row0 + row);
+            int yr_[1] = {tile.row0 + row};
+            mx_y_rows(p, yr_);
+            const int64_t yr = yr_[0];
             if constexpr (GLU) {
                 float h = o < p.OUT ? mx_swiglu(v, u) : 0.f;
                 uint16_t *y = static_cast<uint16_t *>(p.y) + yr * p.ldy + o;
