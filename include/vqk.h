@@ -468,6 +468,16 @@ int vqk_mx_experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, const v
                    int32_t top_k, void *y, int32_t y_type, void *workspace, size_t ws_bytes,
                    void *stream);
 
+/* The same with the routing of vqk_route (below) in front: logits [T, E], rows ld
+ * elements apart; mask [T] or NULL. Padding tokens (mask 0) give rows of zeros. */
+int vqk_mx_moe_workspace(const vqk_mx_weights *gate, const vqk_mx_weights *up,
+                         const vqk_mx_weights *down, int32_t x_type, int64_t T, int32_t top_k,
+                         size_t *bytes);
+int vqk_mx_moe(const vqk_mx_weights *gate, const vqk_mx_weights *up, const vqk_mx_weights *down,
+               const void *x, int32_t x_type, int64_t T, const void *logits, int32_t l_type,
+               int64_t ld, const uint8_t *mask, int32_t top_k, int32_t norm_topk, void *y,
+               int32_t y_type, void *workspace, size_t ws_bytes, void *stream);
+
 /* ---- router -------------------------------------------------------------------
  * The layer calls' routing (softmax, top_k, renormalised when norm_topk != 0)
  * as a call of its own, with what training it needs. logits [T, E] rows ld

@@ -119,6 +119,9 @@ SIGNATURES = {
                                          ctypes.POINTER(c_sz)]),
     "vqk_mx_experts": (c_i32, [_MXW, _MXW, _MXW, c_p, c_i32, c_i64, c_p, c_p, c_i32, c_p, c_i32,
                                c_p, c_sz, c_p]),
+    "vqk_mx_moe_workspace": (c_i32, [_MXW, _MXW, _MXW, c_i32, c_i64, c_i32, ctypes.POINTER(c_sz)]),
+    "vqk_mx_moe": (c_i32, [_MXW, _MXW, _MXW, c_p, c_i32, c_i64, c_p, c_i32, c_i64, c_p, c_i32, c_i32,
+                           c_p, c_i32, c_p, c_sz, c_p]),
     "vqk_route_workspace": (c_i32, [c_i64, c_i64, ctypes.POINTER(c_sz)]),
     "vqk_route": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, c_p, c_i32, c_i32, c_p, c_p, c_p, c_p,
                           c_p, c_p, c_sz, c_p]),

@@ -18,10 +18,12 @@ constexpr int64_t kMxPairsUnsorted = 64;
 constexpr int64_t kMxMaxExperts = 4096;
 
 // Rows per tile of a routing of N pairs over E experts: 16 (the streaming kernel) while
-// experts have a few pairs each, then 32, 64 or 128 (the many-row kernel).
+// experts have a few pairs each, then 32, 64 or 128 (the many-row kernel, whose tiles cost
+// the rows they hold: 60 rows an expert take 111 + 81 us in tiles of 128, 124 + 104 in tiles
+// of 64, 111 + 91 in tiles of 96; 256 experts of 2048 x 512).
 static int mx_tile_rows(int64_t N, int64_t E) {
     const int64_t avg = N / E;
-    return avg <= 12 ? 16 : (avg <= 20 ? 32 : (avg <= 40 ? 64 : (avg <= 80 ? 96 : 128)));
+    return avg <= 12 ? 16 : (avg <= 20 ? 32 : (avg <= 40 ? 64 : 128));
 }
 static int run(const MxCall &c, int rows, hipStream_t st) {
     return rows == 16 && mx_rows_ok(c, 1) ? mx_rows(c, 1, st) : mx_gemm(c, rows, nullptr, 0, st);
@@ -174,6 +176,11 @@ extern "C" int vqk_mx_switch(const vqk_mx_weights *w, const void *x, int32_t x_t
     return run(c, rows, st);
 }
 
+static int experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, const vqk_mx_weights *down,
+                   const MxGeom &g1, const MxGeom &g2, const ExpertsPlan &p, const void *x, int32_t x_type,
+                   int64_t T, const int32_t *ids, const float *wts, int32_t top_k, void *y, int32_t y_type,
+                   uint8_t *ws, hipStream_t st);
+
 extern "C" int vqk_mx_experts_workspace(const vqk_mx_weights *gate, const vqk_mx_weights *up,
                                         const vqk_mx_weights *down, int32_t x_type, int64_t T,
                                         int32_t top_k, size_t *bytes) {
@@ -201,8 +208,15 @@ extern "C" int vqk_mx_experts(const vqk_mx_weights *gate, const vqk_mx_weights *
         return set_error(VQK_ENOSPACE, "mx experts: workspace %zu < %zu", ws_bytes, p.total);
     if (reinterpret_cast<uintptr_t>(workspace) & 255)
         return set_error(VQK_EINVAL, "mx experts: workspace must be 256-byte aligned");
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    return experts(gate, up, down, g1, g2, p, x, x_type, T, ids, wts, top_k, y, y_type,
+                   static_cast<uint8_t *>(workspace), static_cast<hipStream_t>(stream));
+}
+
+static int experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, const vqk_mx_weights *down,
+                   const MxGeom &g1, const MxGeom &g2, const ExpertsPlan &p, const void *x, int32_t x_type,
+                   int64_t T, const int32_t *ids, const float *wts, int32_t top_k, void *y, int32_t y_type,
+                   uint8_t *ws, hipStream_t st) {
+    int rc;
     const bool sorted = p.N > kMxPairsUnsorted;
     const int rows = sorted ? mx_tile_rows(p.N, g1.E) : 16;
     MxCall c{};
@@ -239,4 +253,44 @@ extern "C" int vqk_mx_experts(const vqk_mx_weights *gate, const vqk_mx_weights *
         if ((rc = hip_status(hipGetLastError(), "combine launch"))) return rc;
     }
     return VQK_OK;
+}
+
+// The block of experts with its routing: ids and weights in the workspace.
+static size_t ids_bytes(int64_t N) { return al256(size_t(N) * 4); }
+
+extern "C" int vqk_mx_moe_workspace(const vqk_mx_weights *gate, const vqk_mx_weights *up,
+                                    const vqk_mx_weights *down, int32_t x_type, int64_t T, int32_t top_k,
+                                    size_t *bytes) {
+    MxGeom g1, g2;
+    ExpertsPlan p;
+    const int rc = plan_experts(gate, up, down, x_type, T, top_k, &g1, &g2, &p);
+    if (rc) return rc;
+    if (!bytes) return set_error(VQK_EINVAL, "mx moe: NULL bytes");
+    *bytes = p.total + 2 * ids_bytes(p.N);
+    return VQK_OK;
+}
+
+extern "C" int vqk_mx_moe(const vqk_mx_weights *gate, const vqk_mx_weights *up, const vqk_mx_weights *down,
+                          const void *x, int32_t x_type, int64_t T, const void *logits, int32_t l_type,
+                          int64_t ld, const uint8_t *mask, int32_t top_k, int32_t norm_topk, void *y,
+                          int32_t y_type, void *workspace, size_t ws_bytes, void *stream) {
+    MxGeom g1, g2;
+    ExpertsPlan p;
+    int rc = plan_experts(gate, up, down, x_type, T, top_k, &g1, &g2, &p);
+    if (rc) return rc;
+    if (!out_size(y_type)) return set_error(VQK_EINVAL, "mx moe: y type %d", y_type);
+    if (T == 0) return VQK_OK;
+    if (!x || !logits || !y) return set_error(VQK_EINVAL, "mx moe: NULL pointer");
+    const size_t need = p.total + 2 * ids_bytes(p.N);
+    if (!workspace || ws_bytes < need) return set_error(VQK_ENOSPACE, "mx moe: workspace %zu < %zu", ws_bytes, need);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255)
+        return set_error(VQK_EINVAL, "mx moe: workspace must be 256-byte aligned");
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    int32_t *ids = reinterpret_cast<int32_t *>(ws + p.total);
+    float *wts = reinterpret_cast<float *>(ws + p.total + ids_bytes(p.N));
+    rc = vqk_route(logits, l_type, T, g1.E, ld, mask, top_k, norm_topk, ids, wts, nullptr, nullptr, nullptr,
+                   nullptr, 0, stream);
+    if (rc) return rc;
+    return experts(gate, up, down, g1, g2, p, x, x_type, T, ids, wts, top_k, y, y_type, ws,
+                   static_cast<hipStream_t>(stream));
 }

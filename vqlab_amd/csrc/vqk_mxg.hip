@@ -1,11 +1,6 @@
 // Launch of the many-row MXFP4 products (kernel in vqk_mxg.h).
 #include "vqk_mxg.h"
 
-#ifndef VQ_ST1
-#define VQ_ST1 3
-#define VQ_ST2 3
-#define VQ_ST3 3
-#endif
 namespace vqk {
 
 struct MxRedArgs {
@@ -97,13 +92,13 @@ static int go_op(const MxgArgs &a, int op, int64_t tiles, hipStream_t st) {
 }
 template <bool GLU>
 static int go_bt(const MxgArgs &a, int op, int tile_rows, int64_t tiles, hipStream_t st) {
-    if (tile_rows <= 32) return go_op<1, VQ_ST1, GLU>(a, op, tiles, st);
-    if (tile_rows <= 64) return go_op<2, VQ_ST2, GLU>(a, op, tiles, st);
-    if (tile_rows <= 96) return go_op<3, VQ_ST3, GLU>(a, op, tiles, st);
+    // three stages where registers and LDS leave two workgroups a CU
+    if (tile_rows <= 32) return go_op<1, 3, GLU>(a, op, tiles, st);
+    if (tile_rows <= 64) return go_op<2, 3, GLU>(a, op, tiles, st);
     return go_op<4, 2, GLU>(a, op, tiles, st);
 }
 
-// tile_rows: x rows per tile (32, 64, 96 or 128; the sort's for a sorted routing).
+// tile_rows: x rows per tile (32, 64 or 128; the sort's for a sorted routing).
 int mx_gemm(const MxCall &c, int tile_rows, float *part, size_t part_bytes, hipStream_t st) {
     const bool glu = c.codes[1] != nullptr;
     MxgArgs ga{};

@@ -277,6 +277,7 @@ class MXSwitchGLU(torch.nn.Module):
                 (d.num_experts, d.output_dims, d.input_dims) != (g.num_experts, g.input_dims, g.output_dims):
             raise ValueError("MXSwitchGLU: gate, up [E, I, H] and down [E, H, I] do not fit together")
         self.gate_proj, self.up_proj, self.down_proj = g, u, d
+        self._refs = [ctypes.byref(m._w) for m in (g, u, d)]
         self._sizes = {}
 
     def forward(self, x, ids, weights):
@@ -293,7 +294,7 @@ class MXSwitchGLU(torch.nn.Module):
     def _run(self, x, ids, wts):
         xt, lib = T.act_type(x), L.lib()
         n, k = ids.shape
-        ws = [ctypes.byref(m._w) for m in (self.gate_proj, self.up_proj, self.down_proj)]
+        ws = self._refs
         with T.on_device(x):
             x = x.contiguous()
             y = x.new_empty(x.shape)
@@ -316,15 +317,29 @@ class MXSparseMoeBlock(torch.nn.Module):
         super().__init__()
         self.switch_mlp, self.top_k = switch_mlp, int(top_k)
         self.norm_topk_prob, self.router_weight = bool(norm_topk_prob), router_weight
+        self._sizes = {}
 
     def forward(self, x, logits=None, mask=None):
         if logits is None:
             logits = x.float() @ self.router_weight.float().T
         _no_grad("MXSparseMoeBlock", x, logits)
         g = self.switch_mlp.gate_proj
-        T.require_cuda(x, logits, g._packed[0])
+        T.require_cuda(x, logits, mask, g._packed[0])
         if x.ndim != 2 or x.shape[1] != g.input_dims or logits.shape != (x.shape[0], g.num_experts):
             raise ValueError(f"MXSparseMoeBlock: x {tuple(x.shape)}, logits {tuple(logits.shape)} for "
                              f"{g.num_experts} experts of width {g.input_dims}")
-        ids, w = router.top_k(logits, self.top_k, self.norm_topk_prob, mask)
-        return self.switch_mlp._run(x, ids, w)
+        m = router.mask_bytes(mask, logits)
+        xt, lib, glu, k = T.act_type(x), L.lib(), self.switch_mlp, self.top_k
+        n = x.shape[0]
+        with T.on_device(x):
+            x = x.contiguous()
+            lg, ld = router.rows(logits)
+            y = x.new_empty(x.shape)
+            size = _ws_bytes(self._sizes, (n, xt, k), lib.vqk_mx_moe_workspace, *glu._refs, xt, n, k)
+            work, wp = _work(x, size)
+            rc = lib.vqk_mx_moe(*glu._refs, x.data_ptr(), xt, n, lg.data_ptr(), T.act_type(lg), ld,
+                                None if m is None else m.data_ptr(), k, int(self.norm_topk_prob),
+                                y.data_ptr(), xt, wp, size, T.raw_stream(x))
+            if rc:
+                L.check(rc, "MXSparseMoeBlock")
+        return y

@@ -31,15 +31,15 @@ class Route(NamedTuple):
     tokens: torch.Tensor
 
 
-def _mask_ptr(mask, logits):
+def mask_bytes(mask, logits):
+    """mask [T] (bool / uint8) of logits [T, E] as contiguous bytes, or None."""
     if mask is None:
-        return None, None
+        return None
     if mask.dtype not in (torch.bool, torch.uint8):
         raise ValueError(f"mask must be bool or uint8, got {mask.dtype}")
     if mask.shape != logits.shape[:1]:
         raise ValueError(f"mask {tuple(mask.shape)} for logits {tuple(logits.shape)}")
-    mask = mask.contiguous()
-    return mask, mask.data_ptr()
+    return mask.contiguous()
 
 
 def _check(logits, mask):
@@ -53,7 +53,7 @@ def _f32(g):
     return g if g.dtype == torch.float32 and g.is_contiguous() else g.float().contiguous()
 
 
-def _rows(logits):
+def rows(logits):
     """logits with contiguous rows, and the elements between them."""
     E = logits.shape[1]
     if logits.stride(1) != 1 or logits.stride(0) < E:
@@ -66,8 +66,9 @@ def top_k(logits, k, norm_topk_prob=True, mask=None):
     routing of a serving step. mask [T] (bool / uint8): 0 marks padding, whose ids are -1."""
     _check(logits, mask)
     with T.on_device(logits):
-        lg, ld = _rows(logits)
-        m, mp = _mask_ptr(mask, lg)
+        lg, ld = rows(logits)
+        m = mask_bytes(mask, lg)
+        mp = None if m is None else m.data_ptr()
         n, E = lg.shape
         ids = torch.empty((n, k), dtype=torch.int32, device=lg.device)
         w = torch.empty((n, k), dtype=torch.float32, device=lg.device)
@@ -84,8 +85,9 @@ class _RouteFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, k, norm, mask):
         with T.on_device(logits):
-            lg, ld = _rows(logits)
-            m, mp = _mask_ptr(mask, lg)
+            lg, ld = rows(logits)
+            m = mask_bytes(mask, lg)
+            mp = None if m is None else m.data_ptr()
             n, E = lg.shape
             dev = lg.device
             ids = torch.empty((n, k), dtype=torch.int32, device=dev)
