@@ -109,7 +109,10 @@ def test_quantize_empty():
 
 # ------------------------------------------------------------------- linear
 SHAPES = [(1, 16, 32), (1, 64, 4096), (2, 33, 1), (3, 17, 95), (16, 48, 160), (17, 100, 257), (31, 130, 512),
-          (33, 64, 1056), (64, 80, 128), (65, 40, 224), (130, 272, 640), (300, 129, 1000)]
+          (33, 64, 1056), (64, 80, 128), (65, 40, 224), (130, 272, 640), (300, 129, 1000),
+          # every split of k over the waves, rows too long for them, and x through LDS to its last chunk
+          (1, 32, 8192), (3, 32, 8192), (9, 48, 6144), (16, 16, 5120), (20, 33, 8200), (2, 40, 17408), (5, 24, 768),
+          (12, 20, 1536), (18, 40, 2048), (30, 40, 3000), (32, 16, 4096), (1, 70000, 64)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -308,7 +311,9 @@ def _glu(rng, E, H, I):
 
 
 EXPERTS = [(1, 1, 1, 32, 32), (1, 8, 32, 256, 64), (3, 4, 6, 95, 33), (4, 10, 64, 512, 128), (11, 6, 16, 128, 96),
-           (70, 2, 40, 160, 64), (64, 8, 12, 256, 160), (300, 4, 6, 64, 32), (257, 3, 8, 100, 70)]
+           (70, 2, 40, 160, 64), (64, 8, 12, 256, 160), (300, 4, 6, 64, 32), (257, 3, 8, 100, 70),
+           # rows too long for the streaming kernel, by pair and sorted; few pairs of many chunks; tiles of 32
+           (2, 2, 3, 8192, 32), (30, 2, 12, 8200, 40), (2, 6, 9, 64, 4096), (40, 4, 10, 64, 64)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)

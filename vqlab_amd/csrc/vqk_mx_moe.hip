@@ -13,8 +13,12 @@ namespace vqk {
 
 static size_t al256(size_t v) { return (v + 255) & ~size_t(255); }
 
-// Pairs up to which the products run pair by pair.
-constexpr int64_t kMxPairsUnsorted = 64;
+// Whether a routing runs pair by pair: few pairs, and few of them on one expert
+// (us per block, pair by pair / sorted: 256 experts of 2048 x 512, 64 pairs 31 / 41,
+// 96 48 / 49, 128 50 / 56; 512 of 4096 x 1024, 80 pairs 144 / 145, 160 249 / 227; 64 of
+// 4096 x 1024, 24 pairs 52 / 50, 48 81 / 86, 72 123 / 99; 8 of 2048 x 1024, 16 pairs
+// 21.9 / 22.2, 24 35 / 28).
+static bool mx_by_pair(int64_t N, int64_t E) { return N <= 16 || (N <= 96 && 4 * N <= 3 * E); }
 constexpr int64_t kMxMaxExperts = 4096;
 
 // Rows per tile of a routing of N pairs over E experts: 16 (the streaming kernel) while
@@ -164,11 +168,11 @@ static int make_x(const vqk_mx_weights *w, bool place, const void *x, int32_t ty
 }
 
 static size_t sort_bytes(int64_t N, int64_t E) {
-    return N <= kMxPairsUnsorted ? 0 : al256(seg_sort_bytes(N, E));
+    return mx_by_pair(N, E) ? 0 : al256(seg_sort_bytes(N, E));
 }
 // Sets a call's routing from the ids: unsorted pairs, or sorted into `ws`.
 static int set_routing(MxCall *c, const int32_t *ids, int64_t N, int64_t E, int rows, void *ws, hipStream_t st) {
-    if (N <= kMxPairsUnsorted) {
+    if (mx_by_pair(N, E)) {
         c->ids = ids;
         return VQK_OK;
     }
@@ -206,7 +210,7 @@ static int plan_experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, co
     p->x = 0;
     p->h = plane_bytes(T, g1->NB, p->P);
     p->part = p->h + plane_bytes(p->N, g2->NB, p->P);
-    p->sort = p->part + (p->N <= kMxPairsUnsorted ? 0 : al256(size_t(p->N) * g2->OUT * 4));
+    p->sort = p->part + (mx_by_pair(p->N, g1->E) ? 0 : al256(size_t(p->N) * g2->OUT * 4));
     p->total = p->sort + sort_bytes(p->N, g1->E);
     return VQK_OK;
 }
@@ -254,7 +258,7 @@ extern "C" int vqk_mx_switch(const vqk_mx_weights *w, const void *x, int32_t x_t
     c.y = y; c.y_type = y_type; c.ldy = g.OUT;
     if ((rc = make_x(w, mx_x_in_place(w, x, x_type), x, x_type, T, g.NB, reinterpret_cast<uint16_t *>(ws),
                      &c.x, st))) return rc;
-    const int rows = N <= kMxPairsUnsorted ? 16 : mx_tile_rows(N, g.E);
+    const int rows = mx_by_pair(N, g.E) ? 16 : mx_tile_rows(N, g.E);
     if ((rc = set_routing(&c, eidx, N, g.E, rows, ws + sort_at, st))) return rc;
     return run(c, rows, st);
 }
@@ -300,7 +304,7 @@ static int experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, const v
                    int64_t T, const int32_t *ids, const float *wts, int32_t top_k, void *y, int32_t y_type,
                    uint8_t *ws, hipStream_t st) {
     int rc;
-    const bool sorted = p.N > kMxPairsUnsorted;
+    const bool sorted = !mx_by_pair(p.N, g1.E);
     const int rows = sorted ? mx_tile_rows(p.N, g1.E) : 16;
     MxCall c{};
     c.codes[0] = gate->codes; c.scales[0] = gate->scales;

@@ -36,6 +36,8 @@ int mxf_gemm(const MxfCall &c, float *part, size_t part_bytes, hipStream_t st) {
         a.splits = (groups + a.per - 1) / a.per;
         a.part = part;
     }
+    if (c.xNB * 16 * kMxfRows > INT64_C(0xffffffff))      // offsets inside a tile of x are 32 bits
+        return set_error(VQK_ENOTIMPL, "4-bit product: rows of %lld blocks", (long long)c.xNB);
     const int64_t grid = int64_t(a.nt) * a.nob * a.splits;
     if (grid > INT32_MAX) return set_error(VQK_ENOTIMPL, "4-bit product: grid too large");
     const int rc = launch_with_lds<k_mxf_gemm<kMxfRows / 32, 2>>(dim3(unsigned(grid)), dim3(256),

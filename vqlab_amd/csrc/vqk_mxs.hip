@@ -43,8 +43,15 @@ static RowsPlan rows_plan(int64_t NC, int xn, bool glu, int64_t row_tiles) {
     return ncw <= cap ? RowsPlan{kw, int(ncw)} : RowsPlan{0, 0};
 }
 
+// x goes through LDS for dense tiles of more than two rows; sorted ones hold few
+// as long as this kernel takes them. LDS holds five chunks a wave.
+static bool rows_stage(const MxCall &c) { return !c.ids && !c.meta && c.N > 2; }
+constexpr int kStageChunks = kLdsBytes / (kMxsWaves * 4096);
+
 bool mx_rows_ok(const MxCall &c, int NT) {
-    return (NT == 1 || (NT == 2 && c.x.P == 1)) && rows_plan(c.g.NC, NT * c.x.P, c.codes[1] != nullptr, mx_tiles(c, 16 * NT) * c.g.RT).kw > 0;
+    if (NT != 1 && (NT != 2 || c.x.P != 1)) return false;
+    const RowsPlan pl = rows_plan(c.g.NC, NT * c.x.P, c.codes[1] != nullptr, mx_tiles(c, 16 * NT) * c.g.RT);
+    return pl.kw > 0 && (!rows_stage(c) || pl.ncw <= kStageChunks);
 }
 
 template <int OP, int NT, int P, int NCW, bool GLU>
@@ -62,8 +69,6 @@ static int go(MxsArgs a, int64_t tiles, int kw, hipStream_t st) {
     a.nob = int32_t((a.total_steps + steps - 1) / steps);
     const int64_t grid = int64_t(a.nob) * tiles;
     if (grid > INT32_MAX) return set_error(VQK_ENOTIMPL, "MXFP4 product: grid too large");
-    // dense tiles of more than two rows; sorted ones hold few as long as this kernel takes them
-    a.stage = !a.ids && !a.meta && a.N > 2;
     const size_t sums = kw > 1 ? size_t(2) * kMxsWaves * (GLU ? 2 : 1) * NT * 1024 : 0;
     const size_t xl = a.stage ? size_t(kMxsWaves) * NCW * 4096 : 0;
     return launch_with_lds<k_mx_rows<OP, NT, P, NCW, GLU>>(dim3(unsigned(grid)), dim3(64 * kMxsWaves),
@@ -88,6 +93,7 @@ int mx_rows(const MxCall &c, int NT, hipStream_t st) {
     const int64_t tiles = mx_tiles(c, 16 * NT);
     if (tiles == 0) return VQK_OK;
     const RowsPlan pl = rows_plan(c.g.NC, NT * c.x.P, glu, tiles * c.g.RT);
+    a.stage = rows_stage(c);
     if (c.x.op == kOpF16)
         return NT == 2 ? go_glu<kOpF16, 2, 1>(a, glu, tiles, pl, st) : go_glu<kOpF16, 1, 1>(a, glu, tiles, pl, st);
     if (NT == 2) return go_glu<kOpBF16, 2, 1>(a, glu, tiles, pl, st);
