@@ -313,7 +313,7 @@ def _glu(rng, E, H, I):
 EXPERTS = [(1, 1, 1, 32, 32), (1, 8, 32, 256, 64), (3, 4, 6, 95, 33), (4, 10, 64, 512, 128), (11, 6, 16, 128, 96),
            (70, 2, 40, 160, 64), (64, 8, 12, 256, 160), (300, 4, 6, 64, 32), (257, 3, 8, 100, 70),
            # rows too long for the streaming kernel, by pair and sorted; few pairs of many chunks; tiles of 32
-           (2, 2, 3, 8192, 32), (30, 2, 12, 8200, 40), (2, 6, 9, 64, 4096), (40, 4, 10, 64, 64)]
+           (2, 2, 3, 8192, 32), (30, 2, 12, 8200, 40), (100, 4, 60, 640, 96), (90, 6, 50, 7000, 32), (2, 6, 9, 64, 4096), (40, 4, 10, 64, 64)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)

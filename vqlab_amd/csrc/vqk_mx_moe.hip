@@ -13,24 +13,30 @@ namespace vqk {
 
 static size_t al256(size_t v) { return (v + 255) & ~size_t(255); }
 
-// Whether a routing runs pair by pair: few pairs, and few of them on one expert
-// (us per block, pair by pair / sorted: 256 experts of 2048 x 512, 64 pairs 31 / 41,
-// 96 48 / 49, 128 50 / 56; 512 of 4096 x 1024, 80 pairs 144 / 145, 160 249 / 227; 64 of
-// 4096 x 1024, 24 pairs 52 / 50, 48 81 / 86, 72 123 / 99; 8 of 2048 x 1024, 16 pairs
-// 21.9 / 22.2, 24 35 / 28).
-static bool mx_by_pair(int64_t N, int64_t E) { return N <= 16 || (N <= 96 && 4 * N <= 3 * E); }
+// Whether a routing runs pair by pair: the sort, its tiles and the pass that adds
+// rows cost about 25 us more, and read weights at 5.3 TB/s instead of 3.6 and an
+// expert's once. us per block, pair by pair / sorted: 256 experts of 2048 x 512
+// (1.7 MB a pair), 64 pairs 32 / 49, 128 48 / 64; 512 of 4096 x 1024 (6.7 MB), 30
+// pairs 51 / 64, 60 107 / 98; 64 of 4096 x 1024, 24 pairs 51 / 58, 48 80 / 81; 8 of
+// 2048 x 1024, 16 pairs 21.9 / 22.2, 24 35 / 28.
+static bool mx_by_pair(int64_t N, int64_t E, int64_t pair_bytes) {
+    return N <= 16 || (N <= 2 * E && N * pair_bytes <= INT64_C(256) << 20);
+}
+static int64_t pair_bytes(const MxGeom &g) { return mx_expert_codes(g.RT, g.NC); }
 constexpr int64_t kMxMaxExperts = 4096;
 
-// Rows per tile of a routing of N pairs over E experts: 16 (the streaming kernel) while
-// experts have a few pairs each, then 32, 64 or 128 (the many-row kernel, whose tiles cost
-// the rows they hold: 60 rows an expert take 111 + 81 us in tiles of 128, 124 + 104 in tiles
-// of 64, 111 + 91 in tiles of 96; 256 experts of 2048 x 512).
+// Rows per tile of a sorted routing of N pairs over E experts. Tiles cost the rows
+// they hold (in groups of 32), so a tile is as large as what an expert is likely to
+// have: 60 rows an expert take 111 + 81 us in tiles of 128, 124 + 104 in tiles of 64
+// (256 experts of 2048 x 512); 12 rows 158 us a block on the streaming kernel and 115
+// in tiles of 32 (64 of 4096 x 1024), 1.25 rows 508 and 447 (512 of 4096 x 1024).
 static int mx_tile_rows(int64_t N, int64_t E) {
     const int64_t avg = N / E;
-    return avg <= 12 ? 16 : (avg <= 20 ? 32 : (avg <= 40 ? 64 : 128));
+    return avg <= 20 ? 32 : (avg <= 40 ? 64 : 128);
 }
+// One product: pairs stream the weights where x fits (vqk_mxs.h), tiles else.
 static int run(const MxCall &c, int rows, hipStream_t st) {
-    return rows == 16 && mx_rows_ok(c, 1) ? mx_rows(c, 1, st) : mx_gemm(c, rows, nullptr, 0, st);
+    return c.ids && mx_rows_ok(c, 1) ? mx_rows(c, 1, st) : mx_gemm(c, rows, nullptr, 0, st);
 }
 
 struct CombineArgs {
@@ -167,12 +173,13 @@ static int make_x(const vqk_mx_weights *w, bool place, const void *x, int32_t ty
     return launch_mx_planes(x, type, rows, w->IN, w->IN, false, ws, st);
 }
 
-static size_t sort_bytes(int64_t N, int64_t E) {
-    return mx_by_pair(N, E) ? 0 : al256(seg_sort_bytes(N, E));
+static size_t sort_bytes(int64_t N, int64_t E, int64_t pb) {
+    return mx_by_pair(N, E, pb) ? 0 : al256(seg_sort_bytes(N, E));
 }
 // Sets a call's routing from the ids: unsorted pairs, or sorted into `ws`.
-static int set_routing(MxCall *c, const int32_t *ids, int64_t N, int64_t E, int rows, void *ws, hipStream_t st) {
-    if (mx_by_pair(N, E)) {
+static int set_routing(MxCall *c, bool by_pair, const int32_t *ids, int64_t N, int64_t E, int rows, void *ws,
+                       hipStream_t st) {
+    if (by_pair) {
         c->ids = ids;
         return VQK_OK;
     }
@@ -187,6 +194,7 @@ static int set_routing(MxCall *c, const int32_t *ids, int64_t N, int64_t E, int 
 struct ExpertsPlan {
     int64_t N, IP;
     int P;
+    bool by_pair;
     size_t x, h, part, sort, total;
 };
 static int plan_experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, const vqk_mx_weights *down,
@@ -207,11 +215,13 @@ static int plan_experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, co
     if ((rc = check_pairs(T, p->N, g1->E, "mx experts"))) return rc;
     p->IP = g2->NB * kMxBlock;
     p->P = mx_planes(x_type);
+    const int64_t pb = 2 * pair_bytes(*g1) + pair_bytes(*g2);
+    p->by_pair = mx_by_pair(p->N, g1->E, pb);
     p->x = 0;
     p->h = plane_bytes(T, g1->NB, p->P);
     p->part = p->h + plane_bytes(p->N, g2->NB, p->P);
-    p->sort = p->part + (mx_by_pair(p->N, g1->E) ? 0 : al256(size_t(p->N) * g2->OUT * 4));
-    p->total = p->sort + sort_bytes(p->N, g1->E);
+    p->sort = p->part + (p->by_pair ? 0 : al256(size_t(p->N) * g2->OUT * 4));
+    p->total = p->sort + sort_bytes(p->N, g1->E, pb);
     return VQK_OK;
 }
 
@@ -226,7 +236,7 @@ extern "C" int vqk_mx_switch_workspace(const vqk_mx_weights *w, int32_t x_type, 
     if (rc || (rc = check_pairs(T, N, g.E, "mx switch"))) return rc;
     if (!act_size(x_type)) return set_error(VQK_EINVAL, "mx switch: x type %d", x_type);
     if (!bytes) return set_error(VQK_EINVAL, "mx switch: NULL bytes");
-    *bytes = plane_bytes(T, g.NB, mx_planes(x_type)) + sort_bytes(N, g.E);
+    *bytes = plane_bytes(T, g.NB, mx_planes(x_type)) + sort_bytes(N, g.E, 3 * pair_bytes(g));
     return VQK_OK;
 }
 
@@ -244,7 +254,7 @@ extern "C" int vqk_mx_switch(const vqk_mx_weights *w, const void *x, int32_t x_t
     if (N == 0) return VQK_OK;
     if (!x || !eidx || !y) return set_error(VQK_EINVAL, "mx switch: NULL pointer");
     const size_t sort_at = plane_bytes(T, g.NB, mx_planes(x_type));
-    const size_t need = sort_at + sort_bytes(N, g.E);
+    const size_t need = sort_at + sort_bytes(N, g.E, 3 * pair_bytes(g));
     if (!workspace || ws_bytes < need)
         return set_error(VQK_ENOSPACE, "mx switch: workspace %zu < %zu", ws_bytes, need);
     if (reinterpret_cast<uintptr_t>(workspace) & 255)
@@ -258,8 +268,9 @@ extern "C" int vqk_mx_switch(const vqk_mx_weights *w, const void *x, int32_t x_t
     c.y = y; c.y_type = y_type; c.ldy = g.OUT;
     if ((rc = make_x(w, mx_x_in_place(w, x, x_type), x, x_type, T, g.NB, reinterpret_cast<uint16_t *>(ws),
                      &c.x, st))) return rc;
-    const int rows = mx_by_pair(N, g.E) ? 16 : mx_tile_rows(N, g.E);
-    if ((rc = set_routing(&c, eidx, N, g.E, rows, ws + sort_at, st))) return rc;
+    const bool by_pair = mx_by_pair(N, g.E, 3 * pair_bytes(g));
+    const int rows = mx_tile_rows(N, g.E);
+    if ((rc = set_routing(&c, by_pair, eidx, N, g.E, rows, ws + sort_at, st))) return rc;
     return run(c, rows, st);
 }
 
@@ -304,8 +315,7 @@ static int experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, const v
                    int64_t T, const int32_t *ids, const float *wts, int32_t top_k, void *y, int32_t y_type,
                    uint8_t *ws, hipStream_t st) {
     int rc;
-    const bool sorted = !mx_by_pair(p.N, g1.E);
-    const int rows = sorted ? mx_tile_rows(p.N, g1.E) : 16;
+    const int rows = mx_tile_rows(p.N, g1.E);
     MxCall c{};
     c.codes[0] = gate->codes; c.scales[0] = gate->scales;
     c.codes[1] = up->codes; c.scales[1] = up->scales;
@@ -317,7 +327,7 @@ static int experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, const v
     if ((rc = make_x(gate, place, x, x_type, T, g1.NB, reinterpret_cast<uint16_t *>(ws), &c.x, st))) return rc;
     const int hp = c.x.op == kOpF16 ? 1 : p.P;
     c.y = h; c.ldy = p.IP; c.yplane = p.N * p.IP; c.yp = hp; c.ysorted = true;
-    if ((rc = set_routing(&c, ids, p.N, g1.E, rows, ws + p.sort, st))) return rc;
+    if ((rc = set_routing(&c, p.by_pair, ids, p.N, g1.E, rows, ws + p.sort, st))) return rc;
     if ((rc = run(c, rows, st))) return rc;
     MxCall d = c;                              // the same routing, over the SwiGLU rows
     d.codes[0] = down->codes; d.scales[0] = down->scales;
@@ -325,7 +335,7 @@ static int experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, const v
     d.g = g2;
     d.x = MxX{h, p.IP, p.N * p.IP, hp, c.x.op};
     d.xkrep = 0;
-    if (!sorted) {
+    if (p.by_pair) {
         const DownArgs a{d.codes[0], d.scales[0], g2.E, g2.OUT, int32_t(g2.RT), int32_t(g2.NC), int32_t(g2.NB),
                          top_k, h, p.IP, p.N * p.IP, ids, wts, y, y_type};
         const int64_t grid = T * g2.RT;

@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(64 * kMxsWaves, 2) k_mx_rows(const MxsArgs p) 
 
     u32x4 xf[P][NT][NCW][4];
     auto x_in = [&](int c) { return 4 * (kw * NCW + c) + g < p.NB; };   // this lane's block of x exists
-    if (p.stage) {                            // dense rows only: a tile's rows lie one after the other
+    if (p.stage) {                            // dense rows: a tile's lie one after the other
         uint8_t *xl = smem + wave * (NCW * 4096);
 #pragma unroll
         for (int pl = 0; pl < P; ++pl)

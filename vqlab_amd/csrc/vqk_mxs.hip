@@ -43,13 +43,13 @@ static RowsPlan rows_plan(int64_t NC, int xn, bool glu, int64_t row_tiles) {
     return ncw <= cap ? RowsPlan{kw, int(ncw)} : RowsPlan{0, 0};
 }
 
-// x goes through LDS for dense tiles of more than two rows; sorted ones hold few
-// as long as this kernel takes them. LDS holds five chunks a wave.
-static bool rows_stage(const MxCall &c) { return !c.ids && !c.meta && c.N > 2; }
+// Dense x of more than two rows goes through LDS, which holds five chunks a wave;
+// longer rows are left to the tiles.
+static bool rows_stage(const MxCall &c) { return !c.ids && c.N > 2; }
 constexpr int kStageChunks = kLdsBytes / (kMxsWaves * 4096);
 
 bool mx_rows_ok(const MxCall &c, int NT) {
-    if (NT != 1 && (NT != 2 || c.x.P != 1)) return false;
+    if (c.meta || (NT != 1 && (NT != 2 || c.x.P != 1))) return false;
     const RowsPlan pl = rows_plan(c.g.NC, NT * c.x.P, c.codes[1] != nullptr, mx_tiles(c, 16 * NT) * c.g.RT);
     return pl.kw > 0 && (!rows_stage(c) || pl.ncw <= kStageChunks);
 }
@@ -59,12 +59,11 @@ static int go(MxsArgs a, int64_t tiles, int kw, hipStream_t st) {
     const int RW = kMxsWaves / kw;
     a.kw = kw;
     a.total_steps = int32_t((a.ocover + 16 * RW - 1) / (16 * RW));
-    // row steps per workgroup: one round of workgroups, two to a CU where the registers let them;
-    // tiles of a routing are an upper bound, so walks stay short enough to balance
+    // row steps per workgroup: one round of workgroups, two to a CU where the registers let them
     const int64_t room = 45 + NCW * (16 * NT * P + (GLU ? 18 : 9)) <= 128 ? 512 : 256;
     const int64_t want = tiles > 0 ? (room + tiles - 1) / tiles : 1;
     int64_t steps = (a.total_steps + want - 1) / want;
-    if (a.meta || a.ids) steps = steps > 8 ? 8 : steps;
+    if (a.ids) steps = steps > 8 ? 8 : steps;      // pairs without an expert leave early
     a.steps = int32_t(steps);
     a.nob = int32_t((a.total_steps + steps - 1) / steps);
     const int64_t grid = int64_t(a.nob) * tiles;
