@@ -438,3 +438,77 @@ def test_on_two_streams_at_once():
     torch.cuda.synchronize()
     for i, y in enumerate(got):
         assert torch.equal(y, ref[i % 2])
+
+
+# ----------------------------------------------------------------- refusals
+def test_what_has_no_gradient_says_so():
+    from vqlab_amd import mx
+    rng = np.random.default_rng(6)
+    x, _ = mc.acts(rng, "bf16", 4, 64)
+    x.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        mx.mx_quantize(x)
+    lin, _ = _linear(rng, 32, 64, act="mxfp4")
+    with pytest.raises(RuntimeError, match="no gradient"):
+        lin(x)
+    glu, _ = _glu(rng, 4, 64, 32)
+    ids, w = _dev(np.zeros((4, 2), np.int32), np.ones((4, 2), np.float32))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        glu(x, ids, w)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        glu(x.detach(), ids, w.requires_grad_(True))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        mx.MXSparseMoeBlock(glu, 2)(x, torch.randn(4, 4, device="cuda"))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        glu.gate_proj(x[:, None, None], ids)
+    with torch.no_grad():
+        assert lin(x).shape == (4, 32) and glu(x, ids, w).shape == (4, 64)
+    plain, _ = _linear(rng, 32, 64)
+    d = torch.autograd.grad(plain(x).float().square().sum(), x, create_graph=True)[0]
+    with pytest.raises(RuntimeError):                      # once differentiable
+        d.sum().backward()
+
+
+def test_shapes_and_types_that_do_not_fit():
+    from vqlab_amd import mx
+    rng = np.random.default_rng(7)
+    lin, _ = _linear(rng, 32, 64)
+    glu, _ = _glu(rng, 4, 64, 32)
+    f = torch.zeros(4, 64, device="cuda")
+    for bad in (f[:, :63], f.double(), f.cpu(), torch.zeros((), device="cuda")):
+        with pytest.raises(ValueError):
+            lin(bad)
+    ids, w = _dev(np.zeros((4, 2), np.int32), np.ones((4, 2), np.float32))
+    for x, i, v in ((f[:, :32], ids, w), (f[:3], ids, w), (f, ids[:, :1], w), (f[0], ids, w), (f, ids.cpu(), w)):
+        with pytest.raises(ValueError):
+            glu(x, i, v)
+    blk = mx.MXSparseMoeBlock(glu, top_k=2)
+    for lg, m in ((torch.zeros(4, 5, device="cuda"), None), (torch.zeros(3, 4, device="cuda"), None),
+                  (torch.zeros(4, 4, device="cuda"), torch.ones(3, dtype=torch.bool, device="cuda")),
+                  (torch.zeros(4, 4, device="cuda"), torch.ones(4, device="cuda"))):
+        with pytest.raises(ValueError):
+            blk(f, lg, mask=m)
+    with pytest.raises(ValueError):
+        mx.MXSparseMoeBlock(glu, top_k=5)(f, torch.zeros(4, 4, device="cuda"))
+    with pytest.raises(ValueError):
+        glu.gate_proj(f, ids)
+    with pytest.raises(ValueError):
+        mx.mx_dequantize(*mx.mx_quantize(f), 65)
+    with pytest.raises(ValueError):
+        mx.mx_dequantize(*mx.mx_quantize(f), 64, torch.float64)
+
+
+def test_block_from_router_weight_and_no_tokens():
+    from vqlab_amd import mx
+    rng = np.random.default_rng(8)
+    glu, ws = _glu(rng, 6, 64, 32)
+    rw = torch.randn(6, 64, device="cuda")
+    blk = mx.MXSparseMoeBlock(glu, top_k=2, norm_topk_prob=False, router_weight=rw)
+    x, xv = mc.acts(rng, "fp32", 5, 64)
+    assert torch.equal(blk(x), blk(x, x.float() @ rw.T))
+    assert blk(x[:0]).shape == (0, 64)
+    logits = (x.float() @ rw.T).double().cpu().numpy()
+    r = mc.route(logits, 2, False)
+    ref, bar = mc.experts(xv, r["ids"], r["w"], *ws, 2.0 ** -24)
+    bar += 64 * 2.0 ** -24 * np.abs(ref) + 2.0 ** -24 * (np.abs(ref) + bar)
+    mc.assert_within(blk(x), ref, bar, "block")
