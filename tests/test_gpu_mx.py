@@ -512,3 +512,26 @@ def test_block_from_router_weight_and_no_tokens():
     ref, bar = mc.experts(xv, r["ids"], r["w"], *ws, 2.0 ** -24)
     bar += 64 * 2.0 ** -24 * np.abs(ref) + 2.0 ** -24 * (np.abs(ref) + bar)
     mc.assert_within(blk(x), ref, bar, "block")
+
+
+def test_experts_with_weights_beyond_fp16():
+    """fp16 x where only some of the projections hold fp16 numbers: pairs and sorted."""
+    from vqlab_amd import mx
+    rng = np.random.default_rng(9)
+    H, I, E = 96, 64, 5
+
+    def sw(OUT, IN, lo):
+        codes, scales = mc.weight(rng, E, OUT, IN)
+        scales[rng.random(scales.shape) < 0.2] = lo
+        return mx.MXSwitchLinear(*_dev(codes, scales), IN), mc.values(codes, scales, IN)
+    for los in ((118, 118, 90), (90, 118, 118), (118, 90, 118), (90, 90, 90)):
+        (g, gw), (u, uw), (d, dw) = sw(I, H, los[0]), sw(I, H, los[1]), sw(H, I, los[2])
+        assert [bool(m._w.f16_exact) for m in (g, u, d)] == [lo > 104 for lo in los]
+        glu = mx.MXSwitchGLU(g, u, d)
+        for T in (3, 60):
+            x, xv = mc.acts(rng, "fp16", T, H)
+            ids = np.stack([rng.permutation(E)[:2] for _ in range(T)])
+            w = rng.random((T, 2)).astype(np.float32)
+            ref, bar = mc.experts(xv, ids, w.astype(np.float64), gw, uw, dw, mc.HALF_STEP["fp16"])
+            bar = bar + mc.HALF_STEP["fp16"] * (np.abs(ref) + bar) + 2.0 ** -25
+            mc.assert_within(glu(x, *_dev(ids, w)), ref, bar, f"{los} T={T}")

@@ -39,6 +39,17 @@ static int run(const MxCall &c, int rows, hipStream_t st) {
     return c.ids && mx_rows_ok(c, 1) ? mx_rows(c, 1, st) : mx_gemm(c, rows, nullptr, 0, st);
 }
 
+// The SwiGLU rows that down reads, as bf16 planes (or fp16 rows, 0): pair by pair two
+// of them (16 bits) for 16-bit x, three (24 bits) for fp32. Sorted, they are rounded to
+// x's type, as its own layers would: a second plane would halve the rate of down (2048
+// tokens of 256 experts 237 -> 271 us) to take away a rounding no larger than that of
+// the outputs; where a handful of pairs leaves few outputs, it costs 1.5 us.
+static int mx_h_planes(int32_t x_type, bool by_pair, bool f16_exact) {
+    if (x_type == VQK_F32) return 3;
+    if (by_pair) return 2;
+    return x_type == VQK_BF16 ? 1 : (f16_exact ? 0 : 2);
+}
+
 struct CombineArgs {
     const float *part;
     const int32_t *ids;
@@ -90,10 +101,10 @@ struct DownArgs {
 // leave the sums of a unit, which enter with the pair's weight; the waves meet in
 // LDS in wave order. Against down rows in fp32 and a pass that adds them: one launch
 // and one round trip less (8 pairs of 512 -> 2048: 4.4 us for 4.2 + 4.5).
-template <int OP, int P>
+template <int P>
 __global__ void __launch_bounds__(64 * kMxsWaves) k_mx_down(const DownArgs p) {
     __shared__ float red[kMxsWaves][16];
-    constexpr int U = P == 1 ? 4 : 2;         // units in flight
+    constexpr int U = 2;                      // units in flight (four: 100 us for 89 with 40 pairs of 512 experts)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     const int t = int(blockIdx.x / unsigned(p.RT)), rt = int(blockIdx.x % unsigned(p.RT));
     const uint32_t NC = uint32_t(p.NC), NC4 = (NC + 3) / 4;
@@ -134,9 +145,9 @@ __global__ void __launch_bounds__(64 * kMxsWaves) k_mx_down(const DownArgs p) {
             f32x4 d{};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const u32x4 wf = mx_decode8_op<OP>(w[i][k], s);
+                const u32x4 wf = mx_decode8(w[i][k], s);
 #pragma unroll
-                for (int pl = 0; pl < P; ++pl) d = mx_mma16<OP>(x[i][pl][k], wf, d);
+                for (int pl = 0; pl < P; ++pl) d = mx_mma16<kOpBF16>(x[i][pl][k], wf, d);
             }
             acc += wt[i] * d[0];              // a pair without an expert: 0 times rows of zeros
         }
@@ -219,7 +230,7 @@ static int plan_experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, co
     p->by_pair = mx_by_pair(p->N, g1->E, pb);
     p->x = 0;
     p->h = plane_bytes(T, g1->NB, p->P);
-    p->part = p->h + plane_bytes(p->N, g2->NB, p->P);
+    p->part = p->h + plane_bytes(p->N, g2->NB, x_type == VQK_F32 ? 3 : 2);
     p->sort = p->part + (p->by_pair ? 0 : al256(size_t(p->N) * g2->OUT * 4));
     p->total = p->sort + sort_bytes(p->N, g1->E, pb);
     return VQK_OK;
@@ -322,10 +333,9 @@ static int experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, const v
     c.g = g1;
     c.N = p.N; c.xkrep = top_k;
     uint16_t *h = reinterpret_cast<uint16_t *>(ws + p.h);
-    // fp16 x and SwiGLU rows, or bf16 planes of both
-    const bool place = mx_x_in_place(gate, x, x_type) && (x_type != VQK_F16 || (up->f16_exact && down->f16_exact));
+    const bool place = mx_x_in_place(gate, x, x_type) && (x_type != VQK_F16 || up->f16_exact);
     if ((rc = make_x(gate, place, x, x_type, T, g1.NB, reinterpret_cast<uint16_t *>(ws), &c.x, st))) return rc;
-    const int hp = c.x.op == kOpF16 ? 1 : p.P;
+    const int hp = mx_h_planes(x_type, p.by_pair, down->f16_exact != 0);
     c.y = h; c.ldy = p.IP; c.yplane = p.N * p.IP; c.yp = hp; c.ysorted = true;
     if ((rc = set_routing(&c, p.by_pair, ids, p.N, g1.E, rows, ws + p.sort, st))) return rc;
     if ((rc = run(c, rows, st))) return rc;
@@ -333,7 +343,7 @@ static int experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, const v
     d.codes[0] = down->codes; d.scales[0] = down->scales;
     d.codes[1] = nullptr; d.scales[1] = nullptr;
     d.g = g2;
-    d.x = MxX{h, p.IP, p.N * p.IP, hp, c.x.op};
+    d.x = MxX{h, p.IP, p.N * p.IP, hp ? hp : 1, hp ? kOpBF16 : kOpF16};
     d.xkrep = 0;
     if (p.by_pair) {
         const DownArgs a{d.codes[0], d.scales[0], g2.E, g2.OUT, int32_t(g2.RT), int32_t(g2.NC), int32_t(g2.NB),
@@ -341,10 +351,8 @@ static int experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, const v
         const int64_t grid = T * g2.RT;
         if (grid > INT32_MAX) return set_error(VQK_ENOTIMPL, "mx experts: grid too large");
         const dim3 gr{unsigned(grid)}, b(64 * kMxsWaves);
-        if (c.x.op == kOpF16) hipLaunchKernelGGL((k_mx_down<kOpF16, 1>), gr, b, 0, st, a);
-        else if (hp == 1) hipLaunchKernelGGL((k_mx_down<kOpBF16, 1>), gr, b, 0, st, a);
-        else if (hp == 2) hipLaunchKernelGGL((k_mx_down<kOpBF16, 2>), gr, b, 0, st, a);
-        else hipLaunchKernelGGL((k_mx_down<kOpBF16, 3>), gr, b, 0, st, a);
+        if (hp == 2) hipLaunchKernelGGL((k_mx_down<2>), gr, b, 0, st, a);
+        else hipLaunchKernelGGL((k_mx_down<3>), gr, b, 0, st, a);
         return hip_status(hipGetLastError(), "MXFP4 down launch");
     }
     float *part = reinterpret_cast<float *>(ws + p.part);

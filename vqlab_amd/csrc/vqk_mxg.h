@@ -256,10 +256,10 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
                     const float v = value(0, b, 4 * j + i), u = value(1, b, 4 * j + i);
                     h[i] = o + i < p.OUT ? mx_swiglu(v, u) : 0.f;
                 }
-                for (int pl = 0; pl < (OP == kOpF16 ? 1 : p.yp); ++pl) {
+                for (int pl = 0; pl < max(p.yp, 1); ++pl) {
                     uint16_t q[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) q[i] = OP == kOpF16 ? f32_to_h(h[i]) : mx_plane_next(h[i]);
+                    for (int i = 0; i < 4; ++i) q[i] = p.yp == 0 ? f32_to_h(h[i]) : mx_plane_next(h[i]);
                     u32x2 v2;
                     v2.x = q[0] | (uint32_t(q[1]) << 16);
                     v2.y = q[2] | (uint32_t(q[3]) << 16);
