@@ -7,6 +7,9 @@ modules mirror the reference runtime's interface over torch tensors:
   vqlab_amd.vq_dense   -- vq_dense (VQLinear, VQEmbedding)
   vqlab_amd.moe        -- fused MoE decode layer (SwitchGLU + routing)
   vqlab_amd.artifact   -- VQLab artifact loader (config.json + safetensors)
+and beyond the reference:
+  vqlab_amd.mx         -- MXFP4 weights: quantiser, linears, routed experts
+  vqlab_amd.router     -- softmax top-k routing with counts, losses and gradients
 """
 from . import _lib
 
