@@ -535,3 +535,47 @@ def test_experts_with_weights_beyond_fp16():
             ref, bar = mc.experts(xv, ids, w.astype(np.float64), gw, uw, dw, mc.HALF_STEP["fp16"])
             bar = bar + mc.HALF_STEP["fp16"] * (np.abs(ref) + bar) + 2.0 ** -25
             mc.assert_within(glu(x, *_dev(ids, w)), ref, bar, f"{los} T={T}")
+
+
+def test_copies_stand_alone():
+    """A copied or pickled module describes its own weights, after the first one is gone."""
+    import copy
+    import io
+    from vqlab_amd import mx
+    rng = np.random.default_rng(12)
+    lin, w = _linear(rng, 40, 96)
+    glu, _ = _glu(rng, 6, 64, 32)
+    blk = mx.MXSparseMoeBlock(glu, top_k=2)
+    x, xv = mc.acts(rng, "bf16", 7, 96)
+    z, lg = torch.randn(5, 64, device="cuda"), torch.randn(5, 6, device="cuda")
+    ref = blk(z, lg)
+    twin, blk2 = copy.deepcopy(lin), copy.deepcopy(blk)
+    buf = io.BytesIO()
+    torch.save(lin, buf)
+    lin._packed[0].zero_()
+    glu.down_proj._packed[0].zero_()
+    assert torch.equal(blk2(z, lg), ref)
+    y, bar = mc.product_bar(xv, w, "bf16")
+    mc.assert_within(twin(x), y, bar, "copy")
+    buf.seek(0)
+    mc.assert_within(torch.load(buf, weights_only=False)(x), y, bar, "pickle")
+
+
+def test_no_rows_keep_their_gradient():
+    rng = np.random.default_rng(13)
+    lin, _ = _linear(rng, 40, 96)
+    x = torch.zeros(0, 96, device="cuda", requires_grad=True)
+    y = lin(x)
+    assert y.shape == (0, 40) and torch.autograd.grad(y.sum(), x)[0].shape == (0, 96)
+
+
+def test_more_tokens_than_a_grid_dimension():
+    rng = np.random.default_rng(14)
+    glu, ws = _glu(rng, 2, 32, 32)
+    T = 70001
+    x, xv = mc.acts(rng, "bf16", T, 32)
+    ids = rng.integers(0, 2, (T, 1))
+    y = glu(x, *_dev(ids, np.full((T, 1), 0.5, np.float32)))
+    for part in (slice(0, 40), slice(65500, 65600), slice(T - 40, T)):
+        ref, bar = mc.experts(xv[part], ids[part], np.full((T, 1), 0.5)[part], *ws, mc.HALF_STEP["bf16"])
+        mc.assert_within(y[part], ref, bar + mc.HALF_STEP["bf16"] * (np.abs(ref) + bar), str(part))

@@ -132,6 +132,26 @@ def _work(like, n):
     return t, t.data_ptr()
 
 
+class _Packed(torch.nn.Module):
+    """A module over packed weights: `_packed` tensors, `_shape` (E, OUT, IN), and the descriptor
+    `_w` of them that the library reads, which a copy makes anew."""
+
+    def _set(self, codes, scales, E, OUT, IN):
+        self._shape = (int(E), int(OUT), int(IN))
+        self._packed = _pack(codes, scales, *self._shape)
+        self._w = _desc(self._packed, *self._shape)
+        self._sizes = {}
+
+    def __getstate__(self):
+        state = self.__dict__.copy()
+        del state["_w"]
+        return state
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._w = _desc(self._packed, *self._shape)
+
+
 class _LinearFn(torch.autograd.Function):
     """y = x . W^T with a frozen W; the gradient reaches x."""
 
@@ -146,7 +166,7 @@ class _LinearFn(torch.autograd.Function):
         return ctx.mod._dx(dy), None
 
 
-class MXLinear(torch.nn.Module):
+class MXLinear(_Packed):
     """Bias-free linear whose weight is MXFP4: codes uint8 [OUT, 16 B], scales uint8 [OUT, B]
     (the module keeps its own copy, in the kernels' operand order). in_features may be any width of
     the last block (default: all 32 of it). act: None multiplies x as it is (bf16, fp16 and fp32
@@ -162,9 +182,7 @@ class MXLinear(torch.nn.Module):
         IN = int(scales.shape[-1]) * BLOCK if in_features is None else int(in_features)
         _check_mx(codes, scales, IN, "MXLinear")
         self.in_features, self.out_features, self.act = IN, int(codes.shape[0]), act
-        self._packed = _pack(codes, scales, 1, self.out_features, IN)
-        self._w = _desc(self._packed, 1, self.out_features, IN)
-        self._sizes = {}
+        self._set(codes, scales, 1, self.out_features, IN)
 
     @classmethod
     def from_weight(cls, weight, act=None):
@@ -220,7 +238,7 @@ def _no_grad(what, *ts):
         raise RuntimeError(f"{what} has no gradient: run it under no_grad, or detach its inputs")
 
 
-class MXSwitchLinear(torch.nn.Module):
+class MXSwitchLinear(_Packed):
     """E bias-free linears in MXFP4, one picked by each index: codes uint8 [E, OUT, 16 B], scales
     uint8 [E, OUT, B]. forward(x [..., 1, 1, IN] or [..., k, 1, IN], indices [..., k]) ->
     [..., k, 1, OUT], as VQSwitchLinear; an index outside [0, E) gives zeros. Serving only: no
@@ -233,9 +251,7 @@ class MXSwitchLinear(torch.nn.Module):
         IN = int(scales.shape[-1]) * BLOCK if in_features is None else int(in_features)
         _check_mx(codes, scales, IN, "MXSwitchLinear")
         self.num_experts, self.output_dims, self.input_dims = int(codes.shape[0]), int(codes.shape[1]), IN
-        self._packed = _pack(codes, scales, self.num_experts, self.output_dims, IN)
-        self._w = _desc(self._packed, self.num_experts, self.output_dims, IN)
-        self._sizes = {}
+        self._set(codes, scales, self.num_experts, self.output_dims, IN)
 
     @classmethod
     def from_weight(cls, weight):
@@ -277,8 +293,11 @@ class MXSwitchGLU(torch.nn.Module):
                 (d.num_experts, d.output_dims, d.input_dims) != (g.num_experts, g.input_dims, g.output_dims):
             raise ValueError("MXSwitchGLU: gate, up [E, I, H] and down [E, H, I] do not fit together")
         self.gate_proj, self.up_proj, self.down_proj = g, u, d
-        self._refs = [ctypes.byref(m._w) for m in (g, u, d)]
         self._sizes = {}
+
+    def _refs(self):
+        m = self._modules
+        return [ctypes.byref(m[n]._w) for n in ("gate_proj", "up_proj", "down_proj")]
 
     def forward(self, x, ids, weights):
         T.require_cuda(x, ids, weights, self.gate_proj._packed[0])
@@ -294,7 +313,7 @@ class MXSwitchGLU(torch.nn.Module):
     def _run(self, x, ids, wts):
         xt, lib = T.act_type(x), L.lib()
         n, k = ids.shape
-        ws = self._refs
+        ws = self._refs()
         with T.on_device(x):
             x = x.contiguous()
             y = x.new_empty(x.shape)
@@ -329,15 +348,15 @@ class MXSparseMoeBlock(torch.nn.Module):
             raise ValueError(f"MXSparseMoeBlock: x {tuple(x.shape)}, logits {tuple(logits.shape)} for "
                              f"{g.num_experts} experts of width {g.input_dims}")
         m = router.mask_bytes(mask, logits)
-        xt, lib, glu, k = T.act_type(x), L.lib(), self.switch_mlp, self.top_k
+        xt, lib, ws, k = T.act_type(x), L.lib(), self.switch_mlp._refs(), self.top_k
         n = x.shape[0]
         with T.on_device(x):
             x = x.contiguous()
             lg, ld = router.rows(logits)
             y = x.new_empty(x.shape)
-            size = _ws_bytes(self._sizes, (n, xt, k), lib.vqk_mx_moe_workspace, *glu._refs, xt, n, k)
+            size = _ws_bytes(self._sizes, (n, xt, k), lib.vqk_mx_moe_workspace, *ws, xt, n, k)
             work, wp = _work(x, size)
-            rc = lib.vqk_mx_moe(*glu._refs, x.data_ptr(), xt, n, lg.data_ptr(), T.act_type(lg), ld,
+            rc = lib.vqk_mx_moe(*ws, x.data_ptr(), xt, n, lg.data_ptr(), T.act_type(lg), ld,
                                 None if m is None else m.data_ptr(), k, int(self.norm_topk_prob),
                                 y.data_ptr(), xt, wp, size, T.raw_stream(x))
             if rc:
