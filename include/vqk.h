@@ -458,9 +458,8 @@ int vqk_mx_switch(const vqk_mx_weights *w, const void *x, int32_t x_type, int64_
 
 /* The block of experts: y_t = sum_j wts[t, j] down_e(silu(gate_e x_t) * (up_e x_t)),
  * e = ids[t, j]; gate, up [E, I, H], down [E, H, I]. Pairs whose id is outside
- * [0, E) add nothing, whatever their weight. The SwiGLU rows enter down rounded to
- * x's type, or more precisely where few pairs leave the time for it. ids, wts:
- * [T, top_k], as vqk_route leaves them. */
+ * [0, E) add nothing, whatever their weight. The SwiGLU rows enter down in 16 bits
+ * of bf16's range (24 for fp32 x). ids, wts: [T, top_k], as vqk_route leaves them. */
 int vqk_mx_experts_workspace(const vqk_mx_weights *gate, const vqk_mx_weights *up,
                              const vqk_mx_weights *down, int32_t x_type, int64_t T, int32_t top_k,
                              size_t *bytes);

@@ -201,7 +201,7 @@ struct MxCall {
     void *y;                                  // [row][OUT] in y_type; a SwiGLU pair: rows like x's
     int32_t y_type;
     int64_t ldy, yplane;                      // elements between rows / planes of y
-    int yp;                                   // bf16 planes of a SwiGLU pair's output, 0: fp16 rows
+    int yp;                                   // bf16 planes of a SwiGLU pair's output
     bool ysorted;                             // y rows by sorted position
 };
 

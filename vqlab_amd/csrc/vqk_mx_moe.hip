@@ -5,8 +5,8 @@
 // Few pairs run pair by pair; more are sorted by expert on the device, so that
 // an expert's weights are read once for a tile of its rows. Gate and up are one
 // launch whose epilogue leaves silu(g) * u as the bf16 planes that down reads
-// (in x's precision: one plane for bf16, two for fp16, three for fp32); down
-// leaves fp32 rows by pair, and the last kernel adds them in order of j.
+// (mx_h_planes); down leaves fp32 rows by pair, and the last kernel adds them in
+// order of j.
 #include "vqk_mxs.h"
 
 namespace vqk {
@@ -39,16 +39,14 @@ static int run(const MxCall &c, int rows, hipStream_t st) {
     return c.ids && mx_rows_ok(c, 1) ? mx_rows(c, 1, st) : mx_gemm(c, rows, nullptr, 0, st);
 }
 
-// The SwiGLU rows that down reads, as bf16 planes (or fp16 rows, 0): pair by pair two
-// of them (16 bits) for 16-bit x, three (24 bits) for fp32. Sorted, they are rounded to
-// x's type, as its own layers would: a second plane would halve the rate of down (2048
-// tokens of 256 experts 237 -> 271 us) to take away a rounding no larger than that of
-// the outputs; where a handful of pairs leaves few outputs, it costs 1.5 us.
-static int mx_h_planes(int32_t x_type, bool by_pair, bool f16_exact) {
-    if (x_type == VQK_F32) return 3;
-    if (by_pair) return 2;
-    return x_type == VQK_BF16 ? 1 : (f16_exact ? 0 : 2);
-}
+// The SwiGLU rows that down reads, as bf16 planes: three (24 bits) for fp32 x, two
+// (16 bits, bf16's range) for 16-bit x, however many pairs share the call. They are
+// nobody's output: rounded to x's type as well, they would put an error as large as
+// the outputs' own rounding under it (against 64 bits 0.0026 instead of 0.0017 for
+// bf16), and fp16 rows end at 65504. The second plane is a second product in down: a
+// block of 64 tokens through 512 experts 466 us instead of 459, of 2048 through 256
+// 270 instead of 246.
+constexpr int mx_h_planes(int32_t x_type) { return x_type == VQK_F32 ? 3 : 2; }
 
 struct CombineArgs {
     const float *part;
@@ -230,7 +228,7 @@ static int plan_experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, co
     p->by_pair = mx_by_pair(p->N, g1->E, pb);
     p->x = 0;
     p->h = plane_bytes(T, g1->NB, p->P);
-    p->part = p->h + plane_bytes(p->N, g2->NB, x_type == VQK_F32 ? 3 : 2);
+    p->part = p->h + plane_bytes(p->N, g2->NB, mx_h_planes(x_type));
     p->sort = p->part + (p->by_pair ? 0 : al256(size_t(p->N) * g2->OUT * 4));
     p->total = p->sort + sort_bytes(p->N, g1->E, pb);
     return VQK_OK;
@@ -335,7 +333,7 @@ static int experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, const v
     uint16_t *h = reinterpret_cast<uint16_t *>(ws + p.h);
     const bool place = mx_x_in_place(gate, x, x_type) && (x_type != VQK_F16 || up->f16_exact);
     if ((rc = make_x(gate, place, x, x_type, T, g1.NB, reinterpret_cast<uint16_t *>(ws), &c.x, st))) return rc;
-    const int hp = mx_h_planes(x_type, p.by_pair, down->f16_exact != 0);
+    const int hp = mx_h_planes(x_type);
     c.y = h; c.ldy = p.IP; c.yplane = p.N * p.IP; c.yp = hp; c.ysorted = true;
     if ((rc = set_routing(&c, p.by_pair, ids, p.N, g1.E, rows, ws + p.sort, st))) return rc;
     if ((rc = run(c, rows, st))) return rc;
@@ -343,7 +341,7 @@ static int experts(const vqk_mx_weights *gate, const vqk_mx_weights *up, const v
     d.codes[0] = down->codes; d.scales[0] = down->scales;
     d.codes[1] = nullptr; d.scales[1] = nullptr;
     d.g = g2;
-    d.x = MxX{h, p.IP, p.N * p.IP, hp ? hp : 1, hp ? kOpBF16 : kOpF16};
+    d.x = MxX{h, p.IP, p.N * p.IP, hp, kOpBF16};
     d.xkrep = 0;
     if (p.by_pair) {
         const DownArgs a{d.codes[0], d.scales[0], g2.E, g2.OUT, int32_t(g2.RT), int32_t(g2.NC), int32_t(g2.NB),

@@ -17,8 +17,13 @@
 // fragment (v_cvt_scalef32_pk_bf16_fp4) issue in the shadow of the matrix
 // instructions: one conversion for each of them at BT = 4.
 // The loop exists for every number of 32-row groups that a tile may hold: a
-// routed expert's last rows cost what they are. x in planes (fp16 beyond exact
-// weights, fp32): the chunk's planes one after the other, weights loaded once.
+// routed expert's last rows cost what they are. x in planes (SwiGLU rows, fp16
+// beyond exact weights, fp32): where a tile's rows leave room for all planes in its
+// LDS stage, the planes stand there as more rows, their sums meet, and the weights
+// are loaded and decoded once; otherwise one plane a step, the weights again from
+// L2. (Blocks of experts whose SwiGLU rows stand in two planes: 64 tokens through
+// 512 experts, one or two rows a tile, 466 us folded, 555 in turn; 2048 through 256,
+// about 60 rows, 270 both ways.)
 #pragma once
 
 #include <type_traits>
@@ -35,7 +40,6 @@ constexpr int kMxgRows = 256;                 // weight rows per workgroup
 struct MxgArgs {
     MxsArgs a;
     int32_t ntiles_host;                      // x tiles when they are not counted on the device
-    int32_t planes;                           // bf16 planes of x
     int32_t splits, per;                      // K slices and chunks in each (splits = 1: none)
     float *part;                              // [splits][N][OUT] when splits > 1
 };
@@ -49,6 +53,17 @@ __device__ __forceinline__ f32x16v mx_mma32(u32x4 w, u32x4 x, f32x16v c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, w), __builtin_bit_cast(h8, x), c, 0, 0, 0);
 }
 
+// How a tile of up to 32 * G rows (G = 0: 16) in P planes stands in a stage of 32 * BT
+// rows: `planes` of them, `rows` apart, `groups` of 32 rows each; copies of 16 rows.
+template <int BT, int P, int G>
+struct MxgSpan {
+    static constexpr bool half = G == 0;                  // two planes in one group
+    static constexpr int groups = half ? 1 : G;
+    static constexpr int planes = half ? 2 : (G * P <= BT ? P : 1);
+    static constexpr int rows = half ? 16 : 32 * G;
+    static constexpr int copies = rows * planes / 16;
+};
+
 // What x is past its rows' ends.
 static __device__ __align__(16) uint8_t mxg_zeros[16];
 
@@ -60,14 +75,12 @@ __device__ __forceinline__ void mxg_keep_order() {
 }
 
 // ST: stages of x in LDS and of weights in registers (ST - 1 chunks in flight).
-// PL: x in more planes than one.
-template <int OP, int BT, int ST, bool GLU, bool PL>
+// P: planes of x.
+template <int OP, int BT, int ST, bool GLU, int P>
 __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga) {
     const MxsArgs &p = ga.a;
     constexpr int ROWS = 32 * BT;
     constexpr int STAGE = ROWS * 256;         // bytes of x per chunk
-    constexpr int CPW = STAGE / 1024 / kMxgWaves;
-    static_assert(CPW * kMxgWaves * 1024 == STAGE, "whole copies per wave");
     extern __shared__ __align__(16) uint8_t xs[];       // [ST][STAGE]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 31, g = lane >> 5;
@@ -112,77 +125,80 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
             wo[a] = (rt * NC * 64 + unit) * 16;
             so[a] = (rt * NC4 * 64 + unit) * 4;
         }
-        // the x copies of this lane: 16 bytes of one row each
-        const uint16_t *src[CPW];
-        int piece[CPW], xrow[CPW];
-#pragma unroll
-        for (int j = 0; j < CPW; ++j)
-            xrow[j] = tile.row0 + min((j * kMxgWaves + wave) * 4 + (lane >> 4), tile.nrows - 1);
-        mx_x_rows(p, xrow);
-#pragma unroll
-        for (int j = 0; j < CPW; ++j) {
-            const int n = (j * kMxgWaves + wave) * 4 + (lane >> 4);
-            piece[j] = (lane & 15) ^ (n & 15);
-            src[j] = p.x + int64_t(xrow[j]) * p.xld + piece[j] * 8;
-        }
         struct Weights {
             u32x4 w[2][2];
             uint32_t s[2][2];
         };
         Weights wb[ST];
-        // steps: chunk c_lo + step / P, plane step % P (the weights again for each plane). NA: groups of
-        // 32 rows that the tile holds
-        const int P = PL ? ga.planes : 1, steps = (c_hi - c_lo) * P;
-        auto issue = [&](int step, auto slot, auto na) {
-            const int c = c_lo + (PL ? step / P : step), pl = PL ? step % P : 0;
-            constexpr int S = decltype(slot)::value;
+        auto walk = [&](auto span) {
+            using Sp = decltype(span);
+            // the x copies of this lane: 16 bytes of one row each
+            const uint16_t *src[Sp::copies];
+            int piece[Sp::copies], xrow[Sp::copies];
 #pragma unroll
-            for (int j = 0; j < 2 * decltype(na)::value; ++j) {
-                // past the row's last block: zeros
-                const uint16_t *from = src[j] + pl * p.xplane + int64_t(c) * kMxChunk;
-                from = 4 * c + piece[j] / 4 < p.NB ? from : reinterpret_cast<const uint16_t *>(mxg_zeros);
-                __builtin_amdgcn_global_load_lds((global_void *)from,
-                                                 (lds_void *)(xs + S * STAGE + (j * kMxgWaves + wave) * 1024), 16, 0, 0);
+            for (int j = 0; j < Sp::copies; ++j) {
+                const int n = (j * kMxgWaves + wave) * 4 + (lane >> 4);
+                xrow[j] = tile.row0 + min(n % Sp::rows, tile.nrows - 1);
             }
+            mx_x_rows(p, xrow);
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
+            for (int j = 0; j < Sp::copies; ++j) {
+                const int n = (j * kMxgWaves + wave) * 4 + (lane >> 4);
+                piece[j] = (lane & 15) ^ (n & 15);
+                src[j] = p.x + (n / Sp::rows) * p.xplane + int64_t(xrow[j]) * p.xld + piece[j] * 8;
+            }
+            // steps: chunk c_lo + step / turns, plane step % turns (the weights again for each)
+            constexpr int turns = P / Sp::planes;
+            const int steps = (c_hi - c_lo) * turns;
+            auto issue = [&](int step, auto slot) {
+                const int c = c_lo + step / turns;
+                constexpr int S = decltype(slot)::value;
+#pragma unroll
+                for (int j = 0; j < Sp::copies; ++j) {
+                    // past the row's last block: zeros
+                    const uint16_t *from = src[j] + (step % turns) * p.xplane + int64_t(c) * kMxChunk;
+                    from = 4 * c + piece[j] / 4 < p.NB ? from : reinterpret_cast<const uint16_t *>(mxg_zeros);
+                    __builtin_amdgcn_global_load_lds((global_void *)from,
+                                                     (lds_void *)(xs + S * STAGE + (j * kMxgWaves + wave) * 1024), 16, 0, 0);
+                }
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        wb[S].w[a][q] = *reinterpret_cast<const u32x4 *>(cb[a] + (wo[a] + uint32_t(c) * 1024u + q * 256u));
+                        wb[S].s[a][q] = *reinterpret_cast<const uint32_t *>(sb[a] + (so[a] + uint32_t(c / 4) * 256u + q * 64u));
+                    }
+            };
+            auto mul = [&](int step, auto slot) {
+                constexpr int S = decltype(slot)::value;
+                const Weights &d = wb[S];
+                const int c = c_lo + step / turns;
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    wb[S].w[a][q] = *reinterpret_cast<const u32x4 *>(cb[a] + (wo[a] + uint32_t(c) * 1024u + q * 256u));
-                    wb[S].s[a][q] = *reinterpret_cast<const uint32_t *>(sb[a] + (so[a] + uint32_t(c / 4) * 256u + q * 64u));
-                }
-        };
-        auto mul = [&](int step, auto slot, auto na) {
-            constexpr int S = decltype(slot)::value;
-            const Weights &d = wb[S];
-            const int c = c_lo + (PL ? step / P : step);
+                    float sc[2];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                float sc[2];
+                    for (int a = 0; a < 2; ++a) {
+                        const uint32_t b = (d.s[a][q] >> (8 * (c & 3))) & 255u;
+                        nan[a] = nan[a] || b == 255u;
+                        sc[a] = mx_scale(b == 255u ? 127u : b);
+                    }
 #pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    const uint32_t b = (d.s[a][q] >> (8 * (c & 3))) & 255u;
-                    nan[a] = nan[a] || b == 255u;
-                    sc[a] = mx_scale(b == 255u ? 127u : b);
-                }
+                    for (int h = 0; h < 4; ++h) {
+                        u32x4 wf[2];
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    u32x4 wf[2];
+                        for (int a = 0; a < 2; ++a) wf[a] = mx_decode8_op<OP>(d.w[a][q][h], sc[a]);
+                        const int at = ((8 * g + 4 * q + h) ^ (lane & 15)) * 16 + r * 256;
 #pragma unroll
-                    for (int a = 0; a < 2; ++a) wf[a] = mx_decode8_op<OP>(d.w[a][q][h], sc[a]);
-                    const int at = ((8 * g + 4 * q + h) ^ (lane & 15)) * 16 + r * 256;
+                        for (int b = 0; b < Sp::copies / 2; ++b) {
+                            const u32x4 xv = *reinterpret_cast<const u32x4 *>(xs + S * STAGE + b * 8192 + at);
 #pragma unroll
-                    for (int b = 0; b < decltype(na)::value; ++b) {
-                        const u32x4 xv = *reinterpret_cast<const u32x4 *>(xs + S * STAGE + b * 8192 + at);
-#pragma unroll
-                        for (int a = 0; a < 2; ++a) acc[a][b] = mx_mma32<OP>(wf[a], xv, acc[a][b]);
+                            for (int a = 0; a < 2; ++a)
+                                acc[a][b % Sp::groups] = mx_mma32<OP>(wf[a], xv, acc[a][b % Sp::groups]);
+                        }
                     }
                 }
-            }
-        };
-        // steps: chunk c_lo + step / P, plane step % P
-        auto walk = [&](auto na) {
-            constexpr int OPS = 2 * decltype(na)::value + 8;      // loads of a stage
+            };
+            constexpr int OPS = Sp::copies + 8;           // loads of a stage
             using s0 = std::integral_constant<int, 0>;
             using s1 = std::integral_constant<int, 1>;
             using s2 = std::integral_constant<int, ST - 1>;
@@ -198,15 +214,15 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
                 __builtin_amdgcn_s_barrier();             // (a __syncthreads would wait for every load)
                 mxg_keep_order();
                 issue(min(step + ST - 1, steps - 1),
-                      std::integral_constant<int, (decltype(slot)::value + ST - 1) % ST>{}, na);
+                      std::integral_constant<int, (decltype(slot)::value + ST - 1) % ST>{});
                 mxg_keep_order();
-                if (step < steps) mul(step, slot, na);
+                if (step < steps) mul(step, slot);
             };
             if (steps <= 0) return;
-            issue(0, s0{}, na);
+            issue(0, s0{});
             mxg_keep_order();
             if constexpr (ST == 3) {
-                issue(min(1, steps - 1), s1{}, na);
+                issue(min(1, steps - 1), s1{});
                 mxg_keep_order();
             }
 #pragma unroll 1
@@ -216,12 +232,20 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
                 if constexpr (ST == 3) one(step + 2, s2{});
             }
             wait_vmem();
+            if constexpr (Sp::half) {                     // the second plane's sums are 16 lanes further
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[a][0][i] += __shfl_xor(acc[a][0][i], 16);
+            }
         };
         const int groups = (tile.nrows + 31) / 32;
-        if (BT > 1 && groups <= 1) walk(std::integral_constant<int, 1>{});
-        else if (BT > 2 && groups == 2) walk(std::integral_constant<int, (BT > 2 ? 2 : BT)>{});
-        else if (BT > 3 && groups == 3) walk(std::integral_constant<int, (BT > 3 ? 3 : BT)>{});
-        else walk(std::integral_constant<int, BT>{});
+        if (BT == 1 && P == 2 && tile.nrows <= 16) {
+            if constexpr (BT == 1 && P == 2) walk(MxgSpan<BT, P, 0>{});
+        } else if (BT > 1 && groups <= 1) walk(MxgSpan<BT, P, 1>{});
+        else if (BT > 2 && groups == 2) walk(MxgSpan<BT, P, (BT > 2 ? 2 : BT)>{});
+        else if (BT > 3 && groups == 3) walk(MxgSpan<BT, P, (BT > 3 ? 3 : BT)>{});
+        else walk(MxgSpan<BT, P, BT>{});
     }
 
     // register i of lane l: weight row 8 * (i / 4) + 4 * (l / 32) + i % 4, x row l % 32. A NaN block
@@ -236,6 +260,7 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
         const int o = 8 * (i / 4) + 4 * g + i % 4;
         return (nm[a] >> o) & 1 ? __uint_as_float(0x7fc00000u) : acc[a][b][i];
     };
+    if (GLU && ow >= p.ocover) return;        // whole blocks of 32, as ow is
     int yrow[BT];
 #pragma unroll
     for (int b = 0; b < BT; ++b) yrow[b] = tile.row0 + min(32 * b + r, tile.nrows - 1);
@@ -249,17 +274,16 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int o = ow + 8 * j + 4 * g;
-                if (o >= p.ocover) continue;  // ocover is whole blocks of 32
                 float h[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float v = value(0, b, 4 * j + i), u = value(1, b, 4 * j + i);
                     h[i] = o + i < p.OUT ? mx_swiglu(v, u) : 0.f;
                 }
-                for (int pl = 0; pl < max(p.yp, 1); ++pl) {
+                for (int pl = 0; pl < p.yp; ++pl) {
                     uint16_t q[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) q[i] = p.yp == 0 ? f32_to_h(h[i]) : mx_plane_next(h[i]);
+                    for (int i = 0; i < 4; ++i) q[i] = mx_plane_next(h[i]);
                     u32x2 v2;
                     v2.x = q[0] | (uint32_t(q[1]) << 16);
                     v2.y = q[2] | (uint32_t(q[3]) << 16);

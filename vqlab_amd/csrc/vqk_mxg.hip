@@ -71,31 +71,31 @@ size_t mxg_part_bytes(int64_t N, const MxGeom &g) {
     return s > 1 ? size_t(s) * N * g.OUT * 4 : 0;
 }
 
-template <int OP, int BT, int ST, bool GLU, bool PL>
+template <int OP, int BT, int ST, bool GLU, int P>
 static int go(MxgArgs ga, int64_t tiles, hipStream_t st) {
     MxsArgs &a = ga.a;
     a.nob = int32_t((a.ocover + (GLU ? kMxgRows / 2 : kMxgRows) - 1) / (GLU ? kMxgRows / 2 : kMxgRows));
     const int64_t grid = int64_t(a.nob) * tiles * ga.splits;
     if (grid > INT32_MAX) return set_error(VQK_ENOTIMPL, "MXFP4 product: grid too large");
     ga.ntiles_host = int32_t(tiles);
-    int rc = launch_with_lds<k_mx_gemm<OP, BT, ST, GLU, PL>>(dim3(unsigned(grid)), dim3(64 * kMxgWaves),
-                                                        size_t(ST) * 32 * BT * 256, st, ga);
+    int rc = launch_with_lds<k_mx_gemm<OP, BT, ST, GLU, P>>(dim3(unsigned(grid)), dim3(64 * kMxgWaves),
+                                                       size_t(ST) * 32 * BT * 256, st, ga);
     if (rc || ga.splits == 1) return rc;
     return launch_mx_reduce(ga.part, ga.splits, a.N * a.OUT, a.y, a.y_type, st);
 }
 
 template <int BT, int ST, bool GLU>
-static int go_op(const MxgArgs &a, int op, int64_t tiles, hipStream_t st) {
-    if (op == kOpF16) return go<kOpF16, BT, ST, GLU, false>(a, tiles, st);
-    return a.planes == 1 ? go<kOpBF16, BT, ST, GLU, false>(a, tiles, st)
-                         : go<kOpBF16, BT, ST, GLU, true>(a, tiles, st);
+static int go_op(const MxgArgs &a, int op, int planes, int64_t tiles, hipStream_t st) {
+    if (op == kOpF16) return go<kOpF16, BT, ST, GLU, 1>(a, tiles, st);
+    if (planes == 1) return go<kOpBF16, BT, ST, GLU, 1>(a, tiles, st);
+    return planes == 2 ? go<kOpBF16, BT, ST, GLU, 2>(a, tiles, st) : go<kOpBF16, BT, ST, GLU, 3>(a, tiles, st);
 }
 template <bool GLU>
-static int go_bt(const MxgArgs &a, int op, int tile_rows, int64_t tiles, hipStream_t st) {
+static int go_bt(const MxgArgs &a, int op, int planes, int tile_rows, int64_t tiles, hipStream_t st) {
     // three stages where registers and LDS leave two workgroups a CU
-    if (tile_rows <= 32) return go_op<1, 3, GLU>(a, op, tiles, st);
-    if (tile_rows <= 64) return go_op<2, 3, GLU>(a, op, tiles, st);
-    return go_op<4, 2, GLU>(a, op, tiles, st);
+    if (tile_rows <= 32) return go_op<1, 3, GLU>(a, op, planes, tiles, st);
+    if (tile_rows <= 64) return go_op<2, 3, GLU>(a, op, planes, tiles, st);
+    return go_op<4, 2, GLU>(a, op, planes, tiles, st);
 }
 
 // tile_rows: x rows per tile (32, 64 or 128; the sort's for a sorted routing).
@@ -103,7 +103,6 @@ int mx_gemm(const MxCall &c, int tile_rows, float *part, size_t part_bytes, hipS
     const bool glu = c.codes[1] != nullptr;
     MxgArgs ga{};
     mx_args(c, &ga.a);
-    ga.planes = c.x.P;
     const int64_t tiles = mx_tiles(c, tile_rows);
     if (tiles == 0) return VQK_OK;
     ga.splits = 1;
@@ -116,7 +115,8 @@ int mx_gemm(const MxCall &c, int tile_rows, float *part, size_t part_bytes, hipS
             ga.part = part;
         }
     }
-    return glu ? go_bt<true>(ga, c.x.op, tile_rows, tiles, st) : go_bt<false>(ga, c.x.op, tile_rows, tiles, st);
+    return glu ? go_bt<true>(ga, c.x.op, c.x.P, tile_rows, tiles, st)
+               : go_bt<false>(ga, c.x.op, c.x.P, tile_rows, tiles, st);
 }
 
 }  // namespace vqk

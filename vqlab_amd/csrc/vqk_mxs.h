@@ -236,9 +236,7 @@ __global__ void __launch_bounds__(64 * kMxsWaves, 2) k_mx_rows(const MxsArgs p) 
             if constexpr (GLU) {
                 float h = o < p.OUT ? mx_swiglu(v, u) : 0.f;
                 uint16_t *y = static_cast<uint16_t *>(p.y) + yr * p.ldy + o;
-                if (p.yp == 0) *y = f32_to_h(h);
-                else
-                    for (int pl = 0; pl < p.yp; ++pl) y[pl * p.yplane] = mx_plane_next(h);
+                for (int pl = 0; pl < p.yp; ++pl) y[pl * p.yplane] = mx_plane_next(h);
             } else {
                 store_act(p.y, p.y_type, yr * p.ldy + o, v);
             }

@@ -284,7 +284,8 @@ class MXSwitchLinear(_Packed):
 class MXSwitchGLU(torch.nn.Module):
     """SwitchGLU with MXFP4 projections: forward(x [T, H], ids [T, k], weights [T, k]) ->
     sum_j weights_j * down_j(silu(gate_j(x)) * up_j(x)), [T, H]. Ids outside [0, E) add nothing.
-    The SwiGLU rows are rounded to x's type (few pairs: less). Serving only: no gradient."""
+    The SwiGLU rows are kept in 16 bits of bf16's range (24 for fp32 x). Serving only: no
+    gradient."""
 
     def __init__(self, gate_proj: MXSwitchLinear, up_proj: MXSwitchLinear, down_proj: MXSwitchLinear):
         super().__init__()
