@@ -433,7 +433,8 @@ int vqk_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows,
 
 /* y [N, OUT] = x [N, IN] . W^T, fp32 accumulation, one rounding into y_type
  * (VQK_VIA_F16 as elsewhere). act: VQK_MX_ACT_NONE takes x as it is (every
- * weight and every x enters the matrix cores exactly); VQK_MX_ACT_MXFP4
+ * weight and every finite x enters the matrix cores exactly, but for bits
+ * under 2^-126, which may be dropped); VQK_MX_ACT_MXFP4
  * quantises x's rows as vqk_mx_quantize does and multiplies 4-bit operands.
  * The workspace is 256-byte aligned. */
 #define VQK_MX_ACT_NONE  0

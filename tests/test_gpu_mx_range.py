@@ -67,3 +67,20 @@ def test_swiglu_rows_beyond_fp16(dtype, T):
     ref, bar = mc.experts(xv, ids, w.astype(np.float64), *ws, H_ROUND[dtype])
     bar = bar + mc.HALF_STEP[dtype] * (np.abs(ref) + bar) + (2.0 ** -25 if dtype == "fp16" else 0.0)
     mc.assert_within(glu(x, *_dev(ids, w)), ref, bar, "experts")
+
+
+# ----------------------------------------------------- x beyond bf16's range
+@pytest.mark.parametrize("N", [1, 20, 70, 200])
+def test_fp32_x_above_the_largest_bf16(N):
+    """Every finite fp32 x is finite in the product, forward and backward."""
+    from vqlab_amd import mx
+    rng = np.random.default_rng(N)
+    codes, scales = mc.weight(rng, 48, 96)
+    lin, w = mx.MXLinear(*_dev(codes, scales - 8), 96), mc.values(codes, scales - 8, 96)
+    big = float(np.finfo(np.float32).max)
+    for cols, rows, call in ((96, w, lin), (48, w.T, lin._dx)):
+        x, _ = mc.acts(rng, "fp32", N, cols)
+        x[0, 3], x[N // 2, 17], x[N - 1, cols - 1] = big, -big, big * (1 - 2.0 ** -10)
+        y, bar = mc.product_bar(x.double().cpu().numpy(), rows, "fp32")
+        assert np.abs(y).max() < big
+        mc.assert_within(call(x), y, bar, "large x")

@@ -84,13 +84,15 @@ constexpr uint32_t kMxF16ScaleMin = 104, kMxF16ScaleMax = 140;
 // for bf16, two for fp16 (11 significant bits = 8 + 3), three for fp32 (24).
 constexpr int mx_planes(int32_t type) { return type == VQK_BF16 ? 1 : (type == VQK_F16 ? 2 : 3); }
 
-// Plane pl of v: bf16 of what the planes before it leave. A value that is not
-// finite stands in plane 0 alone.
+// The next plane of a value: bf16 of what the planes before it leave. A value that
+// is not finite stands in plane 0 alone; a finite one that would round past the
+// largest bf16 (2^128 (1 - 2^-9) and up) starts with that number instead, and the
+// next two planes hold the 16 bits under it.
 __device__ __forceinline__ uint16_t mx_plane_next(float &rest) {
-    const uint16_t h = f32_to_bf16(rest);
-    const float f = bf16_to_f32(h);
-    const bool fin = (__float_as_uint(f) & 0x7f800000u) != 0x7f800000u;
-    rest = fin ? rest - f : 0.f;
+    const bool fin = (__float_as_uint(rest) & 0x7f800000u) != 0x7f800000u;
+    uint16_t h = f32_to_bf16(rest);
+    h -= uint16_t(fin && (h & 0x7fffu) == 0x7f80u);
+    rest = fin ? rest - bf16_to_f32(h) : 0.f;
     return h;
 }
 

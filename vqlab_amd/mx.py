@@ -170,8 +170,8 @@ class MXLinear(_Packed):
     """Bias-free linear whose weight is MXFP4: codes uint8 [OUT, 16 B], scales uint8 [OUT, B]
     (the module keeps its own copy, in the kernels' operand order). in_features may be any width of
     the last block (default: all 32 of it). act: None multiplies x as it is (bf16, fp16 and fp32
-    enter exactly, fp32 sums); "mxfp4" quantises x's rows as mx_quantize does. Differentiable in x
-    with act None; the weight is frozen."""
+    enter exactly, but for bits under 2^-126; fp32 sums); "mxfp4" quantises x's rows as mx_quantize
+    does. Differentiable in x with act None; the weight is frozen."""
 
     def __init__(self, codes, scales, in_features=None, act=None):
         super().__init__()
