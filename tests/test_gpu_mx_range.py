@@ -84,3 +84,100 @@ def test_fp32_x_above_the_largest_bf16(N):
         y, bar = mc.product_bar(x.double().cpu().numpy(), rows, "fp32")
         assert np.abs(y).max() < big
         mc.assert_within(call(x), y, bar, "large x")
+
+
+# ------------------------------------------- weights of 2^128 and beyond
+def _huge(rng, E, OUT, IN):
+    """Experts of ordinary weights, but for expert 0: 6 * 2^127 throughout."""
+    codes, scales = mc.weight(rng, E, OUT, IN)
+    codes[0], scales[0] = 0x77, 254
+    return codes, scales
+
+
+def test_values_past_fp32_read_as_infinite():
+    from vqlab_amd import mx
+    codes = np.tile(np.arange(16, dtype=np.uint8) * 17, (4, 1))           # each code twice
+    scales = np.array([[252], [253], [254], [255]], np.uint8)
+    ref = mc.values(codes, scales, 32)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        got = mx.mx_dequantize(*_dev(codes, scales), 32, dtype).double().cpu().numpy()
+        top = float(torch.finfo(dtype).max)
+        want = np.where(np.abs(ref) > top, np.copysign(np.inf, ref), ref)
+        assert np.array_equal(got, want, equal_nan=True)
+
+
+@pytest.mark.parametrize("T,k", [(1, 3), (7, 2), (40, 2)])
+@pytest.mark.parametrize("IN", [96, 640, 1664])
+def test_pairs_without_an_expert_are_zero_beside_an_expert_of_infinities(T, k, IN):
+    from vqlab_amd import mx
+    rng = np.random.default_rng(T + IN)
+    codes, scales = _huge(rng, 6, 48, IN)
+    sw, w = mx.MXSwitchLinear(*_dev(codes, scales), IN), mc.values(codes, scales, IN)
+    x, xv = mc.acts(rng, "bf16", T, 1, 1, IN)
+    ids = rng.integers(1, 6, (T, k))
+    ids[rng.random((T, k)) < 0.4] = -1
+    ids[0, 0], ids[T - 1, k - 1] = -1, 6
+    y = sw(x, *_dev(ids))
+    for t in range(T):
+        for j in range(k):
+            if 1 <= ids[t, j] < 6:
+                ref, bar = mc.product_bar(xv[t, 0], w[ids[t, j]], "bf16")
+                mc.assert_within(y[t, j], ref, bar, f"pair {t}, {j}")
+            else:
+                assert (y[t, j] == 0).all()
+
+
+@pytest.mark.parametrize("T", [1, 5, 40])
+def test_an_expert_that_nobody_chose_changes_nothing(T):
+    from vqlab_amd import mx
+    rng = np.random.default_rng(T)
+    E, H, I, k = 6, 160, 96, 3
+    mods, ws = [], []
+    for OUT, IN in ((I, H), (I, H), (H, I)):
+        codes, scales = _huge(rng, E, OUT, IN)
+        mods.append(mx.MXSwitchLinear(*_dev(codes, scales), IN))
+        ws.append(mc.values(codes, scales, IN))
+    glu = mx.MXSwitchGLU(*mods)
+    x, xv = mc.acts(rng, "bf16", T, H)
+    ids = np.stack([1 + rng.permutation(E - 1)[:k] for _ in range(T)])
+    ids[0, 1] = -1
+    w = rng.random((T, k)).astype(np.float32)
+    ref, bar = mc.experts(xv, ids, w.astype(np.float64), *ws, mc.HALF_STEP["bf16"])
+    mc.assert_within(glu(x, *_dev(ids, w)), ref, bar + mc.HALF_STEP["bf16"] * (np.abs(ref) + bar), "experts")
+
+
+@pytest.mark.parametrize("N", [1, 2, 9, 20, 70])
+@pytest.mark.parametrize("IN", [640, 1152, 5248])
+def test_an_infinite_weight_in_the_last_chunk(N, IN):
+    """Products of positive x with a weight of 2^128 or more are infinite, not NaN."""
+    from vqlab_amd import mx
+    rng = np.random.default_rng(N + IN)
+    codes, scales = mc.weight(rng, 40, IN)
+    codes[7, -16:], scales[7, -1] = 0x77, 254
+    codes[20, -16:], scales[20, -1] = 0xff, 253
+    lin = mx.MXLinear(*_dev(codes, scales), IN)
+    x = (mc.acts(rng, "bf16", N, IN)[0].abs() + 0.5)
+    y = lin(x).float().cpu().numpy()
+    assert (y[:, 7] == np.inf).all() and (y[:, 20] == -np.inf).all()
+    rest = np.delete(np.arange(40), [7, 20])
+    ref, bar = mc.product_bar(x.double().cpu().numpy(), mc.values(codes, scales, IN)[rest], "bf16")
+    mc.assert_within(y[:, rest], ref, bar, "other rows")
+
+
+@pytest.mark.parametrize("N", [20, 70, 200])
+def test_4_bit_products_of_huge_weights(N):
+    """From 65 rows on the matrix instruction takes both scales as they are: a product that fits is
+    finite. Fewer rows multiply by the values, which are infinite."""
+    from vqlab_amd import mx
+    rng = np.random.default_rng(N)
+    codes, scales = mc.weight(rng, 40, 96)
+    codes[7], scales[7] = 0x77, 254
+    lin = mx.MXLinear(*_dev(codes, scales), 96, act="mxfp4")
+    x = ((mc.acts(rng, "fp32", N, 96)[0].abs() + 0.5) * 2.0 ** -100)
+    y = lin(x)
+    q = mc.values(*mc.quantize(x.double().cpu().numpy()), 96)
+    ref, bar = mc.product_bar(q, mc.values(codes, scales, 96), "fp32")
+    if N < 65:
+        assert (y[:, 7] == float("inf")).all()
+        ref, bar, y = np.delete(ref, 7, 1), np.delete(bar, 7, 1), y[:, [i for i in range(40) if i != 7]]
+    mc.assert_within(y, ref, bar, "huge weights")

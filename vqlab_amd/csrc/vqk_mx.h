@@ -7,7 +7,9 @@
 // Three facts carry every kernel here:
 //   * e2m1 * 2^(s - 127) has at most two significant bits and an exponent
 //     inside bf16's, so a bf16 weight is the exact weight
-//     (v_cvt_scalef32_pk_bf16_fp4 makes two of them, scale included);
+//     (v_cvt_scalef32_pk_bf16_fp4 makes two of them, scale included). Only s = 253
+//     from code 4 and s = 254 from code 2 up give 2^128 and more: infinite, in bf16 as
+//     in fp32. The 4-bit products alone multiply those as they are;
 //   * the sum over k may be taken in any order, so a lane of a matrix
 //     instruction can own whole blocks (16 bytes, one scale): in a chunk of 128 k
 //     the lane groups take the chunk's four blocks, and step h multiplies

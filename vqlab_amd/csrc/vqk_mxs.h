@@ -117,7 +117,9 @@ __global__ void __launch_bounds__(64 * kMxsWaves, 2) k_mx_rows(const MxsArgs p) 
         cb[a] = p.codes[a] + ex * mx_expert_codes(p.RT, p.NC);
         sb[a] = p.scales[a] + ex * mx_expert_scales(p.RT, p.NC);
     }
-    // this wave's chunks: kw * NCW ..; past the last one the last stands in, against x of zero
+    // this wave's chunks: kw * NCW ..; past the last one the last stands in, and for a pair without
+    // an expert expert 0: against x of zero, and under a scale of 1, because a weight of 2^128 or
+    // more decodes to infinity, which zero does not cancel
     const uint32_t NC = uint32_t(p.NC), NC4 = (NC + 3) / 4;
     u32x4 w[TT][NCW], wn[TT][NCW];
     uint32_t sc[TT][NCW], scn[TT][NCW];
@@ -205,9 +207,9 @@ __global__ void __launch_bounds__(64 * kMxsWaves, 2) k_mx_rows(const MxsArgs p) 
             for (int b = 0; b < NT; ++b) acc[a][b] = f32x4{};
 #pragma unroll
             for (int c = 0; c < NCW; ++c) {
-                const bool bad = sc[a][c] == 255u;
-                nan = nan || bad;             // a chunk that stands in is of the same row
-                const float s = mx_scale(bad ? 127u : sc[a][c]);
+                const uint32_t e = live && uint32_t(kw * NCW + c) < NC ? sc[a][c] : 127u;
+                nan = nan || e == 255u;
+                const float s = mx_scale(e == 255u ? 127u : e);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const u32x4 wf = mx_decode8_op<OP>(w[a][c][k], s);
@@ -219,8 +221,8 @@ __global__ void __launch_bounds__(64 * kMxsWaves, 2) k_mx_rows(const MxsArgs p) 
                 }
             }
             // a NaN block makes its whole output column NaN, whichever of its lane groups holds it
-            if (__ballot(nan && live)) {
-                int f = nan && live;
+            if (__ballot(nan)) {
+                int f = nan;
                 f |= __shfl_xor(f, 16);
                 f |= __shfl_xor(f, 32);
 #pragma unroll

@@ -64,7 +64,8 @@ def _check_mx(codes, scales, cols, what):
 
 
 def mx_dequantize(codes, scales, cols, dtype=torch.bfloat16):
-    """The values [..., cols] that codes and scales stand for, in dtype (exact in bf16 and fp32)."""
+    """The values [..., cols] that codes and scales stand for, in dtype (exact in bf16 and fp32; 2^128
+    and more, which scales of 253 and 254 can say, are infinite)."""
     T.require_cuda(codes, scales)
     _check_mx(codes, scales, cols, "mx_dequantize")
     if dtype not in T.ACT_TYPES:
