@@ -86,9 +86,16 @@ def _aligned(t, n):
     return t if t.data_ptr() % n == 0 else t.clone()
 
 
+_IDS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+
+
 def _ids32(ids, E):
     """ids as int32; a wider id keeps being outside [0, E) when it is."""
-    return (ids if ids.dtype == torch.int32 else ids.clamp(-1, E).to(torch.int32)).contiguous()
+    if ids.dtype not in _IDS:
+        raise ValueError(f"expert ids must be integers (uint8, int8 .. int64), got {ids.dtype}")
+    if ids.dtype == torch.int64:
+        ids = ids.clamp(-1, E)
+    return ids.to(torch.int32).contiguous()
 
 
 def _desc(packed, E, OUT, IN):
