@@ -4,6 +4,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 import mx_cases as mc
 
@@ -70,3 +71,54 @@ def test_ids_that_are_no_integers_are_refused():
             glu(x, ids, wt)
         with pytest.raises(ValueError, match="ids"):
             glu.gate_proj(x[:, None, None], ids)
+
+
+# ------------------------------------------------- forward-mode derivatives
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("N", [1, 20, 130])
+def test_linear_forward_mode(dtype, N):
+    rng = np.random.default_rng(N)
+    lin, w = _linear(rng, 40, 96)
+    x, xv = mc.acts(rng, dtype, N, 96)
+    t, tv = mc.acts(rng, dtype, N, 96)
+    for leaf in (x, x.clone().requires_grad_(True)):
+        with fw.dual_level():
+            y = fw.unpack_dual(lin(fw.make_dual(leaf, t)))
+            assert y.tangent is not None
+            mc.assert_within(y.primal, *mc.product_bar(xv, w, dtype), "primal")
+            mc.assert_within(y.tangent, *mc.product_bar(tv, w, dtype), "tangent")
+
+
+def test_what_has_no_gradient_has_no_tangent_either():
+    from vqlab_amd import mx, router
+    rng = np.random.default_rng(4)
+    glu, _ = _glu(rng, 4, 64, 32)
+    a4, _ = _linear(rng, 32, 64, act="mxfp4")
+    ids, w = _dev(np.zeros((4, 2), np.int32), np.ones((4, 2), np.float32))
+    x, lg = torch.randn(4, 64, device="cuda"), torch.randn(4, 4, device="cuda")
+    blk = mx.MXSparseMoeBlock(glu, 2)
+    with fw.dual_level():
+        xd, wd, ld = (fw.make_dual(t, torch.ones_like(t)) for t in (x, w, lg))
+        for call in (lambda: mx.mx_quantize(xd), lambda: a4(xd), lambda: glu(xd, ids, w),
+                     lambda: glu(x, ids, wd), lambda: glu.gate_proj(xd[:, None, None], ids),
+                     lambda: blk(xd, lg), lambda: blk(x, ld)):
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no gradient"):
+                call()
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            router.route(ld, 2)
+        assert glu(x, ids, w).shape == (4, 64)             # no tangent: as ever
+        assert fw.unpack_dual(a4(x)).tangent is None
+
+
+def test_forward_over_reverse_is_refused():
+    """A gradient's own derivative would be dropped by the kernels that compute it."""
+    from vqlab_amd import router
+    lin, _ = _linear(np.random.default_rng(5), 40, 96)
+    with fw.dual_level():
+        x = fw.make_dual(torch.randn(3, 96, device="cuda").requires_grad_(True), torch.ones(3, 96, device="cuda"))
+        with pytest.raises(RuntimeError, match="gradient of MXLinear"):
+            torch.autograd.grad(lin(x).square().sum(), x)
+        lg = torch.randn(3, 8, device="cuda", requires_grad=True)
+        c = fw.make_dual(torch.ones((), device="cuda"), torch.ones((), device="cuda"))
+        with pytest.raises(RuntimeError, match="gradient of the router"):
+            torch.autograd.grad(router.route(lg, 2).z * c, lg)

@@ -23,3 +23,21 @@ def test_ids_are_integers(dtype):
     from vqlab_amd import mx
     with pytest.raises(ValueError, match="integers"):
         mx._ids32(torch.zeros(3, dtype=dtype), 8)
+
+
+def test_a_tangent_counts_as_wanting_a_derivative():
+    import torch.autograd.forward_ad as fw
+    from vqlab_amd import _torch as T
+    x = torch.randn(3)
+    assert not T.has_tangent(x)
+    T.no_grad_here("it", x, x)
+    with fw.dual_level():
+        d = fw.make_dual(x, torch.ones(3))
+        assert T.has_tangent(d) and not T.has_tangent(x)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no gradient"):
+            T.no_grad_here("it", x, d)
+    leaf = torch.randn(3, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        T.no_grad_here("it", leaf)
+    with torch.no_grad():
+        T.no_grad_here("it", leaf)

@@ -37,8 +37,7 @@ def mx_quantize(x):
     xt = T.act_type(x)
     if x.ndim == 0:
         raise ValueError("mx_quantize takes rows, got a scalar")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("mx_quantize has no gradient: detach x, or call it under no_grad")
+    T.no_grad_here("mx_quantize", x)
     C, B = x.shape[-1], _blocks(x.shape[-1])
     with T.on_device(x):
         if x.ndim == 2 and x.stride(1) == 1 and x.stride(0) >= C:
@@ -161,7 +160,7 @@ class _Packed(torch.nn.Module):
 
 
 class _LinearFn(torch.autograd.Function):
-    """y = x . W^T with a frozen W; the gradient reaches x."""
+    """y = x . W^T with a frozen W; the gradient reaches x, a tangent of x comes through."""
 
     @staticmethod
     def forward(ctx, x, mod):
@@ -171,7 +170,12 @@ class _LinearFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        T.no_grad_here("The gradient of MXLinear", dy)
         return ctx.mod._dx(dy), None
+
+    @staticmethod
+    def jvp(ctx, dx, _mod):
+        return ctx.mod._product(dx)
 
 
 class MXLinear(_Packed):
@@ -234,16 +238,11 @@ class MXLinear(_Packed):
             raise ValueError(f"MXLinear on {self._packed[0].device}, x on {x.device}")
         if x.ndim == 0 or x.shape[-1] != self.in_features:
             raise ValueError(f"MXLinear: x {tuple(x.shape)} for in_features {self.in_features}")
-        if x.requires_grad and torch.is_grad_enabled():
-            if self.act is not None:
-                raise RuntimeError("MXLinear(act='mxfp4') has no gradient: the rounding of x has none")
+        if self.act is not None:
+            T.no_grad_here("MXLinear(act='mxfp4')", x)
+        elif (x.requires_grad and torch.is_grad_enabled()) or T.has_tangent(x):
             return _LinearFn.apply(x, self)
         return self._product(x)
-
-
-def _no_grad(what, *ts):
-    if any(t.requires_grad for t in ts) and torch.is_grad_enabled():
-        raise RuntimeError(f"{what} has no gradient: run it under no_grad, or detach its inputs")
 
 
 class MXSwitchLinear(_Packed):
@@ -268,7 +267,7 @@ class MXSwitchLinear(_Packed):
 
     def forward(self, x, indices):
         T.require_cuda(x, indices, self._packed[0])
-        _no_grad("MXSwitchLinear", x)
+        T.no_grad_here("MXSwitchLinear", x)
         IN, OUT, k = self.input_dims, self.output_dims, int(indices.shape[-1])
         lead = tuple(indices.shape[:-1])
         if x.ndim < 3 or x.shape[-1] != IN or tuple(x.shape[:-3]) != lead or x.shape[-2] != 1 or \
@@ -310,7 +309,7 @@ class MXSwitchGLU(torch.nn.Module):
 
     def forward(self, x, ids, weights):
         T.require_cuda(x, ids, weights, self.gate_proj._packed[0])
-        _no_grad("MXSwitchGLU", x, weights)
+        T.no_grad_here("MXSwitchGLU", x, weights)
         H = self.gate_proj.input_dims
         if x.ndim != 2 or x.shape[1] != H or ids.ndim != 2 or ids.shape[0] != x.shape[0] or \
                 ids.shape != weights.shape:
@@ -350,7 +349,7 @@ class MXSparseMoeBlock(torch.nn.Module):
     def forward(self, x, logits=None, mask=None):
         if logits is None:
             logits = x.float() @ self.router_weight.float().T
-        _no_grad("MXSparseMoeBlock", x, logits)
+        T.no_grad_here("MXSparseMoeBlock", x, logits)
         g = self.switch_mlp.gate_proj
         T.require_cuda(x, logits, mask, g._packed[0])
         if x.ndim != 2 or x.shape[1] != g.input_dims or logits.shape != (x.shape[0], g.num_experts):

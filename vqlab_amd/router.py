@@ -119,6 +119,7 @@ class _RouteFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, _ids, dw, _counts, db, dz, _tokens):
         lg, ids, w, counts, stats, saved = ctx.saved_tensors
+        T.no_grad_here("The gradient of the router", *(g for g in (dw, db, dz) if g is not None))
         n, E = lg.shape
         with T.on_device(lg):
             d = torch.empty((n, E), dtype=lg.dtype, device=lg.device)
