@@ -122,3 +122,16 @@ def test_forward_over_reverse_is_refused():
         c = fw.make_dual(torch.ones((), device="cuda"), torch.ones((), device="cuda"))
         with pytest.raises(RuntimeError, match="gradient of the router"):
             torch.autograd.grad(router.route(lg, 2).z * c, lg)
+
+
+# ------------------------------------------------------------------- router
+def test_top_k_refuses_logits_that_want_a_gradient():
+    from vqlab_amd import router
+    lg = torch.randn(4, 8, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        router.top_k(lg, 2)
+    with torch.no_grad():
+        ids, w = router.top_k(lg, 2)
+    assert torch.equal(ids, router.top_k(lg.detach(), 2)[0]) and not w.requires_grad
+    with fw.dual_level(), torch.no_grad(), pytest.raises(RuntimeError, match="no gradient"):
+        router.top_k(fw.make_dual(lg.detach(), torch.ones_like(lg)), 2)

@@ -62,9 +62,11 @@ def rows(logits):
 
 
 def top_k(logits, k, norm_topk_prob=True, mask=None):
-    """ids int32 [T, k] and weights fp32 [T, k] of logits [T, E], one launch and no gradient: the
-    routing of a serving step. mask [T] (bool / uint8): 0 marks padding, whose ids are -1."""
+    """ids int32 [T, k] and weights fp32 [T, k] of logits [T, E], one launch: the routing of a
+    serving step. mask [T] (bool / uint8): 0 marks padding, whose ids are -1. Logits that want a
+    gradient are refused: that is route's."""
     _check(logits, mask)
+    T.no_grad_here("router.top_k", logits)
     with T.on_device(logits):
         lg, ld = rows(logits)
         m = mask_bytes(mask, lg)
