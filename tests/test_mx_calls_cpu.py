@@ -41,3 +41,11 @@ def test_a_tangent_counts_as_wanting_a_derivative():
         T.no_grad_here("it", leaf)
     with torch.no_grad():
         T.no_grad_here("it", leaf)
+
+
+@pytest.mark.parametrize("k", [-1, 0, 9])
+def test_router_refuses_other_numbers_of_experts(k):
+    from vqlab_amd import router
+    for call in (router.top_k, router.route):
+        with pytest.raises(ValueError, match="of 8 experts"):
+            call(torch.zeros(4, 8), k)

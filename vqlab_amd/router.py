@@ -42,9 +42,11 @@ def mask_bytes(mask, logits):
     return mask.contiguous()
 
 
-def _check(logits, mask):
+def _check(logits, k, mask):
     if logits.ndim != 2:
         raise ValueError(f"logits must be [T, E], got {tuple(logits.shape)}")
+    if not 1 <= k <= logits.shape[1]:
+        raise ValueError(f"top {k} of {logits.shape[1]} experts")
     T.act_type(logits)
     T.require_cuda(logits, mask)
 
@@ -65,7 +67,8 @@ def top_k(logits, k, norm_topk_prob=True, mask=None):
     """ids int32 [T, k] and weights fp32 [T, k] of logits [T, E], one launch: the routing of a
     serving step. mask [T] (bool / uint8): 0 marks padding, whose ids are -1. Logits that want a
     gradient are refused: that is route's."""
-    _check(logits, mask)
+    k = int(k)
+    _check(logits, k, mask)
     T.no_grad_here("router.top_k", logits)
     with T.on_device(logits):
         lg, ld = rows(logits)
@@ -138,5 +141,6 @@ def route(logits, k, norm_topk_prob=True, mask=None):
     """Route of logits [T, E] (fp16, bf16 or fp32), differentiable in the logits. mask [T] (bool /
     uint8): 0 marks padding, which gets ids -1, weights 0 and a zero gradient and enters neither
     counts nor losses; so does a token whose logits are all -inf."""
-    _check(logits, mask)
-    return Route(*_RouteFn.apply(logits, int(k), int(norm_topk_prob), mask))
+    k = int(k)
+    _check(logits, k, mask)
+    return Route(*_RouteFn.apply(logits, k, int(norm_topk_prob), mask))
