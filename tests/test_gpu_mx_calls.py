@@ -135,3 +135,22 @@ def test_top_k_refuses_logits_that_want_a_gradient():
     assert torch.equal(ids, router.top_k(lg.detach(), 2)[0]) and not w.requires_grad
     with fw.dual_level(), torch.no_grad(), pytest.raises(RuntimeError, match="no gradient"):
         router.top_k(fw.make_dual(lg.detach(), torch.ones_like(lg)), 2)
+
+
+def test_losses_can_be_changed_in_place():
+    """The other outputs and the gradient stay; a changed token count, which the gradient reads, is
+    an error."""
+    from vqlab_amd import router
+    lg = torch.randn(30, 16, device="cuda", requires_grad=True)
+    want = router.route(lg, 4)
+    dref = torch.autograd.grad(0.01 * want.balance + 2 * want.z, lg)[0]
+    r = router.route(lg, 4)
+    r.balance.mul_(0.01)
+    r.z.mul_(2)
+    assert torch.equal(r.z.detach(), 2 * want.z.detach()) and float(r.tokens) == 30
+    assert torch.equal(r.balance.detach(), 0.01 * want.balance.detach())
+    assert torch.equal(torch.autograd.grad(r.balance + r.z, lg)[0], dref)
+    r = router.route(lg, 4)
+    r.tokens.fill_(1e9)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(r.z, lg)

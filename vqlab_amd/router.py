@@ -114,6 +114,8 @@ class _RouteFn(torch.autograd.Function):
                                   stats.data_ptr(), saved.data_ptr(), work.data_ptr(), size,
                                   T.raw_stream(lg)), "route")
         balance, z, tokens = stats.unbind()
+        # no views, so that a loss can be scaled in place: the backward pass reads neither
+        balance, z = balance.data, z.data
         ctx.save_for_backward(lg, ids, w, counts, stats, saved)
         ctx.k, ctx.norm, ctx.ld = k, norm, ld
         ctx.mark_non_differentiable(ids, counts, tokens)
@@ -140,7 +142,8 @@ class _RouteFn(torch.autograd.Function):
 def route(logits, k, norm_topk_prob=True, mask=None):
     """Route of logits [T, E] (fp16, bf16 or fp32), differentiable in the logits. mask [T] (bool /
     uint8): 0 marks padding, which gets ids -1, weights 0 and a zero gradient and enters neither
-    counts nor losses; so does a token whose logits are all -inf."""
+    counts nor losses; so does a token whose logits are all -inf. The gradient reads ids, weights,
+    counts and tokens again: copy them before anything changes them in place, a collective among it."""
     k = int(k)
     _check(logits, k, mask)
     return Route(*_RouteFn.apply(logits, k, int(norm_topk_prob), mask))
