@@ -154,3 +154,11 @@ def test_losses_can_be_changed_in_place():
     r.tokens.fill_(1e9)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         torch.autograd.grad(r.z, lg)
+
+
+# ------------------------------------------------------------------ modules
+def test_a_block_without_logits_says_so():
+    from vqlab_amd import mx
+    glu, _ = _glu(np.random.default_rng(5), 4, 64, 32)
+    with pytest.raises(ValueError, match="router_weight"):
+        mx.MXSparseMoeBlock(glu, 2)(torch.randn(3, 64, device="cuda"))

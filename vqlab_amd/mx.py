@@ -348,6 +348,8 @@ class MXSparseMoeBlock(torch.nn.Module):
 
     def forward(self, x, logits=None, mask=None):
         if logits is None:
+            if self.router_weight is None:
+                raise ValueError("MXSparseMoeBlock without a router_weight needs logits")
             logits = x.float() @ self.router_weight.float().T
         T.no_grad_here("MXSparseMoeBlock", x, logits)
         g = self.switch_mlp.gate_proj
