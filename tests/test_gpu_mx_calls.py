@@ -1,6 +1,8 @@
 """How MXFP4 modules and the router are called and kept: types, derivatives, devices, state."""
 from __future__ import annotations
 
+import io
+
 import numpy as np
 import pytest
 import torch
@@ -162,3 +164,87 @@ def test_a_block_without_logits_says_so():
     glu, _ = _glu(np.random.default_rng(5), 4, 64, 32)
     with pytest.raises(ValueError, match="router_weight"):
         mx.MXSparseMoeBlock(glu, 2)(torch.randn(3, 64, device="cuda"))
+
+
+@pytest.mark.parametrize("E,OUT,IN", [(1, 16, 128), (1, 17, 129), (3, 70, 700), (2, 5, 1), (4, 33, 544)])
+def test_codes_and_scales_come_back(E, OUT, IN):
+    from vqlab_amd import mx
+    rng = np.random.default_rng(OUT)
+    codes, scales = _dev(*mc.weight(rng, E, OUT, IN))
+    sw = mx.MXSwitchLinear(codes, scales, IN)
+    assert torch.equal(sw.codes, codes) and torch.equal(sw.scales, scales)
+    lin = mx.MXLinear(codes[0], scales[0], IN)
+    assert torch.equal(lin.codes, codes[0]) and torch.equal(lin.scales, scales[0])
+
+
+@pytest.mark.parametrize("assign", [False, True])
+def test_state_dict_holds_the_weights(assign):
+    from vqlab_amd import mx
+    rng = np.random.default_rng(6)
+    (glu, ws), (other, _) = _glu(rng, 6, 96, 64), _glu(rng, 6, 96, 64)
+    net = torch.nn.ModuleList([glu, _linear(rng, 40, 96)[0]])
+    net2 = torch.nn.ModuleList([other, _linear(rng, 40, 96)[0]])
+    # weights beyond fp16 in the source only: what is looked up about them follows
+    codes, scales = mc.weight(rng, 40, 96)
+    scales[::3] = 90
+    net[1] = mx.MXLinear(*_dev(codes, scales), 96)
+    assert net2[1]._w.f16_exact and not net[1]._w.f16_exact
+    buf = io.BytesIO()
+    torch.save(net.state_dict(), buf)
+    buf.seek(0)
+    state = torch.load(buf, weights_only=True, map_location="cpu")
+    assert set(state) == {f"0.{p}_proj.{n}" for p in ("gate", "up", "down") for n in ("codes", "scales")} | \
+        {"1.codes", "1.scales"}
+    assert state["1.codes"].shape == (40, 48) and np.array_equal(state["1.scales"].numpy(), scales)
+    net2.load_state_dict(state, assign=assign)
+    assert not net2[1]._w.f16_exact
+    x, h = torch.randn(7, 96, device="cuda"), torch.randn(7, 96, device="cuda").half()
+    ids, w = torch.randint(0, 6, (7, 2), device="cuda"), torch.rand(7, 2, device="cuda")
+    assert torch.equal(net2[0](x, ids, w), net[0](x, ids, w)) and torch.equal(net2[1](h), net[1](h))
+    lost = dict(state)
+    del lost["1.scales"]
+    with pytest.raises(RuntimeError, match="1.scales"):
+        net2.load_state_dict(lost)
+    with pytest.raises(RuntimeError, match="shape"):
+        net2.load_state_dict({**state, "1.codes": state["1.codes"][:20], "1.scales": state["1.scales"][:20]})
+    with pytest.raises(RuntimeError, match="uint8"):
+        net2.load_state_dict({**state, "1.scales": state["1.scales"].int()})
+    assert torch.equal(net2[1](h), net[1](h))              # a refused load leaves the module as it was
+
+
+def test_a_captured_graph_follows_a_load():
+    rng = np.random.default_rng(10)
+    (lin, _), (other, _) = _linear(rng, 40, 96), _linear(rng, 40, 96)
+    x = torch.randn(7, 96, device="cuda", dtype=torch.bfloat16)
+    lin(x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = lin(x)
+    for src in (other, _linear(rng, 40, 96)[0], other):
+        lin.load_state_dict(src.state_dict())
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, src(x))
+
+
+def test_modules_move_with_their_weights():
+    from vqlab_amd import mx
+    rng = np.random.default_rng(7)
+    glu, _ = _glu(rng, 6, 64, 32)
+    blk = mx.MXSparseMoeBlock(glu, 2)
+    x, lg = torch.randn(5, 64, device="cuda"), torch.randn(5, 6, device="cuda")
+    ref = blk(x, lg)
+    blk.to("cpu")
+    assert all(not t.is_cuda for t in glu.up_proj._packed[:2]) and not glu.up_proj.codes.is_cuda
+    ids = torch.zeros(5, 1, dtype=torch.int32, device="cuda")
+    for call in (lambda: blk(x, lg), lambda: glu.gate_proj(x[:, None, None], ids)):
+        with pytest.raises(ValueError, match="device"):
+            call()
+    state = {k: v.clone() for k, v in blk.state_dict().items()}
+    blk.cuda()
+    assert torch.equal(blk(x, lg), ref)
+    assert torch.equal(blk.half()(x, lg), ref)             # codes and scales are no floats
+    assert all(torch.equal(v.cpu(), state[k]) for k, v in blk.state_dict().items())
+    blk.cpu().load_state_dict(state)                       # packed on the GPU, kept where the module is
+    assert torch.equal(blk.cuda()(x, lg), ref)

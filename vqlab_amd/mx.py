@@ -141,13 +141,71 @@ def _work(like, n):
 
 class _Packed(torch.nn.Module):
     """A module over packed weights: `_packed` tensors, `_shape` (E, OUT, IN), and the descriptor
-    `_w` of them that the library reads, which a copy makes anew."""
+    `_w` of them that the library reads, which a copy or a move makes anew. `codes` and `scales`
+    are the rows they were packed from, and what state_dict() holds."""
+
+    _rows = 3                                   # dimensions of codes and scales
 
     def _set(self, codes, scales, E, OUT, IN):
         self._shape = (int(E), int(OUT), int(IN))
-        self._packed = _pack(codes, scales, *self._shape)
-        self._w = _desc(self._packed, *self._shape)
         self._sizes = {}
+        self._keep(_pack(codes, scales, *self._shape))
+
+    def _keep(self, packed):
+        self._packed = packed
+        self._w = _desc(packed, *self._shape)
+
+    def _unpack(self, i, a, b, cols):
+        """Packed tensor i, [E, RT, groups, 4, 16, n], with its row of 16 moved to the front and its
+        last dimensions in the order a, b: rows [E, OUT, cols]."""
+        E, OUT, _ = self._shape
+        t = self._packed[i].view(E, -(-OUT // 16), -1, 4, 16, (16, 4)[i])
+        t = t.permute(0, 1, 4, 2, a, b).reshape(E, -(-OUT // 16) * 16, -1)[:, :OUT, :cols]
+        return (t if self._rows == 3 else t[0]).contiguous()
+
+    @property
+    def codes(self):
+        """Codes uint8 [(E,) OUT, 16 B], unpacked by each access."""
+        return self._unpack(0, 3, 5, 16 * _blocks(self._shape[2]))
+
+    @property
+    def scales(self):
+        """Scales uint8 [(E,) OUT, B], unpacked by each access."""
+        return self._unpack(1, 5, 3, _blocks(self._shape[2]))
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        destination[prefix + "codes"], destination[prefix + "scales"] = self.codes, self.scales
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys,
+                              unexpected_keys, error_msgs):
+        names = (prefix + "codes", prefix + "scales")
+        super()._load_from_state_dict({k: v for k, v in state_dict.items() if k not in names}, prefix,
+                                      local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        lost = [n for n in names if n not in state_dict]
+        if lost:
+            missing_keys.extend(lost)
+            return
+        B = _blocks(self._shape[2])
+        rows = self._shape[3 - self._rows:2]
+        wrong = [f"{n}: {t.dtype} of shape {tuple(t.shape)}, the module holds uint8 of shape {(*rows, c)}"
+                 for n, t, c in zip(names, map(state_dict.get, names), (16 * B, B))
+                 if t.dtype != torch.uint8 or t.shape != (*rows, c)]
+        if wrong:
+            error_msgs.extend(wrong)
+            return
+        here = self._packed[0].device
+        at = here if here.type == "cuda" else "cuda"       # packed by a GPU, kept where the module is
+        new = _pack(*(state_dict[n].to(at) for n in names), *self._shape)
+        for old, t in zip(self._packed, new[:2]):          # in place: captured graphs read these
+            old.copy_(t)
+        self._keep((*self._packed[:2], new[2]))
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        codes, scales, exact = self._packed
+        self._keep((fn(codes).to(torch.uint8), fn(scales).to(torch.uint8), exact))
+        return self
 
     def __getstate__(self):
         state = self.__dict__.copy()
@@ -156,7 +214,7 @@ class _Packed(torch.nn.Module):
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._w = _desc(self._packed, *self._shape)
+        self._keep(self._packed)
 
 
 class _LinearFn(torch.autograd.Function):
@@ -180,10 +238,13 @@ class _LinearFn(torch.autograd.Function):
 
 class MXLinear(_Packed):
     """Bias-free linear whose weight is MXFP4: codes uint8 [OUT, 16 B], scales uint8 [OUT, B]
-    (the module keeps its own copy, in the kernels' operand order). in_features may be any width of
-    the last block (default: all 32 of it). act: None multiplies x as it is (bf16, fp16 and fp32
-    enter exactly, but for bits under 2^-126; fp32 sums); "mxfp4" quantises x's rows as mx_quantize
-    does. Differentiable in x with act None; the weight is frozen."""
+    (the module keeps its own copy, in the kernels' operand order; state_dict holds the rows).
+    in_features may be any width of the last block (default: all 32 of it). act: None multiplies x
+    as it is (bf16, fp16 and fp32 enter exactly, but for bits under 2^-126; fp32 sums); "mxfp4"
+    quantises x's rows as mx_quantize does. Differentiable in x with act None; the weight is
+    frozen."""
+
+    _rows = 2
 
     def __init__(self, codes, scales, in_features=None, act=None):
         super().__init__()
