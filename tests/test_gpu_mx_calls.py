@@ -248,3 +248,18 @@ def test_modules_move_with_their_weights():
     assert all(torch.equal(v.cpu(), state[k]) for k, v in blk.state_dict().items())
     blk.cpu().load_state_dict(state)                       # packed on the GPU, kept where the module is
     assert torch.equal(blk.cuda()(x, lg), ref)
+
+
+def test_projections_on_another_device_are_refused():
+    from vqlab_amd import mx
+    glu, _ = _glu(np.random.default_rng(8), 4, 64, 32)
+    x, lg = torch.randn(5, 64, device="cuda"), torch.randn(5, 4, device="cuda")
+    ids, w = torch.zeros(5, 2, dtype=torch.int32, device="cuda"), torch.rand(5, 2, device="cuda")
+    for name in ("up_proj", "down_proj"):
+        getattr(glu, name).cpu()
+        with pytest.raises(ValueError, match="device"):
+            glu(x, ids, w)
+        with pytest.raises(ValueError, match="device"):
+            mx.MXSparseMoeBlock(glu, 2)(x, lg)
+        getattr(glu, name).cuda()
+    assert glu(x, ids, w).shape == (5, 64)

@@ -364,31 +364,30 @@ class MXSwitchGLU(torch.nn.Module):
         self.gate_proj, self.up_proj, self.down_proj = g, u, d
         self._sizes = {}
 
-    def _refs(self):
+    def _refs(self, *ts):
+        """The projections' descriptors; they and the tensors ts are on one device."""
         m = self._modules
-        return [ctypes.byref(m[n]._w) for n in ("gate_proj", "up_proj", "down_proj")]
+        g, u, d = m["gate_proj"], m["up_proj"], m["down_proj"]
+        T.require_cuda(*ts, g._packed[0], u._packed[0], d._packed[0])
+        return [ctypes.byref(p._w) for p in (g, u, d)]
 
     def forward(self, x, ids, weights):
-        T.require_cuda(x, ids, weights, self.gate_proj._packed[0])
+        refs = self._refs(x, ids, weights)
         T.no_grad_here("MXSwitchGLU", x, weights)
         H = self.gate_proj.input_dims
         if x.ndim != 2 or x.shape[1] != H or ids.ndim != 2 or ids.shape[0] != x.shape[0] or \
                 ids.shape != weights.shape:
             raise ValueError(f"MXSwitchGLU: x {tuple(x.shape)}, ids {tuple(ids.shape)}, weights "
                              f"{tuple(weights.shape)} for hidden size {H}")
-        return self._run(x, _ids32(ids, self.gate_proj.num_experts),
-                         weights.to(torch.float32).contiguous())
-
-    def _run(self, x, ids, wts):
-        xt, lib = T.act_type(x), L.lib()
-        n, k = ids.shape
-        ws = self._refs()
+        xt, lib, (n, k) = T.act_type(x), L.lib(), ids.shape
         with T.on_device(x):
+            ids = _ids32(ids, self.gate_proj.num_experts)
+            wts = weights.to(torch.float32).contiguous()
             x = x.contiguous()
             y = x.new_empty(x.shape)
-            size = _ws_bytes(self._sizes, (n, k, xt), lib.vqk_mx_experts_workspace, *ws, xt, n, k)
+            size = _ws_bytes(self._sizes, (n, k, xt), lib.vqk_mx_experts_workspace, *refs, xt, n, k)
             work, wp = _work(x, size)
-            rc = lib.vqk_mx_experts(*ws, x.data_ptr(), xt, n, ids.data_ptr(), wts.data_ptr(), k,
+            rc = lib.vqk_mx_experts(*refs, x.data_ptr(), xt, n, ids.data_ptr(), wts.data_ptr(), k,
                                     y.data_ptr(), xt, wp, size, T.raw_stream(x))
             if rc:
                 L.check(rc, "MXSwitchGLU")
@@ -414,12 +413,12 @@ class MXSparseMoeBlock(torch.nn.Module):
             logits = x.float() @ self.router_weight.float().T
         T.no_grad_here("MXSparseMoeBlock", x, logits)
         g = self.switch_mlp.gate_proj
-        T.require_cuda(x, logits, mask, g._packed[0])
+        ws = self.switch_mlp._refs(x, logits, mask)
         if x.ndim != 2 or x.shape[1] != g.input_dims or logits.shape != (x.shape[0], g.num_experts):
             raise ValueError(f"MXSparseMoeBlock: x {tuple(x.shape)}, logits {tuple(logits.shape)} for "
                              f"{g.num_experts} experts of width {g.input_dims}")
         m = router.mask_bytes(mask, logits)
-        xt, lib, ws, k = T.act_type(x), L.lib(), self.switch_mlp._refs(), self.top_k
+        xt, lib, k = T.act_type(x), L.lib(), self.top_k
         n = x.shape[0]
         with T.on_device(x):
             x = x.contiguous()
