@@ -263,3 +263,25 @@ def test_projections_on_another_device_are_refused():
             mx.MXSparseMoeBlock(glu, 2)(x, lg)
         getattr(glu, name).cuda()
     assert glu(x, ids, w).shape == (5, 64)
+
+
+# ------------------------------------------------------------------ streams
+@pytest.mark.parametrize("T", [2, 150])
+def test_blocks_on_two_streams_at_once(T):
+    """Pair by pair and sorted: each call has its own workspace."""
+    from vqlab_amd import mx
+    rng = np.random.default_rng(9)
+    glu, _ = _glu(rng, 8, 128, 64)
+    blk = mx.MXSparseMoeBlock(glu, 3)
+    xs = [mc.acts(rng, "fp16", T, 128)[0] for _ in range(2)]
+    lgs = [torch.randn(T, 8, device="cuda") for _ in range(2)]
+    ref = [blk(x, lg) for x, lg in zip(xs, lgs)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(6):
+        for s, x, lg in zip(streams, xs, lgs):
+            with torch.cuda.stream(s):
+                got.append(blk(x, lg))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, ref[i % 2]) for i, y in enumerate(got))
