@@ -44,6 +44,15 @@ struct RouteArgs {
     int32_t *part_c, *part_n;
 };
 
+// What a wave's lanes wrote to LDS before, its other lanes read after. The hardware
+// keeps a wave's LDS accesses in order; the fences, which cost no instruction, hold
+// the compiler to it.
+__device__ __forceinline__ void wave_lds_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <int LT, int NS>
 __device__ __forceinline__ void route_load(const void *l, int64_t base, int E, int lane, float (&v)[NS]) {
 #pragma unroll
@@ -311,6 +320,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_route16(const RouteArgs p) {
 #undef VQK_ROR
         const uint32_t thr = max(row_min(rank < p.k ? lm : 0xffffffffu), kKeyNegInf + 1);
         int run = 0;
+        wave_lds_sync();                      // the last token's candidates are read
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const bool c = live && key[i] >= thr;
@@ -323,7 +333,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_route16(const RouteArgs p) {
         uint64_t c0 = 0, c1 = 0;              // this lane's candidates, or with their ranks settled
         int r0 = 0, r1 = 0;
         if (__ballot(run > kRouteCands) == 0) {
-            __builtin_amdgcn_wave_barrier();
+            wave_lds_sync();
             if (sub < run) c0 = cands[wave][grp][sub];
             if (sub + 16 < run) c1 = cands[wave][grp][sub + 16];
             r0 = c1 > c0;
@@ -400,7 +410,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_route16(const RouteArgs p) {
                 }
             }
             if (w % 4 == 3) __syncthreads();
-            else __builtin_amdgcn_wave_barrier();
+            else wave_lds_sync();
         }
         zsum = wave_sum(zsum);
         for (int o = 16; o < 64; o <<= 1) nlive += __shfl_xor(nlive, o);
@@ -551,9 +561,9 @@ __global__ void __launch_bounds__(kRouteThreads) k_route_bwd(const RouteBwdArgs 
         const float sub = fz * lse - dot - (p.norm ? 0.f : s);
 #pragma unroll
         for (int i = 0; i < NS; ++i) row[lane * NS + i] = 0.f;
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_sync();
         if (id >= 0) row[id] = p.norm ? wdw - w * s : wdw;
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_sync();
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const float d = v[i] * (f[i] + sub) + row[lane * NS + i];
@@ -604,9 +614,9 @@ __global__ void __launch_bounds__(kRouteThreads) k_route_bwd16(const RouteBwdArg
         const float sub_ = fz * lse - dot - (p.norm ? 0.f : s);
 #pragma unroll
         for (int q = 0; q < NS / 4; ++q) *reinterpret_cast<float4 *>(row + 64 * q + 4 * sub) = float4{0.f, 0.f, 0.f, 0.f};
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_sync();
         if (id >= 0) row[id] = p.norm ? wdw - w * s : wdw;
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_sync();
 #pragma unroll
         for (int q = 0; q < NS / 4; ++q) {
             const int e = 64 * q + 4 * sub;
