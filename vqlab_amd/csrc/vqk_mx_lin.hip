@@ -27,7 +27,7 @@ struct DecTArgs {
 // 64 weight rows x one chunk through LDS: 16 bytes of codes in per thread,
 // 16-byte pieces of a transposed row out.
 __global__ void __launch_bounds__(256) k_mx_dec_t(const DecTArgs p) {
-    __shared__ uint16_t tile[128][72];
+    __shared__ __align__(16) uint16_t tile[128][72];     // read in 16-byte pieces
     const int64_t o0 = int64_t(blockIdx.x) * 64, c = blockIdx.y, k0 = c * kMxChunk;
     {
         const int unit = threadIdx.x & 63, o = (threadIdx.x >> 6) * 16 + (unit & 15), g = unit >> 4;
