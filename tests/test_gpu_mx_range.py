@@ -181,3 +181,66 @@ def test_4_bit_products_of_huge_weights(N):
         assert (y[:, 7] == float("inf")).all()
         ref, bar, y = np.delete(ref, 7, 1), np.delete(bar, 7, 1), y[:, [i for i in range(40) if i != 7]]
     mc.assert_within(y, ref, bar, "huge weights")
+
+
+# ------------------------------------------------ tiles, planes, many experts
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("exact", [True, False])
+@pytest.mark.parametrize("counts", [(5, 16, 17, 32), (10, 30, 40, 60), (20, 50, 90, 120), (1, 64, 65, 300)])
+def test_every_way_a_tile_holds_its_planes(dtype, exact, counts):
+    """Experts with 1..4 groups of 32 rows in tiles of 32, 64 and 128, x and SwiGLU rows in one, two
+    and three planes (exact: whether the weights are fp16 numbers)."""
+    rng = np.random.default_rng(sum(counts))
+    E, H, I = len(counts), 160, 288
+    glu, ws = _glu(rng, E, H, I)
+    if not exact:
+        from vqlab_amd import mx
+        mods = []
+        for i, (m, w) in enumerate(zip((glu.gate_proj, glu.up_proj, glu.down_proj), ws)):
+            scales = m.scales.cpu().numpy()
+            scales[:, ::5] = 90
+            codes = m.codes.cpu().numpy()
+            mods.append(mx.MXSwitchLinear(*_dev(codes, scales), m.input_dims))
+            assert not mods[-1]._w.f16_exact
+            ws = (*ws[:i], mc.values(codes, scales, m.input_dims), *ws[i + 1:])
+        glu = mx.MXSwitchGLU(*mods)
+    ids = rng.permutation(np.repeat(np.arange(E), counts))[:, None]
+    x, xv = mc.acts(rng, dtype, len(ids), H)
+    w = rng.random((len(ids), 1)).astype(np.float32)
+    ref, bar = mc.experts(xv, ids, w.astype(np.float64), *ws, H_ROUND[dtype])
+    bar = bar + mc.HALF_STEP[dtype] * (np.abs(ref) + bar) + (2.0 ** -25 if dtype == "fp16" else 0.0)
+    mc.assert_within(glu(x, *_dev(ids, w)), ref, bar, "experts")
+
+
+@pytest.mark.parametrize("T,k", [(3, 4), (1000, 4), (2100, 4)])
+def test_the_most_experts(T, k):
+    rng = np.random.default_rng(T)
+    E, H, I = 4096, 33, 16
+    glu, ws = _glu(rng, E, H, I)
+    x, xv = mc.acts(rng, "bf16", T, H)
+    ids = rng.integers(0, E, (T, k))
+    ids[0] = [0, E - 1, E, -1]
+    w = rng.random((T, k)).astype(np.float32)
+    ref, bar = mc.experts(xv, ids, w.astype(np.float64), *ws, H_ROUND["bf16"])
+    mc.assert_within(glu(x, *_dev(ids, w)), ref, bar + mc.HALF_STEP["bf16"] * (np.abs(ref) + bar), "experts")
+
+
+def test_a_block_of_the_most_experts_and_choices_it_routes():
+    from vqlab_amd import mx
+    rng = np.random.default_rng(11)
+    E, H, I = 2048, 32, 16
+    glu, ws = _glu(rng, E, H, I)
+    for T, k in ((2, 64), (90, 64)):
+        x, xv = mc.acts(rng, "bf16", T, H)
+        lg = rng.standard_normal((T, E)).astype(np.float32)
+        r = mc.route(lg, k)
+        ref, bar = mc.experts(xv, r["ids"], r["w"], *ws, H_ROUND["bf16"])
+        # weights, which sum to 1: exp of a difference rounded once (2 max |l| of it), sums of k terms;
+        # so many parts of the largest expert's output
+        g, u = (np.einsum("th,eih->tei", xv, m) for m in ws[:2])
+        most = np.abs(np.einsum("tei,ehi->teh", g / (1 + np.exp(-g)) * u, ws[2])).max(1)
+        bar = bar + (2 * np.abs(lg).max() + 8 + k) * 2.0 ** -24 * most
+        bar = bar + mc.HALF_STEP["bf16"] * (np.abs(ref) + bar)
+        mc.assert_within(mx.MXSparseMoeBlock(glu, k)(x, *_dev(lg)), ref, bar, "block")
+    with pytest.raises(NotImplementedError):
+        mx.MXSparseMoeBlock(glu, 65)(x, *_dev(lg))
