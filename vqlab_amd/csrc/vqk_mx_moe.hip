@@ -14,11 +14,11 @@ namespace vqk {
 static size_t al256(size_t v) { return (v + 255) & ~size_t(255); }
 
 // Whether a routing runs pair by pair: the sort, its tiles and the pass that adds
-// rows cost about 25 us more, and read weights at 5.3 TB/s instead of 3.6 and an
+// rows cost about 20 us more, and read weights at 5.3 TB/s instead of 3.6 and an
 // expert's once. us per block, pair by pair / sorted: 256 experts of 2048 x 512
-// (1.7 MB a pair), 64 pairs 32 / 49, 128 48 / 64; 512 of 4096 x 1024 (6.7 MB), 30
-// pairs 51 / 64, 60 107 / 98; 64 of 4096 x 1024, 24 pairs 51 / 58, 48 80 / 81; 8 of
-// 2048 x 1024, 16 pairs 21.9 / 22.2, 24 35 / 28.
+// (1.7 MB a pair), 64 pairs 36 / 52, 128 56 / 67; 512 of 4096 x 1024 (6.7 MB), 30
+// pairs 57 / 70, 60 117 / 112; 64 of 4096 x 1024, 24 pairs 55 / 62, 48 87 / 82; 8 of
+// 2048 x 1024, 16 pairs 21 / 42, 24 34 / 42.
 static bool mx_by_pair(int64_t N, int64_t E, int64_t pair_bytes) {
     return N <= 16 || (N <= 2 * E && N * pair_bytes <= INT64_C(256) << 20);
 }
@@ -27,9 +27,10 @@ constexpr int64_t kMxMaxExperts = 4096;
 
 // Rows per tile of a sorted routing of N pairs over E experts. Tiles cost the rows
 // they hold (in groups of 32), so a tile is as large as what an expert is likely to
-// have: 60 rows an expert take 111 + 81 us in tiles of 128, 124 + 104 in tiles of 64
-// (256 experts of 2048 x 512); 12 rows 158 us a block on the streaming kernel and 115
-// in tiles of 32 (64 of 4096 x 1024), 1.25 rows 508 and 447 (512 of 4096 x 1024).
+// have. us per block in tiles of 32 / 64 / 128: 256 experts of 2048 x 512, 12 rows an
+// expert 147 / 154 / 153, 20 162 / 156 / 158, 30 181 / 188 / 185, 40 227 / 215 / 207, 60
+// 278 / 267 / 261; 64 of 4096 x 1024, 12 136 / 139 / 136, 30 159 / 160 / 156, 60 234 / 248 /
+// 219; 512 of 4096 x 1024, 1.25 rows 497 / 545 / 549.
 static int mx_tile_rows(int64_t N, int64_t E) {
     const int64_t avg = N / E;
     return avg <= 20 ? 32 : (avg <= 40 ? 64 : 128);

@@ -8,8 +8,8 @@ NaN (include/vqk.h).
 
   mx_quantize(x) -> codes, scales         mx_dequantize(codes, scales, cols, dtype)
   MXLinear(codes, scales, in_features)    bias-free linear, like VQLinear
-  MXSwitchLinear, MXSwitchGLU             routed experts, like VQSwitchLinear / VQSwitchGLU
-  MXSparseMoeBlock                        routing + experts, like VQSparseMoeBlock
+  MXSwitchLinear                          routed linears, called like VQSwitchLinear
+  MXSwitchGLU, MXSparseMoeBlock           routed experts with their weighted sum, and routing in front
 """
 from __future__ import annotations
 
