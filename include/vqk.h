@@ -393,8 +393,9 @@ int vqk_skipzero_row_table_host(const uint8_t *rowmask, int64_t E,
  * codes (element 2i in the low half of byte i; zeros past C) and a scale byte
  * s: value = e2m1(code) * 2^(s - 127), with e2m1 in {0, .5, 1, 1.5, 2, 3, 4, 6}
  * and the sign in a code's top bit. s = 255: the whole block is NaN. Values of
- * 2^128 and more (s = 253 and 254) are infinite here, as in bf16 and fp32, but for
- * 4-bit by 4-bit products, which take them as they are.
+ * 2^128 and more (s = 253 and 254) are infinite here, as in bf16 and fp32, and make
+ * the outputs that they enter infinite or NaN; only 4-bit by 4-bit products take
+ * them as they are.
  *
  * Weights are kept in operand order, as vqk_mx_pack lays them out once from rows
  * of codes [E, OUT, NB * 16] and scales [E, OUT, NB] (both as vqk_mx_quantize

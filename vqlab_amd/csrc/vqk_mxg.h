@@ -132,6 +132,7 @@ __global__ void __launch_bounds__(64 * kMxgWaves, 2) k_mx_gemm(const MxgArgs ga)
         Weights wb[ST];
         auto walk = [&](auto span) {
             using Sp = decltype(span);
+            static_assert(Sp::rows * Sp::planes <= ROWS && P % Sp::planes == 0, "whole planes in a stage");
             // the x copies of this lane: 16 bytes of one row each
             const uint16_t *src[Sp::copies];
             int piece[Sp::copies], xrow[Sp::copies];
