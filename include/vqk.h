@@ -481,6 +481,89 @@ int vqk_mx_moe(const vqk_mx_weights *gate, const vqk_mx_weights *up, const vqk_m
                int64_t ld, const uint8_t *mask, int32_t top_k, int32_t norm_topk, void *y,
                int32_t y_type, void *workspace, size_t ws_bytes, void *stream);
 
+/* ---- 8-bit weights (e4m3) with a scale for each block of 128 x 128 -------------
+ * No counterpart in the reference: the format that block-scaled 8-bit checkpoints
+ * hold. A weight [OUT, IN] has codes of 8 bits (e4m3, finite: up to 448, 0x7f and
+ * 0xff NaN) and an fp32 scale for each 128 x 128 of it, scales [ceil(OUT / 128),
+ * ceil(IN / 128)]; a row of activations [N, C] has one for each 128 of its columns.
+ * A value is code * scale.
+ *
+ * vqk_f8_quantize: rows x (ldx elements apart; fp16, bf16 or fp32) -> codes
+ * [rows, cols] and scales, that of row n and block b at n * scale_row + b *
+ * scale_block. A block's scale is its largest magnitude / 448, at least 2^-126; a
+ * code is value * (1 / scale) to nearest, ties to even (scale, reciprocal and product
+ * are fp32 numbers). A block with an infinity or NaN has the scale NaN, codes 0.
+ * vqk_f8_quantize_weight: the same for blocks of 128 x 128. vqk_f8_dequantize is the
+ * way back; a scale is for rows_per_scale rows, 1 or 128.
+ *
+ * Products take weights in operand order, which vqk_f8_pack lays out once
+ * (vqk_f8_pack_bytes bytes, 16-byte aligned) and vqk_f8_unpack takes back to rows:
+ *   codes   uint8 [ceil(OUT / 16), ceil(IN / 128), 2, 64, 16]: unit i of half h is
+ *           columns 128 c + 32 (i / 16) + 16 h .. + 15 of row 16 rt + i % 16; codes 0
+ *           past the weight's end
+ *   scales  as above, contiguous
+ * A weight holds less than 4 GB. */
+typedef struct vqk_f8_weights {
+    const uint8_t *codes;
+    const float   *scales;
+    int64_t        OUT;
+    int64_t        IN;
+} vqk_f8_weights;
+int vqk_f8_quantize(const void *x, int32_t x_type, int64_t rows, int64_t cols, int64_t ldx,
+                    uint8_t *codes, float *scales, int64_t scale_row, int64_t scale_block,
+                    void *stream);
+int vqk_f8_quantize_weight(const void *w, int32_t w_type, int64_t OUT, int64_t IN, int64_t ldw,
+                           uint8_t *codes, float *scales, void *stream);
+int vqk_f8_dequantize(const uint8_t *codes, int64_t ldc, const float *scales, int64_t scale_row,
+                      int64_t scale_block, int32_t rows_per_scale, int64_t rows, int64_t cols,
+                      void *out, int32_t out_type, void *stream);
+int vqk_f8_pack_bytes(int64_t OUT, int64_t IN, size_t *bytes);
+int vqk_f8_pack(const uint8_t *codes, int64_t OUT, int64_t IN, uint8_t *packed, void *stream);
+int vqk_f8_unpack(const uint8_t *packed, int64_t OUT, int64_t IN, uint8_t *codes, void *stream);
+
+/* y [N, OUT] = x [N, IN] . W^T: sums in fp32, one rounding into y_type (VQK_VIA_F16
+ * as elsewhere). act: VQK_F8_ACT_NONE takes x as it is (every code and every finite x
+ * enters the matrix cores exactly; with bf16 and fp32 x bits under 2^-110 may be
+ * dropped); VQK_F8_ACT_F8 quantises x's rows as vqk_f8_quantize does. Products of
+ * 8-bit x into a 16-bit y run on the 8-bit matrix instructions, which keep 14 bits of
+ * the largest of eight neighbouring products and what lines up with it of the others;
+ * into an fp32 y every product enters exactly.
+ * vqk_f8_linear_rows takes rows that are in 8 bits already (codes ldc apart, scales
+ * as above). Workspaces are 256-byte aligned and hold nothing between calls. */
+#define VQK_F8_ACT_NONE 0
+#define VQK_F8_ACT_F8   1
+int vqk_f8_linear_workspace(const vqk_f8_weights *w, int32_t x_type, int64_t N, int32_t act,
+                            int32_t y_type, size_t *bytes);
+int vqk_f8_linear(const vqk_f8_weights *w, const void *x, int32_t x_type, int64_t N, int32_t act,
+                  void *y, int32_t y_type, void *workspace, size_t ws_bytes, void *stream);
+int vqk_f8_linear_rows_workspace(const vqk_f8_weights *w, int64_t N, int32_t y_type, size_t *bytes);
+int vqk_f8_linear_rows(const vqk_f8_weights *w, const uint8_t *codes, int64_t ldc,
+                       const float *scales, int64_t scale_row, int64_t scale_block, int64_t N,
+                       void *y, int32_t y_type, void *workspace, size_t ws_bytes, void *stream);
+/* The gradient of x of that product (act NONE): dx [N, IN] = dy [N, OUT] . W. */
+int vqk_f8_linear_dx_workspace(const vqk_f8_weights *w, int32_t dy_type, int64_t N, size_t *bytes);
+int vqk_f8_linear_dx(const vqk_f8_weights *w, const void *dy, int32_t dy_type, int64_t N, void *dx,
+                     int32_t dx_type, void *workspace, size_t ws_bytes, void *stream);
+
+/* RMS norm of rows [N, C] (C at most 16384), with the residual's addition in front:
+ *   h = x + residual, rounded once to their type (without a residual h is x),
+ *   y = h * r * weight, r = 1 / sqrt(mean h^2 + eps)
+ * x and residual: rows ldx, ldr elements apart; h and y contiguous. Either y (the
+ * type of x), or codes [N, C] and scales as vqk_f8_quantize makes them of the fp32 y.
+ * h: with a residual only. r: fp32 [N] for the backward pass, or NULL.
+ * vqk_rms_norm_backward: dx (also the residual's gradient) and dw [C] (w_type) from
+ * dy and dh (the gradient of h, NULL for none), both contiguous; h as the norm took
+ * it, rows ldh apart. The workspace is 16-byte aligned. */
+int vqk_rms_norm(const void *x, int32_t type, int64_t N, int64_t C, int64_t ldx,
+                 const void *residual, int64_t ldr, const void *weight, int32_t w_type, double eps,
+                 void *h, void *y, float *r, uint8_t *codes, float *scales, int64_t scale_row,
+                 int64_t scale_block, void *stream);
+int vqk_rms_norm_backward_workspace(int64_t N, int64_t C, size_t *bytes);
+int vqk_rms_norm_backward(const void *h, int32_t type, int64_t N, int64_t C, int64_t ldh,
+                          const void *weight, int32_t w_type, const float *r, const void *dy,
+                          const void *dh, void *dx, void *dw, void *workspace, size_t ws_bytes,
+                          void *stream);
+
 /* ---- router -------------------------------------------------------------------
  * The layer calls' routing (softmax, top_k, renormalised when norm_topk != 0)
  * as a call of its own, with what training it needs. logits [T, E] rows ld

@@ -21,6 +21,7 @@ VQK_MOE_HEADER_BYTES = 49152             # include/vqk.h: zero before a layer wo
 VQK_VIA_F16 = 0x100                      # output type flag: round through fp16 first
 VQK_X_KEEP = 0x200                       # x type flag (d=8 GEMV): x enters the products unrounded
 VQK_MX_ACT_NONE, VQK_MX_ACT_MXFP4 = range(2)   # include/vqk.h: x of an MXFP4 linear as it is / in 4 bits
+VQK_F8_ACT_NONE, VQK_F8_ACT_F8 = range(2)      # include/vqk.h: x of an 8-bit linear as it is / in 8 bits
 
 c_i32, c_i64, c_p, c_sz = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t
 
@@ -51,7 +52,13 @@ class VQKMXWeights(ctypes.Structure):
                 ("f16_exact", c_i32)]
 
 
+class VQKF8Weights(ctypes.Structure):
+    _fields_ = [("codes", c_p), ("scales", c_p), ("OUT", c_i64), ("IN", c_i64)]
+
+
 _MXW = ctypes.POINTER(VQKMXWeights)
+_F8W = ctypes.POINTER(VQKF8Weights)
+c_f64 = ctypes.c_double
 
 # name -> (restype, argtypes), one entry per function of include/vqk.h
 SIGNATURES = {
@@ -122,6 +129,23 @@ SIGNATURES = {
     "vqk_mx_moe_workspace": (c_i32, [_MXW, _MXW, _MXW, c_i32, c_i64, c_i32, ctypes.POINTER(c_sz)]),
     "vqk_mx_moe": (c_i32, [_MXW, _MXW, _MXW, c_p, c_i32, c_i64, c_p, c_i32, c_i64, c_p, c_i32, c_i32,
                            c_p, c_i32, c_p, c_sz, c_p]),
+    "vqk_f8_quantize": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, c_p, c_p, c_i64, c_i64, c_p]),
+    "vqk_f8_quantize_weight": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, c_p, c_p, c_p]),
+    "vqk_f8_dequantize": (c_i32, [c_p, c_i64, c_p, c_i64, c_i64, c_i32, c_i64, c_i64, c_p, c_i32, c_p]),
+    "vqk_f8_pack_bytes": (c_i32, [c_i64, c_i64, ctypes.POINTER(c_sz)]),
+    "vqk_f8_pack": (c_i32, [c_p, c_i64, c_i64, c_p, c_p]),
+    "vqk_f8_unpack": (c_i32, [c_p, c_i64, c_i64, c_p, c_p]),
+    "vqk_f8_linear_workspace": (c_i32, [_F8W, c_i32, c_i64, c_i32, c_i32, ctypes.POINTER(c_sz)]),
+    "vqk_f8_linear": (c_i32, [_F8W, c_p, c_i32, c_i64, c_i32, c_p, c_i32, c_p, c_sz, c_p]),
+    "vqk_f8_linear_rows_workspace": (c_i32, [_F8W, c_i64, c_i32, ctypes.POINTER(c_sz)]),
+    "vqk_f8_linear_rows": (c_i32, [_F8W, c_p, c_i64, c_p, c_i64, c_i64, c_i64, c_p, c_i32, c_p, c_sz, c_p]),
+    "vqk_f8_linear_dx_workspace": (c_i32, [_F8W, c_i32, c_i64, ctypes.POINTER(c_sz)]),
+    "vqk_f8_linear_dx": (c_i32, [_F8W, c_p, c_i32, c_i64, c_p, c_i32, c_p, c_sz, c_p]),
+    "vqk_rms_norm": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, c_p, c_i64, c_p, c_i32, c_f64, c_p, c_p, c_p,
+                             c_p, c_p, c_i64, c_i64, c_p]),
+    "vqk_rms_norm_backward_workspace": (c_i32, [c_i64, c_i64, ctypes.POINTER(c_sz)]),
+    "vqk_rms_norm_backward": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, c_p, c_i32, c_p, c_p, c_p, c_p, c_p,
+                                      c_p, c_sz, c_p]),
     "vqk_route_workspace": (c_i32, [c_i64, c_i64, ctypes.POINTER(c_sz)]),
     "vqk_route": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, c_p, c_i32, c_i32, c_p, c_p, c_p, c_p,
                           c_p, c_p, c_sz, c_p]),

@@ -1,0 +1,319 @@
+// RMS norm of rows with the residual's addition in front, its output in 8 bits
+// with scales or as it is, and its backward pass.
+//
+//     h = round(x + residual)          (the type of x; what the next layer adds to)
+//     r = 1 / sqrt(sum_c h_c^2 / C + eps),   y = h r w
+//     8 bits: s = max(amax / 448, 2^-126) over 128 of y, code = e4m3(y * (1 / s))
+// and with the gradients dy and dh of both outputs, xhat = h r, g = dy w:
+//     dx = dresidual = r (g - xhat sum_c g xhat / C) + dh,   dw = sum over rows of dy xhat
+//
+// Bound by memory: each input is read once and each output written once. A
+// workgroup of W waves takes a row and holds it in registers, 8 neighbouring
+// columns a piece: few rows are spread over as many waves as they have pieces
+// (latency), many rows take up to four pieces a lane (fewer steps across waves for
+// each row). A block of 128 is 16 lanes of one piece, so its largest magnitude
+// takes four DPP steps. Squares are summed in fp64 (2^127 squared is no fp32
+// number), everything else is fp32. dw: a workgroup adds up its rows in
+// registers, the workgroups' sums meet in a fixed order.
+#include "vqk_f8.h"
+
+namespace vqk {
+
+constexpr int kNormMaxC = 16384;              // 8 waves of 4 pieces
+
+struct NormArgs {
+    const void *x, *res, *w;
+    int64_t N, ldx, ldr;
+    int32_t C, w_type;
+    double eps;
+    void *h, *y;                              // h: NULL without a residual; y: NULL for 8 bits
+    float *r;                                 // [N] or NULL
+    uint8_t *codes;                           // [N][C]
+    float *scales;
+    int64_t sn, sk;
+};
+
+// Sum over the workgroup's W waves, in every thread; `part` is used by one call.
+template <int W>
+__device__ __forceinline__ double norm_sum(double v, double (&part)[W]) {
+    for (int o = 1; o < kWave; o <<= 1) v += __shfl_xor(v, o);
+    if constexpr (W == 1) return v;
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0.;
+#pragma unroll
+    for (int i = 0; i < W; ++i) s += part[i];
+    return s;
+}
+
+__device__ __forceinline__ void norm_store8(void *y, int32_t type, int64_t at, const float (&v)[8], int n, bool vec) {
+    const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
+    if (vec && n >= 8 && type != VQK_F32) {
+        u32x4 o;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const uint16_t lo = type == VQK_BF16 ? f32_to_bf16(v[2 * u]) : f32_to_h(v[2 * u]);
+            const uint16_t hi = type == VQK_BF16 ? f32_to_bf16(v[2 * u + 1]) : f32_to_h(v[2 * u + 1]);
+            o[u] = lo | (uint32_t(hi) << 16);
+        }
+        *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(y) + at) = o;
+        return;
+    }
+    if (n > 0) mx_store4(y, type, at, a, min(n, 4), vec);
+    if (n > 4) mx_store4(y, type, at + 4, b, min(n - 4, 4), vec);
+}
+
+template <int T>
+__device__ __forceinline__ float round_to(float v) {
+    if constexpr (T == VQK_F32) return v;
+    return T == VQK_BF16 ? bf16_to_f32(f32_to_bf16(v)) : h_to_f32(f32_to_h(v));
+}
+
+template <int XT, int W, int P, bool Q>
+__global__ void __launch_bounds__(64 * W) k_rms(const NormArgs p, bool vec, bool vecw) {
+    __shared__ double part[W];
+    const int64_t row = blockIdx.x;
+    float h[P][8], wt[P][8];
+    double sum = 0.;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const int k0 = (i * 64 * W + int(threadIdx.x)) * 8;
+        mx_load8(p.x, XT, row * p.ldx, k0, p.C, vec, h[i]);
+        mx_load8(p.w, p.w_type, 0, k0, p.C, vecw, wt[i]);
+    }
+    if (p.res) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int k0 = (i * 64 * W + int(threadIdx.x)) * 8;
+            float a[8];
+            mx_load8(p.res, XT, row * p.ldr, k0, p.C, vec, a);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) h[i][u] = round_to<XT>(h[i][u] + a[u]);
+            norm_store8(p.h, XT, row * p.C + k0, h[i], p.C - k0, vec);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) sum = __builtin_fma(double(h[i][u]), double(h[i][u]), sum);
+    sum = norm_sum<W>(sum, part);
+    const float r = float(1. / sqrt(sum / double(p.C) + p.eps));
+    if (p.r && threadIdx.x == 0) p.r[row] = r;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const int k0 = (i * 64 * W + int(threadIdx.x)) * 8;
+        float y[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) y[u] = h[i][u] * r * wt[i][u];
+        if constexpr (Q) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                y[u] = k0 + u < p.C ? y[u] : 0.f;              // 0 * r is NaN where r is infinite
+                m = max(m, __float_as_uint(y[u]) & 0x7fffffffu);
+            }
+            const float s = f8_scale(row16_max(m));
+            const u32x2 c = f8_encode8(y, 1.f / s, s == s);
+            if (k0 >= p.C) continue;
+            uint8_t *dst = p.codes + row * p.C + k0;
+            if (vec && k0 + 8 <= p.C) {
+                *reinterpret_cast<u32x2 *>(dst) = c;
+            } else {
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (k0 + u < p.C) dst[u] = uint8_t(c[u / 4] >> (8 * (u % 4)));
+            }
+            if ((threadIdx.x & 15) == 0) p.scales[row * p.sn + (k0 >> 7) * p.sk] = s;
+        } else {
+            norm_store8(p.y, XT, row * p.C + k0, y, p.C - k0, vec);
+        }
+    }
+}
+
+struct NormBwdArgs {
+    const void *h, *w, *dy, *dh;              // dh: NULL for none
+    int64_t N, ldh;
+    int32_t C, w_type;
+    const float *r;
+    void *dx;
+    float *part;                              // [gridDim.x][C]
+};
+
+template <int XT, int W, int P>
+__global__ void __launch_bounds__(64 * W) k_rms_bwd(const NormBwdArgs p, bool vec, bool vecw) {
+    __shared__ double part[2][W];
+    float wt[P][8], dw[P][8] = {};
+#pragma unroll
+    for (int i = 0; i < P; ++i) mx_load8(p.w, p.w_type, 0, (i * 64 * W + int(threadIdx.x)) * 8, p.C, vecw, wt[i]);
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < p.N; row += gridDim.x, turn ^= 1) {
+        float xh[P][8], g[P][8], add[P][8];
+        const float r = p.r[row];
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int k0 = (i * 64 * W + int(threadIdx.x)) * 8;
+            mx_load8(p.h, XT, row * p.ldh, k0, p.C, vec, xh[i]);
+            mx_load8(p.dy, XT, row * p.C, k0, p.C, vec, g[i]);
+            if (p.dh) mx_load8(p.dh, XT, row * p.C, k0, p.C, vec, add[i]);
+        }
+        float dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                xh[i][u] *= r;
+                dw[i][u] = __builtin_fmaf(g[i][u], xh[i][u], dw[i][u]);
+                g[i][u] *= wt[i][u];
+                dot = __builtin_fmaf(g[i][u], xh[i][u], dot);
+            }
+        const float mean = float(norm_sum<W>(double(dot), part[turn]) / double(p.C));
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int k0 = (i * 64 * W + int(threadIdx.x)) * 8;
+            float d[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                d[u] = r * (g[i][u] - xh[i][u] * mean);
+                if (p.dh) d[u] += add[i][u];
+            }
+            norm_store8(p.dx, XT, row * p.C + k0, d, p.C - k0, vec);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const int k0 = (i * 64 * W + int(threadIdx.x)) * 8;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (k0 + u < p.C) p.part[int64_t(blockIdx.x) * p.C + k0 + u] = dw[i][u];
+    }
+}
+
+// dw from the workgroups' sums: 32 columns by 32 slices of the sums a workgroup.
+__global__ void __launch_bounds__(1024) k_rms_dw(const float *part, int rows, int C, void *dw, int32_t type) {
+    __shared__ double s[32][33];
+    const int c = int(blockIdx.x) * 32 + (threadIdx.x & 31), t = threadIdx.x >> 5;
+    double v = 0.;
+    if (c < C)
+        for (int i = t; i < rows; i += 32) v += double(part[int64_t(i) * C + c]);
+    s[t][threadIdx.x & 31] = v;
+    __syncthreads();
+    for (int o = 16; o >= 1; o >>= 1) {
+        if (t < o) s[t][threadIdx.x & 31] += s[t + o][threadIdx.x & 31];
+        __syncthreads();
+    }
+    if (t == 0 && c < C) store_act(dw, type, c, float(s[0][threadIdx.x]));
+}
+
+// Waves to a row and pieces to a lane.
+struct NormPlan { int w, p; };
+// Rows up to which a row is spread over one piece a lane.
+constexpr int64_t kNormSpreadRows = 1024;
+static NormPlan norm_plan(int64_t N, int64_t C) {
+    const int64_t waves = (C + 511) / 512;
+    const int p = N <= kNormSpreadRows && waves <= 16 ? 1 : 4;
+    int w = 1;
+    while (w * p < waves) w *= 2;
+    return NormPlan{w, p};
+}
+// Workgroups of the backward pass: each leaves a row of sums.
+static int64_t norm_bwd_wgs(int64_t N, int64_t C) {
+    const NormPlan pl = norm_plan(N, C);
+    const int64_t most = 2048 / pl.w < 256 ? 256 : 2048 / pl.w;
+    return N < most ? N : most;
+}
+
+template <int XT, bool Q>
+static int go_norm(const NormArgs &a, NormPlan pl, bool vec, bool vecw, hipStream_t st) {
+    const dim3 grid{unsigned(a.N)};
+#define VQK_GO(W, P) if (pl.w == W && pl.p == P) hipLaunchKernelGGL((k_rms<XT, W, P, Q>), grid, dim3(64 * W), 0, st, a, vec, vecw)
+    VQK_GO(1, 1); VQK_GO(2, 1); VQK_GO(4, 1); VQK_GO(8, 1); VQK_GO(16, 1);
+    VQK_GO(1, 4); VQK_GO(2, 4); VQK_GO(4, 4); VQK_GO(8, 4);
+#undef VQK_GO
+    return hip_status(hipGetLastError(), "norm launch");
+}
+template <int XT>
+static int go_norm_bwd(const NormBwdArgs &a, NormPlan pl, unsigned wgs, bool vec, bool vecw, hipStream_t st) {
+#define VQK_GO(W, P) if (pl.w == W && pl.p == P) hipLaunchKernelGGL((k_rms_bwd<XT, W, P>), dim3(wgs), dim3(64 * W), 0, st, a, vec, vecw)
+    VQK_GO(1, 1); VQK_GO(2, 1); VQK_GO(4, 1); VQK_GO(8, 1); VQK_GO(16, 1);
+    VQK_GO(1, 4); VQK_GO(2, 4); VQK_GO(4, 4); VQK_GO(8, 4);
+#undef VQK_GO
+    return hip_status(hipGetLastError(), "norm gradient launch");
+}
+
+static int check_norm(int32_t type, int32_t w_type, int64_t N, int64_t C, double eps, const char *what) {
+    if (!act_size(type) || !act_size(w_type)) return set_error(VQK_EINVAL, "%s: types %d, %d", what, type, w_type);
+    if (N < 0 || N > INT32_MAX || C < 1) return set_error(VQK_EINVAL, "%s: N=%lld C=%lld", what, (long long)N, (long long)C);
+    if (C > kNormMaxC) return set_error(VQK_ENOTIMPL, "%s: rows of %lld > %d", what, (long long)C, kNormMaxC);
+    if (!(eps >= 0.)) return set_error(VQK_EINVAL, "%s: eps=%g", what, eps);
+    return VQK_OK;
+}
+
+static bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace vqk
+
+using namespace vqk;
+
+extern "C" int vqk_rms_norm(const void *x, int32_t type, int64_t N, int64_t C, int64_t ldx, const void *residual,
+                            int64_t ldr, const void *weight, int32_t w_type, double eps, void *h, void *y, float *r,
+                            uint8_t *codes, float *scales, int64_t scale_row, int64_t scale_block, void *stream) {
+    int rc = check_norm(type, w_type, N, C, eps, "rms norm");
+    if (rc) return rc;
+    if (ldx < C || (residual && ldr < C)) return set_error(VQK_EINVAL, "rms norm: rows of %lld apart by %lld, %lld", (long long)C, (long long)ldx, (long long)ldr);
+    if ((y != nullptr) == (codes != nullptr) && N > 0) return set_error(VQK_EINVAL, "rms norm: one of y and codes");
+    if (N == 0) return VQK_OK;
+    if (!x || !weight || (residual && !h) || (codes && !scales)) return set_error(VQK_EINVAL, "rms norm: NULL pointer");
+    if (scale_row < 0 || scale_block < 0) return set_error(VQK_EINVAL, "rms norm: negative stride of scales");
+    const int esz = act_size(type);
+    const NormArgs a{x, residual, weight, N, ldx, ldr, int32_t(C), w_type, eps, h, y, r, codes, scales, scale_row, scale_block};
+    const bool vec = C % 8 == 0 && al16(x) && (ldx * esz) % 16 == 0 &&
+                     (!residual || (al16(residual) && (ldr * esz) % 16 == 0 && al16(h))) &&
+                     (y ? al16(y) : (reinterpret_cast<uintptr_t>(codes) & 7) == 0);
+    const NormPlan pl = norm_plan(N, C);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    switch (type) {
+        case VQK_F16: return y ? go_norm<VQK_F16, false>(a, pl, vec, al16(weight), st) : go_norm<VQK_F16, true>(a, pl, vec, al16(weight), st);
+        case VQK_BF16: return y ? go_norm<VQK_BF16, false>(a, pl, vec, al16(weight), st) : go_norm<VQK_BF16, true>(a, pl, vec, al16(weight), st);
+        default: return y ? go_norm<VQK_F32, false>(a, pl, vec, al16(weight), st) : go_norm<VQK_F32, true>(a, pl, vec, al16(weight), st);
+    }
+}
+
+extern "C" int vqk_rms_norm_backward_workspace(int64_t N, int64_t C, size_t *bytes) {
+    const int rc = check_norm(VQK_F32, VQK_F32, N, C, 0., "rms norm backward");
+    if (rc) return rc;
+    if (!bytes) return set_error(VQK_EINVAL, "rms norm backward: NULL bytes");
+    *bytes = size_t(norm_bwd_wgs(N, C)) * size_t(C) * 4;
+    return VQK_OK;
+}
+
+extern "C" int vqk_rms_norm_backward(const void *h, int32_t type, int64_t N, int64_t C, int64_t ldh, const void *weight,
+                                     int32_t w_type, const float *r, const void *dy, const void *dh, void *dx, void *dw,
+                                     void *workspace, size_t ws_bytes, void *stream) {
+    const int rc = check_norm(type, w_type, N, C, 0., "rms norm backward");
+    if (rc) return rc;
+    if (ldh < C) return set_error(VQK_EINVAL, "rms norm backward: rows of %lld apart by %lld", (long long)C, (long long)ldh);
+    if (!dw || (N > 0 && (!h || !weight || !r || !dy || !dx))) return set_error(VQK_EINVAL, "rms norm backward: NULL pointer");
+    const int64_t wgs = norm_bwd_wgs(N, C);
+    const size_t need = size_t(wgs) * size_t(C) * 4;
+    if (need && (!workspace || ws_bytes < need))
+        return set_error(VQK_ENOSPACE, "rms norm backward: workspace %zu < %zu", ws_bytes, need);
+    if (reinterpret_cast<uintptr_t>(workspace) & 15)
+        return set_error(VQK_EINVAL, "rms norm backward: workspace must be 16-byte aligned");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    float *part = static_cast<float *>(workspace);
+    if (N > 0) {
+        const int esz = act_size(type);
+        const NormBwdArgs a{h, weight, dy, dh, N, ldh, int32_t(C), w_type, r, dx, part};
+        const bool vec = C % 8 == 0 && al16(h) && (ldh * esz) % 16 == 0 && al16(dy) && (!dh || al16(dh)) && al16(dx);
+        const NormPlan pl = norm_plan(N, C);
+        int e;
+        switch (type) {
+            case VQK_F16: e = go_norm_bwd<VQK_F16>(a, pl, unsigned(wgs), vec, al16(weight), st); break;
+            case VQK_BF16: e = go_norm_bwd<VQK_BF16>(a, pl, unsigned(wgs), vec, al16(weight), st); break;
+            default: e = go_norm_bwd<VQK_F32>(a, pl, unsigned(wgs), vec, al16(weight), st);
+        }
+        if (e) return e;
+    }
+    hipLaunchKernelGGL(k_rms_dw, dim3(unsigned((C + 31) / 32)), dim3(1024), 0, st, part, int(wgs), int(C), dw, w_type);
+    return hip_status(hipGetLastError(), "norm weight gradient launch");
+}

@@ -1,0 +1,85 @@
+// Launch of the few-row products of 8-bit weights (kernel in vqk_f8s.h).
+#include "vqk_f8s.h"
+
+namespace vqk {
+
+// Registers of a block: two buffers of weights and their scales, and x.
+constexpr int f8s_regs(int op, int nt, int p) { return 18 + nt * (op == kOpF8 ? 9 : 16 * p + 1); }
+// Blocks a wave that the registers hold.
+constexpr int f8s_cap(int op, int nt, int p) { return 200 / f8s_regs(op, nt, p); }
+
+struct F8sPlan { int kw, ncw; };              // waves along k and blocks a wave; kw = 0: x does not fit
+static F8sPlan f8s_plan(int64_t NC, int cap, int64_t row_tiles) {
+    // about four blocks a wave keep enough weights in flight, and fewer waves along k save the sums;
+    // a small product takes more of them, until each CU has a workgroup
+    int kw = 1;
+    while (kw < kF8sWaves && ((NC + kw - 1) / kw > (cap < 4 ? cap : 4) ||
+                              (NC > kw && row_tiles * kw < 256 * kF8sWaves))) kw *= 2;
+    const int64_t ncw = (NC + kw - 1) / kw;
+    return ncw <= cap ? F8sPlan{kw, int(ncw)} : F8sPlan{0, 0};
+}
+
+static int call_op(const F8Call &c) { return c.a8 ? kOpF8 : c.x.op; }
+static int call_p(const F8Call &c) { return c.a8 ? 1 : c.x.P; }
+static int call_nt(const F8Call &c) { return c.N <= 16 ? 1 : 2; }
+static F8sPlan call_plan(const F8Call &c) {
+    const int nt = call_nt(c);
+    return f8s_plan(c.g.NC, f8s_cap(call_op(c), nt, call_p(c)), (c.N + 16 * nt - 1) / (16 * nt) * c.g.RT);
+}
+
+bool f8_rows_ok(const F8Call &c) {
+    if (c.N > 32 || (call_nt(c) == 2 && call_p(c) != 1)) return false;
+    return call_plan(c).kw > 0;
+}
+
+template <int OP, int NT, int P, int NCW>
+static int go(F8sArgs a, int64_t tiles, int kw, hipStream_t st) {
+    const int RW = kF8sWaves / kw;
+    a.kw = kw;
+    a.total_steps = int32_t((a.OUT + 16 * RW - 1) / (16 * RW));
+    // row steps per workgroup: one round of workgroups, two to a CU where the registers let them
+    const int64_t room = 40 + NCW * f8s_regs(OP, NT, P) <= 128 ? 512 : 256;
+    const int64_t want = (room + tiles - 1) / tiles;
+    const int64_t steps = (a.total_steps + want - 1) / want;
+    a.steps = int32_t(steps);
+    a.nob = int32_t((a.total_steps + steps - 1) / steps);
+    const int64_t grid = int64_t(a.nob) * tiles;
+    const size_t sums = kw > 1 ? size_t(2) * kF8sWaves * NT * 1024 : 0;
+    const size_t xl = a.stage ? size_t(kF8sWaves) * NCW * 16 * (OP == kOpF8 ? 128 : 256) : 0;
+    return launch_with_lds<k_f8_rows<OP, NT, P, NCW>>(dim3(unsigned(grid)), dim3(64 * kF8sWaves),
+                                                     sums > xl ? sums : xl, st, a);
+}
+
+template <int OP, int NT, int P, int NCW = 1>
+static int go_ncw(const F8sArgs &a, int64_t tiles, F8sPlan pl, hipStream_t st) {
+    if (pl.ncw == NCW) return go<OP, NT, P, NCW>(a, tiles, pl.kw, st);
+    if constexpr (NCW < f8s_cap(OP, NT, P)) return go_ncw<OP, NT, P, NCW + 1>(a, tiles, pl, st);
+    return set_error(VQK_EINVAL, "8-bit product: no instance of %d blocks", pl.ncw);
+}
+
+int f8_rows(const F8Call &c, hipStream_t st) {
+    F8sArgs a{};
+    a.codes = c.codes; a.scales = c.scales; a.swo = c.swo; a.swk = c.swk;
+    a.OUT = c.g.OUT; a.IN = c.g.IN; a.N = c.N;
+    a.RT = int32_t(c.g.RT); a.NC = int32_t(c.g.NC);
+    a.sx = c.x8.scales; a.sn = c.x8.sn; a.sk = c.x8.sk;
+    if (c.a8) {
+        a.x = c.x8.codes; a.xld = c.x8.ld;
+    } else {
+        a.x = reinterpret_cast<const uint8_t *>(c.x.x); a.xld = c.x.ld * 2; a.xplane = c.x.plane * 2;
+    }
+    a.y = c.y; a.y_type = c.y_type;
+    a.stage = c.N > 2;
+    const int nt = call_nt(c), P = call_p(c);
+    const F8sPlan pl = call_plan(c);
+    const int64_t tiles = (c.N + 16 * nt - 1) / (16 * nt);
+    switch (call_op(c)) {
+        case kOpF8: return nt == 2 ? go_ncw<kOpF8, 2, 1>(a, tiles, pl, st) : go_ncw<kOpF8, 1, 1>(a, tiles, pl, st);
+        case kOpF16: return nt == 2 ? go_ncw<kOpF16, 2, 1>(a, tiles, pl, st) : go_ncw<kOpF16, 1, 1>(a, tiles, pl, st);
+        default: break;
+    }
+    if (nt == 2) return go_ncw<kOpBF16, 2, 1>(a, tiles, pl, st);
+    return P == 1 ? go_ncw<kOpBF16, 1, 1>(a, tiles, pl, st) : go_ncw<kOpBF16, 1, 3>(a, tiles, pl, st);
+}
+
+}  // namespace vqk
