@@ -596,6 +596,38 @@ int vqk_route_backward(const void *logits, int32_t l_type, int64_t T, int64_t E,
                        const float *dw, const float *dbalance, const float *dz, void *dlogits,
                        void *stream);
 
+/* The same with other scores, a bias and groups of experts:
+ *   s = softmax(logits) or sigmoid(logits), c = s + bias (fp32 [E] or NULL: the choice
+ *   alone goes by it, and no gradient reaches it)
+ *   the experts are `groups` (at most 64) equal runs; a group's score is the sum of the
+ *   group_top (1 or 2) largest c of those of its experts that can be chosen (of what
+ *   there is, where there are fewer), and the top_groups best groups are kept
+ *   ids: the top_k largest c in them, ties to the lower group and the lower id; scores
+ *   are compared in 64 bits (without a bias, experts by their logits)
+ *   wts = scale * s[ids], with norm_topk scale * s[ids] / their sum
+ * An expert whose logit or bias is -inf or NaN is never chosen. balance goes by p =
+ * s / sum(s); the rest is as above, but for saved: fp32 [T, 4], 16-byte aligned. The
+ * workspace is vqk_route_workspace's. */
+#define VQK_SCORE_SOFTMAX 0
+#define VQK_SCORE_SIGMOID 1
+typedef struct vqk_route_form {
+    int32_t      score;
+    int32_t      groups;
+    int32_t      top_groups;
+    int32_t      group_top;
+    float        scale;
+    const float *bias;
+} vqk_route_form;
+int vqk_route_grouped(const void *logits, int32_t l_type, int64_t T, int64_t E, int64_t ld,
+                      const uint8_t *mask, const vqk_route_form *form, int32_t top_k,
+                      int32_t norm_topk, int32_t *ids, float *wts, int32_t *counts, float *stats,
+                      float *saved, void *workspace, size_t ws_bytes, void *stream);
+int vqk_route_grouped_backward(const void *logits, int32_t l_type, int64_t T, int64_t E, int64_t ld,
+                               const vqk_route_form *form, int32_t top_k, int32_t norm_topk,
+                               const int32_t *ids, const float *wts, const int32_t *counts,
+                               const float *stats, const float *saved, const float *dw,
+                               const float *dbalance, const float *dz, void *dlogits, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,7 @@ VQK_MOE_HEADER_BYTES = 49152             # include/vqk.h: zero before a layer wo
 VQK_VIA_F16 = 0x100                      # output type flag: round through fp16 first
 VQK_X_KEEP = 0x200                       # x type flag (d=8 GEMV): x enters the products unrounded
 VQK_MX_ACT_NONE, VQK_MX_ACT_MXFP4 = range(2)   # include/vqk.h: x of an MXFP4 linear as it is / in 4 bits
+VQK_SCORE_SOFTMAX, VQK_SCORE_SIGMOID = range(2)   # include/vqk.h: scores of the router
 VQK_F8_ACT_NONE, VQK_F8_ACT_F8 = range(2)      # include/vqk.h: x of an 8-bit linear as it is / in 8 bits
 
 c_i32, c_i64, c_p, c_sz = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t
@@ -56,7 +57,13 @@ class VQKF8Weights(ctypes.Structure):
     _fields_ = [("codes", c_p), ("scales", c_p), ("OUT", c_i64), ("IN", c_i64)]
 
 
+class VQKRouteForm(ctypes.Structure):
+    _fields_ = [("score", c_i32), ("groups", c_i32), ("top_groups", c_i32), ("group_top", c_i32),
+                ("scale", ctypes.c_float), ("bias", c_p)]
+
+
 _MXW = ctypes.POINTER(VQKMXWeights)
+_FORM = ctypes.POINTER(VQKRouteForm)
 _F8W = ctypes.POINTER(VQKF8Weights)
 c_f64 = ctypes.c_double
 
@@ -151,6 +158,10 @@ SIGNATURES = {
                           c_p, c_p, c_sz, c_p]),
     "vqk_route_backward": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, c_i32, c_i32, c_p, c_p, c_p,
                                    c_p, c_p, c_p, c_p, c_p, c_p, c_p]),
+    "vqk_route_grouped": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, c_p, _FORM, c_i32, c_i32, c_p, c_p, c_p,
+                                  c_p, c_p, c_p, c_sz, c_p]),
+    "vqk_route_grouped_backward": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, _FORM, c_i32, c_i32, c_p, c_p, c_p,
+                                           c_p, c_p, c_p, c_p, c_p, c_p, c_p]),
 }
 
 _LIB = None

@@ -1,0 +1,849 @@
+// Routing by scores with a bias and groups of experts, with what training it needs:
+// tokens per expert, the balance and z losses, the gradient of the logits.
+//
+//   s = sigmoid(l) or softmax(l),  c = s + bias (the bias alone steers the choice)
+//   a group's score: the sum of its group_top (1 or 2) largest c, of the experts that can be chosen
+//   ids = the top_k largest c in the top_groups best groups; ties to the lower group, the lower id
+//   w = scale s[ids] (norm: scale s / sum of the chosen s)
+//   balance = E sum_e c_e / (n k) mean_t p_te,  p = s / sum s;   z = mean_t lse_t^2
+// with gradients g_b, g_z and dw, and f_e = g_b E c_e / (n^2 k):
+//   u_e = p_e (f_e - sum_i f_i p_i) + [e in ids] (norm: w_e dw_e - w_e / scale sum_j w_j dw_j,
+//                                                 else: w_e dw_e)
+//   sigmoid: dl_e = (1 - s_e) u_e;  softmax: dl_e = u_e - (norm: 0, else: p_e sum_j w_j dw_j)
+//   and 2 g_z / n lse softmax(l)_e
+//
+// Which of two scores is larger is a question of 64 bits: in 32, one in some
+// hundred tokens has two near enough to come out in the other order. The choice
+// (choose64) evaluates scores in fp64, a wave a token. From 2048 tokens sixteen lanes
+// take a token in fp32 (k_group16) with a bound on its errors, and only tokens with two
+// scores closer than that, where it matters, are chosen again by choose64. Without a
+// bias experts of equal group are in the order of their logits, which is exact.
+// A sigmoid row far below zero (largest logit under -40) has s = e^l to within fp64's
+// rounding: its weights and p are a softmax, and nothing divides by a vanishing sum.
+// Sums over tokens stay in registers until the wave's last token and meet in a fixed
+// order: every result is the same from call to call.
+#include "vqk_gemv.h"
+#include "vqk_route.h"
+
+namespace vqk {
+
+constexpr int kGroupMaxGroups = 64;
+constexpr int kGroup16MaxE = 512, kGroup16MaxK = 15, kGroup16MaxG = 16;   // a lane for the best left out, too
+constexpr int64_t kGroup16MinT = 2048;
+constexpr float kFarLogit = -40.f;
+
+struct GroupArgs {
+    const void *l;
+    int64_t T, ld;
+    int32_t E, k, norm;
+    const uint8_t *mask;
+    const float *bias;                        // [E] or NULL
+    int32_t G, top_groups, group_top, gs;     // gs = E / G
+    float scale;
+    int32_t *ids;
+    float *wts;
+    float4 *saved;                            // [T] (max, 1 / sum exp, 1 / sum sigmoid, 0), or NULL
+    float *part_p, *part_z;                   // training: per-workgroup partials [wgs][E] and [wgs]
+    int32_t *part_c, *part_n;
+};
+
+// sigmoid(l) and 1 - sigmoid(l), both to their own last bits.
+__device__ __forceinline__ float2 sigmoid2(float l) {
+    const float e = route_exp(-__builtin_fabsf(l)), r = 1.f / (1.f + e);
+    return l >= 0.f ? float2{r, e * r} : float2{e * r, r};
+}
+
+__device__ __forceinline__ uint64_t f64_key(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.);               // -0 as 0
+    return v != v ? 0 : ((b >> 63) ? ~b : (b | (uint64_t(1) << 63)));
+}
+constexpr uint64_t kKey64NegInf = 0x000fffffffffffffull;                   // f64_key(-inf)
+
+__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
+    const uint32_t hi = wave_max_u32(uint32_t(v >> 32));
+    const uint32_t lo = wave_max_u32(uint32_t(v >> 32) == hi ? uint32_t(v) : 0u);
+    return (uint64_t(hi) << 32) | lo;
+}
+
+__device__ __forceinline__ double shfl_f64(double v, int from) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __shfl(uint32_t(b), from), hi = __shfl(uint32_t(b >> 32), from);
+    return __builtin_bit_cast(double, (uint64_t(hi) << 32) | lo);
+}
+
+// The choice for one token by a whole wave: lane holds logits v[i] of experts lane +
+// 64 i (-inf past E), m their largest; lds: E doubles. Returns the lane's choice (lane j
+// the j-th), -1 for none.
+template <int NS, bool SIG>
+__device__ int choose64(const GroupArgs &p, const float (&v)[NS], float m, double *lds, int lane) {
+    double s[NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) s[i] = 0.;
+    if (p.bias || p.G > 1) {
+        double total = 1.;
+        if constexpr (!SIG) {
+            total = 0.;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                s[i] = v[i] == v[i] ? exp(double(v[i]) - double(m)) : 0.;
+                total += s[i];
+            }
+            for (int o = 1; o < 64; o <<= 1) total += shfl_f64(total, lane ^ o);
+        }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int e = lane + 64 * i;
+            s[i] = SIG ? 1. / (1. + exp(-double(v[i]))) : s[i] / total;
+            if (p.bias && e < p.E) s[i] += double(p.bias[e]);
+        }
+    }
+    uint64_t key[NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        // a logit of -inf or NaN, a bias of -inf or NaN: never chosen
+        const bool can = lane + 64 * i < p.E && v[i] > -__builtin_inff() && s[i] > -__builtin_inf();
+        key[i] = can ? f64_key(p.bias ? s[i] : double(v[i])) : 0;
+        if (p.G > 1 && lane + 64 * i < p.E) lds[lane + 64 * i] = can ? s[i] : -__builtin_inf();
+    }
+    if (p.G > 1) {
+        wave_lds_sync();
+        double a = -__builtin_inf(), b = a;   // the group's two largest
+        if (lane < p.G)
+            for (int j = 0; j < p.gs; ++j) {
+                const double c = lds[lane * p.gs + j];
+                b = c > a ? a : (c > b ? c : b);
+                a = c > a ? c : a;
+            }
+        const double mine = p.group_top == 2 && b > -__builtin_inf() ? a + b : a;
+        int rank = 0;
+        for (int j = 0; j < p.G; ++j) {
+            const double o = shfl_f64(mine, j);
+            rank += o > mine || (o == mine && j < lane);
+        }
+        const uint64_t kept = __ballot(lane < p.G && rank < p.top_groups);
+        wave_lds_sync();
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int e = lane + 64 * i;
+            if (e >= p.E || !((kept >> (e / p.gs)) & 1)) key[i] = 0;
+        }
+    }
+    int id = -1;
+    for (int j = 0; j < p.k; ++j) {
+        uint64_t mine = 0;
+        int at = 0;
+#pragma unroll
+        for (int i = NS - 1; i >= 0; --i)
+            if (key[i] >= mine) {
+                mine = key[i];
+                at = i;
+            }
+        const uint64_t top = wave_max_u64(mine);
+        if (top <= kKey64NegInf) break;
+        const int e = int(wave_min_u32(mine == top ? uint32_t(lane + 64 * at) : 0xffffffffu));
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            if (lane + 64 * i == e) key[i] = 0;
+        if (lane == j) id = e;
+    }
+    return id;
+}
+
+// Weight of the choice `id` with logit l (id < 0: 0), from sums over the lanes of a
+// token; sum and biggest: reductions over those lanes.
+template <bool SIG, typename Sum, typename Big>
+__device__ __forceinline__ float group_weight(const GroupArgs &p, int id, float l, float m, float inv, Sum sum, Big biggest) {
+    if (p.norm) {
+        const float top = biggest(id >= 0 ? l : -__builtin_inff());
+        const bool far = !SIG || top < kFarLogit;
+        const float e = id < 0 ? 0.f : (far ? route_exp(l - top) : sigmoid2(l).x);
+        const float t = sum(e);
+        return id < 0 ? 0.f : e / t * p.scale;
+    }
+    return id < 0 ? 0.f : (SIG ? sigmoid2(l).x : route_exp(l - m) * inv) * p.scale;
+}
+
+// ------------------------------------------------------- a wave to a token
+template <int LT, int NS, bool SIG, bool TRAIN>
+__global__ void __launch_bounds__(kRouteThreads) k_group_wave(const GroupArgs p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    double *lds = reinterpret_cast<double *>(smem) + (threadIdx.x >> 6) * p.E;     // [waves][E]
+    int32_t *cnt = reinterpret_cast<int32_t *>(smem + kRouteWaves * 8 * size_t(p.E));   // TRAIN: [E], [E]
+    float *psh = reinterpret_cast<float *>(cnt + p.E);
+    __shared__ float zsh[kRouteWaves];
+    __shared__ int nsh[kRouteWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if constexpr (TRAIN) {
+        for (int e = threadIdx.x; e < p.E; e += kRouteThreads) cnt[e] = 0;
+        __syncthreads();
+    }
+    float psum[NS] = {};
+    float zsum = 0.f;
+    int live = 0;
+    for (int64_t t = int64_t(blockIdx.x) * kRouteWaves + wave; t < p.T; t += int64_t(gridDim.x) * kRouteWaves) {
+        float v[NS];
+        uint32_t best = 0;
+        bool isnan = false;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int e = lane + 64 * i;
+            v[i] = e < p.E ? load_act(p.l, LT, t * p.ld + e) : -__builtin_inff();
+            isnan = isnan || v[i] != v[i];
+            best = max(best, f32_key(v[i]));
+        }
+        best = wave_max_u32(best);
+        const bool anynan = __ballot(isnan) != 0;
+        if (!((!p.mask || p.mask[t] != 0) && (best > kKeyNegInf || anynan))) {
+            if (lane < p.k) {
+                p.ids[t * p.k + lane] = -1;
+                p.wts[t * p.k + lane] = 0.f;
+            }
+            if (p.saved && lane == 0) p.saved[t] = float4{0.f, 0.f, 0.f, 0.f};
+            continue;
+        }
+        const float m = key_f32(best);
+        const int id = choose64<NS, SIG>(p, v, m, lds, lane);
+        float total = 0.f, inv = 0.f, sums = 0.f;
+        if constexpr (!SIG || TRAIN) {
+#pragma unroll
+            for (int i = 0; i < NS; ++i) total += route_exp(v[i] - m);
+            total = wave_sum(total);
+            inv = 1.f / total;
+        }
+        const float l = id >= 0 ? load_act(p.l, LT, t * p.ld + id) : 0.f;
+        float w = group_weight<SIG>(p, id, l, m, inv, [](float x) { return wave_sum(x); }, [](float x) { return wave_max(x); });
+        if (anynan) w = __uint_as_float(0x7fc00000u);
+        if (lane < p.k) {
+            p.ids[t * p.k + lane] = id;
+            p.wts[t * p.k + lane] = w;
+            if (TRAIN && id >= 0) atomicAdd(&cnt[id], 1);
+        }
+        if constexpr (TRAIN) {
+            const float lse = m + logf(total);
+            zsum += lse * lse;
+            ++live;
+            const bool far = !SIG || m < kFarLogit;
+            float f = inv;
+            if (!far) {
+                float s = 0.f;
+#pragma unroll
+                for (int i = 0; i < NS; ++i) s += sigmoid2(v[i]).x;
+                sums = f = 1.f / wave_sum(s);
+            }
+#pragma unroll
+            for (int i = 0; i < NS; ++i) psum[i] += (far ? route_exp(v[i] - m) : sigmoid2(v[i]).x) * f;
+        }
+        if (p.saved && lane == 0) p.saved[t] = float4{m, inv, sums, 0.f};
+    }
+    if constexpr (TRAIN) {
+        for (int w = 0; w < kRouteWaves; ++w) {             // the waves' sums in wave order
+            if (wave == w) {
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    const int e = lane + 64 * i;
+                    if (e < p.E) psh[e] = w ? psh[e] + psum[i] : psum[i];
+                }
+                if (lane == 0) {
+                    zsh[w] = zsum;
+                    nsh[w] = live;
+                }
+            }
+            __syncthreads();
+        }
+        for (int e = threadIdx.x; e < p.E; e += kRouteThreads) {
+            p.part_p[int64_t(blockIdx.x) * p.E + e] = psh[e];
+            p.part_c[int64_t(blockIdx.x) * p.E + e] = cnt[e];
+        }
+        if (threadIdx.x == 0) {
+            float z = 0.f;
+            int n = 0;
+            for (int w = 0; w < kRouteWaves; ++w) {
+                z += zsh[w];
+                n += nsh[w];
+            }
+            p.part_z[blockIdx.x] = z;
+            p.part_n[blockIdx.x] = n;
+        }
+    }
+}
+
+// ------------------------------------------------- sixteen lanes to a token
+// Bounds of what fp32 may get wrong in a comparison of two c (smax: the row's
+// largest s): a sigmoid is 4 units of 2^-23 off at most, a softmax 2^-18 of itself
+// (its sum adds up E terms, 32 in a lane), the sum with the bias half a unit.
+template <bool SIG>
+__device__ __forceinline__ float group_tol(float smax, float c) {
+    return (SIG ? 0x1p-19f : 0x1p-16f) * smax + 0x1p-21f * __builtin_fabsf(c);
+}
+
+// Lane `sub` of a token holds in value 4 q + j expert 64 q + 4 ((sub + 4 q) % 16) + j:
+// whole lines a load, and the lanes of a group shift from one 64 to the next, so that
+// the experts of few groups are not all in the same lanes.
+__device__ __forceinline__ int group16_expert(int i, int sub) { return 64 * (i / 4) + 4 * ((sub + i / 4 * 4) & 15) + i % 4; }
+template <int LT, int NS>
+__device__ __forceinline__ void group16_load(const GroupArgs &p, int64_t t, int sub, bool in, bool vec, float (&v)[NS]) {
+#pragma unroll
+    for (int q = 0; q < NS / 4; ++q) {
+        const int e = group16_expert(4 * q, sub);
+        if (vec) {
+            u32x4 f{};
+            const bool ok = in && e < p.E;
+            if constexpr (LT == VQK_F32) {
+                if (ok) f = *reinterpret_cast<const u32x4 *>(static_cast<const float *>(p.l) + t * p.ld + e);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[4 * q + j] = ok ? __uint_as_float(f[j]) : -__builtin_inff();
+            } else {
+                u32x2 h{};
+                if (ok) h = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(p.l) + t * p.ld + e);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint16_t b = uint16_t(h[j / 2] >> (16 * (j & 1)));
+                    v[4 * q + j] = !ok ? -__builtin_inff() : (LT == VQK_BF16 ? bf16_to_f32(b) : h_to_f32(b));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[4 * q + j] = in && e + j < p.E ? load_act(p.l, LT, t * p.ld + e + j) : -__builtin_inff();
+        }
+    }
+}
+
+// The top k as in k_route16: the k-th largest lane maximum bounds them from below,
+// what reaches it is collected in LDS and ranked, two candidates a lane. One more than
+// top_k is looked at: the best that is left out.
+template <int LT, int NS, bool SIG, bool TRAIN>
+__global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bool vec) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    float *csh = reinterpret_cast<float *>(smem) + (threadIdx.x >> 6) * 4 * p.E;     // [waves][4][E]; choose64: [waves][E] doubles
+    int32_t *cnt = reinterpret_cast<int32_t *>(smem + kRouteWaves * 16 * size_t(p.E));   // TRAIN: [E], [E]
+    float *psh = reinterpret_cast<float *>(cnt + p.E);
+    __shared__ uint64_t cands[kRouteWaves][4][kRouteCands];
+    __shared__ uint64_t sel[kRouteWaves][4][kGroup16MaxK + 1];
+    __shared__ float zsh[kRouteWaves];
+    __shared__ int nsh[kRouteWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int sub = lane & 15, grp = lane >> 4;
+    if constexpr (TRAIN) {
+        for (int e = threadIdx.x; e < p.E; e += kRouteThreads) {
+            cnt[e] = 0;
+            psh[e] = 0.f;
+        }
+        __syncthreads();
+    }
+    float bias[NS];
+    uint32_t gid[NS / 4] = {};                // the experts' groups, four to a word
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int e = group16_expert(i, sub);
+        bias[i] = p.bias && e < p.E ? p.bias[e] : 0.f;
+        gid[i / 4] |= uint32_t(e < p.E ? e / p.gs : 0) << (8 * (i % 4));
+    }
+    float psum[NS] = {};
+    float zsum = 0.f;
+    int nlive = 0;
+    const int64_t stride = int64_t(gridDim.x) * kRouteWaves * 4;
+    for (int64_t t0 = (int64_t(blockIdx.x) * kRouteWaves + wave) * 4; t0 < p.T; t0 += stride) {
+        const int64_t t = t0 + grp;
+        const bool in = t < p.T && (!p.mask || p.mask[t] != 0);
+        float v[NS], c[NS];
+        group16_load<LT, NS>(p, t, sub, in, vec, v);
+        uint32_t best = 0;
+        bool isnan = false;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            isnan = isnan || v[i] != v[i];
+            best = max(best, f32_key(v[i]));
+        }
+        best = row_max(best);
+        const bool anynan = ((__ballot(isnan) >> (grp * 16)) & 0xffffu) != 0;
+        const bool live = in && (best > kKeyNegInf || anynan);
+        const float m = live && best > kKeyNegInf ? key_f32(best) : 0.f;
+        float total = 0.f, inv = 0.f, sums = 0.f;
+        if constexpr (!SIG || TRAIN) {
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                c[i] = live && v[i] == v[i] ? route_exp(v[i] - m) : 0.f;
+                total += c[i];
+            }
+            total = row_sum(total);
+            inv = live ? 1.f / total : 0.f;
+        }
+        const float smax = SIG ? sigmoid2(m).x : inv;
+        const bool far = !SIG || m < kFarLogit;             // p: a softmax
+        float q[TRAIN ? NS : 1];                            // p before its sum
+        if constexpr (TRAIN) {
+#pragma unroll
+            for (int i = 0; i < NS; ++i) q[i] = c[i];
+        }
+        if constexpr (SIG) {
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                c[i] = sigmoid2(v[i]).x;
+                if constexpr (TRAIN) {
+                    s += c[i];
+                    if (!far) q[i] = c[i];
+                }
+            }
+            if constexpr (TRAIN) sums = live && !far ? 1.f / row_sum(s) : 0.f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < NS; ++i) c[i] *= inv;
+        }
+        if (anynan) total = inv = sums = __uint_as_float(live ? 0x7fc00000u : 0u);
+        uint32_t key[NS], lm = 0;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            c[i] += bias[i];
+            const bool can = live && v[i] > -__builtin_inff() && c[i] > -__builtin_inff();
+            key[i] = can ? f32_key(p.bias ? c[i] : v[i]) : 0u;
+            c[i] = can ? c[i] : -__builtin_inff();
+        }
+        bool amb = false;                                   // fp32 does not say which is larger
+        if (p.G > 1) {
+            wave_lds_sync();                                // the last tokens' scores are read
+            float *mine = csh + grp * p.E;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const int e = group16_expert(i, sub);
+                if (e < p.E) mine[e] = c[i];
+            }
+            wave_lds_sync();
+            float a = -__builtin_inff(), b = a;             // the group's two largest
+            if (sub < p.G) {
+                int at = sub % p.gs;                        // lanes start at banks of their own
+                for (int j = 0; j < p.gs; ++j) {
+                    const float x = mine[sub * p.gs + at];
+                    at = at + 1 == p.gs ? 0 : at + 1;
+                    b = fmaxf(b, fminf(a, x));
+                    a = fmaxf(a, x);
+                }
+            }
+            const float g = p.group_top == 2 && b > -__builtin_inff() ? a + b : a;
+            const uint32_t gk = f32_key(g);
+            int rank = 0;
+#define VQK_ROR(N)                                                                    \
+    {                                                                                 \
+        const uint32_t o = dpp_u<0x120 + N>(gk);                                      \
+        const int from = int(dpp_u<0x120 + N>(uint32_t(sub)));                        \
+        rank += from < p.G && (o > gk || (o == gk && from < sub));                    \
+    }
+            VQK_ROR(1) VQK_ROR(2) VQK_ROR(3) VQK_ROR(4) VQK_ROR(5) VQK_ROR(6) VQK_ROR(7) VQK_ROR(8)
+            VQK_ROR(9) VQK_ROR(10) VQK_ROR(11) VQK_ROR(12) VQK_ROR(13) VQK_ROR(14) VQK_ROR(15)
+#undef VQK_ROR
+            const bool keep = sub < p.G && rank < p.top_groups;
+            const uint32_t kept = uint32_t(__ballot(keep) >> (grp * 16)) & 0xffffu;
+            const uint32_t worst = row_min(keep ? gk : 0xffffffffu), next = row_max(sub < p.G && !keep ? gk : 0u);
+            // of a sum each part is as far off as c may be
+            const float mag = p.group_top == 2 ? __builtin_fabsf(a) + (b > -__builtin_inff() ? __builtin_fabsf(b) : 0.f) : __builtin_fabsf(a);
+            const float most = key_f32(row_max(sub < p.G && a > -__builtin_inff() ? f32_key(mag) : f32_key(0.f)));
+            if (next > kKeyNegInf) amb = !(key_f32(worst) - key_f32(next) > 4.f * group_tol<SIG>(smax, most));
+#pragma unroll
+            for (int i = 0; i < NS; ++i) key[i] = (kept >> ((gid[i / 4] >> (8 * (i % 4))) & 255u)) & 1u ? key[i] : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) lm = max(lm, key[i]);
+        // the k-th largest lane maximum; with a bias one rank further, so that the best left out is a
+        // candidate too
+        const int want = p.bias ? p.k + 1 : p.k;
+        int rank = 0;
+#define VQK_ROR(N) rank += dpp_u<0x120 + N>(lm) > lm;
+        VQK_ROR(1) VQK_ROR(2) VQK_ROR(3) VQK_ROR(4) VQK_ROR(5) VQK_ROR(6) VQK_ROR(7) VQK_ROR(8)
+        VQK_ROR(9) VQK_ROR(10) VQK_ROR(11) VQK_ROR(12) VQK_ROR(13) VQK_ROR(14) VQK_ROR(15)
+#undef VQK_ROR
+        const uint32_t thr = max(row_min(rank < want ? lm : 0xffffffffu), kKeyNegInf + 1);
+        int run = 0;
+        wave_lds_sync();                                    // the last token's candidates are read
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const bool in_ = key[i] >= thr;
+            const uint32_t gm = uint32_t(__ballot(in_) >> (grp * 16)) & 0xffffu;
+            const int pos = run + __popc(gm & ((1u << sub) - 1u));
+            if (in_ && pos < kRouteCands)
+                cands[wave][grp][pos] = (uint64_t(key[i]) << 32) | uint32_t(~group16_expert(i, sub));
+            run += __popc(gm);
+        }
+        if (sub <= p.k) sel[wave][grp][sub] = 0;
+        wave_lds_sync();
+        uint64_t c0 = 0, c1 = 0;
+        if (sub < run) c0 = cands[wave][grp][sub];
+        if (sub + 16 < run) c1 = cands[wave][grp][sub + 16];
+        int r0 = c1 > c0, r1 = c0 > c1;
+#define VQK_ROR(N)                                                                              \
+    {                                                                                           \
+        const uint64_t a = dpp_u64<0x120 + N>(c0), b = dpp_u64<0x120 + N>(c1);                  \
+        r0 += int(a > c0) + int(b > c0);                                                        \
+        r1 += int(a > c1) + int(b > c1);                                                        \
+    }
+        VQK_ROR(1) VQK_ROR(2) VQK_ROR(3) VQK_ROR(4) VQK_ROR(5) VQK_ROR(6) VQK_ROR(7) VQK_ROR(8)
+        VQK_ROR(9) VQK_ROR(10) VQK_ROR(11) VQK_ROR(12) VQK_ROR(13) VQK_ROR(14) VQK_ROR(15)
+#undef VQK_ROR
+        if (c0 != 0 && r0 <= p.k) sel[wave][grp][r0] = c0;
+        if (c1 != 0 && r1 <= p.k) sel[wave][grp][r1] = c1;
+        wave_lds_sync();
+        const uint64_t mine = sub < p.k ? sel[wave][grp][sub] : 0, next = sub < p.k ? sel[wave][grp][sub + 1] : 0;
+        int id = mine ? int(~uint32_t(mine)) : -1;
+        float l = id >= 0 ? load_act(p.l, LT, t * p.ld + id) : 0.f;
+        if (p.bias) {
+            bool near = false;
+            if (next) {
+                // equal logits under equal biases are a tie, and the lower id comes first already
+                const int e = int(~uint32_t(next));
+                const float x = key_f32(uint32_t(mine >> 32)), y = key_f32(uint32_t(next >> 32));
+                near = !(x - y > 2.f * group_tol<SIG>(smax, x)) &&
+                       !(l == load_act(p.l, LT, t * p.ld + e) && p.bias[id] == p.bias[e]);
+            }
+            amb = amb || ((__ballot(near) >> (grp * 16)) & 0xffffu) != 0;
+        }
+        amb = live && (amb || run > kRouteCands);
+        const uint64_t again = __ballot(amb);
+        if (again) {
+            for (int g = 0; g < 4; ++g) {
+                if (!((again >> (16 * g)) & 1)) continue;
+                const int64_t tt = t0 + g;
+                float vv[(NS + 3) / 4];
+#pragma unroll
+                for (int i = 0; i < (NS + 3) / 4; ++i) {
+                    const int e = lane + 64 * i;
+                    vv[i] = e < p.E ? load_act(p.l, LT, tt * p.ld + e) : -__builtin_inff();
+                }
+                const float mm = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m), 16 * g));
+                wave_lds_sync();                            // the scores are read
+                const int got = choose64<(NS + 3) / 4, SIG>(p, vv, mm, reinterpret_cast<double *>(csh), lane);
+                const int at = __shfl(got, sub);
+                if (grp == g) id = sub < p.k ? at : -1;
+            }
+            l = id >= 0 ? load_act(p.l, LT, t * p.ld + id) : 0.f;
+        }
+        float w = group_weight<SIG>(p, id, l, m, inv, [](float x) { return row_sum(x); },
+                                    [](float x) { return key_f32(row_max(f32_key(x))); });
+        if (anynan && live) w = __uint_as_float(0x7fc00000u);
+        if (t < p.T && sub < p.k) {
+            p.ids[t * p.k + sub] = id;
+            p.wts[t * p.k + sub] = w;
+            if (TRAIN && id >= 0) atomicAdd(&cnt[id], 1);
+        }
+        if (p.saved && t < p.T && sub == 0) p.saved[t] = live ? float4{m, inv, sums, 0.f} : float4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (TRAIN) {
+            if (live) {
+                const float lse = m + logf(total);
+                if (sub == 0) {
+                    zsum += lse * lse;
+                    ++nlive;
+                }
+                const float f = far ? inv : sums;
+#pragma unroll
+                for (int i = 0; i < NS; ++i) psum[i] += q[TRAIN ? i : 0] * f;
+            }
+        }
+    }
+    if constexpr (TRAIN) {
+        for (int w = 0; w < kRouteWaves * 4; ++w) {         // the tokens' sums in order of wave and row of lanes
+            if (wave == w / 4 && grp == w % 4) {
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    const int e = group16_expert(i, sub);
+                    if (e < p.E) psh[e] += psum[i];
+                }
+            }
+            if (w % 4 == 3) __syncthreads();
+            else wave_lds_sync();
+        }
+        zsum = wave_sum(zsum);
+        for (int o = 16; o < 64; o <<= 1) nlive += __shfl_xor(nlive, o);
+        if (lane == 0) {
+            zsh[wave] = zsum;
+            nsh[wave] = nlive;
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < p.E; e += kRouteThreads) {
+            p.part_p[int64_t(blockIdx.x) * p.E + e] = psh[e];
+            p.part_c[int64_t(blockIdx.x) * p.E + e] = cnt[e];
+        }
+        if (threadIdx.x == 0) {
+            float z = 0.f;
+            int n = 0;
+            for (int w = 0; w < kRouteWaves; ++w) {
+                z += zsh[w];
+                n += nsh[w];
+            }
+            p.part_z[blockIdx.x] = z;
+            p.part_n[blockIdx.x] = n;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- gradient
+struct GroupBwdArgs {
+    const void *l;
+    int64_t T, ld;
+    int32_t E, k, norm;
+    float scale;
+    const int32_t *ids, *counts;
+    const float *wts, *stats;
+    const float4 *saved;
+    const float *dw, *gb, *gz;                // NULL: no gradient of that output
+    void *dl;
+};
+
+// L = 16 lanes to a token (four a wave) or 64; lane `sub` holds experts 4 L q + 4 sub + j.
+template <int LT, int NS, int L, bool SIG>
+__global__ void __launch_bounds__(kRouteThreads) k_group_bwd(const GroupBwdArgs p, bool vec) {
+    extern __shared__ __align__(16) float rows[];           // [waves][64 / L][L * NS]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int sub = lane % L, grp = lane / L;
+    float *row = rows + (wave * (64 / L) + grp) * (L * NS);
+    const float n = p.stats[2];
+    const float fb = p.gb && n > 0.f ? p.gb[0] * (float(p.E) / (n * n * float(p.k))) : 0.f;
+    const float fz = p.gz && n > 0.f ? 2.f * p.gz[0] / n : 0.f;
+    auto sum = [](float x) { return L == 16 ? row_sum(x) : wave_sum(x); };
+    float f[NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int e = 4 * L * (i / 4) + 4 * sub + i % 4;
+        f[i] = e < p.E ? fb * float(p.counts[e]) : 0.f;
+    }
+    const int64_t stride = int64_t(gridDim.x) * kRouteWaves * (64 / L);
+    for (int64_t t0 = (int64_t(blockIdx.x) * kRouteWaves + wave) * (64 / L); t0 < p.T; t0 += stride) {
+        const int64_t t = t0 + grp;
+        const bool in = t < p.T;
+        const float4 sv = in ? p.saved[t] : float4{0.f, 0.f, 0.f, 0.f};
+        const bool live = sv.y != 0.f;        // a live token's sum is at most E
+        float v[NS];
+#pragma unroll
+        for (int q = 0; q < NS / 4; ++q) {
+            const int e = 4 * L * q + 4 * sub;
+            if (vec && live && e < p.E) {
+                if constexpr (LT == VQK_F32) {
+                    const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.l) + t * p.ld + e);
+                    v[4 * q] = a.x; v[4 * q + 1] = a.y; v[4 * q + 2] = a.z; v[4 * q + 3] = a.w;
+                } else {
+                    const u32x2 a = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(p.l) + t * p.ld + e);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint16_t h = uint16_t(a[j / 2] >> (16 * (j & 1)));
+                        v[4 * q + j] = LT == VQK_BF16 ? bf16_to_f32(h) : h_to_f32(h);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    v[4 * q + j] = live && e + j < p.E ? load_act(p.l, LT, t * p.ld + e + j) : -__builtin_inff();
+            }
+        }
+        int id = -1;
+        float wdw = 0.f, w = 0.f;
+        if (p.dw && live && sub < p.k) {
+            id = p.ids[t * p.k + sub];
+            w = p.wts[t * p.k + sub];
+            wdw = id >= 0 ? w * p.dw[t * p.k + sub] : 0.f;
+        }
+        const float s = sum(wdw);
+        const float lse = sv.x - logf(sv.y);
+        const bool far = !SIG || sv.x < kFarLogit;
+        float x[NS];                          // softmax
+        float dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            x[i] = live ? route_exp(v[i] - sv.x) * sv.y : 0.f;
+            dot += f[i] * (far ? x[i] : sigmoid2(v[i]).x * sv.z);
+        }
+        dot = sum(dot);
+        const float sub_ = fz * lse - (SIG || p.norm ? 0.f : s);
+#pragma unroll
+        for (int q = 0; q < NS / 4; ++q) *reinterpret_cast<float4 *>(row + 4 * L * q + 4 * sub) = float4{0.f, 0.f, 0.f, 0.f};
+        wave_lds_sync();
+        if (id >= 0) row[id] = p.norm ? wdw - w / p.scale * s : wdw;
+        wave_lds_sync();
+#pragma unroll
+        for (int q = 0; q < NS / 4; ++q) {
+            const int e = 4 * L * q + 4 * sub;
+            const float4 a = *reinterpret_cast<const float4 *>(row + e);
+            const float add[4] = {a.x, a.y, a.z, a.w};
+            float d[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = 4 * q + j;
+                if constexpr (SIG) {
+                    const float2 g = sigmoid2(v[i]);
+                    d[j] = g.y * ((far ? x[i] : g.x * sv.z) * (f[i] - dot) + add[j]) + x[i] * sub_;
+                } else {
+                    d[j] = x[i] * (f[i] - dot + sub_) + add[j];
+                }
+                if (!live) d[j] = 0.f;
+            }
+            if (!in || e >= p.E) continue;
+            if (vec) {
+                if constexpr (LT == VQK_F32) {
+                    *reinterpret_cast<float4 *>(static_cast<float *>(p.dl) + t * p.E + e) = float4{d[0], d[1], d[2], d[3]};
+                } else {
+                    uint32_t h[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) h[j] = LT == VQK_BF16 ? f32_to_bf16(d[j]) : f32_to_h(d[j]);
+                    u32x2 o;
+                    o.x = h[0] | (h[1] << 16);
+                    o.y = h[2] | (h[3] << 16);
+                    *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(p.dl) + t * p.E + e) = o;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (e + j < p.E) store_act(p.dl, LT, t * p.E + e + j, d[j]);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ launch
+static bool group16_ok(int64_t T, int64_t E, int k, int G) {
+    return T >= kGroup16MinT && E <= kGroup16MaxE && k <= kGroup16MaxK && G <= kGroup16MaxG;
+}
+
+template <int LT, int NS, bool SIG>
+static int go_wave(const GroupArgs &a, bool train, int wgs, hipStream_t st) {
+    const size_t lds = kRouteWaves * 8 * size_t(a.E) + (train ? 8 * size_t(a.E) : 0);
+    if (train) return launch_with_lds<k_group_wave<LT, NS, SIG, true>>(dim3(wgs), dim3(kRouteThreads), lds, st, a);
+    return launch_with_lds<k_group_wave<LT, NS, SIG, false>>(dim3(wgs), dim3(kRouteThreads), lds, st, a);
+}
+template <int LT, int NS, bool SIG>
+static int go_16(const GroupArgs &a, bool train, int wgs, hipStream_t st) {
+    const size_t lds = kRouteWaves * 16 * size_t(a.E) + (train ? 8 * size_t(a.E) : 0);
+    const bool vec = route_vec(a.l, a.ld, a.E, LT);
+    if (train) hipLaunchKernelGGL((k_group16<LT, NS, SIG, true>), dim3(wgs), dim3(kRouteThreads), lds, st, a, vec);
+    else hipLaunchKernelGGL((k_group16<LT, NS, SIG, false>), dim3(wgs), dim3(kRouteThreads), lds, st, a, vec);
+    return hip_status(hipGetLastError(), "router launch");
+}
+template <int LT, bool SIG>
+static int go_group(const GroupArgs &a, bool train, int wgs, hipStream_t st) {
+    const int E = a.E;
+    if (group16_ok(a.T, E, a.k, a.G)) {
+        if (E <= 64) return go_16<LT, 4, SIG>(a, train, wgs, st);
+        if (E <= 128) return go_16<LT, 8, SIG>(a, train, wgs, st);
+        if (E <= 192) return go_16<LT, 12, SIG>(a, train, wgs, st);
+        if (E <= 256) return go_16<LT, 16, SIG>(a, train, wgs, st);
+        if (E <= 384) return go_16<LT, 24, SIG>(a, train, wgs, st);
+        return go_16<LT, 32, SIG>(a, train, wgs, st);
+    }
+    if (E <= 64) return go_wave<LT, 1, SIG>(a, train, wgs, st);
+    if (E <= 128) return go_wave<LT, 2, SIG>(a, train, wgs, st);
+    if (E <= 256) return go_wave<LT, 4, SIG>(a, train, wgs, st);
+    if (E <= 512) return go_wave<LT, 8, SIG>(a, train, wgs, st);
+    if (E <= 1024) return go_wave<LT, 16, SIG>(a, train, wgs, st);
+    return go_wave<LT, 32, SIG>(a, train, wgs, st);
+}
+
+template <int LT, int NS, int L, bool SIG>
+static int go_bwd(const GroupBwdArgs &a, int wgs, hipStream_t st) {
+    const bool vec = route_vec(a.l, a.ld, a.E, LT) && (reinterpret_cast<uintptr_t>(a.dl) & 15) == 0;
+    hipLaunchKernelGGL((k_group_bwd<LT, NS, L, SIG>), dim3(wgs), dim3(kRouteThreads), kRouteWaves * 64 * NS * 4, st, a, vec);
+    return hip_status(hipGetLastError(), "router gradient launch");
+}
+template <int LT, bool SIG>
+static int go_group_bwd(const GroupBwdArgs &a, bool rows16, int wgs, hipStream_t st) {
+    const int E = a.E;
+    if (rows16) {
+        if (E <= 64) return go_bwd<LT, 4, 16, SIG>(a, wgs, st);
+        if (E <= 128) return go_bwd<LT, 8, 16, SIG>(a, wgs, st);
+        if (E <= 192) return go_bwd<LT, 12, 16, SIG>(a, wgs, st);
+        if (E <= 256) return go_bwd<LT, 16, 16, SIG>(a, wgs, st);
+        if (E <= 384) return go_bwd<LT, 24, 16, SIG>(a, wgs, st);
+        return go_bwd<LT, 32, 16, SIG>(a, wgs, st);
+    }
+    if (E <= 256) return go_bwd<LT, 4, 64, SIG>(a, wgs, st);
+    if (E <= 512) return go_bwd<LT, 8, 64, SIG>(a, wgs, st);
+    if (E <= 1024) return go_bwd<LT, 16, 64, SIG>(a, wgs, st);
+    return go_bwd<LT, 32, 64, SIG>(a, wgs, st);
+}
+
+static int check_form(const vqk_route_form *f, int64_t E, int32_t k, const char *what) {
+    if (!f) return set_error(VQK_EINVAL, "%s: NULL form", what);
+    if (f->score != VQK_SCORE_SOFTMAX && f->score != VQK_SCORE_SIGMOID) return set_error(VQK_EINVAL, "%s: score %d", what, f->score);
+    if (f->groups < 1 || E % f->groups || f->top_groups < 1 || f->top_groups > f->groups)
+        return set_error(VQK_EINVAL, "%s: %d of %d groups of %lld experts", what, f->top_groups, f->groups, (long long)E);
+    if (f->groups > kGroupMaxGroups) return set_error(VQK_ENOTIMPL, "%s: %d groups > %d", what, f->groups, kGroupMaxGroups);
+    if (f->group_top != 1 && f->group_top != 2) return set_error(VQK_ENOTIMPL, "%s: a group's score from %d experts", what, f->group_top);
+    if (f->group_top > E / f->groups)
+        return set_error(VQK_EINVAL, "%s: a group's score from %d of %lld experts", what, f->group_top, (long long)(E / f->groups));
+    if (int64_t(k) > f->top_groups * (E / f->groups))
+        return set_error(VQK_EINVAL, "%s: top_k=%d of %lld experts in %d groups", what, k, (long long)(f->top_groups * (E / f->groups)), f->top_groups);
+    if (!(f->scale > 0.f) || f->scale > 3.4028234e38f) return set_error(VQK_EINVAL, "%s: scale %g", what, double(f->scale));
+    return VQK_OK;
+}
+
+}  // namespace vqk
+
+using namespace vqk;
+
+extern "C" int vqk_route_grouped(const void *logits, int32_t l_type, int64_t T, int64_t E, int64_t ld,
+                                 const uint8_t *mask, const vqk_route_form *form, int32_t top_k, int32_t norm_topk,
+                                 int32_t *ids, float *wts, int32_t *counts, float *stats, float *saved, void *workspace,
+                                 size_t ws_bytes, void *stream) {
+    int rc = check_route(l_type, T, E, ld, top_k, "route");
+    if (rc || (rc = check_form(form, E, top_k, "route"))) return rc;
+    const bool train = counts || stats;
+    if (train && (!counts || !stats)) return set_error(VQK_EINVAL, "route: counts and stats come together");
+    if (T > 0 && (!logits || !ids || !wts)) return set_error(VQK_EINVAL, "route: NULL pointer");
+    if (reinterpret_cast<uintptr_t>(saved) & 15) return set_error(VQK_EINVAL, "route: saved must be 16-byte aligned");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    GroupArgs a{};
+    a.l = logits; a.T = T; a.ld = ld;
+    a.E = int32_t(E); a.k = top_k; a.norm = norm_topk;
+    a.mask = mask; a.bias = form->bias;
+    a.G = form->groups; a.top_groups = form->top_groups; a.group_top = form->group_top; a.gs = int32_t(E / form->groups);
+    if (a.top_groups == a.G) a.G = a.top_groups = 1, a.gs = int32_t(E);       // every group is kept
+    a.scale = form->scale;
+    a.ids = ids; a.wts = wts;
+    a.saved = reinterpret_cast<float4 *>(saved);
+    const int wgs = route_wgs_of(T, group16_ok(T, E, top_k, a.G) ? 4 * kRouteWaves : kRouteWaves);
+    FinishArgs f{};
+    if (train) {
+        const size_t need = route_bytes(T, E);
+        if (!workspace || ws_bytes < need) return set_error(VQK_ENOSPACE, "route: workspace %zu < %zu", ws_bytes, need);
+        if (reinterpret_cast<uintptr_t>(workspace) & 15) return set_error(VQK_EINVAL, "route: workspace must be 16-byte aligned");
+        route_parts(workspace, E, wgs, &f, &a.part_p, &a.part_c, &a.part_z, &a.part_n);
+        f.k = top_k; f.counts = counts; f.stats = stats;
+    }
+    if (wgs) {
+        const bool sig = form->score == VQK_SCORE_SIGMOID;
+        switch (l_type) {
+            case VQK_F16: rc = sig ? go_group<VQK_F16, true>(a, train, wgs, st) : go_group<VQK_F16, false>(a, train, wgs, st); break;
+            case VQK_BF16: rc = sig ? go_group<VQK_BF16, true>(a, train, wgs, st) : go_group<VQK_BF16, false>(a, train, wgs, st); break;
+            default: rc = sig ? go_group<VQK_F32, true>(a, train, wgs, st) : go_group<VQK_F32, false>(a, train, wgs, st);
+        }
+        if (rc) return rc;
+    }
+    return train ? route_finish(f, st) : VQK_OK;
+}
+
+extern "C" int vqk_route_grouped_backward(const void *logits, int32_t l_type, int64_t T, int64_t E, int64_t ld,
+                                          const vqk_route_form *form, int32_t top_k, int32_t norm_topk,
+                                          const int32_t *ids, const float *wts, const int32_t *counts,
+                                          const float *stats, const float *saved, const float *dw,
+                                          const float *dbalance, const float *dz, void *dlogits, void *stream) {
+    int rc = check_route(l_type, T, E, ld, top_k, "route backward");
+    if (rc || (rc = check_form(form, E, top_k, "route backward"))) return rc;
+    if (T == 0) return VQK_OK;
+    if (!logits || !ids || !wts || !counts || !stats || !saved || !dlogits)
+        return set_error(VQK_EINVAL, "route backward: NULL pointer");
+    if (reinterpret_cast<uintptr_t>(saved) & 15)
+        return set_error(VQK_EINVAL, "route backward: saved must be 16-byte aligned");
+    GroupBwdArgs a{};
+    a.l = logits; a.T = T; a.ld = ld;
+    a.E = int32_t(E); a.k = top_k; a.norm = norm_topk; a.scale = form->scale;
+    a.ids = ids; a.counts = counts; a.wts = wts; a.stats = stats;
+    a.saved = reinterpret_cast<const float4 *>(saved);
+    a.dw = dw; a.gb = dbalance; a.gz = dz;
+    a.dl = dlogits;
+    const bool rows16 = group16_ok(T, E, top_k, 1);
+    const int per = rows16 ? 4 * kRouteWaves : kRouteWaves;
+    const int64_t w = (T + per - 1) / per;
+    const int wgs = int(w < 2048 ? w : 2048);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const bool sig = form->score == VQK_SCORE_SIGMOID;
+    switch (l_type) {
+        case VQK_F16: return sig ? go_group_bwd<VQK_F16, true>(a, rows16, wgs, st) : go_group_bwd<VQK_F16, false>(a, rows16, wgs, st);
+        case VQK_BF16: return sig ? go_group_bwd<VQK_BF16, true>(a, rows16, wgs, st) : go_group_bwd<VQK_BF16, false>(a, rows16, wgs, st);
+        default: return sig ? go_group_bwd<VQK_F32, true>(a, rows16, wgs, st) : go_group_bwd<VQK_F32, false>(a, rows16, wgs, st);
+    }
+}

@@ -20,16 +20,9 @@
 // (k_route, k_route_bwd). The sums over tokens stay in registers until the wave's
 // last token. All arithmetic is fp32 (the sums over workgroups and the losses
 // fp64). Sums meet in a fixed order: every result is the same from call to call.
-#include "vqk_common.h"
+#include "vqk_route.h"
 
 namespace vqk {
-
-constexpr int kRouteWaves = 4;
-constexpr int kRouteThreads = kRouteWaves * kWave;
-constexpr int kRouteMaxWgs = 768;              // three waves a SIMD: the registers of k_route16
-constexpr int kRouteMaxE = 2048;
-constexpr int kRouteMaxK = 64;
-constexpr uint32_t kKeyNegInf = 0x007fffffu;           // f32_key(-inf); NaN maps below it
 
 struct RouteArgs {
     const void *l;
@@ -44,15 +37,6 @@ struct RouteArgs {
     int32_t *part_c, *part_n;
 };
 
-// What a wave's lanes wrote to LDS before, its other lanes read after. The hardware
-// keeps a wave's LDS accesses in order; the fences, which cost no instruction, hold
-// the compiler to it.
-__device__ __forceinline__ void wave_lds_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 template <int LT, int NS>
 __device__ __forceinline__ void route_load(const void *l, int64_t base, int E, int lane, float (&v)[NS]) {
 #pragma unroll
@@ -60,15 +44,6 @@ __device__ __forceinline__ void route_load(const void *l, int64_t base, int E, i
         const int e = lane * NS + i;
         v[i] = e < E ? load_act(l, LT, base + e) : -__builtin_inff();
     }
-}
-
-// e^d for d <= 0: 2^(d log2 e), the product's rounding error carried along.
-__device__ __forceinline__ float route_exp(float d) {
-    constexpr float hi = 1.44269502162933349609375f, lo = 1.92596299113e-8f;   // log2 e = hi + lo
-    d = d < -200.f ? -200.f : d;              // 0 already (and -inf leaves no NaN; a NaN stays)
-    const float t = d * hi, r = __builtin_fmaf(d, hi, -t) + d * lo;
-    const float e = __builtin_amdgcn_exp2f(t);
-    return __builtin_fmaf(e, 0.693147182f * r, e);
 }
 
 template <int LT, int NS, bool TRAIN>
@@ -195,69 +170,13 @@ __global__ void __launch_bounds__(kRouteThreads) k_route(const RouteArgs p) {
 }
 
 // ------------------------------------------------- sixteen lanes to a token
-template <int CTRL>
-__device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
-    return (uint64_t(dpp_u<CTRL>(uint32_t(v >> 32))) << 32) | dpp_u<CTRL>(uint32_t(v));
-}
-__device__ __forceinline__ uint32_t row_max(uint32_t v) {
-    v = max(v, dpp_u<kDppQuadXor1>(v));
-    v = max(v, dpp_u<kDppQuadXor2>(v));
-    v = max(v, dpp_u<kDppRowHalfMirror>(v));
-    return max(v, dpp_u<kDppRowMirror>(v));
-}
-__device__ __forceinline__ uint32_t row_min(uint32_t v) {
-    v = min(v, dpp_u<kDppQuadXor1>(v));
-    v = min(v, dpp_u<kDppQuadXor2>(v));
-    v = min(v, dpp_u<kDppRowHalfMirror>(v));
-    return min(v, dpp_u<kDppRowMirror>(v));
-}
-// Both partners add the same two values, so every lane ends with the same sum.
-__device__ __forceinline__ float row_sum(float v) {
-    v += dpp_f<kDppQuadXor1>(v);
-    v += dpp_f<kDppQuadXor2>(v);
-    v += dpp_f<kDppRowHalfMirror>(v);
-    return v + dpp_f<kDppRowMirror>(v);
-}
-
-constexpr int kRoute16MaxE = 512, kRoute16MaxK = 16, kRouteCands = 32;
+constexpr int kRoute16MaxE = 512, kRoute16MaxK = 16;
 // Tokens from which they pay: below, a wave a token spreads wider and is less code
 // to fetch (509 tokens of 512 experts: 11 us against 31; 2048 of 256: both 7;
 // 65536 of 256: 118 against 52).
 constexpr int64_t kRoute16MinT = 2048;
 static bool route16_ok(int64_t T, int64_t E, int k) {
     return T >= kRoute16MinT && E <= kRoute16MaxE && k <= kRoute16MaxK;
-}
-
-// Lane `sub` of a token holds experts 64 q + 4 sub + j in value 4 q + j: whole
-// lines a load. VEC: fours are aligned and whole.
-template <int LT, int NS, bool VEC>
-__device__ __forceinline__ void route_load16(const void *l, int64_t base, int E, int sub, bool in, float (&v)[NS]) {
-#pragma unroll
-    for (int q = 0; q < NS / 4; ++q) {
-        const int e = 64 * q + 4 * sub;
-        if constexpr (VEC) {
-            if (in && e < E) {
-                if constexpr (LT == VQK_F32) {
-                    const float4 f = *reinterpret_cast<const float4 *>(static_cast<const float *>(l) + base + e);
-                    v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
-                } else {
-                    const u32x2 f = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(l) + base + e);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint16_t h = uint16_t(f[j / 2] >> (16 * (j & 1)));
-                        v[4 * q + j] = LT == VQK_BF16 ? bf16_to_f32(h) : h_to_f32(h);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[4 * q + j] = -__builtin_inff();
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                v[4 * q + j] = in && e + j < E ? load_act(l, LT, base + e + j) : -__builtin_inff();
-        }
-    }
 }
 
 // How the top k are found: each lane's largest key is ranked against the row's
@@ -435,15 +354,6 @@ __global__ void __launch_bounds__(kRouteThreads) k_route16(const RouteArgs p) {
         }
     }
 }
-
-struct FinishArgs {
-    const float *part_p, *part_z;
-    const int32_t *part_c, *part_n;
-    int32_t wgs, E, k;
-    double *dot;                              // [groups] sums of c_e P_e
-    int32_t *counts;
-    float *stats;                             // balance, z, n
-};
 
 // The partials of 16 experts a workgroup: 64 threads an expert group walk over
 // the routing workgroups, then meet in LDS in a fixed order.
@@ -649,16 +559,35 @@ __global__ void __launch_bounds__(kRouteThreads) k_route_bwd16(const RouteBwdArg
 
 // Workgroups of the forward: one wave to four tokens (k_route16) or to one.
 static int route_wgs(int64_t T, int64_t E, int k) {
-    const int per = route16_ok(T, E, k) ? 4 * kRouteWaves : kRouteWaves;
-    const int64_t w = (T + per - 1) / per;
-    return int(w < kRouteMaxWgs ? w : kRouteMaxWgs);
+    return route_wgs_of(T, route16_ok(T, E, k) ? 4 * kRouteWaves : kRouteWaves);
 }
 
 static int fin_groups(int64_t E) { return int((E + kFinExperts - 1) / kFinExperts); }
 static_assert(kRouteMaxE / kFinExperts <= 512, "one thread each in k_route_losses");
 // Workspace: the groups' fp64 sums, then the workgroups' partials.
-static size_t route_bytes(int64_t T, int64_t E) {          // for any top_k
+size_t route_bytes(int64_t T, int64_t E) {          // for any top_k
     return size_t(fin_groups(E)) * 8 + size_t(route_wgs(T, E, kRouteMaxK)) * (size_t(E) * 8 + 8);
+}
+
+void route_parts(void *workspace, int64_t E, int wgs, FinishArgs *f, float **part_p, int32_t **part_c, float **part_z,
+                 int32_t **part_n) {
+    f->dot = static_cast<double *>(workspace);
+    *part_p = reinterpret_cast<float *>(f->dot + fin_groups(E));
+    *part_c = reinterpret_cast<int32_t *>(*part_p + size_t(wgs) * E);
+    *part_z = reinterpret_cast<float *>(*part_c + size_t(wgs) * E);
+    *part_n = reinterpret_cast<int32_t *>(*part_z + wgs);
+    f->part_p = *part_p; f->part_c = *part_c; f->part_z = *part_z; f->part_n = *part_n;
+    f->wgs = wgs;
+    f->E = int32_t(E);
+}
+
+int route_finish(const FinishArgs &f, hipStream_t st) {
+    const int groups = fin_groups(f.E);
+    hipLaunchKernelGGL(k_route_experts, dim3(groups), dim3(1024), 0, st, f);
+    const int rc = hip_status(hipGetLastError(), "router sums launch");
+    if (rc) return rc;
+    hipLaunchKernelGGL(k_route_losses, dim3(1), dim3(512), 0, st, f, groups);
+    return hip_status(hipGetLastError(), "router losses launch");
 }
 
 template <int LT, int NS>
@@ -673,8 +602,7 @@ static int go_route_bwd(const RouteBwdArgs &a, int wgs, hipStream_t st) {
     return hip_status(hipGetLastError(), "router gradient launch");
 }
 
-// Fours of logits can be loaded (and of the gradient stored) at once.
-static bool route_vec(const void *l, int64_t ld, int64_t E, int lt) {
+bool route_vec(const void *l, int64_t ld, int64_t E, int lt) {
     return E % 4 == 0 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(l) & (lt == VQK_F32 ? 15 : 7)) == 0;
 }
 template <int LT, int NS>
@@ -734,7 +662,7 @@ static int route_bwd_ns(const RouteBwdArgs &a, int wgs, hipStream_t st) {
     return go_route_bwd<LT, 32>(a, wgs, st);
 }
 
-static int check_route(int32_t l_type, int64_t T, int64_t E, int64_t ld, int32_t k, const char *what) {
+int check_route(int32_t l_type, int64_t T, int64_t E, int64_t ld, int32_t k, const char *what) {
     if (!act_size(l_type)) return set_error(VQK_EINVAL, "%s: logits type %d", what, l_type);
     if (T < 0 || E < 1 || ld < E) return set_error(VQK_EINVAL, "%s: T=%lld E=%lld ld=%lld", what, (long long)T, (long long)E, (long long)ld);
     if (E > kRouteMaxE) return set_error(VQK_ENOTIMPL, "%s: E=%lld > %d", what, (long long)E, kRouteMaxE);
@@ -771,14 +699,13 @@ extern "C" int vqk_route(const void *logits, int32_t l_type, int64_t T, int64_t 
     a.mask = mask; a.ids = ids; a.wts = wts;
     a.saved = reinterpret_cast<float2 *>(saved);
     if (reinterpret_cast<uintptr_t>(saved) & 7) return set_error(VQK_EINVAL, "route: saved must be 8-byte aligned");
+    FinishArgs f{};
     if (train) {
         const size_t need = route_bytes(T, E);
         if (!workspace || ws_bytes < need) return set_error(VQK_ENOSPACE, "route: workspace %zu < %zu", ws_bytes, need);
         if (reinterpret_cast<uintptr_t>(workspace) & 15) return set_error(VQK_EINVAL, "route: workspace must be 16-byte aligned");
-        a.part_p = reinterpret_cast<float *>(static_cast<double *>(workspace) + fin_groups(E));
-        a.part_c = reinterpret_cast<int32_t *>(a.part_p + size_t(wgs) * E);
-        a.part_z = reinterpret_cast<float *>(a.part_c + size_t(wgs) * E);
-        a.part_n = reinterpret_cast<int32_t *>(a.part_z + wgs);
+        route_parts(workspace, E, wgs, &f, &a.part_p, &a.part_c, &a.part_z, &a.part_n);
+        f.k = top_k; f.counts = counts; f.stats = stats;
     }
     if (wgs) {
         switch (l_type) {
@@ -788,14 +715,7 @@ extern "C" int vqk_route(const void *logits, int32_t l_type, int64_t T, int64_t 
         }
         if (rc) return rc;
     }
-    if (!train) return VQK_OK;
-    const int groups = fin_groups(E);
-    const FinishArgs f{a.part_p, a.part_z, a.part_c, a.part_n, wgs, int32_t(E), top_k,
-                       static_cast<double *>(workspace), counts, stats};
-    hipLaunchKernelGGL(k_route_experts, dim3(groups), dim3(1024), 0, st, f);
-    if ((rc = hip_status(hipGetLastError(), "router sums launch"))) return rc;
-    hipLaunchKernelGGL(k_route_losses, dim3(1), dim3(512), 0, st, f, groups);
-    return hip_status(hipGetLastError(), "router losses launch");
+    return train ? route_finish(f, st) : VQK_OK;
 }
 
 extern "C" int vqk_route_backward(const void *logits, int32_t l_type, int64_t T, int64_t E, int64_t ld,

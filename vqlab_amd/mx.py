@@ -395,16 +395,23 @@ class MXSwitchGLU(torch.nn.Module):
 
 
 class MXSparseMoeBlock(torch.nn.Module):
-    """Softmax top-k routing and MXFP4 experts: forward(x [T, H], logits [T, E], mask [T]) ->
+    """Top-k routing and MXFP4 experts: forward(x [T, H], logits [T, E], mask [T]) ->
     [T, H]; without logits they are x . router_weight^T. mask: 0 marks padding, whose rows are
-    zero and take no expert's time."""
+    zero and take no expert's time. form: keyword arguments of router.top_k beyond its softmax (score,
+    bias, groups, top_groups, group_top, scale); the bias is a buffer."""
+
+    form = {}
 
     def __init__(self, switch_mlp: MXSwitchGLU, top_k: int, norm_topk_prob: bool = True,
-                 router_weight=None):
+                 router_weight=None, **form):
         super().__init__()
         self.switch_mlp, self.top_k = switch_mlp, int(top_k)
         self.norm_topk_prob, self.router_weight = bool(norm_topk_prob), router_weight
         self._sizes = {}
+        if form:
+            router.form(switch_mlp.gate_proj.num_experts, self.top_k, **form)      # a ValueError where it does not fit
+            self.register_buffer("bias", form.pop("bias", None))
+            self.form = form
 
     def forward(self, x, logits=None, mask=None):
         if logits is None:
@@ -417,6 +424,9 @@ class MXSparseMoeBlock(torch.nn.Module):
         if x.ndim != 2 or x.shape[1] != g.input_dims or logits.shape != (x.shape[0], g.num_experts):
             raise ValueError(f"MXSparseMoeBlock: x {tuple(x.shape)}, logits {tuple(logits.shape)} for "
                              f"{g.num_experts} experts of width {g.input_dims}")
+        bias = self._buffers.get("bias")
+        if self.form or bias is not None:
+            return self.switch_mlp(x, *router.top_k(logits, self.top_k, self.norm_topk_prob, mask, bias=bias, **self.form))
         m = router.mask_bytes(mask, logits)
         xt, lib, k = T.act_type(x), L.lib(), self.top_k
         n = x.shape[0]

@@ -8,6 +8,16 @@ is the one of its MoE block (see vqlab_amd.moe).
     z       = mean_t logsumexp(logits_t)^2
 
 Gradients reach the logits from weights, balance and z.
+
+Other forms of the scores (score, bias, groups, top_groups, group_top, scale of top_k and route):
+
+    s = sigmoid(logits) or softmax(logits); c = s + bias
+    group score = sum of the group_top largest c of a group (groups equal runs of experts)
+    ids = top_k(c) in the top_groups best groups; weights = scale * s[ids] (/ their sum)
+    balance goes by p = s / sum(s)
+
+c is compared in 64 bits (without a bias experts are in the order of their logits). The bias steers
+the choice alone and takes no gradient: a buffer that a training loop moves against the counts.
 """
 from __future__ import annotations
 
@@ -55,6 +65,55 @@ def _f32(g):
     return g if g.dtype == torch.float32 and g.is_contiguous() else g.float().contiguous()
 
 
+SCORES = {"softmax": L.VQK_SCORE_SOFTMAX, "sigmoid": L.VQK_SCORE_SIGMOID}
+
+
+class Form(NamedTuple):
+    """How scores are made and chosen among (see the module's head); `plain` is softmax by itself."""
+    score: str = "softmax"
+    bias: torch.Tensor = None
+    groups: int = 1
+    top_groups: int = 1
+    group_top: int = 2
+    scale: float = 1.0
+
+    @property
+    def plain(self):
+        return self.score == "softmax" and self.bias is None and self.top_groups == self.groups and self.scale == 1.0
+
+
+def form(E, k, score="softmax", bias=None, groups=1, top_groups=None, group_top=None, scale=1.0):
+    """A checked Form for E experts, top_groups all of them and group_top 2 (or the group's size) unless
+    given."""
+    if score not in SCORES:
+        raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
+    groups = int(groups)
+    if groups < 1 or E % groups:
+        raise ValueError(f"{groups} groups of {E} experts")
+    top_groups = groups if top_groups is None else int(top_groups)
+    group_top = min(2, E // groups) if group_top is None else int(group_top)
+    if not 1 <= top_groups <= groups:
+        raise ValueError(f"top {top_groups} of {groups} groups")
+    if not 1 <= group_top <= min(2, E // groups):
+        raise ValueError(f"a group's score from {group_top} of {E // groups} experts (1 or 2 are taken)")
+    if k > top_groups * (E // groups):
+        raise ValueError(f"top {k} of {top_groups * (E // groups)} experts in {top_groups} groups")
+    scale = float(scale)
+    if not 0 < scale <= 3.4e38:
+        raise ValueError(f"scale must be a positive number, got {scale}")
+    if bias is not None:
+        if bias.shape != (E,) or bias.dtype not in T.ACT_TYPES:
+            raise ValueError(f"bias must be float16, bfloat16 or float32 [{E}], got {bias.dtype} {tuple(bias.shape)}")
+        bias = bias.detach().float()
+    return Form(score, bias, groups, top_groups, group_top, scale)
+
+
+def _c_form(f, bias):
+    """The form as the library reads it; bias: its contiguous tensor, or None."""
+    return L.VQKRouteForm(SCORES[f.score], f.groups, f.top_groups, f.group_top, f.scale,
+                          None if bias is None else bias.data_ptr())
+
+
 def rows(logits):
     """logits with contiguous rows, and the elements between them."""
     E = logits.shape[1]
@@ -63,13 +122,20 @@ def rows(logits):
     return logits, max(logits.stride(0), E)
 
 
-def top_k(logits, k, norm_topk_prob=True, mask=None):
+def top_k(logits, k, norm_topk_prob=True, mask=None, score="softmax", bias=None, groups=1, top_groups=None,
+          group_top=None, scale=1.0):
     """ids int32 [T, k] and weights fp32 [T, k] of logits [T, E], one launch: the routing of a
-    serving step. mask [T] (bool / uint8): 0 marks padding, whose ids are -1. Logits that want a
-    gradient are refused: that is route's."""
+    serving step. mask [T] (bool / uint8): 0 marks padding, whose ids are -1. score .. scale: see the
+    module's head. Logits that want a gradient are refused: that is route's."""
     k = int(k)
     _check(logits, k, mask)
+    f = form(logits.shape[1], k, score, bias, groups, top_groups, group_top, scale)
+    T.require_cuda(logits, f.bias)
     T.no_grad_here("router.top_k", logits)
+    return _top_k(logits, k, norm_topk_prob, mask, f)
+
+
+def _top_k(logits, k, norm_topk_prob, mask, f):
     with T.on_device(logits):
         lg, ld = rows(logits)
         m = mask_bytes(mask, lg)
@@ -77,9 +143,16 @@ def top_k(logits, k, norm_topk_prob=True, mask=None):
         n, E = lg.shape
         ids = torch.empty((n, k), dtype=torch.int32, device=lg.device)
         w = torch.empty((n, k), dtype=torch.float32, device=lg.device)
-        L.check(L.lib().vqk_route(lg.data_ptr(), T.act_type(lg), n, E, ld, mp, k,
-                                  int(norm_topk_prob), ids.data_ptr(), w.data_ptr(), None, None,
-                                  None, None, 0, T.raw_stream(lg)), "route")
+        if f.plain:
+            rc = L.lib().vqk_route(lg.data_ptr(), T.act_type(lg), n, E, ld, mp, k, int(norm_topk_prob),
+                                   ids.data_ptr(), w.data_ptr(), None, None, None, None, 0, T.raw_stream(lg))
+        else:
+            b = None if f.bias is None else f.bias.contiguous()
+            rc = L.lib().vqk_route_grouped(lg.data_ptr(), T.act_type(lg), n, E, ld, mp,
+                                           ctypes.byref(_c_form(f, b)), k, int(norm_topk_prob), ids.data_ptr(),
+                                           w.data_ptr(), None, None, None, None, 0, T.raw_stream(lg))
+        if rc:
+            L.check(rc, "route")
     return ids, w
 
 
@@ -88,7 +161,7 @@ _sizes = {}                                     # (tokens, experts) -> workspace
 
 class _RouteFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, k, norm, mask):
+    def forward(ctx, logits, k, norm, mask, f):
         with T.on_device(logits):
             lg, ld = rows(logits)
             m = mask_bytes(mask, lg)
@@ -99,7 +172,7 @@ class _RouteFn(torch.autograd.Function):
             w = torch.empty((n, k), dtype=torch.float32, device=dev)
             counts = torch.empty(E, dtype=torch.int32, device=dev)
             stats = torch.empty(3, dtype=torch.float32, device=dev)
-            saved = torch.empty((n, 2), dtype=torch.float32, device=dev)
+            saved = torch.empty((n, 2 if f.plain else 4), dtype=torch.float32, device=dev)
             lib = L.lib()
             size = _sizes.get((n, E))
             if size is None:
@@ -109,15 +182,20 @@ class _RouteFn(torch.autograd.Function):
                     _sizes.clear()
                 size = _sizes[(n, E)] = ws.value
             work = torch.empty(size, dtype=torch.uint8, device=dev)
-            L.check(lib.vqk_route(lg.data_ptr(), T.act_type(lg), n, E, ld, mp, k, norm,
-                                  ids.data_ptr(), w.data_ptr(), counts.data_ptr(),
-                                  stats.data_ptr(), saved.data_ptr(), work.data_ptr(), size,
-                                  T.raw_stream(lg)), "route")
+            out = (ids.data_ptr(), w.data_ptr(), counts.data_ptr(), stats.data_ptr(), saved.data_ptr(),
+                   work.data_ptr(), size, T.raw_stream(lg))
+            if f.plain:
+                L.check(lib.vqk_route(lg.data_ptr(), T.act_type(lg), n, E, ld, mp, k, norm, *out), "route")
+            else:
+                bias = None if f.bias is None else f.bias.contiguous()
+                L.check(lib.vqk_route_grouped(lg.data_ptr(), T.act_type(lg), n, E, ld, mp,
+                                              ctypes.byref(_c_form(f, bias)), k, norm, *out), "route")
         balance, z, tokens = stats.unbind()
         # no views, so that a loss can be scaled in place: the backward pass reads neither
         balance, z = balance.data, z.data
         ctx.save_for_backward(lg, ids, w, counts, stats, saved)
-        ctx.k, ctx.norm, ctx.ld = k, norm, ld
+        ctx.k, ctx.norm, ctx.ld, ctx.form = k, norm, ld, f._replace(bias=None)      # the gradient reads no bias
+        ctx.plain = f.plain
         ctx.mark_non_differentiable(ids, counts, tokens)
         ctx.set_materialize_grads(False)
         return ids, w, counts, balance, z, tokens
@@ -131,19 +209,27 @@ class _RouteFn(torch.autograd.Function):
         with T.on_device(lg):
             d = torch.empty((n, E), dtype=lg.dtype, device=lg.device)
             grads = [None if g is None else _f32(g) for g in (dw, db, dz)]
-            L.check(L.lib().vqk_route_backward(
-                lg.data_ptr(), T.act_type(lg), n, E, ctx.ld, ctx.k, ctx.norm, ids.data_ptr(),
-                w.data_ptr(), counts.data_ptr(), stats.data_ptr(), saved.data_ptr(),
-                *(None if g is None else g.data_ptr() for g in grads), d.data_ptr(),
-                T.raw_stream(lg)), "route backward")
-        return d, None, None, None
+            at = (ctx.k, ctx.norm, ids.data_ptr(), w.data_ptr(), counts.data_ptr(), stats.data_ptr(),
+                  saved.data_ptr(), *(None if g is None else g.data_ptr() for g in grads), d.data_ptr(),
+                  T.raw_stream(lg))
+            if ctx.plain:
+                rc = L.lib().vqk_route_backward(lg.data_ptr(), T.act_type(lg), n, E, ctx.ld, *at)
+            else:
+                rc = L.lib().vqk_route_grouped_backward(lg.data_ptr(), T.act_type(lg), n, E, ctx.ld,
+                                                        ctypes.byref(_c_form(ctx.form, None)), *at)
+            L.check(rc, "route backward")
+        return d, None, None, None, None
 
 
-def route(logits, k, norm_topk_prob=True, mask=None):
+def route(logits, k, norm_topk_prob=True, mask=None, score="softmax", bias=None, groups=1, top_groups=None,
+          group_top=None, scale=1.0):
     """Route of logits [T, E] (fp16, bf16 or fp32), differentiable in the logits. mask [T] (bool /
     uint8): 0 marks padding, which gets ids -1, weights 0 and a zero gradient and enters neither
-    counts nor losses; so does a token whose logits are all -inf. The gradient reads ids, weights,
-    counts and tokens again: copy them before anything changes them in place, a collective among it."""
+    counts nor losses; so does a token whose logits are all -inf. score .. scale: see the module's
+    head. The gradient reads ids, weights, counts and tokens again: copy them before anything changes
+    them in place, a collective among it."""
     k = int(k)
     _check(logits, k, mask)
-    return Route(*_RouteFn.apply(logits, k, int(norm_topk_prob), mask))
+    f = form(logits.shape[1], k, score, bias, groups, top_groups, group_top, scale)
+    T.require_cuda(logits, f.bias)
+    return Route(*_RouteFn.apply(logits, k, int(norm_topk_prob), mask, f))
