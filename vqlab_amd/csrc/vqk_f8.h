@@ -140,7 +140,7 @@ struct F8Call {
     int64_t N;
     bool a8;                                  // 8-bit x on the 8-bit instructions
     F8X x8;                                   // a8: all; otherwise scales (NULL: none) of x's rows
-    MxX x;                                    // otherwise: op, planes (kOpF16, scales: one)
+    MxX x;                                    // otherwise: op, planes (kOpF16, scales: one); f8_tiles: whole blocks
     void *y;
     int32_t y_type;
 };
@@ -148,10 +148,9 @@ struct F8Call {
 // Few rows (vqk_f8s.h): whether it takes a call, and its launch.
 bool f8_rows_ok(const F8Call &c);
 int f8_rows(const F8Call &c, hipStream_t st);
-// Many rows: 16-bit x (vqk_f8g.h), 8-bit x (vqk_f8t.h). part: room for fp32 K slices.
-size_t f8_gemm_part(int64_t N, const F8Geom &g, int P);
-int f8_gemm(const F8Call &c, float *part, size_t part_bytes, hipStream_t st);
-size_t f8_tiles_part(int64_t N, const F8Geom &g);
+// Many rows (vqk_f8t.h). part: room for the K slices of the last tiles, f8_tiles_part
+// bytes (scaled: 16-bit x with scales).
+size_t f8_tiles_part(int64_t N, const F8Geom &g, bool a8, bool scaled, int P);
 int f8_tiles(const F8Call &c, float *part, size_t part_bytes, hipStream_t st);
 
 }  // namespace vqk

@@ -141,7 +141,12 @@ __global__ void __launch_bounds__(256) k_f8_dequant(const F8Dequant p, int64_t p
         const float s = p.scales[(row >> p.shift) * p.so + (k0 >> 7) * p.sk];
         float v[8];
         f8_decode8(c, v);
-        const float a[4] = {v[0] * s, v[1] * s, v[2] * s, v[3] * s}, b[4] = {v[4] * s, v[5] * s, v[6] * s, v[7] * s};
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            v[u] *= s;
+            asm("" : "+v"(v[u]));             // an fp32 number, not one half of a multiplication that rounds to fp16
+        }
+        const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
         const int64_t at = row * p.cols + k0;
         const int n = int(min(int64_t(8), p.cols - k0));
         mx_store4(p.out, YT, at, a, min(n, 4), vout);

@@ -6,7 +6,7 @@
 // as the codes' values in bf16 where it has 32 (vqk_f8.h).
 // bf16 x enters as it is, fp16 x too (every e4m3 code is an fp16 number), fp32 x as
 // three exact bf16 planes. x that is 16-byte aligned and a multiple of 8 wide is
-// read in place, other x is laid out in the workspace first. The gradient sums over
+// read in place (many rows: whole blocks wide), other x is laid out in the workspace first. The gradient sums over
 // the weight's rows, along which its codes do not lie: they are transposed into the
 // workspace, operand order to operand order, and the same products run on them with
 // the strides of the scales exchanged.
@@ -17,16 +17,35 @@ namespace vqk {
 static size_t al256(size_t v) { return (v + 255) & ~size_t(255); }
 static bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// 16-bit rows [N][IN] to rows ld (a multiple of 8) apart, zero past IN.
-__global__ void __launch_bounds__(256) k_f8_stage16(const uint16_t *x, int64_t N, int64_t IN, int64_t ld, uint16_t *out) {
+// Rows [N][IN] to rows of whole blocks, zero past IN: 16-bit numbers as they are, fp32
+// as three planes.
+template <int XT>
+__global__ void __launch_bounds__(256) k_f8_stage16(const void *x, int64_t N, int64_t IN, int64_t ld, uint16_t *out, bool vec) {
     const int64_t per = ld / 8, i = int64_t(blockIdx.x) * 256 + threadIdx.x;
     if (i >= N * per) return;
     const int64_t row = i / per, k0 = (i - row * per) * 8;
-    u32x4 v{};
+    if constexpr (XT == VQK_F32) {
+        float v[8];
+        mx_load8(x, XT, row * IN, k0, IN, vec, v);
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-        if (k0 + u < IN) v[u / 2] |= uint32_t(x[row * IN + k0 + u]) << (16 * (u & 1));
-    *reinterpret_cast<u32x4 *>(out + row * ld + k0) = v;
+        for (int pl = 0; pl < 3; ++pl) {
+            u32x4 o;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint32_t lo = mx_plane_next(v[2 * u]);
+                o[u] = lo | (uint32_t(mx_plane_next(v[2 * u + 1])) << 16);
+            }
+            *reinterpret_cast<u32x4 *>(out + pl * N * ld + row * ld + k0) = o;
+        }
+    } else {
+        const uint16_t *src = static_cast<const uint16_t *>(x) + row * IN + k0;
+        u32x4 v{};
+        if (vec && k0 + 8 <= IN) v = *reinterpret_cast<const u32x4 *>(src);
+        else
+            for (int u = 0; u < 8; ++u)
+                if (k0 + u < IN) v[u / 2] |= uint32_t(src[u]) << (16 * (u & 1));
+        *reinterpret_cast<u32x4 *>(out + row * ld + k0) = v;
+    }
 }
 
 // 8-bit rows to whole blocks, zero past IN, and their scales block by block.
@@ -118,13 +137,10 @@ static int check_lin(const vqk_f8_weights *w, int64_t N, F8Geom *g, const char *
 }
 
 // x as it is: its layout in the workspace (sized as if it had to be laid out).
-static int16_t x_planes(int32_t type) { return type == VQK_F32 ? 3 : 1; }
-static int64_t x_ld(int64_t IN, int32_t type) { return type == VQK_F32 ? (IN + 31) / 32 * 32 : (IN + 7) / 8 * 8; }
-static size_t x_bytes(int64_t N, int64_t IN, int32_t type) {
-    return al256(size_t(N) * x_ld(IN, type) * 2 * x_planes(type));
-}
+static int x_planes(int32_t type) { return type == VQK_F32 ? 3 : 1; }
+static size_t x_bytes(int64_t N, const F8Geom &g, int32_t type) { return al256(size_t(N) * g.NC * 256 * x_planes(type)); }
 static size_t plain_bytes(const F8Geom &g, int32_t type, int64_t N) {
-    return x_bytes(N, g.IN, type) + f8_gemm_part(N, g, x_planes(type));
+    return x_bytes(N, g, type) + f8_tiles_part(N, g, false, false, x_planes(type));
 }
 // 8-bit x: rows of whole blocks and their scales (and for an fp32 output the codes'
 // values after them), then the K slices.
@@ -135,7 +151,7 @@ static size_t rows_bytes(const F8Geom &g, int64_t N, int32_t y_type) {
     return code_bytes(g, N) + scale_bytes(g, N) + (wide_out(y_type) ? al256(size_t(N) * g.NC * 256) : 0);
 }
 static size_t a8_part(const F8Geom &g, int64_t N, int32_t y_type) {
-    return wide_out(y_type) ? f8_gemm_part(N, g, 1) : f8_tiles_part(N, g);
+    return f8_tiles_part(N, g, !wide_out(y_type), true, 1);
 }
 static size_t a8_bytes(const F8Geom &g, int64_t N, int32_t y_type) { return rows_bytes(g, N, y_type) + a8_part(g, N, y_type); }
 
@@ -145,26 +161,30 @@ static int check_ws(const char *what, size_t need, const void *ws, size_t ws_byt
     return VQK_OK;
 }
 
-// The product of x as it is; ws: plain_bytes.
+// The product of x as it is; ws: plain_bytes. Few rows are read in pieces of 8, many in
+// whole blocks.
 static int plain_product(F8Call c, const void *x, int32_t type, uint8_t *ws, hipStream_t st) {
-    const int64_t N = c.N, IN = c.g.IN, ld = x_ld(IN, type);
-    int rc;
-    if (type == VQK_F32) {
-        if ((rc = launch_mx_planes(x, type, N, IN, IN, false, reinterpret_cast<uint16_t *>(ws), st))) return rc;
-        c.x = MxX{reinterpret_cast<uint16_t *>(ws), ld, N * ld, 3, kOpBF16};
-    } else if (IN % 8 == 0 && al16(x)) {
-        c.x = MxX{static_cast<const uint16_t *>(x), IN, 0, 1, type == VQK_F16 ? kOpF16 : kOpBF16};
-    } else {
+    const int64_t N = c.N, IN = c.g.IN, ld = c.g.NC * kF8Block;
+    const int P = x_planes(type);
+    c.x = MxX{static_cast<const uint16_t *>(x), IN, 0, P, type == VQK_F16 ? kOpF16 : kOpBF16};
+    const bool few = f8_rows_ok(c);
+    if (type == VQK_F32 || !al16(x) || IN % (few ? 8 : kF8Block)) {
         const int64_t wgs = (N * (ld / 8) + 255) / 256;
         if (wgs > INT32_MAX) return set_error(VQK_ENOTIMPL, "activations too large");
-        hipLaunchKernelGGL(k_f8_stage16, dim3(unsigned(wgs)), dim3(256), 0, st, static_cast<const uint16_t *>(x), N, IN, ld,
-                           reinterpret_cast<uint16_t *>(ws));
-        if ((rc = hip_status(hipGetLastError(), "x staging launch"))) return rc;
-        c.x = MxX{reinterpret_cast<uint16_t *>(ws), ld, 0, 1, type == VQK_F16 ? kOpF16 : kOpBF16};
+        uint16_t *out = reinterpret_cast<uint16_t *>(ws);
+        const bool vec = al16(x) && (IN * act_size(type)) % 16 == 0;
+        if (type == VQK_F32) hipLaunchKernelGGL((k_f8_stage16<VQK_F32>), dim3(unsigned(wgs)), dim3(256), 0, st, x, N, IN, ld, out, vec);
+        else hipLaunchKernelGGL((k_f8_stage16<VQK_F16>), dim3(unsigned(wgs)), dim3(256), 0, st, x, N, IN, ld, out, vec);   // 16 bits as they are
+        const int rc = hip_status(hipGetLastError(), "x staging launch");
+        if (rc) return rc;
+        c.x.x = out;
+        c.x.ld = ld;
+        c.x.plane = N * ld;
+        c.g.IN = ld;
     }
-    if (f8_rows_ok(c)) return f8_rows(c, st);
-    const size_t part = f8_gemm_part(N, c.g, c.x.P);
-    return f8_gemm(c, part ? reinterpret_cast<float *>(ws + x_bytes(N, IN, type)) : nullptr, part, st);
+    if (few) return f8_rows(c, st);
+    const size_t part = f8_tiles_part(N, c.g, false, false, P);
+    return f8_tiles(c, part ? reinterpret_cast<float *>(ws + x_bytes(N, c.g, type)) : nullptr, part, st);
 }
 
 // The product of 8-bit rows; ws: a8_bytes (x's codes and scales may be at its start).
@@ -193,7 +213,7 @@ static int a8_product(F8Call c, const F8X &x, uint8_t *ws, hipStream_t st) {
     if (f8_rows_ok(c)) return f8_rows(c, st);
     const size_t part = a8_part(c.g, N, c.y_type);
     float *at = part ? reinterpret_cast<float *>(ws + rows_bytes(c.g, N, c.y_type)) : nullptr;
-    return wide ? f8_gemm(c, at, part, st) : f8_tiles(c, at, part, st);
+    return f8_tiles(c, at, part, st);
 }
 
 static F8Call base_call(const vqk_f8_weights *w, const F8Geom &g, int64_t N, bool a8, void *y, int32_t y_type) {

@@ -18,8 +18,7 @@
 // conversions (16-bit), a fraction of the time in which they can arrive.
 #pragma once
 
-#include "vqk_mxs.h"
-#include "vqk_f8.h"
+#include "vqk_f8t.h"
 
 namespace vqk {
 
@@ -41,8 +40,6 @@ struct F8sArgs {
 };
 
 // OP: kOpF16, kOpBF16, or kOpF8 (8-bit x).
-constexpr int kOpF8 = 2;
-
 template <int OP, int NT, int P, int NCW>
 __global__ void __launch_bounds__(64 * kF8sWaves, 2) k_f8_rows(const F8sArgs p) {
     constexpr bool A8 = OP == kOpF8;
