@@ -47,9 +47,14 @@ struct GroupArgs {
     int32_t *part_c, *part_n;
 };
 
-// sigmoid(l) and 1 - sigmoid(l), both to their own last bits.
+// 1 / x for x in [1, 2]: the reciprocal instruction and one step of Newton's.
+__device__ __forceinline__ float rcp12(float x) {
+    const float r = __builtin_amdgcn_rcpf(x);
+    return __builtin_fmaf(__builtin_fmaf(-x, r, 1.f), r, r);
+}
+// sigmoid(l) and 1 - sigmoid(l), both to their own last bits (a NaN stays).
 __device__ __forceinline__ float2 sigmoid2(float l) {
-    const float e = route_exp(-__builtin_fabsf(l)), r = 1.f / (1.f + e);
+    const float e = route_exp(-__builtin_fabsf(l)), r = rcp12(1.f + e);
     return l >= 0.f ? float2{r, e * r} : float2{e * r, r};
 }
 
@@ -164,6 +169,47 @@ __device__ __forceinline__ float group_weight(const GroupArgs &p, int id, float 
 }
 
 // ------------------------------------------------------- a wave to a token
+// Logits of token t, their largest and whether one is NaN; false: the token is not live.
+template <int LT, int NS>
+__device__ __forceinline__ bool wave_token(const GroupArgs &p, int64_t t, int lane, float (&v)[NS], float *m, bool *anynan) {
+    uint32_t best = 0;
+    bool isnan = false;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int e = lane + 64 * i;
+        v[i] = e < p.E ? load_act(p.l, LT, t * p.ld + e) : -__builtin_inff();
+        isnan = isnan || v[i] != v[i];
+        best = max(best, f32_key(v[i]));
+    }
+    best = wave_max_u32(best);
+    *anynan = __ballot(isnan) != 0;
+    *m = key_f32(best);
+    return (!p.mask || p.mask[t] != 0) && (best > kKeyNegInf || *anynan);
+}
+
+// The choice and its weights, written; inv: 1 / sum exp(l - m) where it is known (softmax).
+template <int LT, int NS, bool SIG>
+__device__ __forceinline__ void wave_choose(const GroupArgs &p, int64_t t, int lane, const float (&v)[NS], float m, float inv,
+                                            bool anynan, double *lds, int32_t *cnt) {
+    const int id = choose64<NS, SIG>(p, v, m, lds, lane);
+    const float l = id >= 0 ? load_act(p.l, LT, t * p.ld + id) : 0.f;
+    float w = group_weight<SIG>(p, id, l, m, inv, [](float x) { return wave_sum(x); }, [](float x) { return wave_max(x); });
+    if (anynan) w = __uint_as_float(0x7fc00000u);
+    if (lane < p.k) {
+        p.ids[t * p.k + lane] = id;
+        p.wts[t * p.k + lane] = w;
+        if (cnt && id >= 0) atomicAdd(&cnt[id], 1);
+    }
+}
+
+template <int NS>
+__device__ __forceinline__ float wave_total(const float (&v)[NS], float m) {
+    float total = 0.f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) total += route_exp(v[i] - m);
+    return wave_sum(total);
+}
+
 template <int LT, int NS, bool SIG, bool TRAIN>
 __global__ void __launch_bounds__(kRouteThreads) k_group_wave(const GroupArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -181,19 +227,9 @@ __global__ void __launch_bounds__(kRouteThreads) k_group_wave(const GroupArgs p)
     float zsum = 0.f;
     int live = 0;
     for (int64_t t = int64_t(blockIdx.x) * kRouteWaves + wave; t < p.T; t += int64_t(gridDim.x) * kRouteWaves) {
-        float v[NS];
-        uint32_t best = 0;
-        bool isnan = false;
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const int e = lane + 64 * i;
-            v[i] = e < p.E ? load_act(p.l, LT, t * p.ld + e) : -__builtin_inff();
-            isnan = isnan || v[i] != v[i];
-            best = max(best, f32_key(v[i]));
-        }
-        best = wave_max_u32(best);
-        const bool anynan = __ballot(isnan) != 0;
-        if (!((!p.mask || p.mask[t] != 0) && (best > kKeyNegInf || anynan))) {
+        float v[NS], m;
+        bool anynan;
+        if (!wave_token<LT>(p, t, lane, v, &m, &anynan)) {
             if (lane < p.k) {
                 p.ids[t * p.k + lane] = -1;
                 p.wts[t * p.k + lane] = 0.f;
@@ -201,23 +237,12 @@ __global__ void __launch_bounds__(kRouteThreads) k_group_wave(const GroupArgs p)
             if (p.saved && lane == 0) p.saved[t] = float4{0.f, 0.f, 0.f, 0.f};
             continue;
         }
-        const float m = key_f32(best);
-        const int id = choose64<NS, SIG>(p, v, m, lds, lane);
         float total = 0.f, inv = 0.f, sums = 0.f;
         if constexpr (!SIG || TRAIN) {
-#pragma unroll
-            for (int i = 0; i < NS; ++i) total += route_exp(v[i] - m);
-            total = wave_sum(total);
+            total = wave_total(v, m);
             inv = 1.f / total;
         }
-        const float l = id >= 0 ? load_act(p.l, LT, t * p.ld + id) : 0.f;
-        float w = group_weight<SIG>(p, id, l, m, inv, [](float x) { return wave_sum(x); }, [](float x) { return wave_max(x); });
-        if (anynan) w = __uint_as_float(0x7fc00000u);
-        if (lane < p.k) {
-            p.ids[t * p.k + lane] = id;
-            p.wts[t * p.k + lane] = w;
-            if (TRAIN && id >= 0) atomicAdd(&cnt[id], 1);
-        }
+        wave_choose<LT, NS, SIG>(p, t, lane, v, m, inv, anynan, lds, TRAIN ? cnt : nullptr);
         if constexpr (TRAIN) {
             const float lse = m + logf(total);
             zsum += lse * lse;
@@ -312,10 +337,13 @@ __device__ __forceinline__ void group16_load(const GroupArgs &p, int64_t t, int 
 // The top k as in k_route16: the k-th largest lane maximum bounds them from below,
 // what reaches it is collected in LDS and ranked, two candidates a lane. One more than
 // top_k is looked at: the best that is left out.
+constexpr int kSecondLook = -2;                // ids[t][0] of a token that choose64 is to choose for
+
 template <int LT, int NS, bool SIG, bool TRAIN>
 __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bool vec) {
     extern __shared__ __align__(16) uint8_t smem[];
-    float *csh = reinterpret_cast<float *>(smem) + (threadIdx.x >> 6) * 4 * p.E;     // [waves][4][E]; choose64: [waves][E] doubles
+    // [waves]: four tokens' scores, as floats or the two largest of every four; choose64: E doubles
+    float *csh = reinterpret_cast<float *>(smem) + (threadIdx.x >> 6) * 4 * p.E;
     int32_t *cnt = reinterpret_cast<int32_t *>(smem + kRouteWaves * 16 * size_t(p.E));   // TRAIN: [E], [E]
     float *psh = reinterpret_cast<float *>(cnt + p.E);
     __shared__ uint64_t cands[kRouteWaves][4][kRouteCands];
@@ -339,43 +367,41 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
         bias[i] = p.bias && e < p.E ? p.bias[e] : 0.f;
         gid[i / 4] |= uint32_t(e < p.E ? e / p.gs : 0) << (8 * (i % 4));
     }
+    const bool fours = p.gs % 4 == 0;
     float psum[NS] = {};
     float zsum = 0.f;
     int nlive = 0;
-    const int64_t stride = int64_t(gridDim.x) * kRouteWaves * 4;
-    for (int64_t t0 = (int64_t(blockIdx.x) * kRouteWaves + wave) * 4; t0 < p.T; t0 += stride) {
+    const int64_t t00 = (int64_t(blockIdx.x) * kRouteWaves + wave) * 4, stride = int64_t(gridDim.x) * kRouteWaves * 4;
+    for (int64_t t0 = t00; t0 < p.T; t0 += stride) {
         const int64_t t = t0 + grp;
         const bool in = t < p.T && (!p.mask || p.mask[t] != 0);
         float v[NS], c[NS];
         group16_load<LT, NS>(p, t, sub, in, vec, v);
-        uint32_t best = 0;
+        float best = -__builtin_inff();
         bool isnan = false;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             isnan = isnan || v[i] != v[i];
-            best = max(best, f32_key(v[i]));
+            best = fmaxf(best, v[i]);         // of a NaN and a number the number
         }
-        best = row_max(best);
+        best = key_f32(row_max(f32_key(best)));
         const bool anynan = ((__ballot(isnan) >> (grp * 16)) & 0xffffu) != 0;
-        const bool live = in && (best > kKeyNegInf || anynan);
-        const float m = live && best > kKeyNegInf ? key_f32(best) : 0.f;
+        const bool live = in && (best > -__builtin_inff() || anynan);
+        const float m = best > -__builtin_inff() ? best : 0.f;
+        const bool far = !SIG || m < kFarLogit;             // p: a softmax
         float total = 0.f, inv = 0.f, sums = 0.f;
+        float q[TRAIN ? NS : 1];                            // p before its sum
         if constexpr (!SIG || TRAIN) {
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                c[i] = live && v[i] == v[i] ? route_exp(v[i] - m) : 0.f;
+                c[i] = v[i] == v[i] ? route_exp(v[i] - m) : 0.f;
                 total += c[i];
+                if constexpr (TRAIN) q[i] = c[i];
             }
             total = row_sum(total);
             inv = live ? 1.f / total : 0.f;
         }
         const float smax = SIG ? sigmoid2(m).x : inv;
-        const bool far = !SIG || m < kFarLogit;             // p: a softmax
-        float q[TRAIN ? NS : 1];                            // p before its sum
-        if constexpr (TRAIN) {
-#pragma unroll
-            for (int i = 0; i < NS; ++i) q[i] = c[i];
-        }
         if constexpr (SIG) {
             float s = 0.f;
 #pragma unroll
@@ -383,7 +409,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
                 c[i] = sigmoid2(v[i]).x;
                 if constexpr (TRAIN) {
                     s += c[i];
-                    if (!far) q[i] = c[i];
+                    q[i] = far ? q[i] : c[i];
                 }
             }
             if constexpr (TRAIN) sums = live && !far ? 1.f / row_sum(s) : 0.f;
@@ -392,6 +418,18 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
             for (int i = 0; i < NS; ++i) c[i] *= inv;
         }
         if (anynan) total = inv = sums = __uint_as_float(live ? 0x7fc00000u : 0u);
+        if constexpr (TRAIN) {
+            if (live) {
+                const float lse = m + logf(total);
+                if (sub == 0) {
+                    zsum += lse * lse;
+                    ++nlive;
+                }
+                const float f = far ? inv : sums;
+#pragma unroll
+                for (int i = 0; i < NS; ++i) psum[i] = __builtin_fmaf(q[TRAIN ? i : 0], f, psum[i]);
+            }
+        }
         uint32_t key[NS], lm = 0;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
@@ -402,22 +440,44 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
         }
         bool amb = false;                                   // fp32 does not say which is larger
         if (p.G > 1) {
-            wave_lds_sync();                                // the last tokens' scores are read
-            float *mine = csh + grp * p.E;
-#pragma unroll
-            for (int i = 0; i < NS; ++i) {
-                const int e = group16_expert(i, sub);
-                if (e < p.E) mine[e] = c[i];
-            }
-            wave_lds_sync();
             float a = -__builtin_inff(), b = a;             // the group's two largest
-            if (sub < p.G) {
-                int at = sub % p.gs;                        // lanes start at banks of their own
-                for (int j = 0; j < p.gs; ++j) {
-                    const float x = mine[sub * p.gs + at];
-                    at = at + 1 == p.gs ? 0 : at + 1;
-                    b = fmaxf(b, fminf(a, x));
-                    a = fmaxf(a, x);
+            wave_lds_sync();                                // the last tokens' scores are read
+            if (fours) {
+                float2 *mine = reinterpret_cast<float2 *>(csh) + grp * (p.E / 4);
+#pragma unroll
+                for (int w = 0; w < NS / 4; ++w) {
+                    const float hi0 = fmaxf(c[4 * w], c[4 * w + 1]), lo0 = fminf(c[4 * w], c[4 * w + 1]);
+                    const float hi1 = fmaxf(c[4 * w + 2], c[4 * w + 3]), lo1 = fminf(c[4 * w + 2], c[4 * w + 3]);
+                    const int e = group16_expert(4 * w, sub);
+                    if (e < p.E) mine[e / 4] = float2{fmaxf(hi0, hi1), fmaxf(fminf(hi0, hi1), fmaxf(lo0, lo1))};
+                }
+                wave_lds_sync();
+                if (sub < p.G) {
+                    const int n = p.gs / 4;
+                    int at = sub % n;                       // lanes start at banks of their own
+                    for (int j = 0; j < n; ++j) {
+                        const float2 x = mine[sub * n + at];
+                        at = at + 1 == n ? 0 : at + 1;
+                        b = fmaxf(fmaxf(b, x.y), fminf(a, x.x));
+                        a = fmaxf(a, x.x);
+                    }
+                }
+            } else {
+                float *mine = csh + grp * p.E;
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    const int e = group16_expert(i, sub);
+                    if (e < p.E) mine[e] = c[i];
+                }
+                wave_lds_sync();
+                if (sub < p.G) {
+                    int at = sub % p.gs;
+                    for (int j = 0; j < p.gs; ++j) {
+                        const float x = mine[sub * p.gs + at];
+                        at = at + 1 == p.gs ? 0 : at + 1;
+                        b = fmaxf(b, fminf(a, x));
+                        a = fmaxf(a, x);
+                    }
                 }
             }
             const float g = p.group_top == 2 && b > -__builtin_inff() ? a + b : a;
@@ -426,7 +486,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
 #define VQK_ROR(N)                                                                    \
     {                                                                                 \
         const uint32_t o = dpp_u<0x120 + N>(gk);                                      \
-        const int from = int(dpp_u<0x120 + N>(uint32_t(sub)));                        \
+        const int from = (sub - N) & 15;                                              \
         rank += from < p.G && (o > gk || (o == gk && from < sub));                    \
     }
             VQK_ROR(1) VQK_ROR(2) VQK_ROR(3) VQK_ROR(4) VQK_ROR(5) VQK_ROR(6) VQK_ROR(7) VQK_ROR(8)
@@ -453,90 +513,73 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
         VQK_ROR(9) VQK_ROR(10) VQK_ROR(11) VQK_ROR(12) VQK_ROR(13) VQK_ROR(14) VQK_ROR(15)
 #undef VQK_ROR
         const uint32_t thr = max(row_min(rank < want ? lm : 0xffffffffu), kKeyNegInf + 1);
-        int run = 0;
+        int mine = 0;                                       // this lane's candidates, and those of the lanes before
+#pragma unroll
+        for (int i = 0; i < NS; ++i) mine += key[i] >= thr;
+        int upto = mine;
+        upto += int(__builtin_amdgcn_update_dpp(0, upto, 0x111, 0xf, 0xf, true));           // row_shr:1, zeros in
+        upto += int(__builtin_amdgcn_update_dpp(0, upto, 0x112, 0xf, 0xf, true));
+        upto += int(__builtin_amdgcn_update_dpp(0, upto, 0x114, 0xf, 0xf, true));
+        upto += int(__builtin_amdgcn_update_dpp(0, upto, 0x118, 0xf, 0xf, true));
+        const int run = int(row_max(uint32_t(upto)));
+        int pos = upto - mine;
         wave_lds_sync();                                    // the last token's candidates are read
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const bool in_ = key[i] >= thr;
-            const uint32_t gm = uint32_t(__ballot(in_) >> (grp * 16)) & 0xffffu;
-            const int pos = run + __popc(gm & ((1u << sub) - 1u));
-            if (in_ && pos < kRouteCands)
-                cands[wave][grp][pos] = (uint64_t(key[i]) << 32) | uint32_t(~group16_expert(i, sub));
-            run += __popc(gm);
-        }
+        for (int i = 0; i < NS; ++i)
+            if (key[i] >= thr) {
+                if (pos < kRouteCands) cands[wave][grp][pos] = (uint64_t(key[i]) << 32) | uint32_t(~group16_expert(i, sub));
+                ++pos;
+            }
         if (sub <= p.k) sel[wave][grp][sub] = 0;
         wave_lds_sync();
-        uint64_t c0 = 0, c1 = 0;
-        if (sub < run) c0 = cands[wave][grp][sub];
-        if (sub + 16 < run) c1 = cands[wave][grp][sub + 16];
-        int r0 = c1 > c0, r1 = c0 > c1;
+        const uint64_t c0 = sub < run ? cands[wave][grp][sub] : 0;
+        int r0 = 0;
+        if (__ballot(run > 16) == 0) {
+#define VQK_ROR(N) r0 += dpp_u64<0x120 + N>(c0) > c0;
+            VQK_ROR(1) VQK_ROR(2) VQK_ROR(3) VQK_ROR(4) VQK_ROR(5) VQK_ROR(6) VQK_ROR(7) VQK_ROR(8)
+            VQK_ROR(9) VQK_ROR(10) VQK_ROR(11) VQK_ROR(12) VQK_ROR(13) VQK_ROR(14) VQK_ROR(15)
+#undef VQK_ROR
+        } else {
+            const uint64_t c1 = sub + 16 < run && sub + 16 < kRouteCands ? cands[wave][grp][sub + 16] : 0;
+            r0 = c1 > c0;
+            int r1 = c0 > c1;
 #define VQK_ROR(N)                                                                              \
     {                                                                                           \
         const uint64_t a = dpp_u64<0x120 + N>(c0), b = dpp_u64<0x120 + N>(c1);                  \
         r0 += int(a > c0) + int(b > c0);                                                        \
         r1 += int(a > c1) + int(b > c1);                                                        \
     }
-        VQK_ROR(1) VQK_ROR(2) VQK_ROR(3) VQK_ROR(4) VQK_ROR(5) VQK_ROR(6) VQK_ROR(7) VQK_ROR(8)
-        VQK_ROR(9) VQK_ROR(10) VQK_ROR(11) VQK_ROR(12) VQK_ROR(13) VQK_ROR(14) VQK_ROR(15)
+            VQK_ROR(1) VQK_ROR(2) VQK_ROR(3) VQK_ROR(4) VQK_ROR(5) VQK_ROR(6) VQK_ROR(7) VQK_ROR(8)
+            VQK_ROR(9) VQK_ROR(10) VQK_ROR(11) VQK_ROR(12) VQK_ROR(13) VQK_ROR(14) VQK_ROR(15)
 #undef VQK_ROR
+            if (c1 != 0 && r1 <= p.k) sel[wave][grp][r1] = c1;
+        }
         if (c0 != 0 && r0 <= p.k) sel[wave][grp][r0] = c0;
-        if (c1 != 0 && r1 <= p.k) sel[wave][grp][r1] = c1;
         wave_lds_sync();
-        const uint64_t mine = sub < p.k ? sel[wave][grp][sub] : 0, next = sub < p.k ? sel[wave][grp][sub + 1] : 0;
-        int id = mine ? int(~uint32_t(mine)) : -1;
-        float l = id >= 0 ? load_act(p.l, LT, t * p.ld + id) : 0.f;
+        const uint64_t got = sub < p.k ? sel[wave][grp][sub] : 0, next = sub < p.k ? sel[wave][grp][sub + 1] : 0;
+        const int id = got ? int(~uint32_t(got)) : -1;
+        const float l = id >= 0 ? load_act(p.l, LT, t * p.ld + id) : 0.f;
         if (p.bias) {
             bool near = false;
             if (next) {
                 // equal logits under equal biases are a tie, and the lower id comes first already
                 const int e = int(~uint32_t(next));
-                const float x = key_f32(uint32_t(mine >> 32)), y = key_f32(uint32_t(next >> 32));
+                const float x = key_f32(uint32_t(got >> 32)), y = key_f32(uint32_t(next >> 32));
                 near = !(x - y > 2.f * group_tol<SIG>(smax, x)) &&
                        !(l == load_act(p.l, LT, t * p.ld + e) && p.bias[id] == p.bias[e]);
             }
             amb = amb || ((__ballot(near) >> (grp * 16)) & 0xffffu) != 0;
         }
         amb = live && (amb || run > kRouteCands);
-        const uint64_t again = __ballot(amb);
-        if (again) {
-            for (int g = 0; g < 4; ++g) {
-                if (!((again >> (16 * g)) & 1)) continue;
-                const int64_t tt = t0 + g;
-                float vv[(NS + 3) / 4];
-#pragma unroll
-                for (int i = 0; i < (NS + 3) / 4; ++i) {
-                    const int e = lane + 64 * i;
-                    vv[i] = e < p.E ? load_act(p.l, LT, tt * p.ld + e) : -__builtin_inff();
-                }
-                const float mm = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m), 16 * g));
-                wave_lds_sync();                            // the scores are read
-                const int got = choose64<(NS + 3) / 4, SIG>(p, vv, mm, reinterpret_cast<double *>(csh), lane);
-                const int at = __shfl(got, sub);
-                if (grp == g) id = sub < p.k ? at : -1;
-            }
-            l = id >= 0 ? load_act(p.l, LT, t * p.ld + id) : 0.f;
-        }
         float w = group_weight<SIG>(p, id, l, m, inv, [](float x) { return row_sum(x); },
                                     [](float x) { return key_f32(row_max(f32_key(x))); });
         if (anynan && live) w = __uint_as_float(0x7fc00000u);
         if (t < p.T && sub < p.k) {
-            p.ids[t * p.k + sub] = id;
+            p.ids[t * p.k + sub] = amb ? kSecondLook : id;
             p.wts[t * p.k + sub] = w;
-            if (TRAIN && id >= 0) atomicAdd(&cnt[id], 1);
+            if (TRAIN && id >= 0 && !amb) atomicAdd(&cnt[id], 1);
         }
         if (p.saved && t < p.T && sub == 0) p.saved[t] = live ? float4{m, inv, sums, 0.f} : float4{0.f, 0.f, 0.f, 0.f};
-        if constexpr (TRAIN) {
-            if (live) {
-                const float lse = m + logf(total);
-                if (sub == 0) {
-                    zsum += lse * lse;
-                    ++nlive;
-                }
-                const float f = far ? inv : sums;
-#pragma unroll
-                for (int i = 0; i < NS; ++i) psum[i] += q[TRAIN ? i : 0] * f;
-            }
-        }
     }
     if constexpr (TRAIN) {
         for (int w = 0; w < kRouteWaves * 4; ++w) {         // the tokens' sums in order of wave and row of lanes
@@ -550,6 +593,22 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
             if (w % 4 == 3) __syncthreads();
             else wave_lds_sync();
         }
+    }
+    // the second look, at this wave's own tokens
+    __syncthreads();
+    for (int64_t t0 = t00; t0 < p.T; t0 += stride) {
+        const uint64_t again = __ballot(sub == 0 && t0 + grp < p.T && p.ids[(t0 + grp) * p.k] == kSecondLook);
+        for (int g = 0; g < 4; ++g) {
+            if (!((again >> (16 * g)) & 1)) continue;
+            float v[(NS + 3) / 4], m;
+            bool anynan;
+            wave_token<LT>(p, t0 + g, lane, v, &m, &anynan);
+            wave_lds_sync();
+            wave_choose<LT, (NS + 3) / 4, SIG>(p, t0 + g, lane, v, m, SIG ? 0.f : 1.f / wave_total(v, m), anynan,
+                                               reinterpret_cast<double *>(csh), TRAIN ? cnt : nullptr);
+        }
+    }
+    if constexpr (TRAIN) {
         zsum = wave_sum(zsum);
         for (int o = 16; o < 64; o <<= 1) nlive += __shfl_xor(nlive, o);
         if (lane == 0) {
