@@ -57,6 +57,15 @@ __device__ __forceinline__ float2 sigmoid2(float l) {
     const float e = route_exp(-__builtin_fabsf(l)), r = rcp12(1.f + e);
     return l >= 0.f ? float2{r, e * r} : float2{e * r, r};
 }
+// The same exponential and sigmoid without a branch and with 0 for a NaN.
+__device__ __forceinline__ float exp0(float d) { return route_exp_in(__builtin_fmaxf(d, -200.f)); }
+__device__ __forceinline__ float sigmoid0(float l) {
+    const float e = exp0(-__builtin_fabsf(l));
+    return (l >= 0.f ? 1.f : e) * rcp12(1.f + e);
+}
+__device__ __forceinline__ float pick(uint32_t mask, float a, float b) {        // bits of a where mask has them, of b elsewhere
+    return __uint_as_float((mask & __float_as_uint(a)) | (~mask & __float_as_uint(b)));
+}
 
 __device__ __forceinline__ uint64_t f64_key(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.);               // -0 as 0
@@ -64,23 +73,32 @@ __device__ __forceinline__ uint64_t f64_key(double v) {
 }
 constexpr uint64_t kKey64NegInf = 0x000fffffffffffffull;                   // f64_key(-inf)
 
-__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
-    const uint32_t hi = wave_max_u32(uint32_t(v >> 32));
-    const uint32_t lo = wave_max_u32(uint32_t(v >> 32) == hi ? uint32_t(v) : 0u);
-    return (uint64_t(hi) << 32) | lo;
-}
-
 __device__ __forceinline__ double shfl_f64(double v, int from) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     const uint32_t lo = __shfl(uint32_t(b), from), hi = __shfl(uint32_t(b >> 32), from);
     return __builtin_bit_cast(double, (uint64_t(hi) << 32) | lo);
 }
+// From a lane that the whole wave agrees on.
+__device__ __forceinline__ uint32_t lane_u32(uint32_t v, int from) { return uint32_t(__builtin_amdgcn_readlane(int(v), from)); }
+__device__ __forceinline__ double lane_f64(double v, int from) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t(lane_u32(uint32_t(b >> 32), from)) << 32) | lane_u32(uint32_t(b), from));
+}
+
+// The experts' biases as choose64 takes them.
+template <int NS>
+__device__ __forceinline__ void wave_bias(const GroupArgs &p, int lane, float (&bias)[NS]) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) bias[i] = p.bias && lane + 64 * i < p.E ? p.bias[lane + 64 * i] : 0.f;
+}
 
 // The choice for one token by a whole wave: lane holds logits v[i] of experts lane +
-// 64 i (-inf past E), m their largest; lds: E doubles. Returns the lane's choice (lane j
-// the j-th), -1 for none.
+// 64 i (-inf past E) and their biases, m is the largest; lds: E doubles. Returns the
+// lane's choice (lane j the j-th), -1 for none, and its logit. 64 tokens are a matter of
+// latency: the lanes share out the groups' experts, and of the wave's reductions only
+// the high word's is made unless two lanes hold the same.
 template <int NS, bool SIG>
-__device__ int choose64(const GroupArgs &p, const float (&v)[NS], float m, double *lds, int lane) {
+__device__ int choose64(const GroupArgs &p, const float (&v)[NS], const float (&bias)[NS], float m, double *lds, int lane, float *l) {
     double s[NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) s[i] = 0.;
@@ -97,9 +115,8 @@ __device__ int choose64(const GroupArgs &p, const float (&v)[NS], float m, doubl
         }
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            const int e = lane + 64 * i;
             s[i] = SIG ? 1. / (1. + exp(-double(v[i]))) : s[i] / total;
-            if (p.bias && e < p.E) s[i] += double(p.bias[e]);
+            if (p.bias) s[i] += double(bias[i]);
         }
     }
     uint64_t key[NS];
@@ -111,26 +128,35 @@ __device__ int choose64(const GroupArgs &p, const float (&v)[NS], float m, doubl
         if (p.G > 1 && lane + 64 * i < p.E) lds[lane + 64 * i] = can ? s[i] : -__builtin_inf();
     }
     if (p.G > 1) {
+        const int lg = 31 - __builtin_clz(64 / p.G);        // 2^lg lanes to a group
+        const int mine = lane >> lg, part = lane & ((1 << lg) - 1);
         wave_lds_sync();
         double a = -__builtin_inf(), b = a;   // the group's two largest
-        if (lane < p.G)
-            for (int j = 0; j < p.gs; ++j) {
-                const double c = lds[lane * p.gs + j];
+        if (mine < p.G)
+            for (int j = part; j < p.gs; j += 1 << lg) {
+                const double c = lds[mine * p.gs + j];
                 b = c > a ? a : (c > b ? c : b);
                 a = c > a ? c : a;
             }
-        const double mine = p.group_top == 2 && b > -__builtin_inf() ? a + b : a;
+        for (int o = 1; o < 1 << lg; o <<= 1) {
+            const double a2 = shfl_f64(a, lane ^ o), b2 = shfl_f64(b, lane ^ o);
+            const double lo = a2 > a ? a : a2;
+            b = b2 > b ? b2 : b;
+            b = lo > b ? lo : b;
+            a = a2 > a ? a2 : a;
+        }
+        const double sum = p.group_top == 2 && b > -__builtin_inf() ? a + b : a;
         int rank = 0;
         for (int j = 0; j < p.G; ++j) {
-            const double o = shfl_f64(mine, j);
-            rank += o > mine || (o == mine && j < lane);
+            const double o = lane_f64(sum, j << lg);
+            rank += o > sum || (o == sum && j < mine);
         }
-        const uint64_t kept = __ballot(lane < p.G && rank < p.top_groups);
+        const uint64_t kept = __ballot(mine < p.G && rank < p.top_groups);
         wave_lds_sync();
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const int e = lane + 64 * i;
-            if (e >= p.E || !((kept >> (e / p.gs)) & 1)) key[i] = 0;
+            if (e >= p.E || !((kept >> ((e / p.gs) << lg)) & 1)) key[i] = 0;
         }
     }
     int id = -1;
@@ -143,13 +169,29 @@ __device__ int choose64(const GroupArgs &p, const float (&v)[NS], float m, doubl
                 mine = key[i];
                 at = i;
             }
-        const uint64_t top = wave_max_u64(mine);
-        if (top <= kKey64NegInf) break;
-        const int e = int(wave_min_u32(mine == top ? uint32_t(lane + 64 * at) : 0xffffffffu));
+        const uint32_t top = wave_max_u32(uint32_t(mine >> 32));
+        uint64_t who = __ballot(uint32_t(mine >> 32) == top);
+        if (who & (who - 1)) {                // more than one: by the low word, then by the id
+            const bool first = uint32_t(mine >> 32) == top;
+            const uint32_t low = wave_max_u32(first ? uint32_t(mine) : 0u);
+            const bool both = first && uint32_t(mine) == low;
+            const int e = int(wave_min_u32(both ? uint32_t(lane + 64 * at) : 0xffffffffu));
+            who = __ballot(both && lane + 64 * at == e);
+        }
+        const int from = __builtin_ctzll(who);
+        const uint64_t best = (uint64_t(top) << 32) | lane_u32(uint32_t(mine), from);
+        if (best <= kKey64NegInf) break;
+        const int e = from + 64 * int(lane_u32(uint32_t(at), from));
+        float le = 0.f;
 #pragma unroll
-        for (int i = 0; i < NS; ++i)
+        for (int i = 0; i < NS; ++i) {
+            if (e >> 6 == i) le = __uint_as_float(lane_u32(__float_as_uint(v[i]), from));
             if (lane + 64 * i == e) key[i] = 0;
-        if (lane == j) id = e;
+        }
+        if (lane == j) {
+            id = e;
+            *l = le;
+        }
     }
     return id;
 }
@@ -188,11 +230,11 @@ __device__ __forceinline__ bool wave_token(const GroupArgs &p, int64_t t, int la
 }
 
 // The choice and its weights, written; inv: 1 / sum exp(l - m) where it is known (softmax).
-template <int LT, int NS, bool SIG>
+template <int NS, bool SIG>
 __device__ __forceinline__ void wave_choose(const GroupArgs &p, int64_t t, int lane, const float (&v)[NS], float m, float inv,
-                                            bool anynan, double *lds, int32_t *cnt) {
-    const int id = choose64<NS, SIG>(p, v, m, lds, lane);
-    const float l = id >= 0 ? load_act(p.l, LT, t * p.ld + id) : 0.f;
+                                            bool anynan, const float (&bias)[NS], double *lds, int32_t *cnt) {
+    float l = 0.f;
+    const int id = choose64<NS, SIG>(p, v, bias, m, lds, lane, &l);
     float w = group_weight<SIG>(p, id, l, m, inv, [](float x) { return wave_sum(x); }, [](float x) { return wave_max(x); });
     if (anynan) w = __uint_as_float(0x7fc00000u);
     if (lane < p.k) {
@@ -223,7 +265,8 @@ __global__ void __launch_bounds__(kRouteThreads) k_group_wave(const GroupArgs p)
         for (int e = threadIdx.x; e < p.E; e += kRouteThreads) cnt[e] = 0;
         __syncthreads();
     }
-    float psum[NS] = {};
+    float bias[NS], psum[NS] = {};
+    wave_bias(p, lane, bias);
     float zsum = 0.f;
     int live = 0;
     for (int64_t t = int64_t(blockIdx.x) * kRouteWaves + wave; t < p.T; t += int64_t(gridDim.x) * kRouteWaves) {
@@ -242,7 +285,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_group_wave(const GroupArgs p)
             total = wave_total(v, m);
             inv = 1.f / total;
         }
-        wave_choose<LT, NS, SIG>(p, t, lane, v, m, inv, anynan, lds, TRAIN ? cnt : nullptr);
+        wave_choose<NS, SIG>(p, t, lane, v, m, inv, anynan, bias, lds, TRAIN ? cnt : nullptr);
         if constexpr (TRAIN) {
             const float lse = m + logf(total);
             zsum += lse * lse;
@@ -305,32 +348,39 @@ __device__ __forceinline__ float group_tol(float smax, float c) {
 // whole lines a load, and the lanes of a group shift from one 64 to the next, so that
 // the experts of few groups are not all in the same lanes.
 __device__ __forceinline__ int group16_expert(int i, int sub) { return 64 * (i / 4) + 4 * ((sub + i / 4 * 4) & 15) + i % 4; }
+// All loads are issued before the first is used: an address past the row or of a token
+// that is not `in` is replaced by the row's, or the first token's, own start.
 template <int LT, int NS>
-__device__ __forceinline__ void group16_load(const GroupArgs &p, int64_t t, int sub, bool in, bool vec, float (&v)[NS]) {
+__device__ __forceinline__ void group16_load(const GroupArgs &p, int64_t t, int sub, int E, bool in, bool vec, float (&v)[NS]) {
+    using T = std::conditional_t<LT == VQK_F32, float, uint16_t>;
+    const T *row = static_cast<const T *>(p.l) + (in ? t * p.ld : 0);
+    if (vec) {
+        using Four = std::conditional_t<LT == VQK_F32, u32x4, u32x2>;
+        Four f[NS / 4];
 #pragma unroll
-    for (int q = 0; q < NS / 4; ++q) {
-        const int e = group16_expert(4 * q, sub);
-        if (vec) {
-            u32x4 f{};
-            const bool ok = in && e < p.E;
-            if constexpr (LT == VQK_F32) {
-                if (ok) f = *reinterpret_cast<const u32x4 *>(static_cast<const float *>(p.l) + t * p.ld + e);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[4 * q + j] = ok ? __uint_as_float(f[j]) : -__builtin_inff();
-            } else {
-                u32x2 h{};
-                if (ok) h = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(p.l) + t * p.ld + e);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint16_t b = uint16_t(h[j / 2] >> (16 * (j & 1)));
-                    v[4 * q + j] = !ok ? -__builtin_inff() : (LT == VQK_BF16 ? bf16_to_f32(b) : h_to_f32(b));
-                }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                v[4 * q + j] = in && e + j < p.E ? load_act(p.l, LT, t * p.ld + e + j) : -__builtin_inff();
+        for (int q = 0; q < NS / 4; ++q) {
+            const int e = group16_expert(4 * q, sub);
+            f[q] = *reinterpret_cast<const Four *>(row + (e < E ? e : 0));
         }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const Four w = f[i / 4];
+            if constexpr (LT == VQK_F32) {
+                v[i] = __uint_as_float(w[i % 4]);
+            } else {
+                const uint16_t h = uint16_t(w[i % 4 / 2] >> (16 * (i & 1)));
+                v[i] = LT == VQK_BF16 ? bf16_to_f32(h) : h_to_f32(h);
+            }
+            v[i] = in && group16_expert(i / 4 * 4, sub) < E ? v[i] : -__builtin_inff();
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int e = group16_expert(i, sub);
+            v[i] = load_act(row, LT, e < E ? e : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) v[i] = in && group16_expert(i, sub) < E ? v[i] : -__builtin_inff();
     }
 }
 
@@ -340,33 +390,35 @@ __device__ __forceinline__ void group16_load(const GroupArgs &p, int64_t t, int 
 constexpr int kSecondLook = -2;                // ids[t][0] of a token that choose64 is to choose for
 
 template <int LT, int NS, bool SIG, bool TRAIN>
-__global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bool vec) {
+__global__ void __launch_bounds__(kRouteThreads, NS <= 16 ? 3 : 1) k_group16(const GroupArgs p, bool vec) {
     extern __shared__ __align__(16) uint8_t smem[];
     // [waves]: four tokens' scores, as floats or the two largest of every four; choose64: E doubles
-    float *csh = reinterpret_cast<float *>(smem) + (threadIdx.x >> 6) * 4 * p.E;
-    int32_t *cnt = reinterpret_cast<int32_t *>(smem + kRouteWaves * 16 * size_t(p.E));   // TRAIN: [E], [E]
-    float *psh = reinterpret_cast<float *>(cnt + p.E);
+    float *csh = reinterpret_cast<float *>(smem) + (threadIdx.x >> 6) * 64 * NS;
+    int32_t *cnt = reinterpret_cast<int32_t *>(smem + kRouteWaves * 256 * NS);           // TRAIN: [16 NS], [16 NS]
+    float *psh = reinterpret_cast<float *>(cnt + 16 * NS);
     __shared__ uint64_t cands[kRouteWaves][4][kRouteCands];
     __shared__ uint64_t sel[kRouteWaves][4][kGroup16MaxK + 1];
     __shared__ float zsh[kRouteWaves];
     __shared__ int nsh[kRouteWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int sub = lane & 15, grp = lane >> 4;
+    const int sub0 = lane & 15, grp = lane >> 4;
     if constexpr (TRAIN) {
-        for (int e = threadIdx.x; e < p.E; e += kRouteThreads) {
+        for (int e = threadIdx.x; e < 16 * NS; e += kRouteThreads) {
             cnt[e] = 0;
             psh[e] = 0.f;
         }
         __syncthreads();
     }
-    float bias[NS];
-    uint32_t gid[NS / 4] = {};                // the experts' groups, four to a word
+    // experts past E have logits of -inf: whatever their bias and group, they are not chosen
+    float bias[NS] = {};
+    if (p.bias) {
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        const int e = group16_expert(i, sub);
-        bias[i] = p.bias && e < p.E ? p.bias[e] : 0.f;
-        gid[i / 4] |= uint32_t(e < p.E ? e / p.gs : 0) << (8 * (i % 4));
+        for (int i = 0; i < NS; ++i) bias[i] = p.bias[min(group16_expert(i, sub0), p.E - 1)];
     }
+    uint32_t gid[NS / 4] = {};                // the experts' groups, four to a word
+    const uint32_t per = ((1u << 20) + p.gs - 1) / p.gs;    // e / gs = e per >> 20: e and gs are at most 512
+#pragma unroll
+    for (int i = 0; i < NS; ++i) gid[i / 4] |= (uint32_t(group16_expert(i, sub0)) * per >> 20) << (8 * (i % 4));
     const bool fours = p.gs % 4 == 0;
     float psum[NS] = {};
     float zsum = 0.f;
@@ -376,7 +428,9 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
         const int64_t t = t0 + grp;
         const bool in = t < p.T && (!p.mask || p.mask[t] != 0);
         float v[NS], c[NS];
-        group16_load<LT, NS>(p, t, sub, in, vec, v);
+        int E = p.E, sub = sub0;
+        asm volatile("" : "+s"(E), "+v"(sub));              // masks and places made anew: kept over the loop they spill
+        group16_load<LT, NS>(p, t, sub, E, in, vec, v);
         float best = -__builtin_inff();
         bool isnan = false;
 #pragma unroll
@@ -394,7 +448,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
         if constexpr (!SIG || TRAIN) {
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                c[i] = v[i] == v[i] ? route_exp(v[i] - m) : 0.f;
+                c[i] = exp0(v[i] - m);
                 total += c[i];
                 if constexpr (TRAIN) q[i] = c[i];
             }
@@ -404,12 +458,13 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
         const float smax = SIG ? sigmoid2(m).x : inv;
         if constexpr (SIG) {
             float s = 0.f;
+            const uint32_t fm = far ? 0xffffffffu : 0u;
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                c[i] = sigmoid2(v[i]).x;
+                c[i] = sigmoid0(v[i]);
                 if constexpr (TRAIN) {
                     s += c[i];
-                    q[i] = far ? q[i] : c[i];
+                    q[i] = pick(fm, q[i], c[i]);
                 }
             }
             if constexpr (TRAIN) sums = live && !far ? 1.f / row_sum(s) : 0.f;
@@ -419,23 +474,20 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
         }
         if (anynan) total = inv = sums = __uint_as_float(live ? 0x7fc00000u : 0u);
         if constexpr (TRAIN) {
-            if (live) {
-                const float lse = m + logf(total);
-                if (sub == 0) {
-                    zsum += lse * lse;
-                    ++nlive;
-                }
-                const float f = far ? inv : sums;
+            const float lse = m + logf(total);
+            zsum += live && sub == 0 ? lse * lse : 0.f;
+            nlive += live && sub == 0;
+            const float f = far ? inv : sums;               // 0 where the token is not live
 #pragma unroll
-                for (int i = 0; i < NS; ++i) psum[i] = __builtin_fmaf(q[TRAIN ? i : 0], f, psum[i]);
-            }
+            for (int i = 0; i < NS; ++i) psum[i] = __builtin_fmaf(q[i], f, psum[i]);
         }
         uint32_t key[NS], lm = 0;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             c[i] += bias[i];
             const bool can = live && v[i] > -__builtin_inff() && c[i] > -__builtin_inff();
-            key[i] = can ? f32_key(p.bias ? c[i] : v[i]) : 0u;
+            const uint32_t b = __float_as_uint((p.bias ? c[i] : v[i]) + 0.f);      // -0 as 0
+            key[i] = can ? b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u) : 0u;    // f32_key of a number
             c[i] = can ? c[i] : -__builtin_inff();
         }
         bool amb = false;                                   // fp32 does not say which is larger
@@ -443,13 +495,12 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
             float a = -__builtin_inff(), b = a;             // the group's two largest
             wave_lds_sync();                                // the last tokens' scores are read
             if (fours) {
-                float2 *mine = reinterpret_cast<float2 *>(csh) + grp * (p.E / 4);
+                float2 *mine = reinterpret_cast<float2 *>(csh) + grp * 4 * NS;
 #pragma unroll
                 for (int w = 0; w < NS / 4; ++w) {
                     const float hi0 = fmaxf(c[4 * w], c[4 * w + 1]), lo0 = fminf(c[4 * w], c[4 * w + 1]);
                     const float hi1 = fmaxf(c[4 * w + 2], c[4 * w + 3]), lo1 = fminf(c[4 * w + 2], c[4 * w + 3]);
-                    const int e = group16_expert(4 * w, sub);
-                    if (e < p.E) mine[e / 4] = float2{fmaxf(hi0, hi1), fmaxf(fminf(hi0, hi1), fmaxf(lo0, lo1))};
+                    mine[group16_expert(4 * w, sub) / 4] = float2{fmaxf(hi0, hi1), fmaxf(fminf(hi0, hi1), fmaxf(lo0, lo1))};
                 }
                 wave_lds_sync();
                 if (sub < p.G) {
@@ -463,12 +514,9 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
                     }
                 }
             } else {
-                float *mine = csh + grp * p.E;
+                float *mine = csh + grp * 16 * NS;
 #pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    const int e = group16_expert(i, sub);
-                    if (e < p.E) mine[e] = c[i];
-                }
+                for (int i = 0; i < NS; ++i) mine[group16_expert(i, sub)] = c[i];
                 wave_lds_sync();
                 if (sub < p.G) {
                     int at = sub % p.gs;
@@ -481,14 +529,10 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
                 }
             }
             const float g = p.group_top == 2 && b > -__builtin_inff() ? a + b : a;
-            const uint32_t gk = f32_key(g);
+            const uint32_t gk = sub < p.G ? f32_key(g) : 0u;
+            const uint64_t gl = (uint64_t(gk) << 32) | uint32_t(15 - sub);
             int rank = 0;
-#define VQK_ROR(N)                                                                    \
-    {                                                                                 \
-        const uint32_t o = dpp_u<0x120 + N>(gk);                                      \
-        const int from = (sub - N) & 15;                                              \
-        rank += from < p.G && (o > gk || (o == gk && from < sub));                    \
-    }
+#define VQK_ROR(N) rank += dpp_u64<0x120 + N>(gl) > gl;
             VQK_ROR(1) VQK_ROR(2) VQK_ROR(3) VQK_ROR(4) VQK_ROR(5) VQK_ROR(6) VQK_ROR(7) VQK_ROR(8)
             VQK_ROR(9) VQK_ROR(10) VQK_ROR(11) VQK_ROR(12) VQK_ROR(13) VQK_ROR(14) VQK_ROR(15)
 #undef VQK_ROR
@@ -500,7 +544,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
             const float most = key_f32(row_max(sub < p.G && a > -__builtin_inff() ? f32_key(mag) : f32_key(0.f)));
             if (next > kKeyNegInf) amb = !(key_f32(worst) - key_f32(next) > 4.f * group_tol<SIG>(smax, most));
 #pragma unroll
-            for (int i = 0; i < NS; ++i) key[i] = (kept >> ((gid[i / 4] >> (8 * (i % 4))) & 255u)) & 1u ? key[i] : 0u;
+            for (int i = 0; i < NS; ++i) key[i] &= uint32_t(-int32_t((kept >> ((gid[i / 4] >> (8 * (i % 4))) & 31u)) & 1u));
         }
 #pragma unroll
         for (int i = 0; i < NS; ++i) lm = max(lm, key[i]);
@@ -585,10 +629,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
         for (int w = 0; w < kRouteWaves * 4; ++w) {         // the tokens' sums in order of wave and row of lanes
             if (wave == w / 4 && grp == w % 4) {
 #pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    const int e = group16_expert(i, sub);
-                    if (e < p.E) psh[e] += psum[i];
-                }
+                for (int i = 0; i < NS; ++i) psh[group16_expert(i, sub0)] += psum[i];
             }
             if (w % 4 == 3) __syncthreads();
             else wave_lds_sync();
@@ -597,15 +638,16 @@ __global__ void __launch_bounds__(kRouteThreads) k_group16(const GroupArgs p, bo
     // the second look, at this wave's own tokens
     __syncthreads();
     for (int64_t t0 = t00; t0 < p.T; t0 += stride) {
-        const uint64_t again = __ballot(sub == 0 && t0 + grp < p.T && p.ids[(t0 + grp) * p.k] == kSecondLook);
+        const uint64_t again = __ballot(sub0 == 0 && t0 + grp < p.T && p.ids[(t0 + grp) * p.k] == kSecondLook);
         for (int g = 0; g < 4; ++g) {
             if (!((again >> (16 * g)) & 1)) continue;
-            float v[(NS + 3) / 4], m;
+            float v[NS / 4], near[NS / 4], m;
             bool anynan;
             wave_token<LT>(p, t0 + g, lane, v, &m, &anynan);
+            wave_bias(p, lane, near);
             wave_lds_sync();
-            wave_choose<LT, (NS + 3) / 4, SIG>(p, t0 + g, lane, v, m, SIG ? 0.f : 1.f / wave_total(v, m), anynan,
-                                               reinterpret_cast<double *>(csh), TRAIN ? cnt : nullptr);
+            wave_choose<NS / 4, SIG>(p, t0 + g, lane, v, m, SIG ? 0.f : 1.f / wave_total(v, m), anynan, near,
+                                     reinterpret_cast<double *>(csh), TRAIN ? cnt : nullptr);
         }
     }
     if constexpr (TRAIN) {
@@ -767,7 +809,7 @@ static int go_wave(const GroupArgs &a, bool train, int wgs, hipStream_t st) {
 }
 template <int LT, int NS, bool SIG>
 static int go_16(const GroupArgs &a, bool train, int wgs, hipStream_t st) {
-    const size_t lds = kRouteWaves * 16 * size_t(a.E) + (train ? 8 * size_t(a.E) : 0);
+    const size_t lds = kRouteWaves * 256 * NS + (train ? 128 * NS : 0);
     const bool vec = route_vec(a.l, a.ld, a.E, LT);
     if (train) hipLaunchKernelGGL((k_group16<LT, NS, SIG, true>), dim3(wgs), dim3(kRouteThreads), lds, st, a, vec);
     else hipLaunchKernelGGL((k_group16<LT, NS, SIG, false>), dim3(wgs), dim3(kRouteThreads), lds, st, a, vec);

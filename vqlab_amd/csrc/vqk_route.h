@@ -23,14 +23,15 @@ __device__ __forceinline__ void wave_lds_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// e^d for d <= 0: 2^(d log2 e), the product's rounding error carried along.
-__device__ __forceinline__ float route_exp(float d) {
+// e^d for -200 <= d <= 0: 2^(d log2 e), the product's rounding error carried along.
+__device__ __forceinline__ float route_exp_in(float d) {
     constexpr float hi = 1.44269502162933349609375f, lo = 1.92596299113e-8f;   // log2 e = hi + lo
-    d = d < -200.f ? -200.f : d;              // 0 already (and -inf leaves no NaN; a NaN stays)
     const float t = d * hi, r = __builtin_fmaf(d, hi, -t) + d * lo;
     const float e = __builtin_amdgcn_exp2f(t);
     return __builtin_fmaf(e, 0.693147182f * r, e);
 }
+// d <= 0: e^-200 is 0 already (and -inf leaves no NaN; a NaN stays).
+__device__ __forceinline__ float route_exp(float d) { return route_exp_in(d < -200.f ? -200.f : d); }
 
 template <int CTRL>
 __device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
