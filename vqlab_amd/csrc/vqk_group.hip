@@ -57,11 +57,11 @@ __device__ __forceinline__ float2 sigmoid2(float l) {
     const float e = route_exp(-__builtin_fabsf(l)), r = rcp12(1.f + e);
     return l >= 0.f ? float2{r, e * r} : float2{e * r, r};
 }
-// The same exponential and sigmoid without a branch and with 0 for a NaN.
+// The same exponential and sigmoid without a branch and with 0 for a NaN (1 - sigmoid: 1).
 __device__ __forceinline__ float exp0(float d) { return route_exp_in(__builtin_fmaxf(d, -200.f)); }
-__device__ __forceinline__ float sigmoid0(float l) {
-    const float e = exp0(-__builtin_fabsf(l));
-    return (l >= 0.f ? 1.f : e) * rcp12(1.f + e);
+__device__ __forceinline__ float2 sigmoid0(float l) {
+    const float e = exp0(-__builtin_fabsf(l)), r = rcp12(1.f + e);
+    return float2{(l >= 0.f ? 1.f : e) * r, (l >= 0.f ? e : 1.f) * r};
 }
 __device__ __forceinline__ float pick(uint32_t mask, float a, float b) {        // bits of a where mask has them, of b elsewhere
     return __uint_as_float((mask & __float_as_uint(a)) | (~mask & __float_as_uint(b)));
@@ -335,6 +335,43 @@ __global__ void __launch_bounds__(kRouteThreads) k_group_wave(const GroupArgs p)
     }
 }
 
+// Logits expert(i) of the row at `base`, -inf for those past E and where the token is not
+// `in` (base: 0). vec: fours are aligned and whole. All loads are issued before the first
+// is used: an address past the row is replaced by the row's own start.
+template <int LT, int NS, typename Expert>
+__device__ __forceinline__ void row_load(const void *l, int64_t base, int E, bool in, bool vec, Expert expert, float (&v)[NS]) {
+    using T = std::conditional_t<LT == VQK_F32, float, uint16_t>;
+    const T *row = static_cast<const T *>(l) + base;
+    if (vec) {
+        using Four = std::conditional_t<LT == VQK_F32, u32x4, u32x2>;
+        Four f[NS / 4];
+#pragma unroll
+        for (int q = 0; q < NS / 4; ++q) {
+            const int e = expert(4 * q);
+            f[q] = *reinterpret_cast<const Four *>(row + (e < E ? e : 0));
+        }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const Four w = f[i / 4];
+            if constexpr (LT == VQK_F32) {
+                v[i] = __uint_as_float(w[i % 4]);
+            } else {
+                const uint16_t h = uint16_t(w[i % 4 / 2] >> (16 * (i & 1)));
+                v[i] = LT == VQK_BF16 ? bf16_to_f32(h) : h_to_f32(h);
+            }
+            v[i] = in && expert(i / 4 * 4) < E ? v[i] : -__builtin_inff();
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int e = expert(i);
+            v[i] = load_act(row, LT, e < E ? e : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) v[i] = in && expert(i) < E ? v[i] : -__builtin_inff();
+    }
+}
+
 // ------------------------------------------------- sixteen lanes to a token
 // Bounds of what fp32 may get wrong in a comparison of two c (smax: the row's
 // largest s): a sigmoid is 4 units of 2^-23 off at most, a softmax 2^-18 of itself
@@ -348,42 +385,6 @@ __device__ __forceinline__ float group_tol(float smax, float c) {
 // whole lines a load, and the lanes of a group shift from one 64 to the next, so that
 // the experts of few groups are not all in the same lanes.
 __device__ __forceinline__ int group16_expert(int i, int sub) { return 64 * (i / 4) + 4 * ((sub + i / 4 * 4) & 15) + i % 4; }
-// All loads are issued before the first is used: an address past the row or of a token
-// that is not `in` is replaced by the row's, or the first token's, own start.
-template <int LT, int NS>
-__device__ __forceinline__ void group16_load(const GroupArgs &p, int64_t t, int sub, int E, bool in, bool vec, float (&v)[NS]) {
-    using T = std::conditional_t<LT == VQK_F32, float, uint16_t>;
-    const T *row = static_cast<const T *>(p.l) + (in ? t * p.ld : 0);
-    if (vec) {
-        using Four = std::conditional_t<LT == VQK_F32, u32x4, u32x2>;
-        Four f[NS / 4];
-#pragma unroll
-        for (int q = 0; q < NS / 4; ++q) {
-            const int e = group16_expert(4 * q, sub);
-            f[q] = *reinterpret_cast<const Four *>(row + (e < E ? e : 0));
-        }
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const Four w = f[i / 4];
-            if constexpr (LT == VQK_F32) {
-                v[i] = __uint_as_float(w[i % 4]);
-            } else {
-                const uint16_t h = uint16_t(w[i % 4 / 2] >> (16 * (i & 1)));
-                v[i] = LT == VQK_BF16 ? bf16_to_f32(h) : h_to_f32(h);
-            }
-            v[i] = in && group16_expert(i / 4 * 4, sub) < E ? v[i] : -__builtin_inff();
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const int e = group16_expert(i, sub);
-            v[i] = load_act(row, LT, e < E ? e : 0);
-        }
-#pragma unroll
-        for (int i = 0; i < NS; ++i) v[i] = in && group16_expert(i, sub) < E ? v[i] : -__builtin_inff();
-    }
-}
-
 // The top k as in k_route16: the k-th largest lane maximum bounds them from below,
 // what reaches it is collected in LDS and ranked, two candidates a lane. One more than
 // top_k is looked at: the best that is left out.
@@ -430,7 +431,7 @@ __global__ void __launch_bounds__(kRouteThreads, NS <= 16 ? 3 : 1) k_group16(con
         float v[NS], c[NS];
         int E = p.E, sub = sub0;
         asm volatile("" : "+s"(E), "+v"(sub));              // masks and places made anew: kept over the loop they spill
-        group16_load<LT, NS>(p, t, sub, E, in, vec, v);
+        row_load<LT, NS>(p.l, in ? t * p.ld : 0, E, in, vec, [=](int i) { return group16_expert(i, sub); }, v);
         float best = -__builtin_inff();
         bool isnan = false;
 #pragma unroll
@@ -461,7 +462,7 @@ __global__ void __launch_bounds__(kRouteThreads, NS <= 16 ? 3 : 1) k_group16(con
             const uint32_t fm = far ? 0xffffffffu : 0u;
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                c[i] = sigmoid0(v[i]);
+                c[i] = sigmoid0(v[i]).x;
                 if constexpr (TRAIN) {
                     s += c[i];
                     q[i] = pick(fm, q[i], c[i]);
@@ -712,27 +713,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_group_bwd(const GroupBwdArgs 
         const float4 sv = in ? p.saved[t] : float4{0.f, 0.f, 0.f, 0.f};
         const bool live = sv.y != 0.f;        // a live token's sum is at most E
         float v[NS];
-#pragma unroll
-        for (int q = 0; q < NS / 4; ++q) {
-            const int e = 4 * L * q + 4 * sub;
-            if (vec && live && e < p.E) {
-                if constexpr (LT == VQK_F32) {
-                    const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.l) + t * p.ld + e);
-                    v[4 * q] = a.x; v[4 * q + 1] = a.y; v[4 * q + 2] = a.z; v[4 * q + 3] = a.w;
-                } else {
-                    const u32x2 a = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(p.l) + t * p.ld + e);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint16_t h = uint16_t(a[j / 2] >> (16 * (j & 1)));
-                        v[4 * q + j] = LT == VQK_BF16 ? bf16_to_f32(h) : h_to_f32(h);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    v[4 * q + j] = live && e + j < p.E ? load_act(p.l, LT, t * p.ld + e + j) : -__builtin_inff();
-            }
-        }
+        row_load<LT, NS>(p.l, live ? t * p.ld : 0, p.E, live, vec, [=](int i) { return 4 * L * (i / 4) + 4 * sub + i % 4; }, v);
         int id = -1;
         float wdw = 0.f, w = 0.f;
         if (p.dw && live && sub < p.k) {
@@ -743,12 +724,19 @@ __global__ void __launch_bounds__(kRouteThreads) k_group_bwd(const GroupBwdArgs 
         const float s = sum(wdw);
         const float lse = sv.x - logf(sv.y);
         const bool far = !SIG || sv.x < kFarLogit;
-        float x[NS];                          // softmax
+        const uint32_t fm = far ? 0xffffffffu : 0u;
+        // softmax, p and 1 - sigmoid; a token that is not live has sums of 0 and logits of -inf
+        float x[NS], pr[SIG ? NS : 1], to1[SIG ? NS : 1];
         float dot = 0.f;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            x[i] = live ? route_exp(v[i] - sv.x) * sv.y : 0.f;
-            dot += f[i] * (far ? x[i] : sigmoid2(v[i]).x * sv.z);
+            x[i] = exp0(v[i] - sv.x) * sv.y;
+            if constexpr (SIG) {
+                const float2 g = sigmoid0(v[i]);
+                pr[i] = pick(fm, x[i], g.x * sv.z);
+                to1[i] = g.y;
+            }
+            dot += f[i] * (SIG ? pr[SIG ? i : 0] : x[i]);
         }
         dot = sum(dot);
         const float sub_ = fz * lse - (SIG || p.norm ? 0.f : s);
@@ -766,13 +754,9 @@ __global__ void __launch_bounds__(kRouteThreads) k_group_bwd(const GroupBwdArgs 
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int i = 4 * q + j;
-                if constexpr (SIG) {
-                    const float2 g = sigmoid2(v[i]);
-                    d[j] = g.y * ((far ? x[i] : g.x * sv.z) * (f[i] - dot) + add[j]) + x[i] * sub_;
-                } else {
-                    d[j] = x[i] * (f[i] - dot + sub_) + add[j];
-                }
-                if (!live) d[j] = 0.f;
+                if constexpr (SIG) d[j] = to1[i] * (pr[i] * (f[i] - dot) + add[j]) + x[i] * sub_;
+                else d[j] = x[i] * (f[i] - dot + sub_) + add[j];
+                d[j] = live ? d[j] : 0.f;
             }
             if (!in || e >= p.E) continue;
             if (vec) {
@@ -938,8 +922,7 @@ extern "C" int vqk_route_grouped_backward(const void *logits, int32_t l_type, in
     a.dl = dlogits;
     const bool rows16 = group16_ok(T, E, top_k, 1);
     const int per = rows16 ? 4 * kRouteWaves : kRouteWaves;
-    const int64_t w = (T + per - 1) / per;
-    const int wgs = int(w < 2048 ? w : 2048);
+    const int wgs = route_wgs_of(T, per);     // resident at once: 65536 tokens over 256 experts 38 us, in 2048 workgroups 45
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool sig = form->score == VQK_SCORE_SIGMOID;
     switch (l_type) {
