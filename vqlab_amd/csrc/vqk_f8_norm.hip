@@ -10,7 +10,7 @@
 // Bound by memory: each input is read once and each output written once. A
 // workgroup of W waves takes a row and holds it in registers, 8 neighbouring
 // columns a piece: few rows are spread over as many waves as they have pieces
-// (latency), many rows take up to four pieces a lane (fewer steps across waves for
+// (latency), many rows take two pieces a lane (fewer steps across waves for
 // each row). A block of 128 is 16 lanes of one piece, so its largest magnitude
 // takes four DPP steps. Squares are summed in fp64 (2^127 squared is no fp32
 // number), everything else is fp32. dw: a workgroup adds up its rows in
@@ -19,7 +19,7 @@
 
 namespace vqk {
 
-constexpr int kNormMaxC = 16384;              // 8 waves of 4 pieces
+constexpr int kNormMaxC = 16384, kNormMaxWaves = 16;      // 2 pieces a lane
 
 struct NormArgs {
     const void *x, *res, *w;
@@ -33,15 +33,32 @@ struct NormArgs {
     int64_t sn, sk;
 };
 
-// Sum over the workgroup's W waves, in every thread; `part` is used by one call.
-template <int W>
-__device__ __forceinline__ double norm_sum(double v, double (&part)[W]) {
-    for (int o = 1; o < kWave; o <<= 1) v += __shfl_xor(v, o);
-    if constexpr (W == 1) return v;
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t(dpp_u<CTRL>(uint32_t(b >> 32))) << 32) | dpp_u<CTRL>(uint32_t(b)));
+}
+__device__ __forceinline__ double lane_f64(double v, int from) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(b)), from));
+    return __builtin_bit_cast(double, (uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(b >> 32)), from))) << 32) | lo);
+}
+// Sum over the workgroup's W waves, in every thread; `part` is used by one call. The
+// barrier waits for LDS alone: loads of the next row stay on their way.
+__device__ __forceinline__ double norm_sum(double v, double (&part)[kNormMaxWaves]) {
+    const int W = int(blockDim.x) >> 6;
+    v += dpp_f64<kDppQuadXor1>(v);
+    v += dpp_f64<kDppQuadXor2>(v);
+    v += dpp_f64<kDppRowHalfMirror>(v);
+    v += dpp_f64<kDppRowMirror>(v);
+    v = (lane_f64(v, 0) + lane_f64(v, 16)) + (lane_f64(v, 32) + lane_f64(v, 48));
+    if (W == 1) return v;
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    __syncthreads();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);       // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
     double s = 0.;
-#pragma unroll
     for (int i = 0; i < W; ++i) s += part[i];
     return s;
 }
@@ -69,22 +86,22 @@ __device__ __forceinline__ float round_to(float v) {
     return T == VQK_BF16 ? bf16_to_f32(f32_to_bf16(v)) : h_to_f32(f32_to_h(v));
 }
 
-template <int XT, int W, int P, bool Q>
-__global__ void __launch_bounds__(64 * W) k_rms(const NormArgs p, bool vec, bool vecw) {
-    __shared__ double part[W];
+template <int XT, int P, bool Q>
+__global__ void __launch_bounds__(64 * kNormMaxWaves) k_rms(const NormArgs p, bool vec, bool vecw) {
+    __shared__ double part[kNormMaxWaves];
     const int64_t row = blockIdx.x;
     float h[P][8], wt[P][8];
     double sum = 0.;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        const int k0 = (i * 64 * W + int(threadIdx.x)) * 8;
+        const int k0 = (i * int(blockDim.x) + int(threadIdx.x)) * 8;
         mx_load8(p.x, XT, row * p.ldx, k0, p.C, vec, h[i]);
         mx_load8(p.w, p.w_type, 0, k0, p.C, vecw, wt[i]);
     }
     if (p.res) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int k0 = (i * 64 * W + int(threadIdx.x)) * 8;
+            const int k0 = (i * int(blockDim.x) + int(threadIdx.x)) * 8;
             float a[8];
             mx_load8(p.res, XT, row * p.ldr, k0, p.C, vec, a);
 #pragma unroll
@@ -96,12 +113,12 @@ __global__ void __launch_bounds__(64 * W) k_rms(const NormArgs p, bool vec, bool
     for (int i = 0; i < P; ++i)
 #pragma unroll
         for (int u = 0; u < 8; ++u) sum = __builtin_fma(double(h[i][u]), double(h[i][u]), sum);
-    sum = norm_sum<W>(sum, part);
+    sum = norm_sum(sum, part);
     const float r = float(1. / sqrt(sum / double(p.C) + p.eps));
     if (p.r && threadIdx.x == 0) p.r[row] = r;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        const int k0 = (i * 64 * W + int(threadIdx.x)) * 8;
+        const int k0 = (i * int(blockDim.x) + int(threadIdx.x)) * 8;
         float y[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) y[u] = h[i][u] * r * wt[i][u];
@@ -139,52 +156,88 @@ struct NormBwdArgs {
     float *part;                              // [gridDim.x][C]
 };
 
-template <int XT, int W, int P>
-__global__ void __launch_bounds__(64 * W) k_rms_bwd(const NormBwdArgs p, bool vec, bool vecw) {
-    __shared__ double part[2][W];
-    float wt[P][8], dw[P][8] = {};
+// Eight neighbouring columns as they lie in memory, zeros past the row.
+template <int XT> struct Raw8 { u32x4 a[XT == VQK_F32 ? 2 : 1]; };
+template <int XT>
+__device__ __forceinline__ Raw8<XT> raw_load8(const void *x, int64_t base, int k0, int C, bool vec) {
+    Raw8<XT> o{};
+    constexpr int E = XT == VQK_F32 ? 4 : 8;  // elements of 16 bytes
+    if (vec) {
+        if (k0 < C) {
+            const u32x4 *from = reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(x) + (base + k0) * (16 / E));
+            o.a[0] = from[0];
+            if constexpr (XT == VQK_F32) o.a[1] = from[1];
+        }
+        return o;
+    }
 #pragma unroll
-    for (int i = 0; i < P; ++i) mx_load8(p.w, p.w_type, 0, (i * 64 * W + int(threadIdx.x)) * 8, p.C, vecw, wt[i]);
+    for (int i = 0; i < 8; ++i) {
+        if (k0 + i >= C) continue;
+        if constexpr (XT == VQK_F32) o.a[i / 4][i % 4] = static_cast<const uint32_t *>(x)[base + k0 + i];
+        else o.a[0][i / 2] |= uint32_t(static_cast<const uint16_t *>(x)[base + k0 + i]) << (16 * (i % 2));
+    }
+    return o;
+}
+template <int XT>
+__device__ __forceinline__ float raw_at(const Raw8<XT> &r, int i) {
+    if constexpr (XT == VQK_F32) return __uint_as_float(r.a[i / 4][i % 4]);
+    const uint16_t h = uint16_t(r.a[0][i / 2] >> (16 * (i % 2)));
+    return XT == VQK_BF16 ? bf16_to_f32(h) : h_to_f32(h);
+}
+
+// The next row is loaded while this one is worked on, as it lies in memory (half the
+// registers of its values); rows of more than 8 waves leave no registers for that.
+template <int XT, int P, int MAXW>
+__global__ void __launch_bounds__(64 * MAXW) k_rms_bwd(const NormBwdArgs p, bool vec, bool vecw) {
+    constexpr bool AHEAD = MAXW <= 8;
+    __shared__ double part[2][kNormMaxWaves];
+    float wt[P][8], dw[P][8] = {};
+    Raw8<XT> h[P], dy[P], dh[P];
+    auto load = [&](int64_t row) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int k0 = (i * int(blockDim.x) + int(threadIdx.x)) * 8;
+            h[i] = raw_load8<XT>(p.h, row * p.ldh, k0, p.C, vec);
+            dy[i] = raw_load8<XT>(p.dy, row * p.C, k0, p.C, vec);
+            dh[i] = p.dh ? raw_load8<XT>(p.dh, row * p.C, k0, p.C, vec) : Raw8<XT>{};
+        }
+    };
+    if (AHEAD) load(blockIdx.x);              // no more workgroups than rows
+#pragma unroll
+    for (int i = 0; i < P; ++i) mx_load8(p.w, p.w_type, 0, (i * int(blockDim.x) + int(threadIdx.x)) * 8, p.C, vecw, wt[i]);
     int turn = 0;
     for (int64_t row = blockIdx.x; row < p.N; row += gridDim.x, turn ^= 1) {
-        float xh[P][8], g[P][8], add[P][8];
+        Raw8<XT> ch[P], cdy[P], cdh[P];
         const float r = p.r[row];
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const int k0 = (i * 64 * W + int(threadIdx.x)) * 8;
-            mx_load8(p.h, XT, row * p.ldh, k0, p.C, vec, xh[i]);
-            mx_load8(p.dy, XT, row * p.C, k0, p.C, vec, g[i]);
-            if (p.dh) mx_load8(p.dh, XT, row * p.C, k0, p.C, vec, add[i]);
-        }
+        if (!AHEAD) load(row);
         float dot = 0.f;
 #pragma unroll
-        for (int i = 0; i < P; ++i)
+        for (int i = 0; i < P; ++i) {
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                xh[i][u] *= r;
-                dw[i][u] = __builtin_fmaf(g[i][u], xh[i][u], dw[i][u]);
-                g[i][u] *= wt[i][u];
-                dot = __builtin_fmaf(g[i][u], xh[i][u], dot);
+                const float d = raw_at(dy[i], u), xh = raw_at(h[i], u) * r;
+                dw[i][u] = __builtin_fmaf(d, xh, dw[i][u]);
+                dot = __builtin_fmaf(d * wt[i][u], xh, dot);
             }
-        const float mean = float(norm_sum<W>(double(dot), part[turn]) / double(p.C));
+            ch[i] = h[i];
+            cdy[i] = dy[i];
+            cdh[i] = dh[i];
+        }
+        if (AHEAD && row + gridDim.x < p.N) load(row + gridDim.x);
+        const float mean = float(norm_sum(double(dot), part[turn]) / double(p.C));
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int k0 = (i * 64 * W + int(threadIdx.x)) * 8;
+            const int k0 = (i * int(blockDim.x) + int(threadIdx.x)) * 8;
             float d[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                d[u] = r * (g[i][u] - xh[i][u] * mean);
-                if (p.dh) d[u] += add[i][u];
-            }
+            for (int u = 0; u < 8; ++u) d[u] = r * (raw_at(cdy[i], u) * wt[i][u] - raw_at(ch[i], u) * r * mean) + raw_at(cdh[i], u);
             norm_store8(p.dx, XT, row * p.C + k0, d, p.C - k0, vec);
         }
     }
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        const int k0 = (i * 64 * W + int(threadIdx.x)) * 8;
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (k0 + u < p.C) p.part[int64_t(blockIdx.x) * p.C + k0 + u] = dw[i][u];
+        const int k0 = (i * int(blockDim.x) + int(threadIdx.x)) * 8;
+        norm_store8(p.part, VQK_F32, int64_t(blockIdx.x) * p.C + k0, dw[i], p.C - k0, vec);
     }
 }
 
@@ -209,34 +262,36 @@ struct NormPlan { int w, p; };
 // Rows up to which a row is spread over one piece a lane.
 constexpr int64_t kNormSpreadRows = 1024;
 static NormPlan norm_plan(int64_t N, int64_t C) {
-    const int64_t waves = (C + 511) / 512;
-    const int p = N <= kNormSpreadRows && waves <= 16 ? 1 : 4;
-    int w = 1;
-    while (w * p < waves) w *= 2;
-    return NormPlan{w, p};
+    const int pieces = int((C + 511) / 512);
+    // 2048 rows of 5120 fp16 to 8 bits: two pieces a lane 18.0 us, one 20.6, four 20.6
+    const int p = N <= kNormSpreadRows && pieces <= kNormMaxWaves ? 1 : 2;
+    return NormPlan{(pieces + p - 1) / p, p};
 }
-// Workgroups of the backward pass: each leaves a row of sums.
+// The backward pass: two pieces a lane, as many workgroups as run at once, each of which
+// leaves a row of sums (16384 rows of 4096, bf16: 2048 waves 117 us with the sums' sum,
+// 1024 waves 134, 4096 waves 135).
+static NormPlan norm_bwd_plan(int64_t C) {
+    const int pieces = int((C + 511) / 512), p = pieces > 1 ? 2 : 1;
+    return NormPlan{(pieces + p - 1) / p, p};
+}
 static int64_t norm_bwd_wgs(int64_t N, int64_t C) {
-    const NormPlan pl = norm_plan(N, C);
-    const int64_t most = 2048 / pl.w < 256 ? 256 : 2048 / pl.w;
+    const int64_t most = 2048 / norm_bwd_plan(C).w;
     return N < most ? N : most;
 }
 
 template <int XT, bool Q>
 static int go_norm(const NormArgs &a, NormPlan pl, bool vec, bool vecw, hipStream_t st) {
-    const dim3 grid{unsigned(a.N)};
-#define VQK_GO(W, P) if (pl.w == W && pl.p == P) hipLaunchKernelGGL((k_rms<XT, W, P, Q>), grid, dim3(64 * W), 0, st, a, vec, vecw)
-    VQK_GO(1, 1); VQK_GO(2, 1); VQK_GO(4, 1); VQK_GO(8, 1); VQK_GO(16, 1);
-    VQK_GO(1, 4); VQK_GO(2, 4); VQK_GO(4, 4); VQK_GO(8, 4);
-#undef VQK_GO
+    const dim3 grid{unsigned(a.N)}, block{unsigned(64 * pl.w)};
+    if (pl.p == 1) hipLaunchKernelGGL((k_rms<XT, 1, Q>), grid, block, 0, st, a, vec, vecw);
+    else hipLaunchKernelGGL((k_rms<XT, 2, Q>), grid, block, 0, st, a, vec, vecw);
     return hip_status(hipGetLastError(), "norm launch");
 }
 template <int XT>
 static int go_norm_bwd(const NormBwdArgs &a, NormPlan pl, unsigned wgs, bool vec, bool vecw, hipStream_t st) {
-#define VQK_GO(W, P) if (pl.w == W && pl.p == P) hipLaunchKernelGGL((k_rms_bwd<XT, W, P>), dim3(wgs), dim3(64 * W), 0, st, a, vec, vecw)
-    VQK_GO(1, 1); VQK_GO(2, 1); VQK_GO(4, 1); VQK_GO(8, 1); VQK_GO(16, 1);
-    VQK_GO(1, 4); VQK_GO(2, 4); VQK_GO(4, 4); VQK_GO(8, 4);
-#undef VQK_GO
+    const dim3 grid{wgs}, block{unsigned(64 * pl.w)};
+    if (pl.p == 1) hipLaunchKernelGGL((k_rms_bwd<XT, 1, 1>), grid, block, 0, st, a, vec, vecw);
+    else if (pl.w <= 8) hipLaunchKernelGGL((k_rms_bwd<XT, 2, 8>), grid, block, 0, st, a, vec, vecw);
+    else hipLaunchKernelGGL((k_rms_bwd<XT, 2, kNormMaxWaves>), grid, block, 0, st, a, vec, vecw);
     return hip_status(hipGetLastError(), "norm gradient launch");
 }
 
@@ -305,7 +360,7 @@ extern "C" int vqk_rms_norm_backward(const void *h, int32_t type, int64_t N, int
         const int esz = act_size(type);
         const NormBwdArgs a{h, weight, dy, dh, N, ldh, int32_t(C), w_type, r, dx, part};
         const bool vec = C % 8 == 0 && al16(h) && (ldh * esz) % 16 == 0 && al16(dy) && (!dh || al16(dh)) && al16(dx);
-        const NormPlan pl = norm_plan(N, C);
+        const NormPlan pl = norm_bwd_plan(C);
         int e;
         switch (type) {
             case VQK_F16: e = go_norm_bwd<VQK_F16>(a, pl, unsigned(wgs), vec, al16(weight), st); break;
