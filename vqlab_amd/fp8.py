@@ -46,9 +46,9 @@ def _rows_in(x, C):
 
 def _rows_out(like, lead, n, C):
     """Room for rows [*lead, C] in 8 bits."""
-    codes = torch.empty((*lead, C), dtype=F8, device=like.device)
-    scales = torch.empty((_blocks(C), n), dtype=torch.float32, device=like.device)
-    return codes, scales, scales.t().view(*lead, _blocks(C))
+    codes = like.new_empty((*lead, C), dtype=F8)
+    scales = torch.empty_strided((n, _blocks(C)), (1, n), dtype=torch.float32, device=like.device)
+    return codes, scales, scales if len(lead) == 1 else scales.view(*lead, _blocks(C))
 
 
 def f8_quantize(x):
@@ -103,7 +103,8 @@ def _strided(codes, scales, C, what):
         raise ValueError(f"{what}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not rows "
                          f"of {C} with a scale for each {BLOCK}")
     codes, n, ldc = _rows_in(codes, C)
-    scales = scales.reshape(n, _blocks(C))             # a view where the strides allow it
+    if scales.ndim != 2:
+        scales = scales.reshape(n, _blocks(C))         # a view where the strides allow it
     if n == 1:                                         # one row: its stride says nothing
         return codes, ldc, scales, 0, scales.stride(1), n
     return codes, ldc, scales, scales.stride(0), scales.stride(1), n
@@ -131,7 +132,7 @@ def f8_dequantize(codes, scales, dtype=torch.bfloat16):
             so, sk, sc = scales.stride(0), scales.stride(1), scales
         else:
             rows, ldc, sc, so, sk, n = _strided(codes, scales, C, "f8_dequantize")
-        out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+        out = codes.new_empty(codes.shape, dtype=dtype)
         L.check(L.lib().vqk_f8_dequantize(rows.data_ptr(), ldc, sc.data_ptr(), so, sk, per, n, C, out.data_ptr(),
                                           T.ACT_TYPES[dtype], T.raw_stream(codes)), "f8_dequantize")
     return out
@@ -343,13 +344,13 @@ def _norm(x, weight, eps, residual, f8, want_r):
         rows, n, ld = _rows_in(x, C)
         res, _, ldr = _rows_in(residual, C) if residual is not None else (None, 0, C)
         w = weight.contiguous()
-        h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        h = None if residual is None else x.new_empty(x.shape)
         r = torch.empty(n, dtype=torch.float32, device=x.device) if want_r else None
         y = codes = scales = None
         if f8:
             codes, scales, view = _rows_out(x, x.shape[:-1], n, C)
         else:
-            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            y = x.new_empty(x.shape)
         at = [None if t is None else t.data_ptr() for t in (res, h, y, r, codes, scales)]
         L.check(L.lib().vqk_rms_norm(rows.data_ptr(), T.act_type(x), n, C, ld, at[0], ldr, w.data_ptr(), T.act_type(w),
                                      float(eps), at[1], at[2], at[3], at[4], at[5], 1, n, T.raw_stream(x)), "rms_norm")
