@@ -444,43 +444,66 @@ __global__ void __launch_bounds__(kRouteThreads, NS <= 16 ? 3 : 1) k_group16(con
         const bool live = in && (best > -__builtin_inff() || anynan);
         const float m = best > -__builtin_inff() ? best : 0.f;
         const bool far = !SIG || m < kFarLogit;             // p: a softmax
-        float total = 0.f, inv = 0.f, sums = 0.f;
-        float q[TRAIN ? NS : 1];                            // p before its sum
-        if constexpr (!SIG || TRAIN) {
+        float lse = 0.f, inv = 0.f, sums = 0.f;
+        if constexpr (!SIG) {
+            float total = 0.f;
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 c[i] = exp0(v[i] - m);
                 total += c[i];
-                if constexpr (TRAIN) q[i] = c[i];
             }
             total = row_sum(total);
             inv = live ? 1.f / total : 0.f;
-        }
-        const float smax = SIG ? sigmoid2(m).x : inv;
-        if constexpr (SIG) {
-            float s = 0.f;
-            const uint32_t fm = far ? 0xffffffffu : 0u;
+            lse = m + logf(total);
+            const float f = anynan && live ? __uint_as_float(0x7fc00000u) : inv;
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                c[i] = sigmoid0(v[i]).x;
+                if constexpr (TRAIN) psum[i] = __builtin_fmaf(c[i], f, psum[i]);
+                c[i] *= inv;
+            }
+        } else {
+            // e^l of the sigmoid's own e^-|l|, unless a row's largest is too far from 0 for its sum
+            float total = 0.f, s = 0.f;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const float e = exp0(-__builtin_fabsf(v[i])), x = rcp12(1.f + e);
+                const bool up = v[i] >= 0.f;
+                c[i] = (up ? 1.f : e) * x;
                 if constexpr (TRAIN) {
                     s += c[i];
-                    q[i] = pick(fm, q[i], c[i]);
+                    total += up ? __builtin_amdgcn_rcpf(e) : e;
                 }
             }
-            if constexpr (TRAIN) sums = live && !far ? 1.f / row_sum(s) : 0.f;
-        } else {
+            if constexpr (TRAIN) {
+                const bool odd = live && !(__builtin_fabsf(m) < -kFarLogit);
+                sums = live && !far ? 1.f / row_sum(s) : 0.f;
+                if (__ballot(odd) == 0) {
+                    total = row_sum(total);
+                    const float em = exp0(-__builtin_fabsf(m));
+                    inv = live ? (m >= 0.f ? 1.f : em) / (total * (m >= 0.f ? em : 1.f)) : 0.f;
+                    lse = logf(total);
+                    sums = anynan && live ? __uint_as_float(0x7fc00000u) : sums;
 #pragma unroll
-            for (int i = 0; i < NS; ++i) c[i] *= inv;
+                    for (int i = 0; i < NS; ++i) psum[i] = __builtin_fmaf(c[i], sums, psum[i]);
+                } else {
+                    total = 0.f;
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) total += exp0(v[i] - m);
+                    total = row_sum(total);
+                    inv = live ? 1.f / total : 0.f;
+                    lse = m + logf(total);
+                    float f = far ? inv : sums;             // 0 where the token is not live
+                    f = anynan && live ? __uint_as_float(0x7fc00000u) : f;
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) psum[i] = __builtin_fmaf(far ? exp0(v[i] - m) : c[i], f, psum[i]);
+                }
+            }
         }
-        if (anynan) total = inv = sums = __uint_as_float(live ? 0x7fc00000u : 0u);
+        const float smax = SIG ? sigmoid2(m).x : inv;
+        if (anynan) lse = inv = sums = __uint_as_float(live ? 0x7fc00000u : 0u);
         if constexpr (TRAIN) {
-            const float lse = m + logf(total);
             zsum += live && sub == 0 ? lse * lse : 0.f;
             nlive += live && sub == 0;
-            const float f = far ? inv : sums;               // 0 where the token is not live
-#pragma unroll
-            for (int i = 0; i < NS; ++i) psum[i] = __builtin_fmaf(q[i], f, psum[i]);
         }
         uint32_t key[NS], lm = 0;
 #pragma unroll
