@@ -336,40 +336,45 @@ __global__ void __launch_bounds__(kRouteThreads) k_group_wave(const GroupArgs p)
 }
 
 // Logits expert(i) of the row at `base`, -inf for those past E and where the token is not
-// `in` (base: 0). vec: fours are aligned and whole. All loads are issued before the first
-// is used: an address past the row is replaced by the row's own start.
+// `in` (base: 0): whole, aligned fours fetched and later turned into values, or one by
+// one. All loads are issued before the first is used: an address past the row is replaced
+// by the row's own start.
+template <int LT> using RowFour = std::conditional_t<LT == VQK_F32, u32x4, u32x2>;
 template <int LT, int NS, typename Expert>
-__device__ __forceinline__ void row_load(const void *l, int64_t base, int E, bool in, bool vec, Expert expert, float (&v)[NS]) {
+__device__ __forceinline__ void row_fetch(const void *l, int64_t base, int E, Expert expert, RowFour<LT> (&f)[NS / 4]) {
     using T = std::conditional_t<LT == VQK_F32, float, uint16_t>;
     const T *row = static_cast<const T *>(l) + base;
-    if (vec) {
-        using Four = std::conditional_t<LT == VQK_F32, u32x4, u32x2>;
-        Four f[NS / 4];
 #pragma unroll
-        for (int q = 0; q < NS / 4; ++q) {
-            const int e = expert(4 * q);
-            f[q] = *reinterpret_cast<const Four *>(row + (e < E ? e : 0));
-        }
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const Four w = f[i / 4];
-            if constexpr (LT == VQK_F32) {
-                v[i] = __uint_as_float(w[i % 4]);
-            } else {
-                const uint16_t h = uint16_t(w[i % 4 / 2] >> (16 * (i & 1)));
-                v[i] = LT == VQK_BF16 ? bf16_to_f32(h) : h_to_f32(h);
-            }
-            v[i] = in && expert(i / 4 * 4) < E ? v[i] : -__builtin_inff();
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const int e = expert(i);
-            v[i] = load_act(row, LT, e < E ? e : 0);
-        }
-#pragma unroll
-        for (int i = 0; i < NS; ++i) v[i] = in && expert(i) < E ? v[i] : -__builtin_inff();
+    for (int q = 0; q < NS / 4; ++q) {
+        const int e = expert(4 * q);
+        f[q] = *reinterpret_cast<const RowFour<LT> *>(row + (e < E ? e : 0));
     }
+}
+template <int LT, int NS, typename Expert>
+__device__ __forceinline__ void row_values(const RowFour<LT> (&f)[NS / 4], int E, bool in, Expert expert, float (&v)[NS]) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const RowFour<LT> w = f[i / 4];
+        if constexpr (LT == VQK_F32) {
+            v[i] = __uint_as_float(w[i % 4]);
+        } else {
+            const uint16_t h = uint16_t(w[i % 4 / 2] >> (16 * (i & 1)));
+            v[i] = LT == VQK_BF16 ? bf16_to_f32(h) : h_to_f32(h);
+        }
+        v[i] = in && expert(i / 4 * 4) < E ? v[i] : -__builtin_inff();
+    }
+}
+template <int LT, int NS, typename Expert>
+__device__ __forceinline__ void row_each(const void *l, int64_t base, int E, bool in, Expert expert, float (&v)[NS]) {
+    using T = std::conditional_t<LT == VQK_F32, float, uint16_t>;
+    const T *row = static_cast<const T *>(l) + base;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int e = expert(i);
+        v[i] = load_act(row, LT, e < E ? e : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) v[i] = in && expert(i) < E ? v[i] : -__builtin_inff();
 }
 
 // ------------------------------------------------- sixteen lanes to a token
@@ -397,6 +402,7 @@ __global__ void __launch_bounds__(kRouteThreads, NS <= 16 ? 3 : 1) k_group16(con
     float *csh = reinterpret_cast<float *>(smem) + (threadIdx.x >> 6) * 64 * NS;
     int32_t *cnt = reinterpret_cast<int32_t *>(smem + kRouteWaves * 256 * NS);           // TRAIN: [16 NS], [16 NS]
     float *psh = reinterpret_cast<float *>(cnt + 16 * NS);
+    __shared__ __align__(16) float bsh[16 * NS];
     __shared__ uint64_t cands[kRouteWaves][4][kRouteCands];
     __shared__ uint64_t sel[kRouteWaves][4][kGroup16MaxK + 1];
     __shared__ float zsh[kRouteWaves];
@@ -411,11 +417,8 @@ __global__ void __launch_bounds__(kRouteThreads, NS <= 16 ? 3 : 1) k_group16(con
         __syncthreads();
     }
     // experts past E have logits of -inf: whatever their bias and group, they are not chosen
-    float bias[NS] = {};
-    if (p.bias) {
-#pragma unroll
-        for (int i = 0; i < NS; ++i) bias[i] = p.bias[min(group16_expert(i, sub0), p.E - 1)];
-    }
+    for (int e = threadIdx.x; e < 16 * NS; e += kRouteThreads) bsh[e] = p.bias ? p.bias[min(e, p.E - 1)] : 0.f;
+    __syncthreads();
     uint32_t gid[NS / 4] = {};                // the experts' groups, four to a word
     const uint32_t per = ((1u << 20) + p.gs - 1) / p.gs;    // e / gs = e per >> 20: e and gs are at most 512
 #pragma unroll
@@ -425,13 +428,25 @@ __global__ void __launch_bounds__(kRouteThreads, NS <= 16 ? 3 : 1) k_group16(con
     float zsum = 0.f;
     int nlive = 0;
     const int64_t t00 = (int64_t(blockIdx.x) * kRouteWaves + wave) * 4, stride = int64_t(gridDim.x) * kRouteWaves * 4;
+    // the next four tokens' logits are on their way while these are ranked
+    RowFour<LT> ahead[NS / 4];
+    bool in_next = false;
+    auto fetch = [&](int64_t t0, int sub, int E) {
+        const int64_t t = t0 + grp;
+        in_next = t < p.T && (!p.mask || p.mask[t] != 0);
+        if (vec) row_fetch<LT, NS>(p.l, in_next ? t * p.ld : 0, E, [=](int i) { return group16_expert(i, sub); }, ahead);
+    };
+    fetch(t00, sub0, p.E);                    // past the last token: the first row's
     for (int64_t t0 = t00; t0 < p.T; t0 += stride) {
         const int64_t t = t0 + grp;
-        const bool in = t < p.T && (!p.mask || p.mask[t] != 0);
         float v[NS], c[NS];
         int E = p.E, sub = sub0;
         asm volatile("" : "+s"(E), "+v"(sub));              // masks and places made anew: kept over the loop they spill
-        row_load<LT, NS>(p.l, in ? t * p.ld : 0, E, in, vec, [=](int i) { return group16_expert(i, sub); }, v);
+        const bool in = in_next;
+        const auto expert = [=](int i) { return group16_expert(i, sub); };
+        if (vec) row_values<LT, NS>(ahead, E, in, expert, v);
+        else row_each<LT, NS>(p.l, in ? t * p.ld : 0, E, in, expert, v);
+        fetch(t0 + stride, sub, E);
         float best = -__builtin_inff();
         bool isnan = false;
 #pragma unroll
@@ -505,6 +520,10 @@ __global__ void __launch_bounds__(kRouteThreads, NS <= 16 ? 3 : 1) k_group16(con
             zsum += live && sub == 0 ? lse * lse : 0.f;
             nlive += live && sub == 0;
         }
+        float bias[NS];
+#pragma unroll
+        for (int q = 0; q < NS / 4; ++q)
+            *reinterpret_cast<float4 *>(bias + 4 * q) = *reinterpret_cast<const float4 *>(bsh + group16_expert(4 * q, sub));
         uint32_t key[NS], lm = 0;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
@@ -736,7 +755,14 @@ __global__ void __launch_bounds__(kRouteThreads) k_group_bwd(const GroupBwdArgs 
         const float4 sv = in ? p.saved[t] : float4{0.f, 0.f, 0.f, 0.f};
         const bool live = sv.y != 0.f;        // a live token's sum is at most E
         float v[NS];
-        row_load<LT, NS>(p.l, live ? t * p.ld : 0, p.E, live, vec, [=](int i) { return 4 * L * (i / 4) + 4 * sub + i % 4; }, v);
+        const auto expert = [=](int i) { return 4 * L * (i / 4) + 4 * sub + i % 4; };
+        if (vec) {
+            RowFour<LT> f4[NS / 4];
+            row_fetch<LT, NS>(p.l, live ? t * p.ld : 0, p.E, expert, f4);
+            row_values<LT, NS>(f4, p.E, live, expert, v);
+        } else {
+            row_each<LT, NS>(p.l, live ? t * p.ld : 0, p.E, live, expert, v);
+        }
         int id = -1;
         float wdw = 0.f, w = 0.f;
         if (p.dw && live && sub < p.k) {
