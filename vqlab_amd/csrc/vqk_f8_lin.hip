@@ -93,7 +93,7 @@ struct F8Trans {
 };
 
 // 128 x 128 codes through LDS: 16 k of a weight row in per unit, 4 x 16 codes
-// turned by byte permutes, 16 weight rows of a k out.
+// turned by byte permutes, 16 weight rows of a k out. 5120 x 17408: 47 us (3.8 TB/s both ways).
 __global__ void __launch_bounds__(256) k_f8_trans(const F8Trans p) {
     constexpr int LD = 144;
     __shared__ __align__(16) uint8_t tile[128 * LD];    // [weight row][k]
