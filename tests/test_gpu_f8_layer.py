@@ -225,6 +225,35 @@ def test_rows_past_2_to_the_31_elements():
     assert torch.equal(gx[-3:], tx) and (gx[:-3] == 0).all() and torch.equal(gw, tw)
 
 
+def test_more_rows_than_a_launch_has_threads_for():
+    """2^25 rows and more: their waves are more than 2^31 threads."""
+    from vqlab_amd import fp8
+    N, C = (1 << 25) + 9, 16
+    x = torch.ones(N, C, device="cuda", dtype=torch.bfloat16)
+    x[-4:] = torch.randn(4, C, device="cuda", dtype=torch.bfloat16)
+    x[1 << 25] = 3.0
+    w = torch.randn(C, device="cuda", dtype=torch.bfloat16)
+    with torch.no_grad():
+        y = fp8.rms_norm(x, w)
+        assert torch.equal(y[-12:], fp8.rms_norm(x[-12:], w)) and torch.equal(y[:-9], y[:1].expand(N - 9, C))
+        rows, few = fp8.rms_norm_f8(x, w), fp8.rms_norm_f8(x[-12:], w)
+        assert torch.equal(rows.codes[-12:].view(torch.uint8), few.codes.view(torch.uint8))
+        assert torch.equal(rows.scales[-12:], few.scales)
+
+
+def test_8_bit_rows_far_apart():
+    """Rows 16 MB and more apart are laid out first."""
+    from vqlab_amd import fp8
+    lin = fp8.F8Linear.from_weight(torch.randn(64, 256, device="cuda"), "fp8")
+    q = fp8.f8_quantize(torch.randn(40, 256, device="cuda", dtype=torch.bfloat16))
+    room = torch.zeros(40, (1 << 24) + 256, device="cuda", dtype=torch.uint8)
+    room[:, :256] = q.codes.view(torch.uint8)
+    far = room[:, :256].view(fp8.F8)
+    assert far.stride(0) > 1 << 24
+    for n in (3, 40):
+        assert torch.equal(lin((far[:n], q.scales[:n])), lin((q.codes[:n], q.scales[:n])))
+
+
 @pytest.mark.parametrize("act", [None, "fp8"])
 def test_linears_past_2_to_the_31_elements(act):
     """x of more than 2^31 elements, then an output of as many: last rows as they are alone."""

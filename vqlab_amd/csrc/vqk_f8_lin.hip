@@ -14,6 +14,8 @@
 
 namespace vqk {
 
+constexpr int64_t kMostWgs = (1 << 24) - 1;   // workgroups of 256: a launch has fewer than 2^32 threads
+
 static size_t al256(size_t v) { return (v + 255) & ~size_t(255); }
 static bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -170,7 +172,7 @@ static int plain_product(F8Call c, const void *x, int32_t type, uint8_t *ws, hip
     const bool few = f8_rows_ok(c);
     if (type == VQK_F32 || !al16(x) || IN % (few ? 8 : kF8Block)) {
         const int64_t wgs = (N * (ld / 8) + 255) / 256;
-        if (wgs > INT32_MAX) return set_error(VQK_ENOTIMPL, "activations too large");
+        if (wgs > kMostWgs) return set_error(VQK_ENOTIMPL, "f8 linear: %lld rows of %lld", (long long)N, (long long)IN);
         uint16_t *out = reinterpret_cast<uint16_t *>(ws);
         const bool vec = al16(x) && (IN * act_size(type)) % 16 == 0;
         if (type == VQK_F32) hipLaunchKernelGGL((k_f8_stage16<VQK_F32>), dim3(unsigned(wgs)), dim3(256), 0, st, x, N, IN, ld, out, vec);
@@ -193,7 +195,8 @@ static int a8_product(F8Call c, const F8X &x, uint8_t *ws, hipStream_t st) {
     uint8_t *codes = ws;
     float *sx = reinterpret_cast<float *>(ws + code_bytes(c.g, N));
     const bool wide = wide_out(c.y_type);
-    const bool place = c.g.IN % 128 == 0 && x.ld % 16 == 0 && al16(x.codes);
+    // in place, if a tile's rows are within reach of 32-bit offsets
+    const bool place = c.g.IN % 128 == 0 && x.ld % 16 == 0 && x.ld < (1 << 24) && al16(x.codes);
     const bool ready = x.codes == ws;         // whole blocks here already
     int rc;
     c.x8 = x;
@@ -202,7 +205,7 @@ static int a8_product(F8Call c, const F8X &x, uint8_t *ws, hipStream_t st) {
         uint8_t *to = wide ? ws + code_bytes(c.g, N) + scale_bytes(c.g, N) : codes;
         const F8Stage s{x.codes, x.ld, N, c.g.IN, c.g.NC, x.scales, x.sn, x.sk, to, ready ? nullptr : sx};
         const int64_t pieces = N * c.g.NC * 8, wgs = (pieces + 255) / 256;
-        if (wgs > INT32_MAX) return set_error(VQK_ENOTIMPL, "f8 linear: too many rows");
+        if (wgs > kMostWgs) return set_error(VQK_ENOTIMPL, "f8 linear: %lld rows of %lld", (long long)N, (long long)c.g.IN);
         if (wide) hipLaunchKernelGGL((k_f8_stage8<true>), dim3(unsigned(wgs)), dim3(256), 0, st, s, pieces);
         else hipLaunchKernelGGL((k_f8_stage8<false>), dim3(unsigned(wgs)), dim3(256), 0, st, s, pieces);
         if ((rc = hip_status(hipGetLastError(), "8-bit row staging launch"))) return rc;

@@ -34,6 +34,7 @@ struct NormArgs {
     uint8_t *codes;                           // [N][C]
     float *scales;
     int64_t sn, sk;
+    int64_t row0;                             // first row of this launch
 };
 
 template <int CTRL>
@@ -92,7 +93,7 @@ __device__ __forceinline__ float round_to(float v) {
 template <int XT, int P, bool Q>
 __global__ void __launch_bounds__(64 * kNormMaxWaves) k_rms(const NormArgs p, bool vec, bool vecw) {
     __shared__ double part[kNormMaxWaves];
-    const int64_t row = blockIdx.x;
+    const int64_t row = p.row0 + blockIdx.x;
     float h[P][8], wt[P][8];
     double sum = 0.;
 #pragma unroll
@@ -283,11 +284,17 @@ static int64_t norm_bwd_wgs(int64_t N, int64_t C) {
 }
 
 template <int XT, bool Q>
-static int go_norm(const NormArgs &a, NormPlan pl, bool vec, bool vecw, hipStream_t st) {
-    const dim3 grid{unsigned(a.N)}, block{unsigned(64 * pl.w)};
-    if (pl.p == 1) hipLaunchKernelGGL((k_rms<XT, 1, Q>), grid, block, 0, st, a, vec, vecw);
-    else hipLaunchKernelGGL((k_rms<XT, 2, Q>), grid, block, 0, st, a, vec, vecw);
-    return hip_status(hipGetLastError(), "norm launch");
+static int go_norm(NormArgs a, NormPlan pl, bool vec, bool vecw, hipStream_t st) {
+    const dim3 block{unsigned(64 * pl.w)};
+    const int64_t most = (INT64_C(1) << 31) / block.x;      // a launch has fewer than 2^32 threads
+    for (; a.row0 < a.N; a.row0 += most) {
+        const dim3 grid{unsigned(a.N - a.row0 < most ? a.N - a.row0 : most)};
+        if (pl.p == 1) hipLaunchKernelGGL((k_rms<XT, 1, Q>), grid, block, 0, st, a, vec, vecw);
+        else hipLaunchKernelGGL((k_rms<XT, 2, Q>), grid, block, 0, st, a, vec, vecw);
+        const int rc = hip_status(hipGetLastError(), "norm launch");
+        if (rc) return rc;
+    }
+    return VQK_OK;
 }
 template <int XT>
 static int go_norm_bwd(const NormBwdArgs &a, NormPlan pl, unsigned wgs, bool vec, bool vecw, hipStream_t st) {
@@ -323,7 +330,7 @@ extern "C" int vqk_rms_norm(const void *x, int32_t type, int64_t N, int64_t C, i
     if (!x || !weight || (residual && !h) || (codes && !scales)) return set_error(VQK_EINVAL, "rms norm: NULL pointer");
     if (scale_row < 0 || scale_block < 0) return set_error(VQK_EINVAL, "rms norm: negative stride of scales");
     const int esz = act_size(type);
-    const NormArgs a{x, residual, weight, N, ldx, ldr, int32_t(C), w_type, eps, h, y, r, codes, scales, scale_row, scale_block};
+    const NormArgs a{x, residual, weight, N, ldx, ldr, int32_t(C), w_type, eps, h, y, r, codes, scales, scale_row, scale_block, 0};
     const bool vec = C % 8 == 0 && al16(x) && (ldx * esz) % 16 == 0 &&
                      (!residual || (al16(residual) && (ldr * esz) % 16 == 0 && al16(h))) &&
                      (y ? al16(y) : (reinterpret_cast<uintptr_t>(codes) & 7) == 0);

@@ -59,7 +59,7 @@ template <int OP, int BN, bool SX, int NST>
 static int go(const F8tArgs &a, hipStream_t st) {
     static_assert(NST * f8t_stage(OP, BN, SX) <= kLdsBytes, "the ring fits LDS");
     const int64_t grid = a.full + int64_t(a.tiles - a.full) * a.splits;
-    if (a.tiles == INT32_MAX || grid > INT32_MAX) return set_error(VQK_ENOTIMPL, "8-bit product: grid too large");
+    if (a.tiles == INT32_MAX || grid >= 1 << 23) return set_error(VQK_ENOTIMPL, "8-bit product: grid too large");
     const int rc = launch_with_lds<k_f8_tiles<OP, BN, SX, NST>>(dim3(unsigned(grid)), dim3(512), size_t(NST) * f8t_stage(OP, BN, SX), st, a);
     if (rc || a.tiles == a.full) return rc;
     hipLaunchKernelGGL(k_f8_reduce<BN>, dim3(BN * kF8tRows / 1024, unsigned(a.tiles - a.full)), dim3(256), 0, st, a);
