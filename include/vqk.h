@@ -529,14 +529,16 @@ int vqk_f8_unpack(const uint8_t *packed, int64_t OUT, int64_t IN, uint8_t *codes
  * the largest of eight neighbouring products and what lines up with it of the others;
  * into an fp32 y every product enters exactly.
  * vqk_f8_linear_rows takes rows that are in 8 bits already (codes ldc apart, scales
- * as above). Workspaces are 256-byte aligned and hold nothing between calls. */
+ * as above). x of act NONE, codes and dy are 16-byte aligned (VQK_EINVAL); workspaces are
+ * 256-byte aligned (NULL where a query says 0) and hold nothing between calls. */
 #define VQK_F8_ACT_NONE 0
 #define VQK_F8_ACT_F8   1
 int vqk_f8_linear_workspace(const vqk_f8_weights *w, int32_t x_type, int64_t N, int32_t act,
                             int32_t y_type, size_t *bytes);
 int vqk_f8_linear(const vqk_f8_weights *w, const void *x, int32_t x_type, int64_t N, int32_t act,
                   void *y, int32_t y_type, void *workspace, size_t ws_bytes, void *stream);
-int vqk_f8_linear_rows_workspace(const vqk_f8_weights *w, int64_t N, int32_t y_type, size_t *bytes);
+int vqk_f8_linear_rows_workspace(const vqk_f8_weights *w, int64_t ldc, int64_t N, int32_t y_type,
+                                 size_t *bytes);
 int vqk_f8_linear_rows(const vqk_f8_weights *w, const uint8_t *codes, int64_t ldc,
                        const float *scales, int64_t scale_row, int64_t scale_block, int64_t N,
                        void *y, int32_t y_type, void *workspace, size_t ws_bytes, void *stream);

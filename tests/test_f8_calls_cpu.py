@@ -23,6 +23,18 @@ def refused(lib, call, rc):
     assert lib.vqk_last_error()
 
 
+def test_workspaces(lib):
+    """What a call reads in place takes none."""
+    w, n = ctypes.byref(L.VQKF8Weights(P, P, 256, 512)), ctypes.c_size_t()
+    size = lambda q, *a: (q(w, *a, ctypes.byref(n)), n.value)
+    assert size(lib.vqk_f8_linear_workspace, L.VQK_BF16, 4, L.VQK_F8_ACT_NONE, L.VQK_BF16) == (0, 0)
+    assert size(lib.vqk_f8_linear_workspace, L.VQK_F32, 4, L.VQK_F8_ACT_NONE, L.VQK_F32) == (0, 3 * 4 * 512 * 2)
+    assert size(lib.vqk_f8_linear_workspace, L.VQK_BF16, 4, L.VQK_F8_ACT_F8, L.VQK_BF16) == (0, 4 * 512 + 256)
+    assert size(lib.vqk_f8_linear_rows_workspace, 512, 4, L.VQK_BF16) == (0, 0)
+    assert size(lib.vqk_f8_linear_rows_workspace, 520, 4, L.VQK_BF16) == (0, 4 * 512 + 256)
+    assert size(lib.vqk_f8_linear_rows_workspace, 512, 4, L.VQK_F32) == (0, 4 * 512 + 256 + 4 * 1024)
+
+
 def test_sizes_of_zero_rows_need_nothing(lib):
     """No rows: nothing is read or launched, whatever the addresses."""
     w = L.VQKF8Weights(P, P, 256, 512)
@@ -72,7 +84,7 @@ def test_pack(lib):
     refused(lib, lib.vqk_f8_unpack(P + 4, 16, 128, P, None), L.VQK_EINVAL)
 
 
-LINEAR = dict(codes=P, scales=P, out=256, inp=512, x=P, xt=L.VQK_BF16, n=4, act=L.VQK_F8_ACT_NONE, y=P, yt=L.VQK_BF16,
+LINEAR = dict(codes=P, scales=P, out=256, inp=500, x=P, xt=L.VQK_BF16, n=4, act=L.VQK_F8_ACT_NONE, y=P, yt=L.VQK_BF16,
               ws=P, short=0)
 
 
@@ -88,7 +100,7 @@ def linear(lib, a):
     (dict(codes=None), L.VQK_EINVAL), (dict(scales=None), L.VQK_EINVAL), (dict(codes=P + 8), L.VQK_EINVAL),
     (dict(out=0), L.VQK_EINVAL), (dict(inp=-1), L.VQK_EINVAL), (dict(n=-1), L.VQK_EINVAL),
     (dict(xt=L.VQK_U32), L.VQK_EINVAL), (dict(yt=L.VQK_U8), L.VQK_EINVAL), (dict(act=2), L.VQK_EINVAL),
-    (dict(x=None), L.VQK_EINVAL), (dict(y=None), L.VQK_EINVAL),
+    (dict(x=None), L.VQK_EINVAL), (dict(y=None), L.VQK_EINVAL), (dict(x=P + 8), L.VQK_EINVAL),
     (dict(ws=P + 64), L.VQK_EINVAL), (dict(ws=None), L.VQK_ENOSPACE), (dict(short=1), L.VQK_ENOSPACE)])
 def test_linear(lib, change, rc):
     refused(lib, linear(lib, LINEAR | change), rc)
@@ -97,19 +109,20 @@ def test_linear(lib, change, rc):
 @pytest.mark.parametrize("change,rc", [
     (dict(x=None), L.VQK_EINVAL), (dict(sc=None), L.VQK_EINVAL), (dict(ld=511), L.VQK_EINVAL),
     (dict(sn=-1), L.VQK_EINVAL), (dict(sk=-1), L.VQK_EINVAL), (dict(y=None), L.VQK_EINVAL),
+    (dict(x=P + 8), L.VQK_EINVAL),
     (dict(yt=L.VQK_I64), L.VQK_EINVAL), (dict(ws=P + 16), L.VQK_EINVAL), (dict(short=1), L.VQK_ENOSPACE)])
 def test_linear_of_rows(lib, change, rc):
     a = dict(x=P, ld=512, sc=P, sn=1, sk=4, n=4, y=P, yt=L.VQK_F32, ws=P, short=0) | change
     w = ctypes.byref(L.VQKF8Weights(P, P, 256, 512))
     n = ctypes.c_size_t()
-    if lib.vqk_f8_linear_rows_workspace(w, a["n"], a["yt"], ctypes.byref(n)):
+    if lib.vqk_f8_linear_rows_workspace(w, a["ld"], a["n"], a["yt"], ctypes.byref(n)):
         n.value = 1 << 40
     refused(lib, lib.vqk_f8_linear_rows(w, a["x"], a["ld"], a["sc"], a["sn"], a["sk"], a["n"], a["y"], a["yt"], a["ws"],
                                         n.value - a["short"], None), rc)
 
 
 @pytest.mark.parametrize("change,rc", [
-    (dict(dy=None), L.VQK_EINVAL), (dict(dx=None), L.VQK_EINVAL), (dict(dt=L.VQK_U16), L.VQK_EINVAL),
+    (dict(dy=None), L.VQK_EINVAL), (dict(dy=P + 4), L.VQK_EINVAL), (dict(dx=None), L.VQK_EINVAL), (dict(dt=L.VQK_U16), L.VQK_EINVAL),
     (dict(yt=7), L.VQK_EINVAL), (dict(ws=P + 128), L.VQK_EINVAL), (dict(short=1), L.VQK_ENOSPACE)])
 def test_linear_gradient(lib, change, rc):
     a = dict(dy=P, dt=L.VQK_F16, n=4, dx=P, yt=L.VQK_F16, ws=P, short=0) | change

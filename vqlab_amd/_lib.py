@@ -144,7 +144,7 @@ SIGNATURES = {
     "vqk_f8_unpack": (c_i32, [c_p, c_i64, c_i64, c_p, c_p]),
     "vqk_f8_linear_workspace": (c_i32, [_F8W, c_i32, c_i64, c_i32, c_i32, ctypes.POINTER(c_sz)]),
     "vqk_f8_linear": (c_i32, [_F8W, c_p, c_i32, c_i64, c_i32, c_p, c_i32, c_p, c_sz, c_p]),
-    "vqk_f8_linear_rows_workspace": (c_i32, [_F8W, c_i64, c_i32, ctypes.POINTER(c_sz)]),
+    "vqk_f8_linear_rows_workspace": (c_i32, [_F8W, c_i64, c_i64, c_i32, ctypes.POINTER(c_sz)]),
     "vqk_f8_linear_rows": (c_i32, [_F8W, c_p, c_i64, c_p, c_i64, c_i64, c_i64, c_p, c_i32, c_p, c_sz, c_p]),
     "vqk_f8_linear_dx_workspace": (c_i32, [_F8W, c_i32, c_i64, ctypes.POINTER(c_sz)]),
     "vqk_f8_linear_dx": (c_i32, [_F8W, c_p, c_i32, c_i64, c_p, c_i32, c_p, c_sz, c_p]),

@@ -5,7 +5,7 @@
 // 8-bit rows run on the 8-bit matrix instructions where the output has 16 bits, and
 // as the codes' values in bf16 where it has 32 (vqk_f8.h).
 // bf16 x enters as it is, fp16 x too (every e4m3 code is an fp16 number), fp32 x as
-// three exact bf16 planes. x that is 16-byte aligned and a multiple of 8 wide is
+// three exact bf16 planes. x that is a multiple of 8 wide is
 // read in place (many rows: whole blocks wide), other x is laid out in the workspace first. The gradient sums over
 // the weight's rows, along which its codes do not lie: they are transposed into the
 // workspace, operand order to operand order, and the same products run on them with
@@ -138,24 +138,57 @@ static int check_lin(const vqk_f8_weights *w, int64_t N, F8Geom *g, const char *
     return VQK_OK;
 }
 
-// x as it is: its layout in the workspace (sized as if it had to be laid out).
+// x as it is: its layout in the workspace, where it cannot be read in place (few rows are
+// read in pieces of 8, many in whole blocks), then the K slices of tiles.
 static int x_planes(int32_t type) { return type == VQK_F32 ? 3 : 1; }
-static size_t x_bytes(int64_t N, const F8Geom &g, int32_t type) { return al256(size_t(N) * g.NC * 256 * x_planes(type)); }
-static size_t plain_bytes(const F8Geom &g, int32_t type, int64_t N) {
-    return x_bytes(N, g, type) + f8_tiles_part(N, g, false, false, x_planes(type));
+struct PlainPlan { bool few, lay; size_t x, part; };
+static PlainPlan plain_plan(const F8Geom &g, int32_t type, int64_t N) {
+    F8Call c{};
+    c.g = g;
+    c.N = N;
+    c.x.P = x_planes(type);
+    c.x.op = type == VQK_F16 ? kOpF16 : kOpBF16;
+    PlainPlan p{};
+    p.few = f8_rows_ok(c);
+    p.lay = type == VQK_F32 || g.IN % (p.few ? 8 : kF8Block);
+    p.x = p.lay ? al256(size_t(N) * g.NC * 256 * c.x.P) : 0;
+    p.part = p.few ? 0 : f8_tiles_part(N, g, false, false, c.x.P);
+    return p;
 }
-// 8-bit x: rows of whole blocks and their scales (and for an fp32 output the codes'
-// values after them), then the K slices.
+static size_t plain_bytes(const F8Geom &g, int32_t type, int64_t N) {
+    const PlainPlan p = plain_plan(g, type, N);
+    return p.x + p.part;
+}
+// 8-bit x that is not in place: rows of whole blocks and their scales (and for an fp32
+// output the codes' values after them); then the K slices.
 static bool wide_out(int32_t y_type) { return (y_type & ~VQK_VIA_F16) == VQK_F32; }
 static size_t code_bytes(const F8Geom &g, int64_t N) { return al256(size_t(N) * g.NC * 128); }
 static size_t scale_bytes(const F8Geom &g, int64_t N) { return al256(size_t(N) * g.NC * 4); }
 static size_t rows_bytes(const F8Geom &g, int64_t N, int32_t y_type) {
     return code_bytes(g, N) + scale_bytes(g, N) + (wide_out(y_type) ? al256(size_t(N) * g.NC * 256) : 0);
 }
-static size_t a8_part(const F8Geom &g, int64_t N, int32_t y_type) {
-    return f8_tiles_part(N, g, !wide_out(y_type), true, 1);
+struct A8Plan { bool few, place; size_t x, part; };
+// ldc: bytes between rows that are in 8 bits already, 0 for rows quantised here.
+static A8Plan a8_plan(const F8Geom &g, int64_t N, int64_t ldc, int32_t y_type) {
+    const bool wide = wide_out(y_type);
+    F8Call c{};
+    c.g = g;
+    c.N = N;
+    c.a8 = !wide;
+    c.x.P = 1;
+    c.x.op = kOpBF16;
+    A8Plan p{};
+    p.few = f8_rows_ok(c);
+    // in place, if a tile's rows are within reach of 32-bit offsets
+    p.place = ldc && !wide && g.IN % 128 == 0 && ldc % 16 == 0 && ldc < (1 << 24);
+    p.x = p.place ? 0 : rows_bytes(g, N, y_type);
+    p.part = p.few ? 0 : f8_tiles_part(N, g, !wide, true, 1);
+    return p;
 }
-static size_t a8_bytes(const F8Geom &g, int64_t N, int32_t y_type) { return rows_bytes(g, N, y_type) + a8_part(g, N, y_type); }
+static size_t a8_bytes(const F8Geom &g, int64_t N, int64_t ldc, int32_t y_type) {
+    const A8Plan p = a8_plan(g, N, ldc, y_type);
+    return p.x + p.part;
+}
 
 static int check_ws(const char *what, size_t need, const void *ws, size_t ws_bytes) {
     if (need && (!ws || ws_bytes < need)) return set_error(VQK_ENOSPACE, "%s: workspace %zu < %zu", what, ws_bytes, need);
@@ -163,18 +196,16 @@ static int check_ws(const char *what, size_t need, const void *ws, size_t ws_byt
     return VQK_OK;
 }
 
-// The product of x as it is; ws: plain_bytes. Few rows are read in pieces of 8, many in
-// whole blocks.
+// The product of x (16-byte aligned) as it is; ws: plain_bytes.
 static int plain_product(F8Call c, const void *x, int32_t type, uint8_t *ws, hipStream_t st) {
     const int64_t N = c.N, IN = c.g.IN, ld = c.g.NC * kF8Block;
-    const int P = x_planes(type);
-    c.x = MxX{static_cast<const uint16_t *>(x), IN, 0, P, type == VQK_F16 ? kOpF16 : kOpBF16};
-    const bool few = f8_rows_ok(c);
-    if (type == VQK_F32 || !al16(x) || IN % (few ? 8 : kF8Block)) {
+    const PlainPlan p = plain_plan(c.g, type, N);
+    c.x = MxX{static_cast<const uint16_t *>(x), IN, 0, x_planes(type), type == VQK_F16 ? kOpF16 : kOpBF16};
+    if (p.lay) {
         const int64_t wgs = (N * (ld / 8) + 255) / 256;
         if (wgs > kMostWgs) return set_error(VQK_ENOTIMPL, "f8 linear: %lld rows of %lld", (long long)N, (long long)IN);
         uint16_t *out = reinterpret_cast<uint16_t *>(ws);
-        const bool vec = al16(x) && (IN * act_size(type)) % 16 == 0;
+        const bool vec = (IN * act_size(type)) % 16 == 0;
         if (type == VQK_F32) hipLaunchKernelGGL((k_f8_stage16<VQK_F32>), dim3(unsigned(wgs)), dim3(256), 0, st, x, N, IN, ld, out, vec);
         else hipLaunchKernelGGL((k_f8_stage16<VQK_F16>), dim3(unsigned(wgs)), dim3(256), 0, st, x, N, IN, ld, out, vec);   // 16 bits as they are
         const int rc = hip_status(hipGetLastError(), "x staging launch");
@@ -184,39 +215,34 @@ static int plain_product(F8Call c, const void *x, int32_t type, uint8_t *ws, hip
         c.x.plane = N * ld;
         c.g.IN = ld;
     }
-    if (few) return f8_rows(c, st);
-    const size_t part = f8_tiles_part(N, c.g, false, false, P);
-    return f8_tiles(c, part ? reinterpret_cast<float *>(ws + x_bytes(N, c.g, type)) : nullptr, part, st);
+    if (p.few) return f8_rows(c, st);
+    return f8_tiles(c, p.part ? reinterpret_cast<float *>(ws + p.x) : nullptr, p.part, st);
 }
 
-// The product of 8-bit rows; ws: a8_bytes (x's codes and scales may be at its start).
-static int a8_product(F8Call c, const F8X &x, uint8_t *ws, hipStream_t st) {
+// The product of 8-bit rows; ws: a8_bytes. here: they are whole blocks at its start, with
+// their scales after them.
+static int a8_product(F8Call c, const F8X &x, bool here, uint8_t *ws, hipStream_t st) {
     const int64_t N = c.N;
-    uint8_t *codes = ws;
-    float *sx = reinterpret_cast<float *>(ws + code_bytes(c.g, N));
+    const A8Plan p = a8_plan(c.g, N, here ? 0 : x.ld, c.y_type);
     const bool wide = wide_out(c.y_type);
-    // in place, if a tile's rows are within reach of 32-bit offsets
-    const bool place = c.g.IN % 128 == 0 && x.ld % 16 == 0 && x.ld < (1 << 24) && al16(x.codes);
-    const bool ready = x.codes == ws;         // whole blocks here already
-    int rc;
     c.x8 = x;
     c.a8 = !wide;
-    if (wide || !(place || ready)) {
-        uint8_t *to = wide ? ws + code_bytes(c.g, N) + scale_bytes(c.g, N) : codes;
-        const F8Stage s{x.codes, x.ld, N, c.g.IN, c.g.NC, x.scales, x.sn, x.sk, to, ready ? nullptr : sx};
+    if (wide || !(p.place || here)) {
+        uint8_t *to = wide ? ws + code_bytes(c.g, N) + scale_bytes(c.g, N) : ws;
+        float *sx = reinterpret_cast<float *>(ws + code_bytes(c.g, N));
+        const F8Stage s{x.codes, x.ld, N, c.g.IN, c.g.NC, x.scales, x.sn, x.sk, to, here ? nullptr : sx};
         const int64_t pieces = N * c.g.NC * 8, wgs = (pieces + 255) / 256;
         if (wgs > kMostWgs) return set_error(VQK_ENOTIMPL, "f8 linear: %lld rows of %lld", (long long)N, (long long)c.g.IN);
         if (wide) hipLaunchKernelGGL((k_f8_stage8<true>), dim3(unsigned(wgs)), dim3(256), 0, st, s, pieces);
         else hipLaunchKernelGGL((k_f8_stage8<false>), dim3(unsigned(wgs)), dim3(256), 0, st, s, pieces);
-        if ((rc = hip_status(hipGetLastError(), "8-bit row staging launch"))) return rc;
-        c.x8 = F8X{codes, c.g.NC * 128, ready ? x.scales : sx, ready ? x.sn : 1, ready ? x.sk : N};
+        const int rc = hip_status(hipGetLastError(), "8-bit row staging launch");
+        if (rc) return rc;
+        c.x8 = F8X{ws, c.g.NC * 128, here ? x.scales : sx, here ? x.sn : 1, here ? x.sk : N};
         if (wide) c.x = MxX{reinterpret_cast<uint16_t *>(to), c.g.NC * 128, 0, 1, kOpBF16};
     }
     if (wide) c.g.IN = c.g.NC * 128;          // x's rows are whole blocks, zero past the weight's columns
-    if (f8_rows_ok(c)) return f8_rows(c, st);
-    const size_t part = a8_part(c.g, N, c.y_type);
-    float *at = part ? reinterpret_cast<float *>(ws + rows_bytes(c.g, N, c.y_type)) : nullptr;
-    return f8_tiles(c, at, part, st);
+    if (p.few) return f8_rows(c, st);
+    return f8_tiles(c, p.part ? reinterpret_cast<float *>(ws + p.x) : nullptr, p.part, st);
 }
 
 static F8Call base_call(const vqk_f8_weights *w, const F8Geom &g, int64_t N, bool a8, void *y, int32_t y_type) {
@@ -248,7 +274,7 @@ extern "C" int vqk_f8_linear_workspace(const vqk_f8_weights *w, int32_t x_type, 
     if (rc || (rc = check_act(act, x_type))) return rc;
     if (!out_size(y_type)) return set_error(VQK_EINVAL, "f8 linear: y type %d", y_type);
     if (!bytes) return set_error(VQK_EINVAL, "f8 linear: NULL bytes");
-    *bytes = N == 0 ? 0 : (act == VQK_F8_ACT_F8 ? a8_bytes(g, N, y_type) : plain_bytes(g, x_type, N));
+    *bytes = N == 0 ? 0 : (act == VQK_F8_ACT_F8 ? a8_bytes(g, N, 0, y_type) : plain_bytes(g, x_type, N));
     return VQK_OK;
 }
 
@@ -260,7 +286,8 @@ extern "C" int vqk_f8_linear(const vqk_f8_weights *w, const void *x, int32_t x_t
     if (!out_size(y_type)) return set_error(VQK_EINVAL, "f8 linear: y type %d", y_type);
     if (N == 0) return VQK_OK;
     if (!x || !y) return set_error(VQK_EINVAL, "f8 linear: NULL pointer");
-    const size_t need = act == VQK_F8_ACT_F8 ? a8_bytes(g, N, y_type) : plain_bytes(g, x_type, N);
+    if (act == VQK_F8_ACT_NONE && !al16(x)) return set_error(VQK_EINVAL, "f8 linear: x must be 16-byte aligned");
+    const size_t need = act == VQK_F8_ACT_F8 ? a8_bytes(g, N, 0, y_type) : plain_bytes(g, x_type, N);
     if ((rc = check_ws("f8 linear", need, workspace, ws_bytes))) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     uint8_t *ws = static_cast<uint8_t *>(workspace);
@@ -269,11 +296,18 @@ extern "C" int vqk_f8_linear(const vqk_f8_weights *w, const void *x, int32_t x_t
     float *sx = reinterpret_cast<float *>(ws + code_bytes(g, N));
     const F8Quant q{x, N, g.IN, g.IN, ws, g.NC * 128, g.NC * 128, sx, 1, N};
     if ((rc = launch_f8_quant(q, x_type, st))) return rc;
-    return a8_product(c, F8X{ws, g.NC * 128, sx, 1, N}, ws, st);
+    return a8_product(c, F8X{ws, g.NC * 128, sx, 1, N}, true, ws, st);
 }
 
-extern "C" int vqk_f8_linear_rows_workspace(const vqk_f8_weights *w, int64_t N, int32_t y_type, size_t *bytes) {
-    return vqk_f8_linear_workspace(w, VQK_F32, N, VQK_F8_ACT_F8, y_type, bytes);
+extern "C" int vqk_f8_linear_rows_workspace(const vqk_f8_weights *w, int64_t ldc, int64_t N, int32_t y_type, size_t *bytes) {
+    F8Geom g;
+    const int rc = check_lin(w, N, &g, "f8 linear of rows");
+    if (rc) return rc;
+    if (!out_size(y_type)) return set_error(VQK_EINVAL, "f8 linear of rows: y type %d", y_type);
+    if (ldc < g.IN) return set_error(VQK_EINVAL, "f8 linear of rows: rows %lld apart", (long long)ldc);
+    if (!bytes) return set_error(VQK_EINVAL, "f8 linear of rows: NULL bytes");
+    *bytes = N == 0 ? 0 : a8_bytes(g, N, ldc, y_type);
+    return VQK_OK;
 }
 
 extern "C" int vqk_f8_linear_rows(const vqk_f8_weights *w, const uint8_t *codes, int64_t ldc, const float *scales,
@@ -287,8 +321,9 @@ extern "C" int vqk_f8_linear_rows(const vqk_f8_weights *w, const uint8_t *codes,
         return set_error(VQK_EINVAL, "f8 linear of rows: strides %lld, %lld, %lld", (long long)ldc, (long long)scale_row, (long long)scale_block);
     if (N == 0) return VQK_OK;
     if (!codes || !scales || !y) return set_error(VQK_EINVAL, "f8 linear of rows: NULL pointer");
-    if ((rc = check_ws("f8 linear of rows", a8_bytes(g, N, y_type), workspace, ws_bytes))) return rc;
-    return a8_product(base_call(w, g, N, true, y, y_type), F8X{codes, ldc, scales, scale_row, scale_block},
+    if (!al16(codes)) return set_error(VQK_EINVAL, "f8 linear of rows: codes must be 16-byte aligned");
+    if ((rc = check_ws("f8 linear of rows", a8_bytes(g, N, ldc, y_type), workspace, ws_bytes))) return rc;
+    return a8_product(base_call(w, g, N, true, y, y_type), F8X{codes, ldc, scales, scale_row, scale_block}, false,
                       static_cast<uint8_t *>(workspace), static_cast<hipStream_t>(stream));
 }
 
@@ -311,6 +346,7 @@ extern "C" int vqk_f8_linear_dx(const vqk_f8_weights *w, const void *dy, int32_t
     if (!act_size(type) || !out_size(dx_type)) return set_error(VQK_EINVAL, "f8 linear dx: types %d, %d", type, dx_type);
     if (N == 0) return VQK_OK;
     if (!dy || !dx) return set_error(VQK_EINVAL, "f8 linear dx: NULL pointer");
+    if (!al16(dy)) return set_error(VQK_EINVAL, "f8 linear dx: dy must be 16-byte aligned");
     const F8Geom t = transposed(g);
     const size_t codes = al256(f8_code_bytes(t.RT, t.NC));
     if (f8_code_bytes(t.RT, t.NC) > INT64_C(0xffffffff) || t.NC > 65535)

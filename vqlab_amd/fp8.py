@@ -44,6 +44,11 @@ def _rows_in(x, C):
     return x, x.numel() // C if C else 0, C
 
 
+def _aligned(x):
+    """x, or a copy of it, at an address that the products read from."""
+    return x.clone() if x.data_ptr() & 15 else x
+
+
 def _rows_out(like, lead, n, C):
     """Room for rows [*lead, C] in 8 bits."""
     codes = like.new_empty((*lead, C), dtype=F8)
@@ -133,8 +138,10 @@ def f8_dequantize(codes, scales, dtype=torch.bfloat16):
         else:
             rows, ldc, sc, so, sk, n = _strided(codes, scales, C, "f8_dequantize")
         out = codes.new_empty(codes.shape, dtype=dtype)
-        L.check(L.lib().vqk_f8_dequantize(rows.data_ptr(), ldc, sc.data_ptr(), so, sk, per, n, C, out.data_ptr(),
-                                          T.ACT_TYPES[dtype], T.raw_stream(codes)), "f8_dequantize")
+        rc = L.lib().vqk_f8_dequantize(rows.data_ptr(), ldc, sc.data_ptr(), so, sk, per, n, C, out.data_ptr(),
+                                       T.ACT_TYPES[dtype], T.raw_stream(codes))
+        if rc:
+            L.check(rc, "f8_dequantize")
     return out
 
 
@@ -204,7 +211,7 @@ class F8Linear(torch.nn.Module):
 
     def _keep(self, packed, scales):
         self._packed = (packed, scales)
-        self._w = L.VQKF8Weights(packed.data_ptr(), scales.data_ptr(), self.out_features, self.in_features)
+        self._w = ctypes.byref(L.VQKF8Weights(packed.data_ptr(), scales.data_ptr(), self.out_features, self.in_features))
 
     @property
     def codes(self):
@@ -263,11 +270,11 @@ class F8Linear(torch.nn.Module):
     def _product(self, x, out_dtype):
         IN, OUT = self.in_features, self.out_features
         act = L.VQK_F8_ACT_NONE if self.act is None else L.VQK_F8_ACT_F8
-        xt, yt, lib, w = T.act_type(x), T.ACT_TYPES[out_dtype], L.lib(), ctypes.byref(self._w)
+        xt, yt, lib, w = T.act_type(x), T.ACT_TYPES[out_dtype], L.lib(), self._w
         with T.on_device(x):
-            xf = T.rows_of(x, IN)
+            xf = _aligned(T.rows_of(x, IN))
             N = xf.shape[0]
-            y = torch.empty((*x.shape[:-1], OUT), dtype=out_dtype, device=x.device)
+            y = x.new_empty((*x.shape[:-1], OUT), dtype=out_dtype)
             size = _ws_bytes(self._sizes, (N, xt, yt), lib.vqk_f8_linear_workspace, w, xt, N, act, yt)
             work, wp = _work(x, size)
             rc = lib.vqk_f8_linear(w, xf.data_ptr(), xt, N, act, y.data_ptr(), yt, wp, size, T.raw_stream(x))
@@ -276,12 +283,14 @@ class F8Linear(torch.nn.Module):
         return y
 
     def _rows_product(self, rows, out_dtype):
-        lib, w = L.lib(), ctypes.byref(self._w)
+        lib, w = L.lib(), self._w
         with T.on_device(rows.codes):
             codes, ldc, scales, sn, sk, N = _strided(*rows, self.in_features, "F8Linear")
-            y = torch.empty((*rows.codes.shape[:-1], self.out_features), dtype=out_dtype, device=codes.device)
+            if codes.data_ptr() & 15:
+                codes, ldc = codes.clone(memory_format=torch.contiguous_format), self.in_features
+            y = scales.new_empty((*rows.codes.shape[:-1], self.out_features), dtype=out_dtype)
             yt = T.ACT_TYPES[out_dtype]
-            size = _ws_bytes(self._sizes, (N, "rows", yt), lib.vqk_f8_linear_rows_workspace, w, N, yt)
+            size = _ws_bytes(self._sizes, (N, ldc, yt, "rows"), lib.vqk_f8_linear_rows_workspace, w, ldc, N, yt)
             work, wp = _work(codes, size)
             rc = lib.vqk_f8_linear_rows(w, codes.data_ptr(), ldc, scales.data_ptr(), sn, sk, N, y.data_ptr(),
                                         yt, wp, size, T.raw_stream(codes))
@@ -291,9 +300,9 @@ class F8Linear(torch.nn.Module):
 
     def _dx(self, dy, dtype):
         IN, OUT = self.in_features, self.out_features
-        dt, lib, w = T.act_type(dy), L.lib(), ctypes.byref(self._w)
+        dt, lib, w = T.act_type(dy), L.lib(), self._w
         with T.on_device(dy):
-            d = T.rows_of(dy, OUT)
+            d = _aligned(T.rows_of(dy, OUT))
             N = d.shape[0]
             dx = torch.empty((*dy.shape[:-1], IN), dtype=dtype, device=dy.device)
             size = _ws_bytes(self._sizes, (N, dt, "dx"), lib.vqk_f8_linear_dx_workspace, w, dt, N)
@@ -352,8 +361,10 @@ def _norm(x, weight, eps, residual, f8, want_r):
         else:
             y = x.new_empty(x.shape)
         at = [None if t is None else t.data_ptr() for t in (res, h, y, r, codes, scales)]
-        L.check(L.lib().vqk_rms_norm(rows.data_ptr(), T.act_type(x), n, C, ld, at[0], ldr, w.data_ptr(), T.act_type(w),
-                                     float(eps), at[1], at[2], at[3], at[4], at[5], 1, n, T.raw_stream(x)), "rms_norm")
+        rc = L.lib().vqk_rms_norm(rows.data_ptr(), T.act_type(x), n, C, ld, at[0], ldr, w.data_ptr(), T.act_type(w),
+                                  float(eps), at[1], at[2], at[3], at[4], at[5], 1, n, T.raw_stream(x))
+        if rc:
+            L.check(rc, "rms_norm")
     return h, r, F8Rows(codes, view) if f8 else y
 
 

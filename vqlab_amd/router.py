@@ -141,8 +141,8 @@ def _top_k(logits, k, norm_topk_prob, mask, f):
         m = mask_bytes(mask, lg)
         mp = None if m is None else m.data_ptr()
         n, E = lg.shape
-        ids = torch.empty((n, k), dtype=torch.int32, device=lg.device)
-        w = torch.empty((n, k), dtype=torch.float32, device=lg.device)
+        ids = lg.new_empty((n, k), dtype=torch.int32)
+        w = lg.new_empty((n, k), dtype=torch.float32)
         if f.plain:
             rc = L.lib().vqk_route(lg.data_ptr(), T.act_type(lg), n, E, ld, mp, k, int(norm_topk_prob),
                                    ids.data_ptr(), w.data_ptr(), None, None, None, None, 0, T.raw_stream(lg))
