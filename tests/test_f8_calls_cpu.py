@@ -202,7 +202,7 @@ def test_route_arguments(lib):
 @pytest.mark.parametrize("change,words", [
     (dict(score="tanh"), "score must be"), (dict(groups=0), "0 groups"), (dict(groups=7), "7 groups"),
     (dict(groups=8, top_groups=9), "top 9 of 8"), (dict(groups=8, top_groups=0), "top 0 of 8"),
-    (dict(groups=8, group_top=3), "from 3 of 8"), (dict(groups=64, group_top=2), "from 2 of 1"),
+    (dict(groups=8, group_top=3), "from 3 experts"), (dict(groups=8, group_top=0), "from 0 experts"),
     (dict(groups=16, top_groups=1), "top 6 of 4"), (dict(scale=0), "positive"), (dict(scale=float("nan")), "positive"),
     (dict(bias=torch.zeros(63)), "bias must be"), (dict(bias=torch.zeros(64, dtype=torch.float64)), "bias must be")])
 def test_python_forms(change, words):
@@ -216,7 +216,7 @@ def test_python_defaults():
     f = router.form(64, 6, groups=8)
     assert f.plain and (f.top_groups, f.group_top) == (8, 2)
     assert not router.form(64, 6, scale=2.0).plain and not router.form(64, 6, groups=8, top_groups=2).plain
-    assert router.form(8, 2, groups=8).group_top == 1
+    assert router.form(8, 2, groups=8, top_groups=3).group_top == 2       # of groups of one: that one
 
 
 def test_python_calls_want_a_gpu():

@@ -102,3 +102,18 @@ def test_far_and_near_rows_side_by_side():
     gb, gz = torch.tensor(0.7, device="cuda"), torch.tensor(0.2, device="cuda")
     d, = torch.autograd.grad((r.weights, r.balance, r.z), lg, (dw, gb, gz))
     tg._check(lg, 6, r, grads=((dw, gb, gz), d, "fp32"), group_top=2, **form)
+
+
+@pytest.mark.parametrize("T", [7, 4100])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_groups_of_one_expert(T, score):
+    """Scored by two experts where there is one: by that one."""
+    from vqlab_amd import router
+    rng = np.random.default_rng(T)
+    for bias in (None, torch.from_numpy((0.1 * rng.standard_normal(16)).astype(np.float32)).cuda()):
+        lg = torch.from_numpy(rng.standard_normal((T, 16)).astype(np.float32)).cuda()
+        f = dict(score=score, groups=16, top_groups=9, group_top=2, bias=bias, scale=2.5)
+        r = router.route(lg, 6, **f)
+        tg._check(lg, 6, r, **f)
+        one = router.route(lg, 6, **dict(f, group_top=1))
+        assert torch.equal(r.ids, one.ids) and torch.equal(r.weights, one.weights)

@@ -904,8 +904,6 @@ static int check_form(const vqk_route_form *f, int64_t E, int32_t k, const char 
         return set_error(VQK_EINVAL, "%s: %d of %d groups of %lld experts", what, f->top_groups, f->groups, (long long)E);
     if (f->groups > kGroupMaxGroups) return set_error(VQK_ENOTIMPL, "%s: %d groups > %d", what, f->groups, kGroupMaxGroups);
     if (f->group_top != 1 && f->group_top != 2) return set_error(VQK_ENOTIMPL, "%s: a group's score from %d experts", what, f->group_top);
-    if (f->group_top > E / f->groups)
-        return set_error(VQK_EINVAL, "%s: a group's score from %d of %lld experts", what, f->group_top, (long long)(E / f->groups));
     if (int64_t(k) > f->top_groups * (E / f->groups))
         return set_error(VQK_EINVAL, "%s: top_k=%d of %lld experts in %d groups", what, k, (long long)(f->top_groups * (E / f->groups)), f->top_groups);
     if (!(f->scale > 0.f) || f->scale > 3.4028234e38f) return set_error(VQK_EINVAL, "%s: scale %g", what, double(f->scale));

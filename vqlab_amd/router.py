@@ -83,19 +83,19 @@ class Form(NamedTuple):
 
 
 def form(E, k, score="softmax", bias=None, groups=1, top_groups=None, group_top=None, scale=1.0):
-    """A checked Form for E experts, top_groups all of them and group_top 2 (or the group's size) unless
-    given."""
+    """A checked Form for E experts, top_groups all of them and group_top 2 unless given (a group of one
+    expert scores as that)."""
     if score not in SCORES:
         raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
     groups = int(groups)
     if groups < 1 or E % groups:
         raise ValueError(f"{groups} groups of {E} experts")
     top_groups = groups if top_groups is None else int(top_groups)
-    group_top = min(2, E // groups) if group_top is None else int(group_top)
+    group_top = 2 if group_top is None else int(group_top)
     if not 1 <= top_groups <= groups:
         raise ValueError(f"top {top_groups} of {groups} groups")
-    if not 1 <= group_top <= min(2, E // groups):
-        raise ValueError(f"a group's score from {group_top} of {E // groups} experts (1 or 2 are taken)")
+    if group_top not in (1, 2):
+        raise ValueError(f"a group's score from {group_top} experts (1 or 2 are taken)")
     if k > top_groups * (E // groups):
         raise ValueError(f"top {k} of {top_groups * (E // groups)} experts in {top_groups} groups")
     scale = float(scale)
