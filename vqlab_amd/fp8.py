@@ -354,7 +354,7 @@ def _norm(x, weight, eps, residual, f8, want_r):
         res, _, ldr = _rows_in(residual, C) if residual is not None else (None, 0, C)
         w = weight.contiguous()
         h = None if residual is None else x.new_empty(x.shape)
-        r = torch.empty(n, dtype=torch.float32, device=x.device) if want_r else None
+        r = x.new_empty(n, dtype=torch.float32) if want_r else None
         y = codes = scales = None
         if f8:
             codes, scales, view = _rows_out(x, x.shape[:-1], n, C)
@@ -384,7 +384,9 @@ class _NormFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh=None):
         h, weight, r = ctx.saved_tensors
-        T.no_grad_here("The gradient of rms_norm", *(g for g in (dy, dh) if g is not None))
+        for g in (dy, dh):
+            if g is not None:
+                T.no_grad_here("The gradient of rms_norm", g)
         if dy is None:                                 # through h alone
             return dh, None, dh if ctx.has_res else None, None
         C = h.shape[-1]
@@ -393,13 +395,14 @@ class _NormFn(torch.autograd.Function):
             rows, n, ld = _rows_in(h, C)
             w, dy = weight.contiguous(), dy.contiguous()
             dh = None if dh is None else dh.contiguous()
-            dx, dw = torch.empty(h.shape, dtype=h.dtype, device=h.device), torch.empty_like(w)
+            dx, dw = h.new_empty(h.shape), w.new_empty(C)
             size = _ws_bytes(_norm_sizes, (n, C), lib.vqk_rms_norm_backward_workspace, n, C)
             work, wp = _work(h, size)
-            L.check(lib.vqk_rms_norm_backward(rows.data_ptr(), T.act_type(h), n, C, ld, w.data_ptr(), T.act_type(w),
-                                              r.data_ptr(), dy.data_ptr(), None if dh is None else dh.data_ptr(),
-                                              dx.data_ptr(), dw.data_ptr(), wp, size, T.raw_stream(h)),
-                    "rms_norm gradient")
+            rc = lib.vqk_rms_norm_backward(rows.data_ptr(), T.act_type(h), n, C, ld, w.data_ptr(), T.act_type(w),
+                                           r.data_ptr(), dy.data_ptr(), None if dh is None else dh.data_ptr(),
+                                           dx.data_ptr(), dw.data_ptr(), wp, size, T.raw_stream(h))
+            if rc:
+                L.check(rc, "rms_norm gradient")
         return dx, dw, dx if ctx.has_res else None, None
 
 

@@ -167,12 +167,12 @@ class _RouteFn(torch.autograd.Function):
             m = mask_bytes(mask, lg)
             mp = None if m is None else m.data_ptr()
             n, E = lg.shape
-            dev = lg.device
-            ids = torch.empty((n, k), dtype=torch.int32, device=dev)
-            w = torch.empty((n, k), dtype=torch.float32, device=dev)
-            counts = torch.empty(E, dtype=torch.int32, device=dev)
-            stats = torch.empty(3, dtype=torch.float32, device=dev)
-            saved = torch.empty((n, 2 if f.plain else 4), dtype=torch.float32, device=dev)
+            plain = f.plain
+            ids = lg.new_empty((n, k), dtype=torch.int32)
+            w = lg.new_empty((n, k), dtype=torch.float32)
+            counts = lg.new_empty(E, dtype=torch.int32)
+            stats = lg.new_empty(3, dtype=torch.float32)
+            saved = lg.new_empty((n, 2 if plain else 4), dtype=torch.float32)
             lib = L.lib()
             size = _sizes.get((n, E))
             if size is None:
@@ -181,21 +181,23 @@ class _RouteFn(torch.autograd.Function):
                 if len(_sizes) > 4096:
                     _sizes.clear()
                 size = _sizes[(n, E)] = ws.value
-            work = torch.empty(size, dtype=torch.uint8, device=dev)
+            work = lg.new_empty(size, dtype=torch.uint8)
             out = (ids.data_ptr(), w.data_ptr(), counts.data_ptr(), stats.data_ptr(), saved.data_ptr(),
                    work.data_ptr(), size, T.raw_stream(lg))
-            if f.plain:
-                L.check(lib.vqk_route(lg.data_ptr(), T.act_type(lg), n, E, ld, mp, k, norm, *out), "route")
+            if plain:
+                c_form, rc = None, lib.vqk_route(lg.data_ptr(), T.act_type(lg), n, E, ld, mp, k, norm, *out)
             else:
                 bias = None if f.bias is None else f.bias.contiguous()
-                L.check(lib.vqk_route_grouped(lg.data_ptr(), T.act_type(lg), n, E, ld, mp,
-                                              ctypes.byref(_c_form(f, bias)), k, norm, *out), "route")
+                c_form = _c_form(f, bias)
+                rc = lib.vqk_route_grouped(lg.data_ptr(), T.act_type(lg), n, E, ld, mp, ctypes.byref(c_form), k, norm, *out)
+                c_form.bias = None                          # the gradient reads no bias
+            if rc:
+                L.check(rc, "route")
         balance, z, tokens = stats.unbind()
         # no views, so that a loss can be scaled in place: the backward pass reads neither
         balance, z = balance.data, z.data
         ctx.save_for_backward(lg, ids, w, counts, stats, saved)
-        ctx.k, ctx.norm, ctx.ld, ctx.form = k, norm, ld, f._replace(bias=None)      # the gradient reads no bias
-        ctx.plain = f.plain
+        ctx.k, ctx.norm, ctx.ld, ctx.form = k, norm, ld, c_form
         ctx.mark_non_differentiable(ids, counts, tokens)
         ctx.set_materialize_grads(False)
         return ids, w, counts, balance, z, tokens
@@ -204,20 +206,23 @@ class _RouteFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, _ids, dw, _counts, db, dz, _tokens):
         lg, ids, w, counts, stats, saved = ctx.saved_tensors
-        T.no_grad_here("The gradient of the router", *(g for g in (dw, db, dz) if g is not None))
+        for g in (dw, db, dz):
+            if g is not None:
+                T.no_grad_here("The gradient of the router", g)
         n, E = lg.shape
         with T.on_device(lg):
-            d = torch.empty((n, E), dtype=lg.dtype, device=lg.device)
+            d = lg.new_empty((n, E))
             grads = [None if g is None else _f32(g) for g in (dw, db, dz)]
             at = (ctx.k, ctx.norm, ids.data_ptr(), w.data_ptr(), counts.data_ptr(), stats.data_ptr(),
                   saved.data_ptr(), *(None if g is None else g.data_ptr() for g in grads), d.data_ptr(),
                   T.raw_stream(lg))
-            if ctx.plain:
+            if ctx.form is None:
                 rc = L.lib().vqk_route_backward(lg.data_ptr(), T.act_type(lg), n, E, ctx.ld, *at)
             else:
                 rc = L.lib().vqk_route_grouped_backward(lg.data_ptr(), T.act_type(lg), n, E, ctx.ld,
-                                                        ctypes.byref(_c_form(ctx.form, None)), *at)
-            L.check(rc, "route backward")
+                                                        ctypes.byref(ctx.form), *at)
+            if rc:
+                L.check(rc, "route backward")
         return d, None, None, None, None
 
 
