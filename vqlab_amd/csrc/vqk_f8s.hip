@@ -6,7 +6,7 @@ namespace vqk {
 // Registers of a block: two buffers of weights and their scales, and x.
 constexpr int f8s_regs(int op, int nt, int p) { return 18 + nt * (op == kOpF8 ? 9 : 16 * p + 1); }
 // Blocks a wave that the registers hold.
-constexpr int f8s_cap(int op, int nt, int p) { return 200 / f8s_regs(op, nt, p); }
+constexpr int f8s_cap(int op, int nt, int p) { return 208 / f8s_regs(op, nt, p); }
 
 struct F8sPlan { int kw, ncw; };              // waves along k and blocks a wave; kw = 0: x does not fit
 static F8sPlan f8s_plan(int64_t NC, int cap, int64_t row_tiles) {
