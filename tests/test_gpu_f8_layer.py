@@ -358,3 +358,14 @@ def test_router_forms_are_refused():
     wide = torch.randn(3, 1024, device="cuda")
     with pytest.raises(NotImplementedError):
         router.top_k(wide, 4, groups=128, top_groups=64)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("N,OUT,IN", [(1, 100, 5121), (2, 64, 8000), (3, 2000, 7400), (16, 33, 17408), (17, 130, 4104),
+                                      (20, 5120, 6016), (32, 48, 20001), (9, 16, 120000)])
+def test_few_rows_of_many_blocks(dtype, N, OUT, IN):
+    """Rows of more blocks than eight waves hold: ranges of k, added up in their order."""
+    import test_gpu_f8 as tf
+    tf.test_linear(dtype, N, OUT, IN)
+    tf.test_linear_8_bit_activations(dtype, N, OUT, IN)
+    tf.test_linear_gradient(dtype, N, min(IN, 9000), OUT)

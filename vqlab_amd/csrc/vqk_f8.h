@@ -146,8 +146,10 @@ struct F8Call {
 };
 
 // Few rows (vqk_f8s.h): whether it takes a call, and its launch.
+// part: room for the sums of ranges of k, f8_rows_part bytes.
 bool f8_rows_ok(const F8Call &c);
-int f8_rows(const F8Call &c, hipStream_t st);
+size_t f8_rows_part(const F8Call &c);
+int f8_rows(const F8Call &c, float *part, size_t part_bytes, hipStream_t st);
 // Many rows (vqk_f8t.h). part: room for the K slices of the last tiles, f8_tiles_part
 // bytes (scaled: 16-bit x with scales).
 size_t f8_tiles_part(int64_t N, const F8Geom &g, bool a8, bool scaled, int P);

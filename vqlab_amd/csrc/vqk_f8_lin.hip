@@ -152,7 +152,7 @@ static PlainPlan plain_plan(const F8Geom &g, int32_t type, int64_t N) {
     p.few = f8_rows_ok(c);
     p.lay = type == VQK_F32 || g.IN % (p.few ? 8 : kF8Block);
     p.x = p.lay ? al256(size_t(N) * g.NC * 256 * c.x.P) : 0;
-    p.part = p.few ? 0 : f8_tiles_part(N, g, false, false, c.x.P);
+    p.part = p.few ? f8_rows_part(c) : f8_tiles_part(N, g, false, false, c.x.P);
     return p;
 }
 static size_t plain_bytes(const F8Geom &g, int32_t type, int64_t N) {
@@ -182,7 +182,7 @@ static A8Plan a8_plan(const F8Geom &g, int64_t N, int64_t ldc, int32_t y_type) {
     // in place, if a tile's rows are within reach of 32-bit offsets
     p.place = ldc && !wide && g.IN % 128 == 0 && ldc % 16 == 0 && ldc < (1 << 24);
     p.x = p.place ? 0 : rows_bytes(g, N, y_type);
-    p.part = p.few ? 0 : f8_tiles_part(N, g, !wide, true, 1);
+    p.part = p.few ? f8_rows_part(c) : f8_tiles_part(N, g, !wide, true, 1);
     return p;
 }
 static size_t a8_bytes(const F8Geom &g, int64_t N, int64_t ldc, int32_t y_type) {
@@ -215,8 +215,8 @@ static int plain_product(F8Call c, const void *x, int32_t type, uint8_t *ws, hip
         c.x.plane = N * ld;
         c.g.IN = ld;
     }
-    if (p.few) return f8_rows(c, st);
-    return f8_tiles(c, p.part ? reinterpret_cast<float *>(ws + p.x) : nullptr, p.part, st);
+    float *part = p.part ? reinterpret_cast<float *>(ws + p.x) : nullptr;
+    return p.few ? f8_rows(c, part, p.part, st) : f8_tiles(c, part, p.part, st);
 }
 
 // The product of 8-bit rows; ws: a8_bytes. here: they are whole blocks at its start, with
@@ -241,8 +241,8 @@ static int a8_product(F8Call c, const F8X &x, bool here, uint8_t *ws, hipStream_
         if (wide) c.x = MxX{reinterpret_cast<uint16_t *>(to), c.g.NC * 128, 0, 1, kOpBF16};
     }
     if (wide) c.g.IN = c.g.NC * 128;          // x's rows are whole blocks, zero past the weight's columns
-    if (p.few) return f8_rows(c, st);
-    return f8_tiles(c, p.part ? reinterpret_cast<float *>(ws + p.x) : nullptr, p.part, st);
+    float *part = p.part ? reinterpret_cast<float *>(ws + p.x) : nullptr;
+    return p.few ? f8_rows(c, part, p.part, st) : f8_tiles(c, part, p.part, st);
 }
 
 static F8Call base_call(const vqk_f8_weights *w, const F8Geom &g, int64_t N, bool a8, void *y, int32_t y_type) {

@@ -12,6 +12,8 @@
 // four neighbouring outputs of one x row and that row's scales are one number a
 // lane. The fp32 sums of KW > 1 waves meet in LDS in wave order, two buffers in
 // turn, one barrier a step.
+// Rows of more blocks than eight waves hold (kF8sWaves times the registers' NCW) are cut
+// into ks ranges of k, a workgroup each, whose sums a second kernel adds up.
 // x comes from its rows where there are one or two, otherwise through LDS, copied
 // in whole lines (8 KB or less a wave at a time).
 // Bound by HBM: 2 KB of weights take a wave 32 cycles (8-bit x) or 64 and the
@@ -38,7 +40,9 @@ struct F8sArgs {
     int64_t sn, sk;
     void *y;
     int32_t y_type;
-    int32_t nob, kw, steps, total_steps, stage;
+    int32_t nob, kw, ks, steps, total_steps, stage;
+    int32_t even, more;                       // blocks of a share of k (kw * ks of them), shares with one more
+    float *part;                              // ks > 1: sums of each range of k, [ks][N][OUT]
 };
 
 // OP: kOpF16, kOpBF16, or kOpF8 (8-bit x).
@@ -53,12 +57,15 @@ __global__ void __launch_bounds__(64 * kF8sWaves, 2) k_f8_rows(const F8sArgs p) 
     const int r = lane & 15, g = lane >> 4;
     const int KW = p.kw, RW = kF8sWaves / KW;
     const int kw = wave % KW, rw = wave / KW;
-    const int t = int(blockIdx.x / unsigned(p.nob)), part = int(blockIdx.x % unsigned(p.nob));
+    const int t = int(blockIdx.x / unsigned(p.nob)) / p.ks, z = int(blockIdx.x / unsigned(p.nob)) % p.ks;
+    const int part = int(blockIdx.x % unsigned(p.nob));
     const int row0 = t * 16 * NT, nrows = int(min(int64_t(16 * NT), p.N - row0));
     const int s_lo = part * p.steps, s_hi = min(p.total_steps, s_lo + p.steps);
     if (s_lo >= s_hi) return;
 
-    const int c0 = kw * NCW, nc = min(NCW, p.NC - c0);  // this wave's blocks (none: nc < 1)
+    // this wave's blocks: an even share of them all, NCW at most
+    const int share = z * KW + kw;
+    const int c0 = share * p.even + min(share, p.more), nc = p.even + (share < p.more);
     u32x4 wn[NCW][2];
     float swn[NCW];
     auto load_w = [&](int step) {
@@ -176,8 +183,14 @@ __global__ void __launch_bounds__(64 * kF8sWaves, 2) k_f8_rows(const F8sArgs p) 
             float q[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) q[i] = OP == kOpBF16 ? v[i] * kF8Up : v[i];
-            const bool al = (p.OUT & 3) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
-            mx_store4(p.y, p.y_type, int64_t(row0 + n) * p.OUT + o, q, int(min(int64_t(4), p.OUT - o)), al);
+            const int64_t at = int64_t(row0 + n) * p.OUT + o;
+            const int count = int(min(int64_t(4), p.OUT - o));
+            if (p.ks > 1) {
+                mx_store4(p.part, VQK_F32, int64_t(z) * p.N * p.OUT + at, q, count, (p.OUT & 3) == 0);
+            } else {
+                const bool al = (p.OUT & 3) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
+                mx_store4(p.y, p.y_type, at, q, count, al);
+            }
         };
         if (KW == 1) {
 #pragma unroll
