@@ -369,3 +369,83 @@ def test_few_rows_of_many_blocks(dtype, N, OUT, IN):
     tf.test_linear(dtype, N, OUT, IN)
     tf.test_linear_8_bit_activations(dtype, N, OUT, IN)
     tf.test_linear_gradient(dtype, N, min(IN, 9000), OUT)
+
+
+def _within(got, ref, mag, n, dtype, more=0.0):
+    """fc.product_bar's bar, on the GPU: n exact products summed in fp32, scales, slices, one rounding."""
+    acc = (n + 20) * EPS * mag + more
+    step = mc.HALF_STEP[dtype] * (ref.abs() + acc)
+    bar = acc + (step.clamp(min=2.0 ** -25) if dtype == "fp16" else step)
+    bad = ((got.double() - ref).abs() > bar).sum()
+    assert int(bad) == 0, f"{int(bad)} of {ref.numel()}"
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("N,OUT,IN", [(49, 4096, 10240), (64, 4100, 10300), (100, 10240, 4096), (129, 4096, 10240),
+                                      (200, 10300, 4100), (333, 5120, 8192), (700, 4096, 4096),
+                                      (14001, 300, 260), (17000, 257, 384), (20011, 100, 513)])
+def test_tiles(dtype, N, OUT, IN):
+    """Products large enough for tiles, whatever x: few of them cut along k, and many small ones. In 64 bits
+    on the GPU."""
+    from vqlab_amd import fp8
+    rng = np.random.default_rng(N + OUT + IN)
+    codes, s, w = fc.weight(rng, OUT, IN)
+    codes, s = torch.from_numpy(codes).cuda(), torch.from_numpy(s).cuda()
+    lin, lin8 = fp8.F8Linear(codes, s), fp8.F8Linear(codes, s, "fp8")
+    w = torch.from_numpy(w).cuda()
+    torch.manual_seed(N)
+    x = torch.randn(N, IN, device="cuda").to(mc.torch_dtype(dtype)).requires_grad_()
+    y = lin(x)
+    xd, aw = x.detach().double(), w.abs()
+    _within(y.detach(), xd @ w.t(), xd.abs() @ aw.t(), IN, dtype)
+    dy = torch.randn_like(y)
+    dx, = torch.autograd.grad(y, x, dy)
+    dd = dy.double()
+    _within(dx, dd @ w, dd.abs() @ aw, OUT, dtype)
+    # 8-bit x: exact into fp32; into 16 bits each group of eight products may lose 7 * 2^-13 of its largest
+    q = fp8.f8_quantize(x.detach())
+    xd = q.codes.float().double() * q.scales.double().repeat_interleave(128, 1)[:, :IN]
+    ref, mag = xd @ w.t(), xd.abs() @ aw.t()
+    _within(lin8(q, out_dtype=torch.float32), ref, mag, IN, "fp32")
+    if dtype != "fp32":
+        pad = lambda t: torch.nn.functional.pad(t.abs().float(), (0, -IN % 8)).unflatten(1, (-1, 8))
+        a, b = pad(xd), pad(w)
+        top = torch.stack([(a[n][None] * b).amax(-1).sum(-1) for n in range(N)]).double()
+        _within(lin8(x.detach()), ref, mag, IN, dtype, 1.01 * 7 * 2.0 ** -13 * top)
+
+
+@pytest.mark.parametrize("act", [None, "fp8"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("N,OUT,IN", [(100, 4160, 10304), (9000, 300, 1100)])
+def test_tiles_keep_to_their_rows(dtype, N, OUT, IN, act):
+    """NaN, infinities and far values of x, codes and scales that are NaN: what they do not meet is as ever."""
+    from vqlab_amd import fp8
+    rng = np.random.default_rng(N + IN)
+    codes, s, w = fc.weight(rng, OUT, IN)
+    codes[11, 77], codes[270, IN - 1] = 0x7f, 0xff
+    s[1, 2] = np.nan                                       # weight rows 128 .. 255
+    w = fc.weight_values(fc.decode(codes), s)
+    lin = fp8.F8Linear(torch.from_numpy(codes).cuda(), torch.from_numpy(s).cuda(), act)
+    w = torch.from_numpy(w).cuda()
+    torch.manual_seed(N)
+    x = torch.randn(N, IN, device="cuda")
+    far = 2.0 ** 12 if dtype == "fp16" else 2.0 ** 100
+    x[5] *= far
+    x[6] /= far
+    x = x.to(mc.torch_dtype(dtype))
+    x[17, 3], x[18, IN - 1], x[19, 200] = float("nan"), float("inf"), -float("inf")
+    with torch.no_grad():
+        out = torch.float32 if act else x.dtype
+        y = lin(x, out_dtype=out)
+        if act:
+            q = fp8.f8_quantize(x)
+            xd = q.codes.float().double() * q.scales.double().repeat_interleave(128, 1)[:, :IN]
+        else:
+            xd = x.double()
+    xd = xd.nan_to_num(nan=float("nan"), posinf=float("nan"), neginf=float("nan"))
+    ref, mag = xd @ w.t(), xd.abs() @ w.abs().t()
+    assert ref.isnan().any(0)[[11, 128, 255, 270]].all() and ref.isnan().any(1)[[17, 18, 19]].all()
+    fine = ref.isfinite()
+    assert not y[~fine].isfinite().any()
+    # x / far in fp16 has numbers below the smallest normal one, which are exact all the same
+    _within(torch.where(fine, y.double(), 0), torch.where(fine, ref, 0), torch.where(fine, mag, 0), IN, "fp32" if act else dtype)

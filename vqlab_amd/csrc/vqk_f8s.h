@@ -1,5 +1,5 @@
 // Products of 8-bit weights with few rows of x: the weights are streamed once
-// past up to 16 * NT rows.
+// past up to 16 * NT rows, and again for the next ones.
 //
 //     y[n, o] = sum_b f[n, o, b] sum_{k in b} w8[o, k] x[n, k]
 //     f = sw[o / 128, b], with x in 8 bits (or codes' values in 16) times sx[n, b]
@@ -15,7 +15,7 @@
 // Rows of more blocks than eight waves hold (kF8sWaves times the registers' NCW) are cut
 // into ks ranges of k, a workgroup each, whose sums a second kernel adds up.
 // x comes from its rows where there are one or two, otherwise through LDS, copied
-// in whole lines (8 KB or less a wave at a time).
+// in whole lines (20 KB or less a wave at a time).
 // Bound by HBM: 2 KB of weights take a wave 32 cycles (8-bit x) or 64 and the
 // conversions (16-bit), a fraction of the time in which they can arrive. Measured:
 // 5120 to 17408, 8 rows of 8 bits 17.5 us (5.1 TB/s), 20 rows 19.0 (4.7); one row of bf16,

@@ -21,14 +21,22 @@ static F8sPlan f8s_plan(int64_t NC, int cap, int64_t row_tiles) {
 
 static int call_op(const F8Call &c) { return c.a8 ? kOpF8 : c.x.op; }
 static int call_p(const F8Call &c) { return c.a8 ? 1 : c.x.P; }
-static int call_nt(const F8Call &c) { return c.N <= 16 ? 1 : 2; }
+static int call_nt(const F8Call &c) { return c.N <= 16 || call_p(c) != 1 ? 1 : 2; }
+static int64_t call_tiles(const F8Call &c) { return (c.N + 16 * call_nt(c) - 1) / (16 * call_nt(c)); }
 static F8sPlan call_plan(const F8Call &c) {
-    const int nt = call_nt(c);
-    return f8s_plan(c.g.NC, f8s_cap(call_op(c), nt, call_p(c)), (c.N + 16 * nt - 1) / (16 * nt) * c.g.RT);
+    return f8s_plan(c.g.NC, f8s_cap(call_op(c), call_nt(c), call_p(c)), call_tiles(c) * c.g.RT);
 }
 
+// Up to one tile of x (fp32: three) always: the weights pass once. More while the passes over
+// them stay short of what tiles of 256 weight rows cost in slices of k and their sum. bf16 x
+// in us, this way / by tiles: 4096 squared, 64 rows 11.7 / 17.1, 128 rows (67 MB in all)
+// 13.4 / 21.0, 192 (100 MB) 22.1 / 19.1; 1024 squared, 1024 rows (33 MB) 10.3 / 14.2; 512
+// squared, 8192 rows (67 MB, 256 tiles) 14.0 / 12.0; 5120 to 17408, 64 rows (178 MB) 41 / 30.
+// fp32 x: 4096 squared, 96 rows (100 MB) 29 / 32, 192 43 / 39; 5120 to 17408, 48 rows 54 / 61.
 bool f8_rows_ok(const F8Call &c) {
-    return c.N <= 32 && !(call_nt(c) == 2 && call_p(c) != 1);
+    const int64_t tiles = call_tiles(c);
+    const bool one = call_p(c) == 1;
+    return tiles <= (one ? 1 : 3) || tiles * f8_code_bytes(c.g.RT, c.g.NC) <= (one ? (tiles <= 16 ? 72 : 36) : 96) << 20;
 }
 
 size_t f8_rows_part(const F8Call &c) {
@@ -104,7 +112,7 @@ int f8_rows(const F8Call &c, float *part, size_t part_bytes, hipStream_t st) {
     if (need > part_bytes || (need && !part)) return set_error(VQK_ENOSPACE, "8-bit product: workspace %zu < %zu", part_bytes, need);
     a.ks = pl.ks;
     a.part = part;
-    const int64_t tiles = (c.N + 16 * nt - 1) / (16 * nt);
+    const int64_t tiles = call_tiles(c);
     switch (call_op(c)) {
         case kOpF8: return nt == 2 ? go_ncw<kOpF8, 2, 1>(a, tiles, pl, st) : go_ncw<kOpF8, 1, 1>(a, tiles, pl, st);
         case kOpF16: return nt == 2 ? go_ncw<kOpF16, 2, 1>(a, tiles, pl, st) : go_ncw<kOpF16, 1, 1>(a, tiles, pl, st);
