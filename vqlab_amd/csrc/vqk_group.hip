@@ -387,10 +387,12 @@ __device__ __forceinline__ void row_each(const void *l, int64_t base, int E, boo
 // ------------------------------------------------- sixteen lanes to a token
 // Bounds of what fp32 may get wrong in a comparison of two c (smax: the row's
 // largest s): a sigmoid is 4 units of 2^-23 off at most, a softmax 2^-18 of itself
-// (its sum adds up E terms, 32 in a lane), the sum with the bias half a unit.
+// (its sum adds up E terms, 32 in a lane), the sum with the bias half a unit. An
+// exponential below 2^-126 comes out as 0, which costs a sigmoid up to that much whatever
+// smax is: four times it, two scores to a group's sum on each side of the comparison.
 template <bool SIG>
 __device__ __forceinline__ float group_tol(float smax, float c) {
-    return (SIG ? 0x1p-19f : 0x1p-16f) * smax + 0x1p-21f * __builtin_fabsf(c);
+    return (SIG ? __builtin_fmaf(0x1p-19f, smax, 0x1p-124f) : 0x1p-16f * smax) + 0x1p-21f * __builtin_fabsf(c);
 }
 
 // Lane `sub` of a token holds in value 4 q + j expert 64 q + 4 ((sub + 4 q) % 16) + j:
