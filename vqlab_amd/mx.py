@@ -398,7 +398,8 @@ class MXSparseMoeBlock(torch.nn.Module):
     """Top-k routing and MXFP4 experts: forward(x [T, H], logits [T, E], mask [T]) ->
     [T, H]; without logits they are x . router_weight^T. mask: 0 marks padding, whose rows are
     zero and take no expert's time. form: keyword arguments of router.top_k beyond its softmax (score,
-    bias, groups, top_groups, group_top, scale); the bias is a buffer."""
+    bias, groups, top_groups, group_top, scale); the bias is a buffer, whose type casts of the module
+    leave as it is."""
 
     form = {}
 
@@ -412,6 +413,22 @@ class MXSparseMoeBlock(torch.nn.Module):
             router.form(switch_mlp.gate_proj.num_experts, self.top_k, **form)      # a ValueError where it does not fit
             self.register_buffer("bias", form.pop("bias", None))
             self.form = form
+
+    def _apply(self, fn, recurse=True):
+        bias = self._buffers.get("bias")
+        if bias is None:
+            return super()._apply(fn, recurse)
+        self._buffers["bias"] = None
+        try:
+            super()._apply(fn, recurse)
+            # as bytes, whose values casts keep: a rounded bias chooses other experts
+            flat = bias.detach().contiguous().view(torch.uint8)
+            moved = fn(flat)
+            if moved is not flat:
+                bias = moved.to(torch.uint8).view(bias.dtype)
+        finally:
+            self._buffers["bias"] = bias
+        return self
 
     def forward(self, x, logits=None, mask=None):
         if logits is None:
