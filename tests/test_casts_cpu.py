@@ -1,11 +1,13 @@
-"""Casts of modules over quantised weights: the routing bias, which decides exactly, keeps
-its bits. On the CPU, over modules whose device work is left out."""
+"""Casts of modules over quantised weights: what decides exactly (the routing bias, the scales of 8-bit
+weights) keeps its bits. On the CPU, over modules whose device work is left out."""
 from __future__ import annotations
+
+import copy
 
 import pytest
 import torch
 
-from vqlab_amd import mx
+from vqlab_amd import fp8, mx
 
 CASTS = [lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.double(), lambda m: m.to(torch.bfloat16),
          lambda m: m.type(torch.float16), lambda m: m.type(torch.bfloat16), lambda m: m.to("cpu")]
@@ -55,3 +57,19 @@ def test_blocks_without_a_bias():
     assert m.bias is None and "bias" not in m.state_dict()
     plain = mx.MXSparseMoeBlock(Experts(16), 2, router_weight=torch.nn.Parameter(torch.randn(16, 8))).half()
     assert plain.router_weight.dtype == torch.float16
+
+@pytest.mark.parametrize("cast", CASTS, ids=NAMES)
+def test_scales_of_8_bit_weights_keep_their_bits(cast):
+    g = torch.Generator().manual_seed(2)
+    packed = torch.randint(0, 256, (16 * 2 * 256,), generator=g).to(torch.uint8)
+    scales = 2.0 ** (200 * torch.rand(1, 2, generator=g) - 120)
+    lin = fp8.F8Linear.__new__(fp8.F8Linear)
+    torch.nn.Module.__init__(lin)
+    lin.out_features, lin.in_features, lin.act, lin._sizes = 32, 256, None, {}
+    lin._keep(packed, scales)
+    cast(lin)
+    assert torch.equal(lin._packed[0], packed) and lin._packed[0].dtype == torch.uint8
+    assert torch.equal(lin._packed[1], scales) and lin._packed[1].dtype == torch.float32
+    assert lin._packed[1].shape == (1, 2)
+    other = copy.deepcopy(lin)
+    assert torch.equal(other._packed[1], scales) and other._packed[1].data_ptr() != lin._packed[1].data_ptr()

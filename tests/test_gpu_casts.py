@@ -31,3 +31,17 @@ def test_the_block_chooses_the_same_after_casts(T):
                  lambda: block.cpu().cuda(), lambda: block.type(torch.float16)):
         cast()
         assert block.bias.dtype == torch.float32 and block.bias.is_cuda and torch.equal(block(x, lg), want)
+
+
+@pytest.mark.parametrize("act", [None, "fp8"])
+def test_8_bit_linears_after_casts(act):
+    from vqlab_amd import fp8
+    torch.manual_seed(1)
+    lin = fp8.F8Linear.from_weight(torch.randn(200, 300, device="cuda") * torch.logspace(-6, 6, 300, device="cuda"), act)
+    x = torch.randn(9, 300, device="cuda")
+    want, codes, scales = lin(x), lin.codes.view(torch.uint8), lin.scales
+    for cast in (lambda: lin.half(), lambda: lin.type(torch.float16), lambda: lin.type(torch.bfloat16),
+                 lambda: lin.cpu().type(torch.float16).cuda()):
+        cast()
+        assert torch.equal(lin.codes.view(torch.uint8), codes) and torch.equal(lin.scales, scales)
+        assert torch.equal(lin(x), want)

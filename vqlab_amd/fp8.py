@@ -254,8 +254,8 @@ class F8Linear(torch.nn.Module):
     def _apply(self, fn, recurse=True):
         super()._apply(fn, recurse)
         packed, scales = self._packed
-        # as integers, which casts of floating-point tensors leave alone
-        self._keep(fn(packed).to(torch.uint8), fn(scales.view(torch.int32)).to(torch.int32).view(torch.float32))
+        # as bytes, whose values casts keep (type() casts integers too)
+        self._keep(fn(packed).to(torch.uint8), fn(scales.view(torch.uint8)).to(torch.uint8).view(torch.float32))
         return self
 
     def __getstate__(self):
