@@ -527,7 +527,9 @@ int vqk_f8_unpack(const uint8_t *packed, int64_t OUT, int64_t IN, uint8_t *codes
  * dropped); VQK_F8_ACT_F8 quantises x's rows as vqk_f8_quantize does. Products of
  * 8-bit x into a 16-bit y run on the 8-bit matrix instructions, which keep 14 bits of
  * the largest of eight neighbouring products and what lines up with it of the others;
- * into an fp32 y every product enters exactly.
+ * into an fp32 y every product enters exactly. The scales of a row and of a weight are
+ * multiplied into one fp32 number first: a block keeps fewer bits where that is below 2^-126
+ * (blocks of outputs under 2^-101), and is infinite or NaN where it is 2^128 or more.
  * vqk_f8_linear_rows takes rows that are in 8 bits already (codes ldc apart, scales
  * as above). x of act NONE, codes and dy are 16-byte aligned (VQK_EINVAL); workspaces are
  * 256-byte aligned (NULL where a query says 0) and hold nothing between calls. */
@@ -552,7 +554,8 @@ int vqk_f8_linear_dx(const vqk_f8_weights *w, const void *dy, int32_t dy_type, i
  *   y = h * r * weight, r = 1 / sqrt(mean h^2 + eps)
  * x and residual: rows ldx, ldr elements apart; h and y contiguous. Either y (the
  * type of x), or codes [N, C] and scales as vqk_f8_quantize makes them of the fp32 y.
- * h: with a residual only. r: fp32 [N] for the backward pass, or NULL.
+ * h: with a residual only. r: fp32 [N] for the backward pass, or NULL; an fp32 number, so with
+ * eps 0 a row whose root mean square is under 2^-128 comes out infinite, a row of zeros NaN.
  * vqk_rms_norm_backward: dx (also the residual's gradient) and dw [C] (w_type) from
  * dy and dh (the gradient of h, NULL for none), both contiguous; h as the norm took
  * it, rows ldh apart. The workspace is 16-byte aligned. */

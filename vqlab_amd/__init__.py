@@ -9,7 +9,9 @@ modules mirror the reference runtime's interface over torch tensors:
   vqlab_amd.artifact   -- VQLab artifact loader (config.json + safetensors)
 and beyond the reference:
   vqlab_amd.mx         -- MXFP4 weights: quantiser, linears, routed experts
-  vqlab_amd.router     -- softmax top-k routing with counts, losses and gradients
+  vqlab_amd.fp8        -- 8-bit (e4m3) weights with block scales: quantisers, linears; RMS norm
+  vqlab_amd.router     -- top-k routing (softmax or sigmoid, a bias, groups of experts) with counts,
+                          losses and gradients
 """
 from . import _lib
 

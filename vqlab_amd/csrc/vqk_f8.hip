@@ -7,8 +7,8 @@
 // which rounds to 448. A block with an infinity or NaN gets the scale NaN and
 // codes 0, and reads back as NaN. Bound by memory: a row's block is 16 lanes of
 // 8 values, so a wave's loads are contiguous, and the largest magnitude takes
-// four DPP steps inside the lanes' row. Measured: 2048 rows of 5120 bf16 9.3 us (3.4 TB/s,
-// out of the MALL in part), 20 rows 3.3, back to bf16 8.3.
+// four DPP steps inside the lanes' row. Measured: 2048 rows of 5120 bf16 9.6 us (3.3 TB/s,
+// out of the MALL in part), 20 rows 3.2, back to bf16 8.4.
 #include "vqk_f8.h"
 
 namespace vqk {

@@ -5,8 +5,8 @@
 // 8-bit rows run on the 8-bit matrix instructions where the output has 16 bits, and
 // as the codes' values in bf16 where it has 32 (vqk_f8.h).
 // bf16 x enters as it is, fp16 x too (every e4m3 code is an fp16 number), fp32 x as
-// three exact bf16 planes. x that is a multiple of 8 wide is
-// read in place (many rows: whole blocks wide), other x is laid out in the workspace first. The gradient sums over
+// three exact bf16 planes. x that is a multiple of 8 wide is read in place (many rows:
+// whole blocks wide), other x is laid out in the workspace first. The gradient sums over
 // the weight's rows, along which its codes do not lie: they are transposed into the
 // workspace, operand order to operand order, and the same products run on them with
 // the strides of the scales exchanged.
@@ -95,7 +95,7 @@ struct F8Trans {
 };
 
 // 128 x 128 codes through LDS: 16 k of a weight row in per unit, 4 x 16 codes
-// turned by byte permutes, 16 weight rows of a k out. 5120 x 17408: 47 us (3.8 TB/s both ways).
+// turned by byte permutes, 16 weight rows of a k out. 5120 x 17408: 48 us (3.7 TB/s both ways).
 __global__ void __launch_bounds__(256) k_f8_trans(const F8Trans p) {
     constexpr int LD = 144;
     __shared__ __align__(16) uint8_t tile[128 * LD];    // [weight row][k]

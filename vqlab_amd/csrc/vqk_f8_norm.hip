@@ -15,9 +15,9 @@
 // takes four DPP steps. Squares are summed in fp64 (2^127 squared is no fp32
 // number), everything else is fp32. dw: a workgroup adds up its rows in
 // registers, the workgroups' sums meet in a fixed order.
-// Measured: one row of 4096 to 8 bits 3.1 us, 2048 rows of 5120 fp16 18 (4.1 TB/s), 16384
-// rows of 4096 bf16 with h 87 (6.1 TB/s, out of the MALL in part), backward 113
-// (4.75 TB/s) and 6.5 for dw.
+// Measured: one row of 4096 to 8 bits 3.0 us, 2048 rows of 5120 fp16 18 (4.1 TB/s), 16384
+// rows of 4096 bf16 with h 87 (6.2 TB/s, out of the MALL in part), backward 112
+// (4.8 TB/s) and 6.2 for dw.
 #include "vqk_f8.h"
 
 namespace vqk {
@@ -190,7 +190,8 @@ __device__ __forceinline__ float raw_at(const Raw8<XT> &r, int i) {
 }
 
 // The next row is loaded while this one is worked on, as it lies in memory (half the
-// registers of its values); rows of more than 8 waves leave no registers for that.
+// registers of its values); rows of more than 8 waves leave no registers for that (the 128
+// of 1024 threads: those kernels spill 3 to 11).
 template <int XT, int P, int MAXW>
 __global__ void __launch_bounds__(64 * MAXW) k_rms_bwd(const NormBwdArgs p, bool vec, bool vecw) {
     constexpr bool AHEAD = MAXW <= 8;

@@ -19,7 +19,7 @@
 // Bound by HBM: 2 KB of weights take a wave 32 cycles (8-bit x) or 64 and the
 // conversions (16-bit), a fraction of the time in which they can arrive. Measured:
 // 5120 to 17408, 8 rows of 8 bits 17.5 us (5.1 TB/s), 20 rows 19.0 (4.7); one row of bf16,
-// 4096 to 4096, 7.0 us, a chain of launch, first load, products and the waves' sum.
+// 4096 to 4096, 6.5 us, a chain of launch, first load, products and the waves' sum.
 #pragma once
 
 #include "vqk_f8t.h"

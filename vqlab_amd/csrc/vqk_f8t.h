@@ -15,12 +15,12 @@
 // What bounds the tile: accumulators are VALU operands, so they, the weights and two
 // tiles of sums share 256 registers (two waves a SIMD): BN up to 256 with 8-bit x, 192
 // with 16-bit x, whose two buffers fill LDS, too.
-// Measured (us, slices' sum included): 2048 rows of 5120 to 17408, 8-bit x 196 (1.86 PF; the
+// Measured (us, slices' sum included): 2048 rows of 5120 to 17408, 8-bit x 203 (1.8 PF; the
 // same loop without its copies and barriers 2.4 PF, so the matrix cores and the
 // multiply-adds behind them are what it waits for); 2048 rows of 17408 to 5120, bf16 x
-// 412 (0.89 PF; 320 tiles are 1.25 rounds), its gradient 366 (1.0 PF) after the
-// transposition; 333 rows of 17408 to 5120, fp16 x 88 (384 rows' work at 0.78 PF, 15 us of
-// them slices).
+// 415 (0.88 PF; 320 tiles are 1.25 rounds), its gradient 374 (0.98 PF) after the
+// transposition; 333 rows of 17408 to 5120, fp16 x 87 (384 rows' work at 0.78 PF, 7.4 us of
+// them the slices' sum). The long ones are 5 to 10 % shorter on a cool chip.
 // Whole rounds of tiles run as they are; the tiles of the last, partial round are cut
 // along k, so that every CU has a part, into fp32 partials summed in a fixed order.
 #pragma once

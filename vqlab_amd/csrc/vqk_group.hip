@@ -24,7 +24,7 @@
 // order: every result is the same from call to call.
 // Bound by instructions: 65536 tokens over 256 experts in 8 groups read 67 MB in 70 us
 // (1800 vector instructions for four tokens, issued 65 % of the time at three waves a
-// SIMD), the gradient moves twice that in 37 (3.6 TB/s). 64 tokens: 8.8 us, one wave's
+// SIMD), the gradient moves twice that in 37 (3.6 TB/s). 64 tokens: 8.9 us, one wave's
 // chain of loads, fp64 exponentials, groups and k maxima.
 #include "vqk_gemv.h"
 #include "vqk_route.h"

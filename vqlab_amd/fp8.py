@@ -408,8 +408,8 @@ class _NormFn(torch.autograd.Function):
 
 def rms_norm(x, weight, eps=1e-6, residual=None):
     """y = h / sqrt(mean(h^2) + eps) * weight over the last dimension of x [..., C] (fp16, bf16, fp32; C at
-    most 16384), h = x + residual rounded once to their type; with a residual y, h, otherwise y.
-    Differentiable in x, residual and weight."""
+    most 16384), h = x + residual rounded once to their type; with a residual y, h, otherwise y. eps 0 is
+    for rows of a root mean square of 2^-128 and more. Differentiable in x, residual and weight."""
     _check_norm(x, weight, eps, residual, "rms_norm")
     ts = (x, weight) if residual is None else (x, weight, residual)
     for t in ts:
